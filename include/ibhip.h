@@ -68,6 +68,7 @@ int         ibh_memcpy_d2d(void* dst, const void* src, size_t bytes, void* strea
  * reference counterpart (the CPU kernels have no such failure). */
 #define IBH_DEVERR_TILE_WAIT 1   /* a bounded wait inside the tile GEMV expired */
 #define IBH_DEVERR_PQ_WS     2   /* a PQ workspace that ibh_pq_workspace_init did not prepare */
+#define IBH_DEVERR_KV4_TABLE 4   /* a 4-bit cache whose table names a page, or whose lens a length, that it has not */
 int         ibh_device_errors(int clear);
 
 /* ── quantized matvec, device pointers ─────────────────────── */
@@ -198,6 +199,80 @@ int ibh_attn_set_split(int on);
  * the query heads of a KV head together from one coalesced key tile in LDS
  * (head_dim 64 or 128), 0 one head per launch row.  Same bits either way. */
 int ibh_attn_exact_set_grouped(int on);
+
+/* ── paged 4-bit KV cache, device pointers ─────────────────── */
+
+/* No counterpart in the reference, whose 4-bit cache (kv_bits 4 above) holds
+ * one sequence with one scale per position and head: a cache of n_seq
+ * sequences in pages of 64 positions, each 64 dims of a position held as
+ * 4-bit codes with their own fp16 scale and middle (4.5 bits an element).
+ *
+ * Every device array belongs to the caller and may change between calls, and
+ * between the replays of a captured graph:
+ *   pool   n_pages pages of ibh_kv4_page_bytes(n_kv, head_dim) bytes, on 16
+ *          bytes;
+ *   table  [n_seq][max_pages]: the page that holds positions 64 j .. 64 j + 63
+ *          of a sequence.  Entries behind a sequence's last page are not read.
+ *          Sequences may share full pages, not one that is appended to;
+ *   lens   [n_seq] positions held, 0 .. 64 max_pages; 0 leaves a sequence out.
+ * head_dim 64, 128, 192 or 256.  A page number outside the pool or a length
+ * outside the row raises IBH_DEVERR_KV4_TABLE (ibh_device_errors): nothing is
+ * stored for it, what would be computed from it is NaN, the other sequences
+ * are served.  An element stands for mid + scale * (code - 8). */
+#define IBH_KV4_PAGE 64
+typedef struct {
+    void* pool;
+    const int32_t* table;
+    int32_t* lens;             /* written by ibh_kv4_evict only */
+    int n_pages, n_seq, max_pages, n_kv, head_dim;
+} ibh_kv4_cache;
+size_t ibh_kv4_page_bytes(int n_kv, int head_dim);
+
+/* Stores the last n_new positions of every sequence: lens already counts
+ * them, so row i of k, v ([n_seq][n_new] rows of n_kv * head_dim floats,
+ * kv_stride floats apart) goes to position lens - n_new + i; rows that would
+ * lie before position 0 are left out, which serves sequences with fewer new
+ * positions (their rows at the end).  Per 64 dims: lo, hi of the elements
+ * (held to +-65504), scale = fp16((hi - lo) / 15), mid = fp16(lo + 8 scale),
+ * code = 8 + (x - mid) / scale rounded to nearest (ties to even) and held to
+ * 0 .. 15, exactly; 8 where scale is 0.  A NaN makes its 64 dims NaN. */
+int ibh_kv4_append(const ibh_kv4_cache* cache, const float* k, const float* v, int n_new, int kv_stride,
+                   void* stream);
+/* The values that the last n positions of every sequence stand for, rows as
+ * ibh_kv4_append takes them; rows before position 0 are left as they are. */
+int ibh_kv4_read(const ibh_kv4_cache* cache, float* k, float* v, int n, int kv_stride, void* stream);
+
+/* Attention of the last n_q positions of every sequence (1: a decode step;
+ * more: a verify step or a chunk of a prompt, whose rows ibh_kv4_append has
+ * stored): query i sits at position lens - n_q + i and sees the positions up
+ * to its own.  q [n_seq][n_q] rows of n_heads * head_dim floats, q_stride
+ * floats apart; out [n_seq][n_q][n_heads * head_dim].  Head h reads KV head
+ * h / (n_heads / n_kv), scores are q.k / sqrt(head_dim).  A query that sees
+ * nothing gives zeros.
+ * With weights (both or neither): weights_out[n_seq][n_kv][64 max_pages] =
+ * weights_in + the softmax probabilities that the queries and heads of the KV
+ * head gave each position; 0 behind a sequence's length.  The two may be the
+ * same array.
+ * `ws` >= ibh_kv4_attn_workspace_bytes on 16 bytes, NULL = library workspace;
+ * calls that share one must not overlap in time. */
+size_t ibh_kv4_attn_workspace_bytes(const ibh_kv4_cache* cache, int n_heads, int n_q);
+int    ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float* q, int n_heads, int n_q, int q_stride,
+                    const float* weights_in, float* weights_out, void* ws, size_t ws_bytes, void* stream);
+
+/* Cuts every sequence of more than `budget` positions to `budget`: each KV
+ * head keeps the first `sink` and the last `recent` positions and, of the
+ * others, the budget - sink - recent of largest weight (weights_src, as
+ * ibh_kv4_attn accumulates them; equal weights keep the lower position, NaN
+ * ranks below all), in their order.  dst receives the kept rows, weights_dst
+ * their weights (0 behind them), dst->lens the new lengths, kept
+ * [n_seq][n_kv][budget] the positions they had (-1 behind them).  The slots
+ * behind the last kept one of a page are cleared; dst pages without a kept
+ * position are left as they are.
+ * In place: dst with src's pool, table, lens and weights.  Otherwise dst has
+ * its own table, lens and weights, and pages that src does not use; src is
+ * left as it was.  sink + recent <= budget <= 64 dst->max_pages. */
+int ibh_kv4_evict(const ibh_kv4_cache* src, const ibh_kv4_cache* dst, const float* weights_src, float* weights_dst,
+                  int budget, int sink, int recent, int32_t* kept, void* stream);
 
 /* ── product-quantised LUT matvec, device pointers ─────────── */
 

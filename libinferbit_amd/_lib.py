@@ -43,6 +43,12 @@ SIGNATURES = {
     "ibh_attn_decode": (I, [P, P, P, P, P, P, I, I, I, I, I, P, SZ, P]),
     "ibh_attn_exact_set_grouped": (I, [I]),
     "ibh_attn_set_split": (I, [I]),
+    "ibh_kv4_page_bytes": (SZ, [I, I]),
+    "ibh_kv4_append": (I, [P, P, P, I, I, P]),
+    "ibh_kv4_read": (I, [P, P, P, I, I, P]),
+    "ibh_kv4_attn_workspace_bytes": (SZ, [P, I, I]),
+    "ibh_kv4_attn": (I, [P, P, P, I, I, I, P, P, P, SZ, P]),
+    "ibh_kv4_evict": (I, [P, P, P, P, I, I, I, P, P]),
     "ibh_pq_workspace_bytes": (SZ, [P]),
     "ibh_pq_workspace_init": (I, [P, SZ, P]),
     "ibh_pq_matmul_fp32_host": (I, [P, P, P]),
@@ -157,6 +163,12 @@ class PqTensor(C.Structure):
 class PqSampleParams(C.Structure):
     """ib_pq_sample_params (src/pq_decode.h:499-504)."""
     _fields_ = [("temperature", C.c_float), ("top_k", C.c_int), ("top_p", C.c_float), ("seed", C.c_uint32)]
+
+
+class Kv4Desc(C.Structure):
+    """ibh_kv4_cache (include/ibhip.h)."""
+    _fields_ = [(n, P) for n in ("pool", "table", "lens")] + \
+               [(n, I) for n in ("n_pages", "n_seq", "max_pages", "n_kv", "head_dim")]
 
 
 class PqPolicy(C.Structure):

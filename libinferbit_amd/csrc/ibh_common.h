@@ -45,6 +45,7 @@ hipStream_t ibh_resolve_stream(void* s);
 // collects them.
 int ibh_tile_errors(bool clear);
 int ibh_pq_errors(bool clear);
+int ibh_kv4_errors(bool clear);
 
 // ── device helpers ─────────────────────────────────────────────────────────
 namespace ibh {

@@ -15,7 +15,7 @@ import ctypes
 
 import numpy as np
 
-from ._lib import Int4gTensor, PqPolicy, PqTensor, check, lib
+from ._lib import Int4gTensor, Kv4Desc, PqPolicy, PqTensor, check, lib
 
 SCALE_F16, SCALE_F32 = 0, 1
 
@@ -103,6 +103,114 @@ def attn_decode(out, q, kdata, vdata, kscales, vscales, pos: int, n_heads: int, 
     """ib_attn_head_task for all heads of a layer (src/forward.c:449-504)."""
     check(lib().ibh_attn_decode(_ptr(out), _ptr(q), _ptr(kdata), _ptr(vdata), _optptr(kscales), _optptr(vscales),
                                 pos, n_heads, n_kv, head_dim, kv_bits, None, 0, _stream()), "ibh_attn_decode")
+
+
+KV4_PAGE = 64
+
+
+class Kv4Cache:
+    """A paged 4-bit KV cache (ibh_kv4_cache): `pool` uint8 [n_pages,
+    kv4_page_bytes], `table` int32 [n_seq, max_pages], `lens` int32 [n_seq],
+    all contiguous on one GPU and kept by reference.  Calls on it run on that
+    GPU, on its current stream."""
+
+    def __init__(self, pool, table, lens, n_kv: int, head_dim: int):
+        if table.dim() != 2 or lens.dim() != 1 or table.shape[0] != lens.shape[0]:
+            raise ValueError("table must be [n_seq, max_pages] and lens [n_seq]")
+        if table.dtype != torch.int32 or lens.dtype != torch.int32 or pool.dtype != torch.uint8:
+            raise TypeError("a cache is a uint8 pool with an int32 table and int32 lens")
+        self.device = pool.device
+        self.pool, self.table, self.lens = pool, table, lens
+        self.n_seq, self.max_pages = table.shape
+        self.n_kv, self.head_dim = n_kv, head_dim
+        size = lib().ibh_kv4_page_bytes(n_kv, head_dim)
+        if not size or pool.numel() % size:
+            raise ValueError(f"the pool is not whole pages of {n_kv} heads of {head_dim}")
+        self.desc = Kv4Desc(_ptr(pool), self._on(table), self._on(lens), pool.numel() // size, self.n_seq,
+                            self.max_pages, n_kv, head_dim)
+        self.ref = ctypes.byref(self.desc)
+
+    def _on(self, t, dtype=None, numel=None):
+        """t's address, if it is a contiguous tensor of this cache's GPU with the given type and size."""
+        if t.device != self.device:
+            raise ValueError(f"operand on {t.device}, the cache is on {self.device}")
+        if dtype is not None and t.dtype != dtype:
+            raise TypeError(f"operand must be {dtype}, got {t.dtype}")
+        if numel is not None and t.numel() != numel:
+            raise ValueError(f"operand must have {numel} elements, got {t.numel()}")
+        return _ptr(t)
+
+    def _rows(self, t, width: int):
+        """(address, rows per sequence, floats between rows) of [n_seq, n, width] fp32 rows with unit inner stride."""
+        if t.device != self.device or not t.is_cuda:
+            raise ValueError(f"operand on {t.device}, the cache is on {self.device}")
+        if t.dtype != torch.float32:
+            raise TypeError(f"operand must be torch.float32, got {t.dtype}")
+        if t.dim() != 3 or t.shape[0] != self.n_seq or t.shape[2] != width:
+            raise ValueError(f"operand must be [{self.n_seq}, n, {width}], got {list(t.shape)}")
+        n = t.shape[1]
+        s0, s1, s2 = t.stride()
+        if n == 1:
+            s1 = s0 if self.n_seq > 1 else width
+        if s2 != 1 or s1 < width or (self.n_seq > 1 and s0 != n * s1):
+            raise ValueError("rows must be evenly spaced with contiguous elements")
+        return t.data_ptr(), n, s1
+
+    def _stream(self):
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _call(self, name: str, *args) -> None:
+        if torch.cuda.current_device() == self.device.index:
+            check(getattr(lib(), name)(*args, self._stream()), name)
+        else:
+            with torch.cuda.device(self.device):
+                check(getattr(lib(), name)(*args, self._stream()), name)
+
+
+def kv4_append(cache: Kv4Cache, k, v) -> None:
+    """Stores k, v [n_seq, n_new, n_kv * head_dim] as the last n_new positions of every sequence (lens counts them)."""
+    width = cache.n_kv * cache.head_dim
+    (pk, n, sk), (pv, nv, sv) = cache._rows(k, width), cache._rows(v, width)
+    if n != nv or sk != sv:
+        raise ValueError("k and v must have the same rows")
+    cache._call("ibh_kv4_append", cache.ref, pk, pv, n, sk)
+
+
+def kv4_read(cache: Kv4Cache, k, v) -> None:
+    """The values of the last k.shape[1] positions of every sequence into k, v [n_seq, n, n_kv * head_dim]."""
+    width = cache.n_kv * cache.head_dim
+    (pk, n, sk), (pv, nv, sv) = cache._rows(k, width), cache._rows(v, width)
+    if n != nv or sk != sv:
+        raise ValueError("k and v must have the same rows")
+    cache._call("ibh_kv4_read", cache.ref, pk, pv, n, sk)
+
+
+def kv4_attn(out, q, cache: Kv4Cache, n_heads: int, weights_in=None, weights_out=None, ws=None) -> None:
+    """Attention of the last q.shape[1] positions of every sequence: q [n_seq, n_q, n_heads * head_dim] (rows may be
+    spaced), out the same, contiguous; weights fp32 [n_seq, n_kv, 64 * max_pages], accumulated from in to out."""
+    pq, n_q, sq = cache._rows(q, n_heads * cache.head_dim)
+    po = cache._on(out, torch.float32, q.numel())
+    if (weights_in is None) != (weights_out is None):
+        raise ValueError("weights_in and weights_out go together")
+    wi = wo = None
+    if weights_in is not None:
+        size = cache.n_seq * cache.n_kv * cache.max_pages * KV4_PAGE
+        wi, wo = (cache._on(w, torch.float32, size) for w in (weights_in, weights_out))
+    if ws is None:
+        need = lib().ibh_kv4_attn_workspace_bytes(cache.ref, n_heads, n_q)
+        ws = torch.empty(need, dtype=torch.uint8, device=cache.device)
+    cache._call("ibh_kv4_attn", cache.ref, po, pq, n_heads, n_q, sq, wi, wo, cache._on(ws), ws.numel())
+
+
+def kv4_evict(src: Kv4Cache, dst: Kv4Cache, weights_src, weights_dst, budget: int, sink: int, recent: int,
+              kept) -> None:
+    """Cuts every sequence to `budget` positions by accumulated weight: rows, weights and lengths into dst (src itself
+    for in place), the kept positions into kept int32 [n_seq, n_kv, budget]."""
+    n = src.n_seq * src.n_kv
+    src._call("ibh_kv4_evict", src.ref, dst.ref,
+              src._on(weights_src, torch.float32, n * src.max_pages * KV4_PAGE),
+              src._on(weights_dst, torch.float32, n * dst.max_pages * KV4_PAGE), budget, sink, recent,
+              src._on(kept, torch.int32, n * budget))
 
 
 class PqDeviceTensor:
