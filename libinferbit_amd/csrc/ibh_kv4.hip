@@ -223,113 +223,451 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4 c, float* __restrict_
 }
 
 // ── attention ────────────────────────────────────────────────────────────────
-// Block (head, query, sequence): one pass over the pages with the running
-// maximum and sum; the row's maximum and sum go to `stat` for the weights.
-__global__ __launch_bounds__(256) void kv4_attn_rows(Kv4 c, float* __restrict__ out, const float* __restrict__ q,
-                                                     int n_heads, int n_q, int q_stride, float scale,
-                                                     float2* __restrict__ stat) {
-    __shared__ float qs[256], sc[kPage], sv[kPage][4], mv[kPage][4], red[2];
-    int b = blockIdx.x;
-    const int hq = b % n_heads; b /= n_heads;
-    const int qi = b % n_q, seq = b / n_q;
-    const int hdg = c.hd / 64, h = hq / (n_heads / c.n_kv);
-    const int tid = threadIdx.x;
-    bool bad;
-    const int len = seq_len(c, seq, &bad);
-    const int n = max(0, len - n_q + qi + 1);            // positions that this query sees
-    if (tid < c.hd) qs[tid] = q[((size_t)seq * n_q + qi) * (size_t)q_stride + hq * c.hd + tid];
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    for (int p = 0; p * kPage < n; p++) {
-        const uint8_t* pg = page_at(c, seq, p, h);
-        if (!pg) { bad = true; break; }
-        const int t = tid >> 2, cq = tid & 3;
-        __syncthreads();
-        float s = 0.f;
-        for (int g = 0; g < hdg; g++) {
-            const uint32_t pr = ((const uint32_t*)(pg + 32 * c.hd))[g * 64 + slot_of(t)];
-            const uint8_t* kb = pg + key_off(t, g, cq, hdg);
-            const float ks = h2f(pr), km = h2f(pr >> 16);
-            for (int e = 0; e < 16; e++) {
-                const int cd = kb[(e >> 3) * 4 + (e & 3)] >> (e & 4) & 15;
-                s = fmaf(qs[64 * g + 16 * cq + e], fmaf(ks, (float)(cd - 8), km), s);
-            }
-        }
-        s += __shfl_xor(s, 1, kWave);
-        s += __shfl_xor(s, 2, kWave);
-        if (cq == 0) sc[t] = p * kPage + t < n ? s * scale : -INFINITY;
-        if (cq < hdg) {
-            const uint32_t pr = ((const uint32_t*)(pg + 68 * c.hd))[cq * 64 + slot_of(t)];
-            sv[t][cq] = h2f(pr);
-            mv[t][cq] = h2f(pr >> 16);
-        }
-        __syncthreads();
-        if (tid < 64) {
-            const float x = sc[tid];
-            const float mn = fmaxf(m, wave_max(x));      // at least one position of the page is seen
-            const float e = x == -INFINITY ? 0.f : expf(x - mn);
-            const float a = expf(m - mn);
-            l = l * a + wave_sum(e);
-            m = mn;
-            sc[tid] = e;
-            if (tid == 0) red[0] = a;
-        }
-        __syncthreads();
-        if (tid < c.hd) {
-            o *= red[0];
-            for (int tt = 0; tt < min(kPage, n - p * kPage); tt++) {
-                const int cd = pg[36 * c.hd + val_off(tid, (tt & 15) >> 1) + (tt >> 4)] >> (4 * (tt & 1)) & 15;
-                o = fmaf(sc[tt], fmaf(sv[tt][tid >> 6], (float)(cd - 8), mv[tt][tid >> 6]), o);
-            }
-        }
-    }
-    if (tid == 0) {
-        red[0] = l;
-        if (bad) raise_table();
-        if (stat) stat[((size_t)seq * n_q + qi) * n_heads + hq] = bad ? make_float2(0.f, NAN) : make_float2(m, l);
-    }
-    __syncthreads();
-    if (tid < c.hd)
-        out[(((size_t)seq * n_q + qi) * n_heads + hq) * c.hd + tid] = bad ? NAN : (n ? o / red[0] : 0.f);
+// The matrix cores multiply the codes as they lie.  The other operand of each
+// product is written in three signed base-256 digits, x = step * (65536 d0 +
+// 256 d1 + d2) with |x| <= 127 * 65536 step (23 bits below the largest element
+// of a query, or of a page's p * scale), so every product and sum is exact in
+// int32 and what is rounded is rounded as in fp32.  A tile is 4 query rows (a
+// row is one head of one query) as the 16 rows of the MFMA's first operand:
+// row 4 i + j is digit j of query row i, j < 3.  The result leaves lane l with
+// the digits' sums of query row l / 16 and column l % 16, so they are joined
+// in the lane.  Codes are 0 .. 15; a product with -8 in every place, used as
+// the accumulator, centres them.
+typedef int i4_t __attribute__((ext_vector_type(4)));
+typedef int i4_alias __attribute__((ext_vector_type(4), may_alias));
+typedef uint32_t u32_alias __attribute__((may_alias));
+
+constexpr float kDigitMax = 8323072.f;                   // 127 * 65536
+constexpr float kTiny = 1e-30f;                          // below this a query, or a page's p * scale, counts as zero
+
+__device__ __forceinline__ i4_t unpack16(uint32_t a, uint32_t b) {
+    constexpr uint32_t M = 0x0f0f0f0fu;
+    return i4_t{(int)(a & M), (int)((a >> 4) & M), (int)(b & M), (int)((b >> 4) & M)};
+}
+__device__ __forceinline__ i4_t mfma16(i4_t a, i4_t b, i4_t c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ float join_digits(i4_t c) { return fmaf((float)((c[0] << 8) + c[1]), 256.f, (float)c[2]); }
+// v_exp_f32: at most one unit in the last place off, results below 2^-126 are 0
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+// Sum over the 16 lanes of a row, every lane getting it.
+__device__ __forceinline__ float row16_sum(float v) {
+    v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, false));
+    v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, false));
+    v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x124, 0xF, 0xF, false));
+    v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x128, 0xF, 0xF, false));
+    return v;
 }
 
-// Accumulated weights: block (page, KV head, sequence) scores its 64 positions
-// again for every row of the head and adds e^(s - m) / l.
-__global__ __launch_bounds__(256) void kv4_attn_weights(Kv4 c, const float* __restrict__ q, int n_heads, int n_q,
-                                                        int q_stride, float scale, const float2* __restrict__ stat,
-                                                        const float* __restrict__ win, float* __restrict__ wout) {
+// A head's part of a page in registers: the keys' half, then the values'.
+template <int HDG>
+struct PageK {
+    uint4 c[2][HDG], p[HDG];
+    __device__ __forceinline__ void load(const uint8_t* pg, int lane) {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int g = 0; g < HDG; g++) c[u][g] = *(const uint4*)(pg + (u * HDG + g) * 1024 + lane * 16);
+#pragma unroll
+        for (int g = 0; g < HDG; g++) p[g] = *(const uint4*)(pg + 2048 * HDG + g * 256 + (lane & 15) * 16);
+    }
+};
+template <int HDG>
+struct PageV {
+    uint4 c[2 * HDG], p[HDG];
+    __device__ __forceinline__ void load(const uint8_t* pg, int lane) {
+#pragma unroll
+        for (int j = 0; j < 2 * HDG; j++) c[j] = *(const uint4*)(pg + 2304 * HDG + j * 1024 + lane * 16);
+#pragma unroll
+        for (int g = 0; g < HDG; g++) p[g] = *(const uint4*)(pg + 4352 * HDG + g * 256 + (lane & 15) * 16);
+    }
+};
+__device__ __forceinline__ uint32_t part4(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// What a launch of the attention kernels works on.
+struct AttnArgs {
+    float* out;
+    const float* q;
+    int n_heads, n_q, q_stride;
+    float scale;                                         // log2(e) / sqrt(head_dim)
+    int chunk, n_split, n_tile;                          // pages of a block, blocks of a row tile, row tiles of a KV head
+    float* part;                                         // [seq][KV head][row][split][head_dim], when n_split > 1
+    float2* part_ml;                                     // [seq][KV head][row][split] maximum (log2) and sum
+    float* lse;                                          // [seq][KV head][row] log2 of the row's sum, when weights are wanted
+    i4_t* digits;                                        // [seq][KV head][4-row tile][group][lane]
+    float* rowc;                                         // [seq][KV head][row][1 + groups] step * scale, sums of the query in steps
+};
+
+// Block: `chunk` pages of one (sequence, KV head), RT tiles of 4 query rows,
+// four wavefronts that take the block's pages in turn, each with its own
+// running maximum and sums, joined at the end.
+template <int HDG, int RT>
+__global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4 c, AttnArgs a) {
+    constexpr int HD = 64 * HDG, ROWS = 4 * RT;
+    __shared__ __align__(16) int8_t digs[RT * HDG * 1024];   // [tile][group][16][64]
+    __shared__ __align__(16) int8_t turn[4][HDG][4 * 320];   // a wavefront's p * scale digits, 64 B a row, a query row on 320
+    __shared__ float rc[ROWS][1 + HDG];
+    __shared__ float ob[4][4][HD];
+    __shared__ float mlw[4][4][2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int li = lane & 15, lq = lane >> 4;
+    // the KV head runs fastest over the blocks, so that blocks which share a
+    // head's pages share an XCD's L2 where the heads are a multiple of 8; the
+    // row tiles with the most positions come first
     int b = blockIdx.x;
-    const int p = b % c.max_pages; b /= c.max_pages;
-    const int h = b % c.n_kv, seq = b / c.n_kv;
-    const int hdg = c.hd / 64, grp = n_heads / c.n_kv;
+    const int h = b % c.n_kv; b /= c.n_kv;
+    const int rt = a.n_tile - 1 - b % a.n_tile; b /= a.n_tile;
+    const int split = b % a.n_split, seq = b / a.n_split;
+    const int grp = a.n_heads / c.n_kv, n_rows = a.n_q * grp;
     bool bad;
     const int len = seq_len(c, seq, &bad);
-    const int t = threadIdx.x >> 2, cq = threadIdx.x & 3, pos = p * kPage + t;
-    const size_t at = ((size_t)seq * c.n_kv + h) * c.max_pages * kPage + pos;
-    float acc = 0.f;
-    if (p * kPage < len) {
-        const uint8_t* pg = page_at(c, seq, p, h);
-        bad |= !pg;
-        for (int r = 0; pg && r < n_q * grp; r++) {
-            const int qi = r / grp, hq = h * grp + r % grp;
-            if (p * kPage > len - n_q + qi) continue;
-            const float* qr = q + ((size_t)seq * n_q + qi) * (size_t)q_stride + hq * c.hd;
-            float s = 0.f;
-            for (int g = 0; g < hdg; g++) {
-                const uint32_t pr = ((const uint32_t*)(pg + 32 * c.hd))[g * 64 + slot_of(t)];
-                const uint8_t* kb = pg + key_off(t, g, cq, hdg);
-                const float ks = h2f(pr), km = h2f(pr >> 16);
-                for (int e = 0; e < 16; e++) {
-                    const int cd = kb[(e >> 3) * 4 + (e & 3)] >> (e & 4) & 15;
-                    s = fmaf(qr[64 * g + 16 * cq + e], fmaf(ks, (float)(cd - 8), km), s);
-                }
-            }
-            s += __shfl_xor(s, 1, kWave);
-            s += __shfl_xor(s, 2, kWave);
-            const float2 ml = stat[((size_t)seq * n_q + qi) * n_heads + hq];
-            if (pos <= len - n_q + qi) acc += expf(s * scale - ml.x) / ml.y;
+    const int row0 = rt * ROWS;
+    // the last position that each row sees; rows past the last copy it
+    const int lim_min = len - a.n_q + row0 / grp, lim_max = len - a.n_q + min(row0 + ROWS - 1, n_rows - 1) / grp;
+    const int pages = lim_max < 0 ? 0 : lim_max / kPage + 1;
+    const int p0 = split * a.chunk, p1 = min(p0 + a.chunk, pages);
+    if (split > 0 && p0 >= pages) return;
+    int lim[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) lim[t] = len - a.n_q + min(row0 + 4 * t + lq, n_rows - 1) / grp;
+
+    const size_t sh = (size_t)seq * c.n_kv + h;
+    PageK<HDG> kn;
+    PageV<HDG> vn;
+    int p = p0 + wave;
+    const uint8_t* pg = nullptr;
+    if (p < p1) {
+        pg = page_at(c, seq, p, h);
+        if (pg) { kn.load(pg, lane); vn.load(pg, lane); }
+        else bad = true;
+    }
+
+    // the query rows as digits
+    for (int r = wave; r < ROWS; r += 4) {
+        const int row = min(row0 + r, n_rows - 1);
+        const float* src = a.q + ((size_t)seq * a.n_q + row / grp) * (size_t)a.q_stride + (h * grp + row % grp) * HD;
+        float x[HDG], mx = 0.f;
+#pragma unroll
+        for (int g = 0; g < HDG; g++) {
+            x[g] = src[64 * g + lane];
+            mx = fmaxf(mx, fabsf(x[g]));
+        }
+        mx = wave_max_dpp(mx);
+        const float step = mx > kTiny ? mx / kDigitMax : 1.f, inv = mx > kTiny ? kDigitMax / mx : 0.f;
+#pragma unroll
+        for (int g = 0; g < HDG; g++) {
+            const int j = (int)rintf(x[g] * inv) + 0x8080;   // the two low digits offset by 128 each
+            int8_t* d = digs + ((r >> 2) * HDG + g) * 1024 + (r & 3) * 256 + lane;
+            d[0] = (int8_t)(j >> 16);
+            d[64] = (int8_t)((j >> 8) ^ 0x80);
+            d[128] = (int8_t)(j ^ 0x80);
+            d[192] = 0;
+            const float sum = wave_sum_dpp(x[g]) / step;
+            if (lane == 0) rc[r][1 + g] = sum;
+        }
+        if (lane == 0) rc[r][0] = step * a.scale;
+    }
+    __syncthreads();
+    i4_t qa[RT][HDG];
+    float kf[RT], qsum[RT][HDG];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        kf[t] = rc[4 * t + lq][0];
+#pragma unroll
+        for (int g = 0; g < HDG; g++) {
+            qa[t][g] = *(const i4_alias*)(digs + (t * HDG + g) * 1024 + li * 64 + lq * 16);
+            qsum[t][g] = rc[4 * t + lq][1 + g];
         }
     }
-    if (cq == 0) wout[at] = pos < len ? (bad ? NAN : win[at] + acc) : 0.f;
+    if (a.lse && split == 0) {
+        const size_t tiles = (n_rows + 3) / 4;
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+            if ((t & 3) == wave && row0 + 4 * t < n_rows) {
+#pragma unroll
+                for (int g = 0; g < HDG; g++) a.digits[((sh * tiles + row0 / 4 + t) * HDG + g) * 64 + lane] = qa[t][g];
+                const int row = row0 + 4 * t + lq;
+                if (li <= HDG && row < n_rows) a.rowc[(sh * n_rows + row) * (1 + HDG) + li] = rc[4 * t + lq][li];
+            }
+    }
+
+    float m[RT], l[RT], o[RT][4 * HDG], om[RT][HDG];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        m[t] = -INFINITY;
+        l[t] = 0.f;
+#pragma unroll
+        for (int d = 0; d < 4 * HDG; d++) o[t][d] = 0.f;
+#pragma unroll
+        for (int g = 0; g < HDG; g++) om[t][g] = 0.f;
+    }
+    const i4_t zero = {0, 0, 0, 0}, minus8 = {(int)0xf8f8f8f8, (int)0xf8f8f8f8, (int)0xf8f8f8f8, (int)0xf8f8f8f8};
+    int8_t* const tw = &turn[wave][0][0];
+
+    for (; p < p1; p += 4) {
+        const bool here = pg != nullptr;
+        PageK<HDG> kc = kn;
+        PageV<HDG> vc = vn;
+        if (p + 4 < p1) {
+            pg = page_at(c, seq, p + 4, h);
+            if (pg) { kn.load(pg, lane); vn.load(pg, lane); }
+            else bad = true;
+        }
+        if (!here) continue;
+        const bool masked = p * kPage + kPage - 1 > lim_min;
+        float ks[4][HDG], km[4][HDG], vs[4][HDG], vm[4][HDG];
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+#pragma unroll
+            for (int g = 0; g < HDG; g++) {
+                const uint32_t kp = part4(kc.p[g], s), vp = part4(vc.p[g], s);
+                ks[s][g] = h2f(kp);
+                km[s][g] = h2f(kp >> 16);
+                vs[s][g] = h2f(vp);
+                vm[s][g] = h2f(vp >> 16);
+            }
+        i4_t kb[4][HDG], vb[4 * HDG];
+#pragma unroll
+        for (int g = 0; g < HDG; g++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                kb[2 * u][g] = unpack16(kc.c[u][g].x, kc.c[u][g].y);
+                kb[2 * u + 1][g] = unpack16(kc.c[u][g].z, kc.c[u][g].w);
+                vb[4 * g + 2 * u] = unpack16(vc.c[2 * g + u].x, vc.c[2 * g + u].y);
+                vb[4 * g + 2 * u + 1] = unpack16(vc.c[2 * g + u].z, vc.c[2 * g + u].w);
+            }
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int g = 0; g < HDG; g++) {
+                const i4_t init = mfma16(qa[t][g], minus8, zero);
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    const float f = join_digits(mfma16(qa[t][g], kb[s][g], init));
+                    x[s] = fmaf(ks[s][g], f, fmaf(km[s][g], qsum[t][g], x[s]));
+                }
+            }
+            bool ok[4] = {true, true, true, true};
+            if (masked) {
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    ok[s] = p * kPage + 16 * s + li <= lim[t];
+                    x[s] = ok[s] ? x[s] : -INFINITY;
+                }
+            }
+            const float top = dpp_row_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+            if (__any(top > m[t])) {
+                const float mn = fmaxf(m[t], top);
+                const float al = mn == -INFINITY ? 1.f : exp2_((m[t] - mn) * kf[t]);
+                m[t] = mn;
+                l[t] *= al;
+#pragma unroll
+                for (int d = 0; d < 4 * HDG; d++) o[t][d] *= al;
+#pragma unroll
+                for (int g = 0; g < HDG; g++) om[t][g] *= al;
+            }
+            const float mk = m[t] == -INFINITY ? 0.f : -m[t] * kf[t];
+            float e[4];
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                e[s] = exp2_(fmaf(x[s], kf[t], mk));
+                l[t] += e[s];
+            }
+#pragma unroll
+            for (int g = 0; g < HDG; g++) {
+                float w[4];
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    w[s] = e[s] * vs[s][g];
+                    float me = e[s] * vm[s][g];
+                    if (masked) {                            // stale pairs may be anything
+                        w[s] = ok[s] ? w[s] : 0.f;
+                        me = ok[s] ? me : 0.f;
+                    }
+                    om[t][g] += me;
+                }
+                const float wm = dpp_row_max(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])));
+                const float inv = wm > kTiny ? kDigitMax * __builtin_amdgcn_rcpf(wm) : 0.f;
+                const float ws = wm > kTiny ? wm * (1.f / kDigitMax) : 0.f;
+                uint32_t j[4];
+#pragma unroll
+                for (int s = 0; s < 4; s++) j[s] = (uint32_t)fmaf(w[s], inv, 32896.5f);
+                // bytes of the four slots 4 li + s, one word a digit
+                const uint32_t a01 = __builtin_amdgcn_perm(j[1], j[0], 0x05010400), a23 = __builtin_amdgcn_perm(j[3], j[2], 0x05010400);
+                const uint32_t b01 = __builtin_amdgcn_perm(j[1], j[0], 0x0c0c0602), b23 = __builtin_amdgcn_perm(j[3], j[2], 0x06020c0c);
+                u32_alias* d = (u32_alias*)(tw + g * 1280 + lq * 320 + li * 4);
+                d[0] = b01 | b23;
+                d[16] = __builtin_amdgcn_perm(a23, a01, 0x07060302) ^ 0x80808080u;
+                d[32] = __builtin_amdgcn_perm(a23, a01, 0x05040100) ^ 0x80808080u;
+                __builtin_amdgcn_wave_barrier();
+                const i4_t wa = *(const i4_alias*)(tw + g * 1280 + (li >> 2) * 320 + (li & 3) * 64 + lq * 16);
+                __builtin_amdgcn_wave_barrier();
+                const i4_t init = mfma16(wa, minus8, zero);
+#pragma unroll
+                for (int d4 = 0; d4 < 4; d4++)
+                    o[t][4 * g + d4] = fmaf(join_digits(mfma16(wa, vb[4 * g + d4], init)), ws, o[t][4 * g + d4]);
+            }
+        }
+    }
+
+    // the four wavefronts' sums, a tile at a time
+    const bool any_bad = __syncthreads_or(bad);
+    if (any_bad && tid == 0) raise_table();
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const float ls = row16_sum(l[t]);
+        if (li == 0) {
+            mlw[wave][lq][0] = m[t] == -INFINITY ? -INFINITY : m[t] * kf[t];
+            mlw[wave][lq][1] = ls;
+        }
+#pragma unroll
+        for (int g = 0; g < HDG; g++) {
+            const float mid = row16_sum(om[t][g]);
+#pragma unroll
+            for (int d = 0; d < 4; d++) ob[wave][lq][64 * g + 16 * d + li] = o[t][4 * g + d] + mid;
+        }
+        __syncthreads();
+        const int r = wave, row = row0 + 4 * t + r;
+        if (row < n_rows) {
+            float mm = fmaxf(fmaxf(mlw[0][r][0], mlw[1][r][0]), fmaxf(mlw[2][r][0], mlw[3][r][0]));
+            float f[4], sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                f[w] = mlw[w][r][0] == -INFINITY && mlw[w][r][1] == 0.f ? 0.f : exp2_(mlw[w][r][0] - mm);
+                sum = fmaf(f[w], mlw[w][r][1], sum);
+            }
+            if (any_bad) sum = NAN;
+            const size_t rr = sh * n_rows + row;
+            const size_t to = a.n_split > 1 ? (rr * a.n_split + split) * HD
+                                            : ((size_t)seq * a.n_q + row / grp) * (size_t)a.n_heads * HD + (h * grp + row % grp) * HD;
+            float* dst = (a.n_split > 1 ? a.part : a.out) + to;
+            const float norm = a.n_split > 1 ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
+#pragma unroll
+            for (int g = 0; g < HDG; g++) {
+                float y = 0.f;
+#pragma unroll
+                for (int w = 0; w < 4; w++) y = fmaf(f[w], ob[w][r][64 * g + lane], y);
+                dst[64 * g + lane] = y * norm;
+            }
+            if (lane == 0) {
+                if (a.n_split > 1) a.part_ml[rr * a.n_split + split] = make_float2(mm, sum);
+                else if (a.lse) a.lse[rr] = sum == 0.f ? INFINITY : mm + log2f(sum);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Joins the splits of a query row: block (row, KV head, sequence), a thread a dim.
+template <int HDG>
+__global__ __launch_bounds__(64 * HDG) void kv4_attn_join(Kv4 c, AttnArgs a, int rows_per_tile) {
+    constexpr int HD = 64 * HDG;
+    const int grp = a.n_heads / c.n_kv, n_rows = a.n_q * grp;
+    const size_t rr = blockIdx.x;
+    const int row = rr % n_rows;
+    const size_t sh = rr / n_rows;
+    const int h = sh % c.n_kv, seq = sh / c.n_kv;
+    bool bad;
+    const int len = seq_len(c, seq, &bad);
+    const int last = min(row / rows_per_tile * rows_per_tile + rows_per_tile, n_rows) - 1;
+    const int lim = len - a.n_q + last / grp;            // as the row's tile was cut
+    const int n = lim < 0 ? 1 : (lim / kPage + a.chunk) / a.chunk;
+    const float2* ml = a.part_ml + rr * a.n_split;
+    const float* po = a.part + rr * a.n_split * HD;
+    float mm = -INFINITY;
+    for (int i = 0; i < n; i++) mm = fmaxf(mm, ml[i].x);
+    float sum = 0.f, y = 0.f;
+    for (int i = 0; i < n; i++) {
+        const float2 v = ml[i];
+        const float f = v.x == -INFINITY && v.y == 0.f ? 0.f : exp2_(v.x - mm);
+        sum = fmaf(f, v.y, sum);
+        y = fmaf(f, po[(size_t)i * HD + threadIdx.x], y);
+    }
+    a.out[((size_t)seq * a.n_q + row / grp) * (size_t)a.n_heads * HD + (h * grp + row % grp) * HD + threadIdx.x] =
+        sum == 0.f ? 0.f : y / sum;
+    if (threadIdx.x == 0 && a.lse) a.lse[rr] = sum == 0.f ? INFINITY : mm + log2f(sum);
+}
+
+// Accumulated weights: a wavefront scores one page again for every row of its
+// KV head and adds 2^(s - lse).
+template <int HDG>
+__global__ __launch_bounds__(256) void kv4_attn_weights(Kv4 c, AttnArgs a, const float* win, float* wout) {
+    const int lane = threadIdx.x & 63, li = lane & 15, lq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int b = blockIdx.x;
+    const int h = b % c.n_kv; b /= c.n_kv;
+    const int np = (c.max_pages + 3) / 4;
+    const int p = b % np * 4 + wave, seq = b / np;
+    if (p >= c.max_pages) return;
+    const int grp = a.n_heads / c.n_kv, n_rows = a.n_q * grp;
+    bool bad;
+    const int len = seq_len(c, seq, &bad);
+    const size_t sh = (size_t)seq * c.n_kv + h;
+    const size_t at = (sh * c.max_pages + p) * kPage + lane;
+    if (p * kPage >= len) {
+        wout[at] = 0.f;
+        return;
+    }
+    const float old = win[at];
+    const uint8_t* pg = page_at(c, seq, p, h);
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    if (pg && !bad) {
+        PageK<HDG> kc;
+        kc.load(pg, lane);
+        i4_t kb[4][HDG];
+        float ks[4][HDG], km[4][HDG];
+#pragma unroll
+        for (int g = 0; g < HDG; g++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                kb[2 * u][g] = unpack16(kc.c[u][g].x, kc.c[u][g].y);
+                kb[2 * u + 1][g] = unpack16(kc.c[u][g].z, kc.c[u][g].w);
+            }
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+#pragma unroll
+            for (int g = 0; g < HDG; g++) {
+                const uint32_t kp = part4(kc.p[g], s);
+                ks[s][g] = h2f(kp);
+                km[s][g] = h2f(kp >> 16);
+            }
+        const i4_t zero = {0, 0, 0, 0}, minus8 = {(int)0xf8f8f8f8, (int)0xf8f8f8f8, (int)0xf8f8f8f8, (int)0xf8f8f8f8};
+        const int tiles = (n_rows + 3) / 4;
+        // queries before the page's first position see nothing of it
+        const int t0 = max(0, p * kPage - (len - a.n_q)) * grp / 4;
+        for (int t = t0; t < tiles; t++) {
+            const int row = min(4 * t + lq, n_rows - 1);
+            const float* rcp = a.rowc + (sh * n_rows + row) * (1 + HDG);
+            const float kf = rcp[0], lse = a.lse[sh * n_rows + row];
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int g = 0; g < HDG; g++) {
+                const i4_t qa = a.digits[((sh * tiles + t) * HDG + g) * 64 + lane];
+                const float qs = rcp[1 + g];
+                const i4_t init = mfma16(qa, minus8, zero);
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+                    x[s] = fmaf(ks[s][g], join_digits(mfma16(qa, kb[s][g], init)), fmaf(km[s][g], qs, x[s]));
+            }
+            const int lim = 4 * t + lq < n_rows ? len - a.n_q + row / grp : -1;
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+                acc[s] += p * kPage + 16 * s + li <= lim ? exp2_(fmaf(x[s], kf, -lse)) : 0.f;
+        }
+    } else {
+        bad = true;
+    }
+    if (bad) {
+        if (lane == 0) raise_table();
+        wout[at] = p * kPage + lane < len ? NAN : 0.f;
+        return;
+    }
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+        acc[s] += __shfl_xor(acc[s], 16, kWave);
+        acc[s] += __shfl_xor(acc[s], 32, kWave);
+    }
+    const float add = lq == 0 ? acc[0] : lq == 1 ? acc[1] : lq == 2 ? acc[2] : acc[3];
+    wout[at] = p * kPage + lane < len ? old + add : 0.f;
 }
 
 // ── eviction ─────────────────────────────────────────────────────────────────
@@ -575,42 +913,87 @@ extern "C" int ibh_kv4_read(const ibh_kv4_cache* cache, float* k, float* v, int 
     return IBH_OK;
 }
 
+// How a call is cut: row tiles of 4 rt query rows, blocks of `chunk` pages.
+struct AttnPlan {
+    int rt, n_tile, chunk, n_split;
+    size_t part, part_ml, lse, digits, rowc, bytes;      // offsets into the workspace
+};
+static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q) {
+    AttnPlan p;
+    const size_t n_rows = (size_t)n_q * (n_heads / c->n_kv), hdg = c->head_dim / 64;
+    const size_t heads = (size_t)c->n_seq * c->n_kv;
+    p.rt = n_rows <= 4 ? 1 : n_rows <= 8 ? 2 : n_rows <= 16 || hdg > 2 ? 4 : 8;
+    p.n_tile = (int)((n_rows + 4 * p.rt - 1) / (4 * p.rt));
+    const size_t work = heads * p.n_tile * c->max_pages, want = 2048;
+    const size_t chunk = (work + want - 1) / want;
+    p.chunk = (int)((chunk + 3) / 4 * 4);
+    p.n_split = (c->max_pages + p.chunk - 1) / p.chunk;
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
+    p.part = take(p.n_split > 1 ? heads * n_rows * p.n_split * c->head_dim * sizeof(float) : 0);
+    p.part_ml = take(p.n_split > 1 ? heads * n_rows * p.n_split * sizeof(float2) : 0);
+    p.lse = take(heads * n_rows * sizeof(float));
+    p.digits = take(heads * ((n_rows + 3) / 4) * hdg * 1024);
+    p.rowc = take(heads * n_rows * (1 + hdg) * sizeof(float));
+    p.bytes = at;
+    return p;
+}
+
 extern "C" size_t ibh_kv4_attn_workspace_bytes(const ibh_kv4_cache* cache, int n_heads, int n_q) {
-    if (!cache || cache->n_seq <= 0 || n_heads <= 0 || n_q <= 0) return 0;
-    return (size_t)cache->n_seq * n_q * n_heads * sizeof(float2);
+    if (!cache || cache->n_seq <= 0 || cache->n_kv <= 0 || cache->max_pages <= 0 || cache->head_dim < 64 ||
+        cache->head_dim > 256 || cache->head_dim % 64 || n_heads <= 0 || n_heads % cache->n_kv || n_q <= 0)
+        return 0;
+    return attn_plan(cache, n_heads, n_q).bytes;
+}
+
+template <int HDG>
+static void launch_attn(const Kv4& c, const AttnArgs& a, const AttnPlan& p, size_t blocks, size_t rows,
+                        const float* win, float* wout, size_t wblocks, hipStream_t st) {
+    if (p.rt == 1) kv4_attn_kernel<HDG, 1><<<(unsigned)blocks, 256, 0, st>>>(c, a);
+    else if (p.rt == 2) kv4_attn_kernel<HDG, 2><<<(unsigned)blocks, 256, 0, st>>>(c, a);
+    else if (p.rt == 4) kv4_attn_kernel<HDG, 4><<<(unsigned)blocks, 256, 0, st>>>(c, a);
+    else if constexpr (HDG <= 2) kv4_attn_kernel<HDG, 8><<<(unsigned)blocks, 256, 0, st>>>(c, a);
+    if (p.n_split > 1) kv4_attn_join<HDG><<<(unsigned)rows, 64 * HDG, 0, st>>>(c, a, 4 * p.rt);
+    if (wout) kv4_attn_weights<HDG><<<(unsigned)wblocks, 256, 0, st>>>(c, a, win, wout);
 }
 
 extern "C" int ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float* q, int n_heads, int n_q, int q_stride,
                             const float* weights_in, float* weights_out, void* ws, size_t ws_bytes, void* stream) {
     if (!cache_ok(cache, "ibh_kv4_attn")) return IBH_ERROR_PARAM;
-    if (!out || !q || n_heads <= 0 || n_heads % cache->n_kv || n_q <= 0 || (size_t)q_stride < (size_t)n_heads * cache->head_dim ||
+    if (!out || !q || n_heads <= 0 || n_heads % cache->n_kv || n_q <= 0 ||
+        (int64_t)q_stride < (int64_t)n_heads * cache->head_dim || (int64_t)n_q * n_heads > 0x7fffffff / 16 ||
         !weights_in != !weights_out) {
         ibh_set_error("ibh_kv4_attn: invalid arguments (heads=%d/%d n_q=%d q_stride=%d; weights_in and weights_out "
                       "both or neither)", n_heads, cache->n_kv, n_q, q_stride);
         return IBH_ERROR_PARAM;
     }
-    const size_t need = ibh_kv4_attn_workspace_bytes(cache, n_heads, n_q);
+    const AttnPlan p = attn_plan(cache, n_heads, n_q);
     if (!ws) {
-        ws = ibh_workspace(need);
-        ws_bytes = ws ? need : 0;
+        ws = ibh_workspace(p.bytes);
+        ws_bytes = ws ? p.bytes : 0;
     }
-    if (!ws || ws_bytes < need || ((uintptr_t)ws & 15)) {
-        ibh_set_error("ibh_kv4_attn: workspace of %zu bytes on 16 bytes needed", need);
+    if (!ws || ws_bytes < p.bytes || ((uintptr_t)ws & 15)) {
+        ibh_set_error("ibh_kv4_attn: workspace of %zu bytes on 16 bytes needed", p.bytes);
         return IBH_ERROR_MEMORY;
     }
-    const size_t rows = (size_t)cache->n_seq * n_q * n_heads;
-    const size_t wb = (size_t)cache->n_seq * cache->n_kv * cache->max_pages;
-    if (!grid_ok(rows, "ibh_kv4_attn") || !grid_ok(wb, "ibh_kv4_attn")) return IBH_ERROR_PARAM;
-    const float scale = 1.0f / sqrtf((float)cache->head_dim);
+    const size_t heads = (size_t)cache->n_seq * cache->n_kv;
+    const size_t blocks = heads * p.n_tile * p.n_split, rows = heads * n_q * (n_heads / cache->n_kv);
+    const size_t wblocks = heads * ((cache->max_pages + 3) / 4);
+    if (!grid_ok(blocks, "ibh_kv4_attn") || !grid_ok(rows, "ibh_kv4_attn") || !grid_ok(wblocks, "ibh_kv4_attn"))
+        return IBH_ERROR_PARAM;
+    char* w = (char*)ws;
+    AttnArgs a{out, q, n_heads, n_q, q_stride, (float)(1.4426950408889634 / sqrt((double)cache->head_dim)), p.chunk,
+               p.n_split, p.n_tile, (float*)(w + p.part), (float2*)(w + p.part_ml),
+               weights_out ? (float*)(w + p.lse) : nullptr, (i4_t*)(w + p.digits), (float*)(w + p.rowc)};
+    const Kv4 c = device_of(cache);
     hipStream_t st = ibh_resolve_stream(stream);
-    float2* stat = (float2*)ws;
-    kv4_attn_rows<<<(unsigned)rows, 256, 0, st>>>(device_of(cache), out, q, n_heads, n_q, q_stride, scale, stat);
-    IBH_CHECK_LAUNCH("ibh_kv4_attn");
-    if (weights_out) {
-        kv4_attn_weights<<<(unsigned)wb, 256, 0, st>>>(device_of(cache), q, n_heads, n_q, q_stride, scale, stat,
-                                                       weights_in, weights_out);
-        IBH_CHECK_LAUNCH("ibh_kv4_attn (weights)");
+    switch (cache->head_dim / 64) {
+        case 1: launch_attn<1>(c, a, p, blocks, rows, weights_in, weights_out, wblocks, st); break;
+        case 2: launch_attn<2>(c, a, p, blocks, rows, weights_in, weights_out, wblocks, st); break;
+        case 3: launch_attn<3>(c, a, p, blocks, rows, weights_in, weights_out, wblocks, st); break;
+        default: launch_attn<4>(c, a, p, blocks, rows, weights_in, weights_out, wblocks, st); break;
     }
+    IBH_CHECK_LAUNCH("ibh_kv4_attn");
     return IBH_OK;
 }
 
