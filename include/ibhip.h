@@ -253,9 +253,10 @@ int ibh_kv4_read(const ibh_kv4_cache* cache, float* k, float* v, int n, int kv_s
  * weights_in + the softmax probabilities that the queries and heads of the KV
  * head gave each position; 0 behind a sequence's length.  The two may be the
  * same array.
- * `ws` >= ibh_kv4_attn_workspace_bytes on 16 bytes, NULL = library workspace;
- * calls that share one must not overlap in time. */
-size_t ibh_kv4_attn_workspace_bytes(const ibh_kv4_cache* cache, int n_heads, int n_q);
+ * `ws` >= ibh_kv4_attn_workspace_bytes (weights != 0: of a call with weights)
+ * on 16 bytes, NULL = library workspace; calls that share one must not overlap
+ * in time. */
+size_t ibh_kv4_attn_workspace_bytes(const ibh_kv4_cache* cache, int n_heads, int n_q, int weights);
 int    ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float* q, int n_heads, int n_q, int q_stride,
                     const float* weights_in, float* weights_out, void* ws, size_t ws_bytes, void* stream);
 

@@ -46,7 +46,7 @@ SIGNATURES = {
     "ibh_kv4_page_bytes": (SZ, [I, I]),
     "ibh_kv4_append": (I, [P, P, P, I, I, P]),
     "ibh_kv4_read": (I, [P, P, P, I, I, P]),
-    "ibh_kv4_attn_workspace_bytes": (SZ, [P, I, I]),
+    "ibh_kv4_attn_workspace_bytes": (SZ, [P, I, I, I]),
     "ibh_kv4_attn": (I, [P, P, P, I, I, I, P, P, P, SZ, P]),
     "ibh_kv4_evict": (I, [P, P, P, P, I, I, I, P, P]),
     "ibh_pq_workspace_bytes": (SZ, [P]),

@@ -36,6 +36,9 @@ HIPCC_FLAGS = [
 # VGPRs: with the AGPR form the register allocator copies every accumulator
 # through v_accvgpr moves on each K step.
 EXTRA_FLAGS = {
+    # The 4-bit cache's attention reads every product right away: results in
+    # VGPRs save a v_accvgpr_read for each.
+    "ibh_kv4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "ibh_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 

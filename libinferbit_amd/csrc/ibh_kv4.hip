@@ -16,6 +16,8 @@
 // An element stands for mid + scale * (code - 8).
 #include "ibh_common.h"
 
+#include <type_traits>
+
 using namespace ibh;
 
 namespace {
@@ -36,12 +38,23 @@ __device__ __forceinline__ void raise_table() {
     __hip_atomic_fetch_or(&ibh_kv4_err, (unsigned)IBH_DEVERR_KV4_TABLE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// Read through the scalar cache: no kernel that reads the table or the lengths
+// here writes them (kv4_move writes lengths and reads none).
+__device__ __forceinline__ int ld_uniform(const int32_t* p) {
+    return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
+}
 // A sequence's length; one outside its table row is cut to it and reported.
 __device__ __forceinline__ int seq_len(const Kv4& c, int seq, bool* bad) {
-    const int n = c.lens[seq], cap = c.max_pages * kPage;
+    const int n = ld_uniform(c.lens + seq), cap = c.max_pages * kPage;
     const int m = n < 0 ? 0 : (n > cap ? cap : n);
     *bad = m != n;
     return m;
+}
+// page_at() where all arguments are the same for the whole wavefront.
+__device__ __forceinline__ const uint8_t* page_of_wave(const Kv4& c, int seq, int p, int h) {
+    const int id = ld_uniform(c.table + (size_t)seq * c.max_pages + p);
+    if ((unsigned)id >= (unsigned)c.n_pages) return nullptr;
+    return c.pool + ((size_t)id * c.n_kv + h) * (size_t)(72 * c.hd);
 }
 // Head h's part of page p of a sequence, or null where the table names no page of the pool.
 __device__ __forceinline__ uint8_t* page_at(const Kv4& c, int seq, int p, int h) {
@@ -238,6 +251,7 @@ typedef int i4_alias __attribute__((ext_vector_type(4), may_alias));
 typedef uint32_t u32_alias __attribute__((may_alias));
 
 constexpr float kDigitMax = 8323072.f;                   // 127 * 65536
+constexpr int kMaxSplit = 4096;                          // blocks of one row tile
 constexpr float kTiny = 1e-30f;                          // below this a query, or a page's p * scale, counts as zero
 
 __device__ __forceinline__ i4_t unpack16(uint32_t a, uint32_t b) {
@@ -248,6 +262,16 @@ __device__ __forceinline__ i4_t mfma16(i4_t a, i4_t b, i4_t c) { return __builti
 __device__ __forceinline__ float join_digits(i4_t c) { return fmaf((float)((c[0] << 8) + c[1]), 256.f, (float)c[2]); }
 // v_exp_f32: at most one unit in the last place off, results below 2^-126 are 0
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+// Largest value of the 16 lanes of a row, every lane getting it: v_max_f32
+// with its first operand moved across lanes (the two wait states that a moved
+// operand needs after its write stand before each).
+__device__ __forceinline__ float row16_max(float v) {
+    asm("s_nop 1\n\tv_max_f32_dpp %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_ror:4 row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_ror:8 row_mask:0xf bank_mask:0xf\n\ts_nop 1" : "+v"(v));
+    return v;
+}
 // Sum over the 16 lanes of a row, every lane getting it.
 __device__ __forceinline__ float row16_sum(float v) {
     v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, false));
@@ -257,29 +281,30 @@ __device__ __forceinline__ float row16_sum(float v) {
     return v;
 }
 
-// A head's part of a page in registers: the keys' half, then the values'.
-template <int HDG>
-struct PageK {
-    uint4 c[2][HDG], p[HDG];
-    __device__ __forceinline__ void load(const uint8_t* pg, int lane) {
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int g = 0; g < HDG; g++) c[u][g] = *(const uint4*)(pg + (u * HDG + g) * 1024 + lane * 16);
-#pragma unroll
-        for (int g = 0; g < HDG; g++) p[g] = *(const uint4*)(pg + 2048 * HDG + g * 256 + (lane & 15) * 16);
-    }
-};
-template <int HDG>
-struct PageV {
-    uint4 c[2 * HDG], p[HDG];
-    __device__ __forceinline__ void load(const uint8_t* pg, int lane) {
-#pragma unroll
-        for (int j = 0; j < 2 * HDG; j++) c[j] = *(const uint4*)(pg + 2304 * HDG + j * 1024 + lane * 16);
-#pragma unroll
-        for (int g = 0; g < HDG; g++) p[g] = *(const uint4*)(pg + 4352 * HDG + g * 256 + (lane & 15) * 16);
-    }
-};
+// A lane's operands in a head's part of a page; at = 16 lane.  Pages that one
+// block alone reads are loaded past the caches (NT): 604 MB are read at 7.0
+// TB/s so, at 6.1 by ordinary loads.
+template <bool NT>
+__device__ __forceinline__ uint4 ld16(const uint8_t* p) {
+    if constexpr (NT) return ld_stream16(p);
+    else return *(const uint4*)p;
+}
+template <int HDG, bool NT>
+__device__ __forceinline__ uint4 key_codes(const uint8_t* pg, int u, int g, unsigned at) {   // positions 32 u .., dims 64 g ..
+    return ld16<NT>(pg + at + (u * HDG + g) * 1024);
+}
+template <int HDG, bool NT>
+__device__ __forceinline__ uint4 key_pairs(const uint8_t* pg, int g, unsigned at) {          // positions 16 s + lane % 16
+    return ld16<NT>(pg + (at & 255) + 2048 * HDG + g * 256);
+}
+template <int HDG, bool NT>
+__device__ __forceinline__ uint4 val_codes(const uint8_t* pg, int j, unsigned at) {          // dims 32 j ..
+    return ld16<NT>(pg + at + 2304 * HDG + j * 1024);
+}
+template <int HDG, bool NT>
+__device__ __forceinline__ uint4 val_pairs(const uint8_t* pg, int g, unsigned at) {
+    return ld16<NT>(pg + (at & 255) + 4352 * HDG + g * 256);
+}
 __device__ __forceinline__ uint32_t part4(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // What a launch of the attention kernels works on.
@@ -296,11 +321,14 @@ struct AttnArgs {
     float* rowc;                                         // [seq][KV head][row][1 + groups] step * scale, sums of the query in steps
 };
 
+// Wavefronts a SIMD holds: what the registers of a page and RT tiles leave.
+constexpr int attn_waves(int hdg, int rt) { return hdg * rt == 1 ? 4 : hdg * rt == 2 ? 3 : hdg * rt >= 8 && hdg > 2 ? 1 : 2; }
+
 // Block: `chunk` pages of one (sequence, KV head), RT tiles of 4 query rows,
 // four wavefronts that take the block's pages in turn, each with its own
 // running maximum and sums, joined at the end.
 template <int HDG, int RT>
-__global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4 c, AttnArgs a) {
+__global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 c, AttnArgs a) {
     constexpr int HD = 64 * HDG, ROWS = 4 * RT;
     __shared__ __align__(16) int8_t digs[RT * HDG * 1024];   // [tile][group][16][64]
     __shared__ __align__(16) int8_t turn[4][HDG][4 * 320];   // a wavefront's p * scale digits, 64 B a row, a query row on 320
@@ -330,14 +358,33 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4 c, AttnArgs a) {
     for (int t = 0; t < RT; t++) lim[t] = len - a.n_q + min(row0 + 4 * t + lq, n_rows - 1) / grp;
 
     const size_t sh = (size_t)seq * c.n_kv + h;
-    PageK<HDG> kn;
-    PageV<HDG> vn;
+    // a page no table entry names is left out of the sums (the block reports
+    // it at its end and gives NaN): its wavefront goes on to its next page
+    auto next_page = [&](int& p) -> const uint8_t* {
+        for (; p < p1; p += 4) {
+            const uint8_t* pg = page_of_wave(c, seq, p, h);
+            if (pg) return pg;
+            bad = true;
+        }
+        return nullptr;
+    };
+    uint4 kc[2][HDG], kp[HDG], vc[2 * HDG], vp[HDG];     // the page's codes and pairs
+    unsigned at = 16 * lane;
     int p = p0 + wave;
-    const uint8_t* pg = nullptr;
-    if (p < p1) {
-        pg = page_at(c, seq, p, h);
-        if (pg) { kn.load(pg, lane); vn.load(pg, lane); }
-        else bad = true;
+    const uint8_t* pg = next_page(p);
+    if (pg) {
+#pragma unroll
+        for (int g = 0; g < HDG; g++) {
+            kc[0][g] = key_codes<HDG, RT <= 2>(pg, 0, g, at);
+            kc[1][g] = key_codes<HDG, RT <= 2>(pg, 1, g, at);
+            kp[g] = key_pairs<HDG, RT <= 2>(pg, g, at);
+        }
+#pragma unroll
+        for (int g = 0; g < HDG; g++) {
+            vc[2 * g] = val_codes<HDG, RT <= 2>(pg, 2 * g, at);
+            vc[2 * g + 1] = val_codes<HDG, RT <= 2>(pg, 2 * g + 1, at);
+            vp[g] = val_pairs<HDG, RT <= 2>(pg, g, at);
+        }
     }
 
     // the query rows as digits
@@ -377,7 +424,7 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4 c, AttnArgs a) {
             qsum[t][g] = rc[4 * t + lq][1 + g];
         }
     }
-    if (a.lse && split == 0) {
+    if (a.digits && split == 0) {
         const size_t tiles = (n_rows + 3) / 4;
 #pragma unroll
         for (int t = 0; t < RT; t++)
@@ -402,90 +449,91 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4 c, AttnArgs a) {
     const i4_t zero = {0, 0, 0, 0}, minus8 = {(int)0xf8f8f8f8, (int)0xf8f8f8f8, (int)0xf8f8f8f8, (int)0xf8f8f8f8};
     int8_t* const tw = &turn[wave][0][0];
 
-    for (; p < p1; p += 4) {
-        const bool here = pg != nullptr;
-        PageK<HDG> kc = kn;
-        PageV<HDG> vc = vn;
-        if (p + 4 < p1) {
-            pg = page_at(c, seq, p + 4, h);
-            if (pg) { kn.load(pg, lane); vn.load(pg, lane); }
-            else bad = true;
-        }
-        if (!here) continue;
-        const bool masked = p * kPage + kPage - 1 > lim_min;
-        float ks[4][HDG], km[4][HDG], vs[4][HDG], vm[4][HDG];
+    // One page, MASKED where some row of the block does not see all of it.
+    // Each register is refilled from the wavefront's next page (nx) as soon as
+    // its content has been taken apart; behind the last page every lane reads
+    // one place of this page again (at = 0), which costs less than a branch.
+    auto step = [&](int pos0, const uint8_t* nx, auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
+        float e[RT][4];
+        {
+            i4_t kb[4][HDG];
 #pragma unroll
-        for (int s = 0; s < 4; s++)
+            for (int g = 0; g < HDG; g++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    kb[2 * u][g] = unpack16(kc[u][g].x, kc[u][g].y);
+                    kb[2 * u + 1][g] = unpack16(kc[u][g].z, kc[u][g].w);
+                }
 #pragma unroll
             for (int g = 0; g < HDG; g++) {
-                const uint32_t kp = part4(kc.p[g], s), vp = part4(vc.p[g], s);
-                ks[s][g] = h2f(kp);
-                km[s][g] = h2f(kp >> 16);
-                vs[s][g] = h2f(vp);
-                vm[s][g] = h2f(vp >> 16);
+                kc[0][g] = key_codes<HDG, RT <= 2>(nx, 0, g, at);
+                kc[1][g] = key_codes<HDG, RT <= 2>(nx, 1, g, at);
             }
-        i4_t kb[4][HDG], vb[4 * HDG];
 #pragma unroll
-        for (int g = 0; g < HDG; g++)
+            for (int t = 0; t < RT; t++) {
+                float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int g = 0; g < HDG; g++) {
+                    const i4_t init = mfma16(qa[t][g], minus8, zero);
+#pragma unroll
+                    for (int s = 0; s < 4; s++) {
+                        const uint32_t pr = part4(kp[g], s);
+                        const float f = join_digits(mfma16(qa[t][g], kb[s][g], init));
+                        x[s] = fmaf(h2f(pr), f, fmaf(h2f(pr >> 16), qsum[t][g], x[s]));
+                    }
+                }
+                if constexpr (MASKED) {
+#pragma unroll
+                    for (int s = 0; s < 4; s++) x[s] = pos0 + 16 * s + li <= lim[t] ? x[s] : -INFINITY;
+                }
+                const float top = row16_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+                if (__any(top > m[t])) {
+                    const float mn = fmaxf(m[t], top);
+                    const float al = mn == -INFINITY ? 1.f : exp2_((m[t] - mn) * kf[t]);
+                    m[t] = mn;
+                    l[t] *= al;
+#pragma unroll
+                    for (int d = 0; d < 4 * HDG; d++) o[t][d] *= al;
+#pragma unroll
+                    for (int g = 0; g < HDG; g++) om[t][g] *= al;
+                }
+                const float mk = m[t] == -INFINITY ? 0.f : -m[t] * kf[t];
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    e[t][s] = exp2_(fmaf(x[s], kf[t], mk));
+                    l[t] += e[t][s];
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < HDG; g++) kp[g] = key_pairs<HDG, RT <= 2>(nx, g, at);
+        }
+#pragma unroll
+        for (int g = 0; g < HDG; g++) {
+            i4_t vb[4];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                kb[2 * u][g] = unpack16(kc.c[u][g].x, kc.c[u][g].y);
-                kb[2 * u + 1][g] = unpack16(kc.c[u][g].z, kc.c[u][g].w);
-                vb[4 * g + 2 * u] = unpack16(vc.c[2 * g + u].x, vc.c[2 * g + u].y);
-                vb[4 * g + 2 * u + 1] = unpack16(vc.c[2 * g + u].z, vc.c[2 * g + u].w);
+                vb[2 * u] = unpack16(vc[2 * g + u].x, vc[2 * g + u].y);
+                vb[2 * u + 1] = unpack16(vc[2 * g + u].z, vc[2 * g + u].w);
             }
+            vc[2 * g] = val_codes<HDG, RT <= 2>(nx, 2 * g, at);
+            vc[2 * g + 1] = val_codes<HDG, RT <= 2>(nx, 2 * g + 1, at);
 #pragma unroll
-        for (int t = 0; t < RT; t++) {
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int g = 0; g < HDG; g++) {
-                const i4_t init = mfma16(qa[t][g], minus8, zero);
-#pragma unroll
-                for (int s = 0; s < 4; s++) {
-                    const float f = join_digits(mfma16(qa[t][g], kb[s][g], init));
-                    x[s] = fmaf(ks[s][g], f, fmaf(km[s][g], qsum[t][g], x[s]));
-                }
-            }
-            bool ok[4] = {true, true, true, true};
-            if (masked) {
-#pragma unroll
-                for (int s = 0; s < 4; s++) {
-                    ok[s] = p * kPage + 16 * s + li <= lim[t];
-                    x[s] = ok[s] ? x[s] : -INFINITY;
-                }
-            }
-            const float top = dpp_row_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-            if (__any(top > m[t])) {
-                const float mn = fmaxf(m[t], top);
-                const float al = mn == -INFINITY ? 1.f : exp2_((m[t] - mn) * kf[t]);
-                m[t] = mn;
-                l[t] *= al;
-#pragma unroll
-                for (int d = 0; d < 4 * HDG; d++) o[t][d] *= al;
-#pragma unroll
-                for (int g = 0; g < HDG; g++) om[t][g] *= al;
-            }
-            const float mk = m[t] == -INFINITY ? 0.f : -m[t] * kf[t];
-            float e[4];
-#pragma unroll
-            for (int s = 0; s < 4; s++) {
-                e[s] = exp2_(fmaf(x[s], kf[t], mk));
-                l[t] += e[s];
-            }
-#pragma unroll
-            for (int g = 0; g < HDG; g++) {
+            for (int t = 0; t < RT; t++) {
                 float w[4];
 #pragma unroll
                 for (int s = 0; s < 4; s++) {
-                    w[s] = e[s] * vs[s][g];
-                    float me = e[s] * vm[s][g];
-                    if (masked) {                            // stale pairs may be anything
-                        w[s] = ok[s] ? w[s] : 0.f;
-                        me = ok[s] ? me : 0.f;
+                    const uint32_t pr = part4(vp[g], s);
+                    w[s] = e[t][s] * h2f(pr);
+                    if constexpr (MASKED) {                  // stale pairs may be anything
+                        const bool ok = pos0 + 16 * s + li <= lim[t];
+                        w[s] = ok ? w[s] : 0.f;
+                        om[t][g] += ok ? e[t][s] * h2f(pr >> 16) : 0.f;
+                    } else {
+                        om[t][g] = fmaf(e[t][s], h2f(pr >> 16), om[t][g]);
                     }
-                    om[t][g] += me;
                 }
-                const float wm = dpp_row_max(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])));
+                const float wm = row16_max(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])));
                 const float inv = wm > kTiny ? kDigitMax * __builtin_amdgcn_rcpf(wm) : 0.f;
                 const float ws = wm > kTiny ? wm * (1.f / kDigitMax) : 0.f;
                 uint32_t j[4];
@@ -504,10 +552,25 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4 c, AttnArgs a) {
                 const i4_t init = mfma16(wa, minus8, zero);
 #pragma unroll
                 for (int d4 = 0; d4 < 4; d4++)
-                    o[t][4 * g + d4] = fmaf(join_digits(mfma16(wa, vb[4 * g + d4], init)), ws, o[t][4 * g + d4]);
+                    o[t][4 * g + d4] = fmaf(join_digits(mfma16(wa, vb[d4], init)), ws, o[t][4 * g + d4]);
             }
+            vp[g] = val_pairs<HDG, RT <= 2>(nx, g, at);
         }
-    }
+    };
+    // pages that every row sees, then the others
+    const int full = min(p1, (lim_min + 1) >> 6);
+    auto run = [&](int end, auto masked) {
+        while (pg && p < end) {
+            int pn = p + 4;
+            const uint8_t* nx = next_page(pn);
+            if (!nx) at = 0;
+            step(p * kPage, nx ? nx : pg, masked);
+            pg = nx;
+            p = pn;
+        }
+    };
+    run(full, std::false_type{});
+    run(p1, std::true_type{});
 
     // the four wavefronts' sums, a tile at a time
     const bool any_bad = __syncthreads_or(bad);
@@ -557,117 +620,261 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4 c, AttnArgs a) {
     }
 }
 
-// Joins the splits of a query row: block (row, KV head, sequence), a thread a dim.
-template <int HDG>
-__global__ __launch_bounds__(64 * HDG) void kv4_attn_join(Kv4 c, AttnArgs a, int rows_per_tile) {
-    constexpr int HD = 64 * HDG;
-    const int grp = a.n_heads / c.n_kv, n_rows = a.n_q * grp;
-    const size_t rr = blockIdx.x;
-    const int row = rr % n_rows;
-    const size_t sh = rr / n_rows;
-    const int h = sh % c.n_kv, seq = sh / c.n_kv;
-    bool bad;
-    const int len = seq_len(c, seq, &bad);
-    const int last = min(row / rows_per_tile * rows_per_tile + rows_per_tile, n_rows) - 1;
-    const int lim = len - a.n_q + last / grp;            // as the row's tile was cut
-    const int n = lim < 0 ? 1 : (lim / kPage + a.chunk) / a.chunk;
-    const float2* ml = a.part_ml + rr * a.n_split;
-    const float* po = a.part + rr * a.n_split * HD;
-    float mm = -INFINITY;
-    for (int i = 0; i < n; i++) mm = fmaxf(mm, ml[i].x);
-    float sum = 0.f, y = 0.f;
-    for (int i = 0; i < n; i++) {
-        const float2 v = ml[i];
-        const float f = v.x == -INFINITY && v.y == 0.f ? 0.f : exp2_(v.x - mm);
-        sum = fmaf(f, v.y, sum);
-        y = fmaf(f, po[(size_t)i * HD + threadIdx.x], y);
-    }
-    a.out[((size_t)seq * a.n_q + row / grp) * (size_t)a.n_heads * HD + (h * grp + row % grp) * HD + threadIdx.x] =
-        sum == 0.f ? 0.f : y / sum;
-    if (threadIdx.x == 0 && a.lse) a.lse[rr] = sum == 0.f ? INFINITY : mm + log2f(sum);
+// Blocks of a row's tile that had work: as kv4_attn_kernel cut the pages.
+__device__ __forceinline__ int splits_of(const AttnArgs& a, int len, int row, int grp, int n_rows, int tile_rows) {
+    const int last = min(row / tile_rows * tile_rows + tile_rows, n_rows) - 1;
+    const int lim = len - a.n_q + last / grp;
+    return lim < 0 ? 1 : (lim / kPage + a.chunk) / a.chunk;
 }
 
-// Accumulated weights: a wavefront scores one page again for every row of its
-// KV head and adds 2^(s - lse).
+// A page's keys, and 2^(score - lse) of its positions summed over the rows of
+// tiles t0, t0 + dt, .. < t1: lane l of sum() returns position l's (the rows'
+// digits, step * scale, sums, lse and last positions as the callers give them).
 template <int HDG>
-__global__ __launch_bounds__(256) void kv4_attn_weights(Kv4 c, AttnArgs a, const float* win, float* wout) {
-    const int lane = threadIdx.x & 63, li = lane & 15, lq = lane >> 4;
+struct PageWeights {
+    uint4 kc[2][HDG], kp[HDG];
+    __device__ __forceinline__ void load(const uint8_t* pg, int lane) {
+        const unsigned at = 16 * lane;
+#pragma unroll
+        for (int g = 0; g < HDG; g++) {
+            kc[0][g] = key_codes<HDG, false>(pg, 0, g, at);
+            kc[1][g] = key_codes<HDG, false>(pg, 1, g, at);
+            kp[g] = key_pairs<HDG, false>(pg, g, at);
+        }
+    }
+    template <class Rows>
+    __device__ __forceinline__ float sum(const i4_t* digits, int pos0, int lane, int t0, int t1, int dt, Rows rows) const {
+        const int li = lane & 15, lq = lane >> 4;
+        const i4_t zero = {0, 0, 0, 0}, minus8 = {(int)0xf8f8f8f8, (int)0xf8f8f8f8, (int)0xf8f8f8f8, (int)0xf8f8f8f8};
+        i4_t kb[4][HDG], qa[HDG];
+#pragma unroll
+        for (int g = 0; g < HDG; g++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                kb[2 * u][g] = unpack16(kc[u][g].x, kc[u][g].y);
+                kb[2 * u + 1][g] = unpack16(kc[u][g].z, kc[u][g].w);
+            }
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        float kf, lse, qs[HDG];
+        int lim;                                         // the last position that the lane's row sees
+        if (t0 < t1) {
+#pragma unroll
+            for (int g = 0; g < HDG; g++) qa[g] = digits[((size_t)t0 * HDG + g) * 64 + lane];
+            rows(t0, lq, kf, lse, qs, lim);
+        }
+        for (int t = t0; t < t1; t += dt) {
+            // the next tile's rows are loaded while this one's are multiplied
+            const int tn = t + dt < t1 ? t + dt : t;
+            i4_t qn[HDG];
+            float kfn, lsen, qsn[HDG];
+            int limn;
+#pragma unroll
+            for (int g = 0; g < HDG; g++) qn[g] = digits[((size_t)tn * HDG + g) * 64 + lane];
+            rows(tn, lq, kfn, lsen, qsn, limn);
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int g = 0; g < HDG; g++) {
+                const i4_t init = mfma16(qa[g], minus8, zero);
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    const uint32_t pr = part4(kp[g], s);
+                    x[s] = fmaf(h2f(pr), join_digits(mfma16(qa[g], kb[s][g], init)), fmaf(h2f(pr >> 16), qs[g], x[s]));
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 4; s++) acc[s] += pos0 + 16 * s + li <= lim ? exp2_(fmaf(x[s], kf, -lse)) : 0.f;
+            kf = kfn;
+            lse = lsen;
+            lim = limn;
+#pragma unroll
+            for (int g = 0; g < HDG; g++) {
+                qa[g] = qn[g];
+                qs[g] = qsn[g];
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            acc[s] += __shfl_xor(acc[s], 16, kWave);
+            acc[s] += __shfl_xor(acc[s], 32, kWave);
+        }
+        return lq == 0 ? acc[0] : lq == 1 ? acc[1] : lq == 2 ? acc[2] : acc[3];
+    }
+};
+
+constexpr int kFinishPages = 4;                          // pages of a weights block
+
+// Maximum (log2) and sum of a query row over its splits, by one wavefront.
+__device__ __forceinline__ float row_lse(const float2* ml, int n, int lane) {
+    float m = -INFINITY, s = 0.f;
+    for (int i = lane; i < n; i += 64) m = fmaxf(m, ml[i].x);
+    m = wave_max_dpp(m);
+    for (int i = lane; i < n; i += 64) {
+        const float2 v = ml[i];
+        s = fmaf(v.x == -INFINITY && v.y == 0.f ? 0.f : exp2_(v.x - m), v.y, s);
+    }
+    s = wave_sum_dpp(s);
+    return s == 0.f ? INFINITY : m + log2f(s);
+}
+
+// What is left after the pages' blocks.  Blocks below n_join join the splits
+// of a query row: 16 HDG threads hold four dims each, the other threads take
+// other splits, so that all partial sums are in flight together.  The others,
+// where one row tile holds all rows, score a page a wavefront again for the
+// accumulated weights; they take lse from the splits' maxima and sums
+// themselves, so that they need not wait for the joining blocks.  (Scores kept
+// by the first kernel instead cost it 9 us of 26 at 32 sequences of up to 4096
+// positions: 1 KB stored a page, behind which its loads wait.)
+template <int HDG, int RT>
+__global__ __launch_bounds__(256) void kv4_attn_finish(Kv4 c, AttnArgs a, unsigned n_join, const float* win, float* wout) {
+    constexpr int HD = 64 * HDG, TD = HD / 4, CLS = 256 / TD;
+    __shared__ float f[kMaxSplit];
+    __shared__ float4 ob[CLS][TD];
+    __shared__ float red[2][4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = a.n_heads / c.n_kv, n_rows = a.n_q * grp;
+    bool bad;
+    if (blockIdx.x < n_join) {
+        const size_t rr = blockIdx.x, sh = rr / n_rows;
+        const int row = rr % n_rows, h = sh % c.n_kv, seq = sh / c.n_kv;
+        const int len = seq_len(c, seq, &bad);
+        const int n = splits_of(a, len, row, grp, n_rows, 4 * RT);
+        const float2* ml = a.part_ml + rr * a.n_split;
+        const int td = tid % TD, cl = tid / TD;
+        const float4* po = (const float4*)(a.part + rr * a.n_split * HD) + td;
+        float4 first = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (cl < CLS && cl < n) first = po[(size_t)cl * TD];
+        float mm = -INFINITY;
+        for (int i = tid; i < n; i += 256) mm = fmaxf(mm, ml[i].x);
+        mm = wave_max_dpp(mm);
+        if (lane == 0) red[0][wave] = mm;
+        __syncthreads();
+        mm = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+        float sum = 0.f;
+        for (int i = tid; i < n; i += 256) {
+            const float2 v = ml[i];
+            const float w = v.x == -INFINITY && v.y == 0.f ? 0.f : exp2_(v.x - mm);
+            f[i] = w;
+            sum = fmaf(w, v.y, sum);
+        }
+        sum = wave_sum_dpp(sum);
+        if (lane == 0) red[1][wave] = sum;
+        __syncthreads();
+        sum = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+        if (cl < CLS) {
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (cl < n) {
+                const float w = f[cl];
+                y = make_float4(w * first.x, w * first.y, w * first.z, w * first.w);
+            }
+#pragma unroll 4
+            for (int i = cl + CLS; i < n; i += CLS) {
+                const float4 v = po[(size_t)i * TD];
+                const float w = f[i];
+                y.x = fmaf(w, v.x, y.x);
+                y.y = fmaf(w, v.y, y.y);
+                y.z = fmaf(w, v.z, y.z);
+                y.w = fmaf(w, v.w, y.w);
+            }
+            ob[cl][td] = y;
+        }
+        __syncthreads();
+        if (tid < HD) {
+            float y = 0.f;
+#pragma unroll
+            for (int k = 0; k < CLS; k++) y += ((const float*)&ob[k][0])[tid];
+            a.out[((size_t)seq * a.n_q + row / grp) * (size_t)a.n_heads * HD + (h * grp + row % grp) * HD + tid] =
+                sum == 0.f ? 0.f : y / sum;
+        }
+        if (tid == 0 && a.lse) a.lse[rr] = sum == 0.f ? INFINITY : mm + log2f(sum);
+        return;
+    }
+    unsigned b = blockIdx.x - n_join;
+    const int h = b % c.n_kv; b /= c.n_kv;
+    const int np = (c.max_pages + kFinishPages - 1) / kFinishPages;
+    const int p0 = b % np * kFinishPages, seq = b / np;
+    const size_t sh = (size_t)seq * c.n_kv + h;
+    const int len = seq_len(c, seq, &bad);
+    const int p = p0 + wave;
+    const bool here = p * kPage < len;
+    const size_t at = (sh * c.max_pages + p) * kPage + lane;
+    const float old = here ? win[at] : 0.f;
+    const uint8_t* pg = here ? page_of_wave(c, seq, p, h) : nullptr;
+    PageWeights<HDG> pw;
+    if (pg) pw.load(pg, lane);
+    if (p0 * kPage < len) {
+        const int n = splits_of(a, len, 0, grp, n_rows, 4 * RT);
+        for (int r = wave; r < n_rows; r += 4) {
+            const float lse = row_lse(a.part_ml + (sh * n_rows + r) * a.n_split, n, lane);
+            if (lane == 0) f[r] = lse;
+        }
+    }
+    __syncthreads();
+    if (p >= c.max_pages) return;
+    float add = NAN;
+    if (pg && !bad) {
+        const int tiles = (n_rows + 3) / 4;
+        add = pw.sum(a.digits + sh * tiles * HDG * 64, p * kPage, lane, 0, tiles, 1,
+            [&](int t, int lq, float& kf, float& lse, float* qs, int& lim) {
+                const int r = 4 * t + lq, row = min(r, n_rows - 1);
+                const float* rcp = a.rowc + (sh * n_rows + row) * (1 + HDG);
+                kf = rcp[0];
+                lse = f[row];
+#pragma unroll
+                for (int g = 0; g < HDG; g++) qs[g] = rcp[1 + g];
+                lim = r < n_rows ? len - a.n_q + row / grp : -1;
+            });
+    } else if (here && lane == 0) {
+        raise_table();
+    }
+    wout[at] = p * kPage + lane < len ? old + add : 0.f;
+}
+
+// Accumulated weights where the rows fill several tiles: block (KV head, page,
+// sequence), its wavefronts take the tiles in turn.
+constexpr int kWeightWaves = 8;
+template <int HDG>
+__global__ __launch_bounds__(64 * kWeightWaves) void kv4_attn_weights(Kv4 c, AttnArgs a, const float* win, float* wout) {
+    __shared__ float part[kWeightWaves][kPage];
+    const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int b = blockIdx.x;
     const int h = b % c.n_kv; b /= c.n_kv;
-    const int np = (c.max_pages + 3) / 4;
-    const int p = b % np * 4 + wave, seq = b / np;
-    if (p >= c.max_pages) return;
-    const int grp = a.n_heads / c.n_kv, n_rows = a.n_q * grp;
+    const int p = b % c.max_pages, seq = b / c.max_pages;
+    const int grp = a.n_heads / c.n_kv, n_rows = a.n_q * grp, tiles = (n_rows + 3) / 4;
     bool bad;
     const int len = seq_len(c, seq, &bad);
     const size_t sh = (size_t)seq * c.n_kv + h;
     const size_t at = (sh * c.max_pages + p) * kPage + lane;
     if (p * kPage >= len) {
-        wout[at] = 0.f;
+        if (wave == 0) wout[at] = 0.f;
         return;
     }
-    const float old = win[at];
-    const uint8_t* pg = page_at(c, seq, p, h);
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    const uint8_t* pg = page_of_wave(c, seq, p, h);
     if (pg && !bad) {
-        PageK<HDG> kc;
-        kc.load(pg, lane);
-        i4_t kb[4][HDG];
-        float ks[4][HDG], km[4][HDG];
-#pragma unroll
-        for (int g = 0; g < HDG; g++)
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                kb[2 * u][g] = unpack16(kc.c[u][g].x, kc.c[u][g].y);
-                kb[2 * u + 1][g] = unpack16(kc.c[u][g].z, kc.c[u][g].w);
-            }
-#pragma unroll
-        for (int s = 0; s < 4; s++)
-#pragma unroll
-            for (int g = 0; g < HDG; g++) {
-                const uint32_t kp = part4(kc.p[g], s);
-                ks[s][g] = h2f(kp);
-                km[s][g] = h2f(kp >> 16);
-            }
-        const i4_t zero = {0, 0, 0, 0}, minus8 = {(int)0xf8f8f8f8, (int)0xf8f8f8f8, (int)0xf8f8f8f8, (int)0xf8f8f8f8};
-        const int tiles = (n_rows + 3) / 4;
+        PageWeights<HDG> pw;
+        pw.load(pg, lane);
         // queries before the page's first position see nothing of it
         const int t0 = max(0, p * kPage - (len - a.n_q)) * grp / 4;
-        for (int t = t0; t < tiles; t++) {
-            const int row = min(4 * t + lq, n_rows - 1);
-            const float* rcp = a.rowc + (sh * n_rows + row) * (1 + HDG);
-            const float kf = rcp[0], lse = a.lse[sh * n_rows + row];
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
+        part[wave][lane] = pw.sum(a.digits + sh * tiles * HDG * 64, p * kPage, lane, t0 + wave, tiles, kWeightWaves,
+            [&](int t, int lq, float& kf, float& lse, float* qs, int& lim) {
+                const int r = 4 * t + lq, row = min(r, n_rows - 1);
+                const float* rcp = a.rowc + (sh * n_rows + row) * (1 + HDG);
+                kf = rcp[0];
+                lse = a.lse[sh * n_rows + row];
 #pragma unroll
-            for (int g = 0; g < HDG; g++) {
-                const i4_t qa = a.digits[((sh * tiles + t) * HDG + g) * 64 + lane];
-                const float qs = rcp[1 + g];
-                const i4_t init = mfma16(qa, minus8, zero);
-#pragma unroll
-                for (int s = 0; s < 4; s++)
-                    x[s] = fmaf(ks[s][g], join_digits(mfma16(qa, kb[s][g], init)), fmaf(km[s][g], qs, x[s]));
-            }
-            const int lim = 4 * t + lq < n_rows ? len - a.n_q + row / grp : -1;
-#pragma unroll
-            for (int s = 0; s < 4; s++)
-                acc[s] += p * kPage + 16 * s + li <= lim ? exp2_(fmaf(x[s], kf, -lse)) : 0.f;
-        }
+                for (int g = 0; g < HDG; g++) qs[g] = rcp[1 + g];
+                lim = r < n_rows ? len - a.n_q + row / grp : -1;
+            });
     } else {
-        bad = true;
+        if (threadIdx.x == 0) raise_table();
+        part[wave][lane] = NAN;
     }
-    if (bad) {
-        if (lane == 0) raise_table();
-        wout[at] = p * kPage + lane < len ? NAN : 0.f;
-        return;
-    }
+    __syncthreads();
+    if (wave) return;
+    float add = 0.f;
 #pragma unroll
-    for (int s = 0; s < 4; s++) {
-        acc[s] += __shfl_xor(acc[s], 16, kWave);
-        acc[s] += __shfl_xor(acc[s], 32, kWave);
-    }
-    const float add = lq == 0 ? acc[0] : lq == 1 ? acc[1] : lq == 2 ? acc[2] : acc[3];
-    wout[at] = p * kPage + lane < len ? old + add : 0.f;
+    for (int w = 0; w < kWeightWaves; w++) add += part[w][lane];
+    wout[at] = p * kPage + lane < len ? win[at] + add : 0.f;
 }
 
 // ── eviction ─────────────────────────────────────────────────────────────────
@@ -916,45 +1123,55 @@ extern "C" int ibh_kv4_read(const ibh_kv4_cache* cache, float* k, float* v, int 
 // How a call is cut: row tiles of 4 rt query rows, blocks of `chunk` pages.
 struct AttnPlan {
     int rt, n_tile, chunk, n_split;
+    bool joint;                                          // the weights in the launch that joins the splits
     size_t part, part_ml, lse, digits, rowc, bytes;      // offsets into the workspace
 };
-static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q) {
+static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool weights) {
     AttnPlan p;
     const size_t n_rows = (size_t)n_q * (n_heads / c->n_kv), hdg = c->head_dim / 64;
     const size_t heads = (size_t)c->n_seq * c->n_kv;
-    p.rt = n_rows <= 4 ? 1 : n_rows <= 8 ? 2 : n_rows <= 16 || hdg > 2 ? 4 : 8;
+    p.rt = n_rows <= 4 ? 1 : n_rows <= 8 || hdg > 2 ? 2 : 4;
     p.n_tile = (int)((n_rows + 4 * p.rt - 1) / (4 * p.rt));
-    const size_t work = heads * p.n_tile * c->max_pages, want = 2048;
-    const size_t chunk = (work + want - 1) / want;
+    const size_t work = heads * p.n_tile * c->max_pages, want = p.rt <= 2 ? 2048 : 1024;
+    size_t chunk = (work + want - 1) / want;
+    chunk = max(chunk, ((size_t)c->max_pages + kMaxSplit - 1) / kMaxSplit);
     p.chunk = (int)((chunk + 3) / 4 * 4);
     p.n_split = (c->max_pages + p.chunk - 1) / p.chunk;
+    p.joint = weights && p.n_tile == 1 && p.n_split > 1;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
     p.part = take(p.n_split > 1 ? heads * n_rows * p.n_split * c->head_dim * sizeof(float) : 0);
     p.part_ml = take(p.n_split > 1 ? heads * n_rows * p.n_split * sizeof(float2) : 0);
-    p.lse = take(heads * n_rows * sizeof(float));
-    p.digits = take(heads * ((n_rows + 3) / 4) * hdg * 1024);
-    p.rowc = take(heads * n_rows * (1 + hdg) * sizeof(float));
+    p.lse = take(weights && !p.joint ? heads * n_rows * sizeof(float) : 0);
+    p.digits = take(weights ? heads * ((n_rows + 3) / 4) * hdg * 1024 : 0);
+    p.rowc = take(weights ? heads * n_rows * (1 + hdg) * sizeof(float) : 0);
     p.bytes = at;
     return p;
 }
 
-extern "C" size_t ibh_kv4_attn_workspace_bytes(const ibh_kv4_cache* cache, int n_heads, int n_q) {
+extern "C" size_t ibh_kv4_attn_workspace_bytes(const ibh_kv4_cache* cache, int n_heads, int n_q, int weights) {
     if (!cache || cache->n_seq <= 0 || cache->n_kv <= 0 || cache->max_pages <= 0 || cache->head_dim < 64 ||
         cache->head_dim > 256 || cache->head_dim % 64 || n_heads <= 0 || n_heads % cache->n_kv || n_q <= 0)
         return 0;
-    return attn_plan(cache, n_heads, n_q).bytes;
+    return attn_plan(cache, n_heads, n_q, weights != 0).bytes;
 }
 
+template <int HDG, int RT>
+static void launch_attn_rt(const Kv4& c, const AttnArgs& a, const AttnPlan& p, size_t heads, const float* win,
+                           float* wout, hipStream_t st) {
+    const size_t rows = p.n_split > 1 ? heads * a.n_q * (a.n_heads / c.n_kv) : 0;
+    kv4_attn_kernel<HDG, RT><<<(unsigned)(heads * p.n_tile * p.n_split), 256, 0, st>>>(c, a);
+    const size_t wb = p.joint ? heads * ((c.max_pages + kFinishPages - 1) / kFinishPages) : 0;
+    if (rows + wb) kv4_attn_finish<HDG, RT><<<(unsigned)(rows + wb), 256, 0, st>>>(c, a, (unsigned)rows, win, wout);
+    if (wout && !p.joint)
+        kv4_attn_weights<HDG><<<(unsigned)(heads * c.max_pages), 64 * kWeightWaves, 0, st>>>(c, a, win, wout);
+}
 template <int HDG>
-static void launch_attn(const Kv4& c, const AttnArgs& a, const AttnPlan& p, size_t blocks, size_t rows,
-                        const float* win, float* wout, size_t wblocks, hipStream_t st) {
-    if (p.rt == 1) kv4_attn_kernel<HDG, 1><<<(unsigned)blocks, 256, 0, st>>>(c, a);
-    else if (p.rt == 2) kv4_attn_kernel<HDG, 2><<<(unsigned)blocks, 256, 0, st>>>(c, a);
-    else if (p.rt == 4) kv4_attn_kernel<HDG, 4><<<(unsigned)blocks, 256, 0, st>>>(c, a);
-    else if constexpr (HDG <= 2) kv4_attn_kernel<HDG, 8><<<(unsigned)blocks, 256, 0, st>>>(c, a);
-    if (p.n_split > 1) kv4_attn_join<HDG><<<(unsigned)rows, 64 * HDG, 0, st>>>(c, a, 4 * p.rt);
-    if (wout) kv4_attn_weights<HDG><<<(unsigned)wblocks, 256, 0, st>>>(c, a, win, wout);
+static void launch_attn(const Kv4& c, const AttnArgs& a, const AttnPlan& p, size_t heads, const float* win,
+                        float* wout, hipStream_t st) {
+    if (p.rt == 1) launch_attn_rt<HDG, 1>(c, a, p, heads, win, wout, st);
+    else if (p.rt == 2) launch_attn_rt<HDG, 2>(c, a, p, heads, win, wout, st);
+    else if constexpr (HDG <= 2) launch_attn_rt<HDG, 4>(c, a, p, heads, win, wout, st);
 }
 
 extern "C" int ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float* q, int n_heads, int n_q, int q_stride,
@@ -967,7 +1184,7 @@ extern "C" int ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float*
                       "both or neither)", n_heads, cache->n_kv, n_q, q_stride);
         return IBH_ERROR_PARAM;
     }
-    const AttnPlan p = attn_plan(cache, n_heads, n_q);
+    const AttnPlan p = attn_plan(cache, n_heads, n_q, weights_out != nullptr);
     if (!ws) {
         ws = ibh_workspace(p.bytes);
         ws_bytes = ws ? p.bytes : 0;
@@ -977,21 +1194,21 @@ extern "C" int ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float*
         return IBH_ERROR_MEMORY;
     }
     const size_t heads = (size_t)cache->n_seq * cache->n_kv;
-    const size_t blocks = heads * p.n_tile * p.n_split, rows = heads * n_q * (n_heads / cache->n_kv);
-    const size_t wblocks = heads * ((cache->max_pages + 3) / 4);
-    if (!grid_ok(blocks, "ibh_kv4_attn") || !grid_ok(rows, "ibh_kv4_attn") || !grid_ok(wblocks, "ibh_kv4_attn"))
+    if (!grid_ok(heads * p.n_tile * p.n_split, "ibh_kv4_attn") ||
+        !grid_ok(heads * n_q * (n_heads / cache->n_kv) + heads * cache->max_pages, "ibh_kv4_attn"))
         return IBH_ERROR_PARAM;
     char* w = (char*)ws;
     AttnArgs a{out, q, n_heads, n_q, q_stride, (float)(1.4426950408889634 / sqrt((double)cache->head_dim)), p.chunk,
                p.n_split, p.n_tile, (float*)(w + p.part), (float2*)(w + p.part_ml),
-               weights_out ? (float*)(w + p.lse) : nullptr, (i4_t*)(w + p.digits), (float*)(w + p.rowc)};
+               weights_out && !p.joint ? (float*)(w + p.lse) : nullptr,
+               weights_out ? (i4_t*)(w + p.digits) : nullptr, (float*)(w + p.rowc)};
     const Kv4 c = device_of(cache);
     hipStream_t st = ibh_resolve_stream(stream);
     switch (cache->head_dim / 64) {
-        case 1: launch_attn<1>(c, a, p, blocks, rows, weights_in, weights_out, wblocks, st); break;
-        case 2: launch_attn<2>(c, a, p, blocks, rows, weights_in, weights_out, wblocks, st); break;
-        case 3: launch_attn<3>(c, a, p, blocks, rows, weights_in, weights_out, wblocks, st); break;
-        default: launch_attn<4>(c, a, p, blocks, rows, weights_in, weights_out, wblocks, st); break;
+        case 1: launch_attn<1>(c, a, p, heads, weights_in, weights_out, st); break;
+        case 2: launch_attn<2>(c, a, p, heads, weights_in, weights_out, st); break;
+        case 3: launch_attn<3>(c, a, p, heads, weights_in, weights_out, st); break;
+        default: launch_attn<4>(c, a, p, heads, weights_in, weights_out, st); break;
     }
     IBH_CHECK_LAUNCH("ibh_kv4_attn");
     return IBH_OK;

@@ -197,7 +197,7 @@ def kv4_attn(out, q, cache: Kv4Cache, n_heads: int, weights_in=None, weights_out
         size = cache.n_seq * cache.n_kv * cache.max_pages * KV4_PAGE
         wi, wo = (cache._on(w, torch.float32, size) for w in (weights_in, weights_out))
     if ws is None:
-        need = lib().ibh_kv4_attn_workspace_bytes(cache.ref, n_heads, n_q)
+        need = lib().ibh_kv4_attn_workspace_bytes(cache.ref, n_heads, n_q, wi is not None)
         ws = torch.empty(need, dtype=torch.uint8, device=cache.device)
     cache._call("ibh_kv4_attn", cache.ref, po, pq, n_heads, n_q, sq, wi, wo, cache._on(ws), ws.numel())
 

@@ -98,8 +98,8 @@ def test_sizes():
     assert L.ibh_kv4_page_bytes(8, 128) == 8 * 9216
     for kv, hd in ((0, 128), (8, 96), (8, 0), (-1, 64), (8, 320)):
         assert L.ibh_kv4_page_bytes(kv, hd) == 0
-    assert L.ibh_kv4_attn_workspace_bytes(C.byref(desc()), 4, 1) > 0
-    assert L.ibh_kv4_attn_workspace_bytes(C.byref(desc()), 0, 1) == 0
+    assert L.ibh_kv4_attn_workspace_bytes(C.byref(desc()), 4, 1, 0) > 0
+    assert L.ibh_kv4_attn_workspace_bytes(C.byref(desc()), 0, 1, 1) == 0
 
 
 def test_python_wrappers_refuse():

@@ -439,7 +439,7 @@ def test_graph_replay_follows_lens_and_table(ops):
     k, v = (torch.randn(n, 1, n_kv * hd, device="cuda") for _ in range(2))
     out, w = torch.empty_like(q), torch.zeros(n, n_kv, 320, device="cuda")
     import libinferbit_amd as L
-    ws = torch.empty(L.lib().ibh_kv4_attn_workspace_bytes(m.cache.ref, n_heads, 1), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(L.lib().ibh_kv4_attn_workspace_bytes(m.cache.ref, n_heads, 1, 1), dtype=torch.uint8, device="cuda")
 
     def step():
         m.dlens.add_(1)
