@@ -50,11 +50,13 @@ __device__ __forceinline__ int seq_len(const Kv4& c, int seq, bool* bad) {
     *bad = m != n;
     return m;
 }
-// page_at() where all arguments are the same for the whole wavefront.
-__device__ __forceinline__ const uint8_t* page_of_wave(const Kv4& c, int seq, int p, int h) {
-    const int id = ld_uniform(c.table + (size_t)seq * c.max_pages + p);
+__device__ __forceinline__ const uint8_t* page_by_id(const Kv4& c, int id, int h) {
     if ((unsigned)id >= (unsigned)c.n_pages) return nullptr;
     return c.pool + ((size_t)id * c.n_kv + h) * (size_t)(72 * c.hd);
+}
+// page_at() where all arguments are the same for the whole wavefront.
+__device__ __forceinline__ const uint8_t* page_of_wave(const Kv4& c, int seq, int p, int h) {
+    return page_by_id(c, ld_uniform(c.table + (size_t)seq * c.max_pages + p), h);
 }
 // Head h's part of page p of a sequence, or null where the table names no page of the pool.
 __device__ __forceinline__ uint8_t* page_at(const Kv4& c, int seq, int p, int h) {
@@ -238,7 +240,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4 c, float* __restrict_
 // ── attention ────────────────────────────────────────────────────────────────
 // The matrix cores multiply the codes as they lie.  The other operand of each
 // product is written in three signed base-256 digits, x = step * (65536 d0 +
-// 256 d1 + d2) with |x| <= 127 * 65536 step (23 bits below the largest element
+// 256 d1 + d2) with |x| <= 63.5 * 65536 step (22 bits below the largest element
 // of a query, or of a page's p * scale), so every product and sum is exact in
 // int32 and what is rounded is rounded as in fp32.  A tile is 4 query rows (a
 // row is one head of one query) as the 16 rows of the MFMA's first operand:
@@ -250,7 +252,9 @@ typedef int i4_t __attribute__((ext_vector_type(4)));
 typedef int i4_alias __attribute__((ext_vector_type(4), may_alias));
 typedef uint32_t u32_alias __attribute__((may_alias));
 
-constexpr float kDigitMax = 8323072.f;                   // 127 * 65536
+// 63.5 * 65536: 64 products of such a number with -8 .. 7 fit 31 bits, so the
+// three digits' sums are joined as integers, by shifts
+constexpr float kDigitMax = 4161536.f;
 constexpr int kMaxSplit = 4096;                          // blocks of one row tile
 constexpr float kTiny = 1e-30f;                          // below this a query, or a page's p * scale, counts as zero
 
@@ -259,7 +263,7 @@ __device__ __forceinline__ i4_t unpack16(uint32_t a, uint32_t b) {
     return i4_t{(int)(a & M), (int)((a >> 4) & M), (int)(b & M), (int)((b >> 4) & M)};
 }
 __device__ __forceinline__ i4_t mfma16(i4_t a, i4_t b, i4_t c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ float join_digits(i4_t c) { return fmaf((float)((c[0] << 8) + c[1]), 256.f, (float)c[2]); }
+__device__ __forceinline__ float join_digits(i4_t c) { return (float)((c[0] << 16) + ((c[1] << 8) + c[2])); }
 // v_exp_f32: at most one unit in the last place off, results below 2^-126 are 0
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 // Largest value of the 16 lanes of a row, every lane getting it: v_max_f32
@@ -319,6 +323,7 @@ struct AttnArgs {
     float* lse;                                          // [seq][KV head][row] log2 of the row's sum, when weights are wanted
     i4_t* digits;                                        // [seq][KV head][4-row tile][group][lane]
     float* rowc;                                         // [seq][KV head][row][1 + groups] step * scale, sums of the query in steps
+    float4* scores;                                      // [seq][KV head][page][tile][lane] scores (log2), -inf where not seen
 };
 
 // Wavefronts a SIMD holds: what the registers of a page and RT tiles leave.
@@ -327,7 +332,7 @@ constexpr int attn_waves(int hdg, int rt) { return hdg * rt == 1 ? 4 : hdg * rt 
 // Block: `chunk` pages of one (sequence, KV head), RT tiles of 4 query rows,
 // four wavefronts that take the block's pages in turn, each with its own
 // running maximum and sums, joined at the end.
-template <int HDG, int RT>
+template <int HDG, int RT, bool SCORES>
 __global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 c, AttnArgs a) {
     constexpr int HD = 64 * HDG, ROWS = 4 * RT;
     __shared__ __align__(16) int8_t digs[RT * HDG * 1024];   // [tile][group][16][64]
@@ -345,13 +350,17 @@ __global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 
     const int rt = a.n_tile - 1 - b % a.n_tile; b /= a.n_tile;
     const int split = b % a.n_split, seq = b / a.n_split;
     const int grp = a.n_heads / c.n_kv, n_rows = a.n_q * grp;
+    // the first page's number with the length, not behind it
+    const int p0 = split * a.chunk;
+    int p = p0 + wave;
+    const int id0 = ld_uniform(c.table + (size_t)seq * c.max_pages + min(p, c.max_pages - 1));
     bool bad;
     const int len = seq_len(c, seq, &bad);
     const int row0 = rt * ROWS;
     // the last position that each row sees; rows past the last copy it
     const int lim_min = len - a.n_q + row0 / grp, lim_max = len - a.n_q + min(row0 + ROWS - 1, n_rows - 1) / grp;
     const int pages = lim_max < 0 ? 0 : lim_max / kPage + 1;
-    const int p0 = split * a.chunk, p1 = min(p0 + a.chunk, pages);
+    const int p1 = min(p0 + a.chunk, pages);
     if (split > 0 && p0 >= pages) return;
     int lim[RT];
 #pragma unroll
@@ -370,8 +379,12 @@ __global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 
     };
     uint4 kc[2][HDG], kp[HDG], vc[2 * HDG], vp[HDG];     // the page's codes and pairs
     unsigned at = 16 * lane;
-    int p = p0 + wave;
-    const uint8_t* pg = next_page(p);
+    const uint8_t* pg = p < p1 ? page_by_id(c, id0, h) : nullptr;
+    if (!pg && p < p1) {
+        bad = true;
+        p += 4;
+        pg = next_page(p);
+    }
     if (pg) {
 #pragma unroll
         for (int g = 0; g < HDG; g++) {
@@ -455,7 +468,7 @@ __global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 
     // one place of this page again (at = 0), which costs less than a branch.
     auto step = [&](int pos0, const uint8_t* nx, auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
-        float e[RT][4];
+        float e[RT][4], y[RT][4];
         {
             i4_t kb[4][HDG];
 #pragma unroll
@@ -486,6 +499,10 @@ __global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 
                 if constexpr (MASKED) {
 #pragma unroll
                     for (int s = 0; s < 4; s++) x[s] = pos0 + 16 * s + li <= lim[t] ? x[s] : -INFINITY;
+                }
+                if constexpr (SCORES) {
+#pragma unroll
+                    for (int s = 0; s < 4; s++) y[t][s] = x[s] * kf[t];
                 }
                 const float top = row16_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
                 if (__any(top > m[t])) {
@@ -534,8 +551,8 @@ __global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 
                     }
                 }
                 const float wm = row16_max(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])));
-                const float inv = wm > kTiny ? kDigitMax * __builtin_amdgcn_rcpf(wm) : 0.f;
-                const float ws = wm > kTiny ? wm * (1.f / kDigitMax) : 0.f;
+                const float wt = fmaxf(wm, kTiny);
+                const float inv = kDigitMax * __builtin_amdgcn_rcpf(wt), ws = wt * (1.f / kDigitMax);
                 uint32_t j[4];
 #pragma unroll
                 for (int s = 0; s < 4; s++) j[s] = (uint32_t)fmaf(w[s], inv, 32896.5f);
@@ -555,6 +572,15 @@ __global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 
                     o[t][4 * g + d4] = fmaf(join_digits(mfma16(wa, vb[d4], init)), ws, o[t][4 * g + d4]);
             }
             vp[g] = val_pairs<HDG, RT <= 2>(nx, g, at);
+        }
+        if constexpr (SCORES) {
+            // behind the next page's loads: a wait for a load waits for every store before it
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                typedef float f4_t __attribute__((ext_vector_type(4)));
+                __builtin_nontemporal_store(f4_t{y[t][0], y[t][1], y[t][2], y[t][3]},
+                                            (f4_t*)(a.scores + ((sh * c.max_pages + (pos0 >> 6)) * RT + t) * 64 + lane));
+            }
         }
     };
     // pages that every row sees, then the others
@@ -664,13 +690,19 @@ struct PageWeights {
         }
         for (int t = t0; t < t1; t += dt) {
             // the next tile's rows are loaded while this one's are multiplied
-            const int tn = t + dt < t1 ? t + dt : t;
             i4_t qn[HDG];
-            float kfn, lsen, qsn[HDG];
-            int limn;
+            float kfn = 0.f, lsen = 0.f, qsn[HDG];
+            int limn = -1;
 #pragma unroll
-            for (int g = 0; g < HDG; g++) qn[g] = digits[((size_t)tn * HDG + g) * 64 + lane];
-            rows(tn, lq, kfn, lsen, qsn, limn);
+            for (int g = 0; g < HDG; g++) {
+                qn[g] = zero;
+                qsn[g] = 0.f;
+            }
+            if (t + dt < t1) {
+#pragma unroll
+                for (int g = 0; g < HDG; g++) qn[g] = digits[((size_t)(t + dt) * HDG + g) * 64 + lane];
+                rows(t + dt, lq, kfn, lsen, qsn, limn);
+            }
             float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int g = 0; g < HDG; g++) {
@@ -701,18 +733,16 @@ struct PageWeights {
     }
 };
 
-constexpr int kFinishPages = 4;                          // pages of a weights block
-
-// Maximum (log2) and sum of a query row over its splits, by one wavefront.
-__device__ __forceinline__ float row_lse(const float2* ml, int n, int lane) {
+// log2 of a query row's sum over its splits, by the 16 lanes of a row.
+__device__ __forceinline__ float row_lse(const float2* ml, int n, int li) {
     float m = -INFINITY, s = 0.f;
-    for (int i = lane; i < n; i += 64) m = fmaxf(m, ml[i].x);
-    m = wave_max_dpp(m);
-    for (int i = lane; i < n; i += 64) {
+    for (int i = li; i < n; i += 16) m = fmaxf(m, ml[i].x);
+    m = row16_max(m);
+    for (int i = li; i < n; i += 16) {
         const float2 v = ml[i];
         s = fmaf(v.x == -INFINITY && v.y == 0.f ? 0.f : exp2_(v.x - m), v.y, s);
     }
-    s = wave_sum_dpp(s);
+    s = row16_sum(s);
     return s == 0.f ? INFINITY : m + log2f(s);
 }
 
@@ -790,42 +820,39 @@ __global__ __launch_bounds__(256) void kv4_attn_finish(Kv4 c, AttnArgs a, unsign
     }
     unsigned b = blockIdx.x - n_join;
     const int h = b % c.n_kv; b /= c.n_kv;
-    const int np = (c.max_pages + kFinishPages - 1) / kFinishPages;
-    const int p0 = b % np * kFinishPages, seq = b / np;
+    const int np = (c.max_pages + 3) / 4;
+    const int p = b % np * 4 + wave, seq = b / np;
+    if (p >= c.max_pages) return;
     const size_t sh = (size_t)seq * c.n_kv + h;
     const int len = seq_len(c, seq, &bad);
-    const int p = p0 + wave;
-    const bool here = p * kPage < len;
     const size_t at = (sh * c.max_pages + p) * kPage + lane;
-    const float old = here ? win[at] : 0.f;
-    const uint8_t* pg = here ? page_of_wave(c, seq, p, h) : nullptr;
-    PageWeights<HDG> pw;
-    if (pg) pw.load(pg, lane);
-    if (p0 * kPage < len) {
-        const int n = splits_of(a, len, 0, grp, n_rows, 4 * RT);
-        for (int r = wave; r < n_rows; r += 4) {
-            const float lse = row_lse(a.part_ml + (sh * n_rows + r) * a.n_split, n, lane);
-            if (lane == 0) f[r] = lse;
-        }
+    if (p * kPage >= len) {
+        wout[at] = 0.f;
+        return;
     }
-    __syncthreads();
-    if (p >= c.max_pages) return;
-    float add = NAN;
-    if (pg && !bad) {
-        const int tiles = (n_rows + 3) / 4;
-        add = pw.sum(a.digits + sh * tiles * HDG * 64, p * kPage, lane, 0, tiles, 1,
-            [&](int t, int lq, float& kf, float& lse, float* qs, int& lim) {
-                const int r = 4 * t + lq, row = min(r, n_rows - 1);
-                const float* rcp = a.rowc + (sh * n_rows + row) * (1 + HDG);
-                kf = rcp[0];
-                lse = f[row];
+    const float old = win[at];
+    float4 x[RT];
 #pragma unroll
-                for (int g = 0; g < HDG; g++) qs[g] = rcp[1 + g];
-                lim = r < n_rows ? len - a.n_q + row / grp : -1;
-            });
-    } else if (here && lane == 0) {
-        raise_table();
+    for (int t = 0; t < RT; t++) x[t] = a.scores[((sh * c.max_pages + p) * RT + t) * 64 + lane];
+    const int n = splits_of(a, len, 0, grp, n_rows, 4 * RT);
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    const int lq = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int r = 4 * t + lq;
+        float lse = row_lse(a.part_ml + (sh * n_rows + min(r, n_rows - 1)) * a.n_split, n, lane & 15);
+        if (r >= n_rows) lse = INFINITY;
+        acc[0] += exp2_(x[t].x - lse);
+        acc[1] += exp2_(x[t].y - lse);
+        acc[2] += exp2_(x[t].z - lse);
+        acc[3] += exp2_(x[t].w - lse);
     }
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+        acc[s] += __shfl_xor(acc[s], 16, kWave);
+        acc[s] += __shfl_xor(acc[s], 32, kWave);
+    }
+    const float add = lq == 0 ? acc[0] : lq == 1 ? acc[1] : lq == 2 ? acc[2] : acc[3];
     wout[at] = p * kPage + lane < len ? old + add : 0.f;
 }
 
@@ -1124,7 +1151,7 @@ extern "C" int ibh_kv4_read(const ibh_kv4_cache* cache, float* k, float* v, int 
 struct AttnPlan {
     int rt, n_tile, chunk, n_split;
     bool joint;                                          // the weights in the launch that joins the splits
-    size_t part, part_ml, lse, digits, rowc, bytes;      // offsets into the workspace
+    size_t part, part_ml, lse, digits, rowc, score, bytes;      // offsets into the workspace
 };
 static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool weights) {
     AttnPlan p;
@@ -1137,14 +1164,15 @@ static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool wei
     chunk = max(chunk, ((size_t)c->max_pages + kMaxSplit - 1) / kMaxSplit);
     p.chunk = (int)((chunk + 3) / 4 * 4);
     p.n_split = (c->max_pages + p.chunk - 1) / p.chunk;
-    p.joint = weights && p.n_tile == 1 && p.n_split > 1;
+    p.joint = weights && p.n_tile == 1 && p.n_split > 1 && p.rt <= 2;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
     p.part = take(p.n_split > 1 ? heads * n_rows * p.n_split * c->head_dim * sizeof(float) : 0);
     p.part_ml = take(p.n_split > 1 ? heads * n_rows * p.n_split * sizeof(float2) : 0);
     p.lse = take(weights && !p.joint ? heads * n_rows * sizeof(float) : 0);
-    p.digits = take(weights ? heads * ((n_rows + 3) / 4) * hdg * 1024 : 0);
-    p.rowc = take(weights ? heads * n_rows * (1 + hdg) * sizeof(float) : 0);
+    p.digits = take(weights && !p.joint ? heads * ((n_rows + 3) / 4) * hdg * 1024 : 0);
+    p.rowc = take(weights && !p.joint ? heads * n_rows * (1 + hdg) * sizeof(float) : 0);
+    p.score = take(p.joint ? heads * c->max_pages * p.rt * 1024 : 0);
     p.bytes = at;
     return p;
 }
@@ -1160,8 +1188,12 @@ template <int HDG, int RT>
 static void launch_attn_rt(const Kv4& c, const AttnArgs& a, const AttnPlan& p, size_t heads, const float* win,
                            float* wout, hipStream_t st) {
     const size_t rows = p.n_split > 1 ? heads * a.n_q * (a.n_heads / c.n_kv) : 0;
-    kv4_attn_kernel<HDG, RT><<<(unsigned)(heads * p.n_tile * p.n_split), 256, 0, st>>>(c, a);
-    const size_t wb = p.joint ? heads * ((c.max_pages + kFinishPages - 1) / kFinishPages) : 0;
+    const unsigned blocks = (unsigned)(heads * p.n_tile * p.n_split);
+    if constexpr (RT <= 2) {
+        if (p.joint) kv4_attn_kernel<HDG, RT, true><<<blocks, 256, 0, st>>>(c, a);
+    }
+    if (!p.joint) kv4_attn_kernel<HDG, RT, false><<<blocks, 256, 0, st>>>(c, a);
+    const size_t wb = p.joint ? heads * ((c.max_pages + 3) / 4) : 0;
     if (rows + wb) kv4_attn_finish<HDG, RT><<<(unsigned)(rows + wb), 256, 0, st>>>(c, a, (unsigned)rows, win, wout);
     if (wout && !p.joint)
         kv4_attn_weights<HDG><<<(unsigned)(heads * c.max_pages), 64 * kWeightWaves, 0, st>>>(c, a, win, wout);
@@ -1201,7 +1233,7 @@ extern "C" int ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float*
     AttnArgs a{out, q, n_heads, n_q, q_stride, (float)(1.4426950408889634 / sqrt((double)cache->head_dim)), p.chunk,
                p.n_split, p.n_tile, (float*)(w + p.part), (float2*)(w + p.part_ml),
                weights_out && !p.joint ? (float*)(w + p.lse) : nullptr,
-               weights_out ? (i4_t*)(w + p.digits) : nullptr, (float*)(w + p.rowc)};
+               weights_out && !p.joint ? (i4_t*)(w + p.digits) : nullptr, (float*)(w + p.rowc), (float4*)(w + p.score)};
     const Kv4 c = device_of(cache);
     hipStream_t st = ibh_resolve_stream(stream);
     switch (cache->head_dim / 64) {
