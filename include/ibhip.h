@@ -271,9 +271,13 @@ int    ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float* q, int 
  * position are left as they are.
  * In place: dst with src's pool, table, lens and weights.  Otherwise dst has
  * its own table, lens and weights, and pages that src does not use; src is
- * left as it was.  sink + recent <= budget <= 64 dst->max_pages. */
-int ibh_kv4_evict(const ibh_kv4_cache* src, const ibh_kv4_cache* dst, const float* weights_src, float* weights_dst,
-                  int budget, int sink, int recent, int32_t* kept, void* stream);
+ * left as it was.  sink + recent <= budget <= 64 dst->max_pages.
+ * `ws` >= ibh_kv4_evict_workspace_bytes(src) (0 for rows of up to 16384
+ * positions) on 16 bytes, NULL = library workspace; calls that share one must
+ * not overlap in time. */
+size_t ibh_kv4_evict_workspace_bytes(const ibh_kv4_cache* src);
+int    ibh_kv4_evict(const ibh_kv4_cache* src, const ibh_kv4_cache* dst, const float* weights_src, float* weights_dst,
+                     int budget, int sink, int recent, int32_t* kept, void* ws, size_t ws_bytes, void* stream);
 
 /* ── product-quantised LUT matvec, device pointers ─────────── */
 

@@ -48,7 +48,8 @@ SIGNATURES = {
     "ibh_kv4_read": (I, [P, P, P, I, I, P]),
     "ibh_kv4_attn_workspace_bytes": (SZ, [P, I, I, I]),
     "ibh_kv4_attn": (I, [P, P, P, I, I, I, P, P, P, SZ, P]),
-    "ibh_kv4_evict": (I, [P, P, P, P, I, I, I, P, P]),
+    "ibh_kv4_evict_workspace_bytes": (SZ, [P]),
+    "ibh_kv4_evict": (I, [P, P, P, P, I, I, I, P, P, SZ, P]),
     "ibh_pq_workspace_bytes": (SZ, [P]),
     "ibh_pq_workspace_init": (I, [P, SZ, P]),
     "ibh_pq_matmul_fp32_host": (I, [P, P, P]),

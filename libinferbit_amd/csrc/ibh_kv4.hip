@@ -913,78 +913,23 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
 }
 
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
+constexpr int kSelKeys = 16;                             // ranks a thread of the one-block selection holds
+constexpr int kSelMost = kSelThreads * kSelKeys;         // longest row of it
 
-// Block (KV head, sequence): the need-th largest weight of positions
-// [sink, len - recent) byte by byte from the top (a histogram of the ranks
-// that share the bytes found so far), then the kept positions in order:
-// wavefront w counts and then emits its own stretch of the positions.
-__global__ __launch_bounds__(kSelThreads) void kv4_select(Kv4 c, const float* __restrict__ w, int budget, int sink,
-                                                          int recent, int32_t* __restrict__ kept) {
-    __shared__ unsigned hist[256];
-    __shared__ unsigned pick[2];
-    __shared__ int cnt[kSelWaves][2];
-    const int seq = blockIdx.x / c.n_kv;
-    bool bad;
-    const int len = seq_len(c, seq, &bad);
-    const float* wr = w + (size_t)blockIdx.x * c.max_pages * kPage;
-    int32_t* kr = kept + (size_t)blockIdx.x * budget;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (bad && tid == 0) raise_table();
-    if (bad || len <= budget) {
-        for (int i = tid; i < budget; i += kSelThreads) kr[i] = !bad && i < len ? i : -1;
-        return;
-    }
-    const int z = len - recent;                          // candidates [sink, z)
-    unsigned need = budget - sink - recent, prefix = 0, mask = 0;
-    for (int shift = 24; need && shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int i = sink + tid; i < z; i += kSelThreads) {
-            const uint32_t r = rank_of(wr[i]);
-            if ((r & mask) == prefix) atomicAdd(&hist[(r >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            unsigned left = need;
-            int d = 255;
-            for (; d > 0 && hist[d] < left; d--) left -= hist[d];
-            pick[0] = d;
-            pick[1] = left;
-        }
-        __syncthreads();
-        prefix |= pick[0] << shift;
-        mask |= 255u << shift;
-        need = pick[1];
-    }
-    // kept: rank above the prefix, and the first `need` of those equal to it
-    const bool none = budget == sink + recent;
-    const int per = (len + kSelWaves * 64 - 1) / (kSelWaves * 64) * 64;
-    const int a = wave * per, e = min(len, a + per);
-    int above = 0, equal = 0;
-    for (int i0 = a; i0 < e; i0 += 64) {
+// Emits the kept positions of a wavefront's stretch a .. e - 1 in order: those
+// not for choice (before sink, from z on), those above `cut`, and of those
+// equal to it the ones whose count among all equals is below `equals`.
+template <class Rank>
+__device__ __forceinline__ void emit_kept(int32_t* kr, int a, int e, int sink, int z, uint32_t cut, bool choose,
+                                          int at, int eqs, int equals, int lane, Rank rank) {
+    const unsigned long long low = (1ull << lane) - 1;
+    for (int i0 = a, j = 0; i0 < e; i0 += 64, j++) {
         const int i = i0 + lane;
-        const bool cand = i < e && i >= sink && i < z;
-        const uint32_t r = cand ? rank_of(wr[i]) : 0u;
-        const bool sure = i < e && (!cand || (!none && r > prefix));
-        const bool eq = cand && !none && r == prefix;
-        above += __popcll(__ballot(sure));
-        equal += __popcll(__ballot(eq));
-    }
-    if (lane == 0) { cnt[wave][0] = above; cnt[wave][1] = equal; }
-    __syncthreads();
-    int at = 0, eqs = 0;                                 // kept entries and equal ranks before this stretch
-    for (int k = 0; k < wave; k++) {
-        at += cnt[k][0];
-        eqs += cnt[k][1];
-    }
-    at += min(eqs, (int)need);
-    for (int i0 = a; i0 < e; i0 += 64) {
-        const int i = i0 + lane;
-        const bool cand = i < e && i >= sink && i < z;
-        const uint32_t r = cand ? rank_of(wr[i]) : 0u;
-        const bool eq = cand && !none && r == prefix;
-        const unsigned long long be = __ballot(eq), low = (1ull << lane) - 1;
-        const bool keep = i < e && (!cand || (!none && r > prefix) || (eq && eqs + __popcll(be & low) < (int)need));
+        const bool in = i < e, cand = in && i >= sink && i < z;
+        const uint32_t r = rank(i, j, cand);
+        const bool eq = cand && choose && r == cut;
+        const unsigned long long be = __ballot(eq);
+        const bool keep = in && (!cand || (choose && r > cut) || (eq && eqs + __popcll(be & low) < equals));
         const unsigned long long bk = __ballot(keep);
         if (keep) kr[at + __popcll(bk & low)] = i;
         at += __popcll(bk);
@@ -992,76 +937,338 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select(Kv4 c, const float* __
     }
 }
 
-// Moves the kept positions: block (first page, KV head, sequence) gathers a
-// page of the destination into LDS and writes it.  In place (`serial`) a block
-// takes all pages of its head in order: a kept position never lies before its
-// destination, so page p's sources are in pages >= p, and page p is written
-// only after pages <= p have been gathered.
-__global__ __launch_bounds__(256) void kv4_move(Kv4 src, Kv4 dst, const float* w_src, float* w_dst, int budget,
-                                                const int32_t* __restrict__ kept, int serial) {
-    extern __shared__ __align__(16) uint8_t buf[];       // 72 hd bytes
-    __shared__ int from[kPage];
-    __shared__ float wt[kPage];
-    const int hd = src.hd, hdg = hd / 64, tid = threadIdx.x;
+// Rows of up to 16384 positions: block (KV head, sequence), the ranks in
+// registers.  The need-th largest is built bit by bit from the top: a bit
+// stays set while at least `need` ranks are no smaller (a ballot a register, a
+// wave's count in LDS, one barrier a bit), which takes no atomics and the
+// same time for any distribution.
+__global__ __launch_bounds__(kSelThreads) void kv4_select(Kv4 c, const float* __restrict__ w, int budget, int sink,
+                                                          int recent, int32_t* __restrict__ kept) {
+    __shared__ int cnt[2][kSelWaves];
+    __shared__ int cnt2[kSelWaves][2];
+    const int seq = blockIdx.x / c.n_kv;
+    bool bad;
+    const int len = seq_len(c, seq, &bad);
+    const float* wr = w + (size_t)blockIdx.x * c.max_pages * kPage;
+    int32_t* kr = kept + (size_t)blockIdx.x * budget;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (bad && tid == 0) raise_table();
+    if (bad || len <= budget) {
+        for (int i = tid; i < budget; i += kSelThreads) kr[i] = !bad && i < len ? i : -1;
+        return;
+    }
+    const int z = len - recent;                          // candidates [sink, z)
+    const int need = budget - sink - recent;
+    const int per = (len + kSelWaves * 64 - 1) / (kSelWaves * 64) * 64;   // positions of a wavefront
+    const int a = wave * per, e = min(len, a + per);
+    uint32_t key[kSelKeys];                              // 0 where nothing is to choose: never counted, a bit is set in every trial
+#pragma unroll
+    for (int j = 0; j < kSelKeys; j++) {
+        const int i = a + 64 * j + lane;
+        key[j] = i < e && i >= sink && i < z ? rank_of(wr[i]) : 0u;
+    }
+    uint32_t cut = 0;
+    const bool choose = need > 0;
+    if (choose)
+        for (int bit = 31; bit >= 0; bit--) {
+            const uint32_t trial = cut | (1u << bit);
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < kSelKeys; j++)
+                if (64 * j < per) n += __popcll(__ballot(key[j] >= trial));
+            if (lane == 0) cnt[bit & 1][wave] = n;
+            __syncthreads();
+            int sum = 0;
+#pragma unroll
+            for (int k = 0; k < kSelWaves; k++) sum += cnt[bit & 1][k];
+            if (sum >= need) cut = trial;
+        }
+    int above = 0, equal = 0;
+#pragma unroll
+    for (int j = 0; j < kSelKeys; j++)
+        if (64 * j < per) {
+            const int i = a + 64 * j + lane;
+            const bool in = i < e, cand = in && i >= sink && i < z;
+            above += __popcll(__ballot(in && (!cand || (choose && key[j] > cut))));
+            equal += __popcll(__ballot(cand && choose && key[j] == cut));
+        }
+    if (lane == 0) { cnt2[wave][0] = above; cnt2[wave][1] = equal; }
+    __syncthreads();
+    int total = 0, at = 0, eqs = 0;                      // all that are sure; kept and equal before this stretch
+#pragma unroll
+    for (int k = 0; k < kSelWaves; k++) {
+        total += cnt2[k][0];
+        if (k < wave) {
+            at += cnt2[k][0];
+            eqs += cnt2[k][1];
+        }
+    }
+    const int equals = budget - total;                   // how many of the equal ones are kept
+    at += min(eqs, equals);
+    const unsigned long long low = (1ull << lane) - 1;
+#pragma unroll
+    for (int j = 0; j < kSelKeys; j++)
+        if (64 * j < per) {
+            const int i = a + 64 * j + lane;
+            const bool in = i < e, cand = in && i >= sink && i < z, eq = cand && choose && key[j] == cut;
+            const unsigned long long be = __ballot(eq);
+            const bool keep = in && (!cand || (choose && key[j] > cut) || (eq && eqs + __popcll(be & low) < equals));
+            const unsigned long long bk = __ballot(keep);
+            if (keep) kr[at + __popcll(bk & low)] = i;
+            at += __popcll(bk);
+            eqs += __popcll(be);
+        }
+}
+
+// Longer rows: up to 32 blocks a row, each with its own segment, in four
+// launches.  Launch 0, 1, 2 count the segment's ranks by their top 11, middle
+// 11 and low 10 bits, among those whose higher bits are the cut's; every block
+// of the next launch adds up the segments' counts and finds the next bits of
+// the cut for itself.  Launch 3 counts what the segments before its own keep
+// from the same counts, and emits.
+constexpr int kSegs = 32, kBins = 2048;
+struct LongSel {
+    uint32_t* hist;                                      // [row][launch 0..2][segment][kBins]
+    uint32_t* above;                                     // [row][launch 1, 2][segment] ranks above the cut's bits so far, in its group
+    int seg, n_seg;                                      // positions of a segment, segments of a row
+    int budget, sink, recent;
+};
+__device__ __forceinline__ int bin_shift(int level) { return level == 0 ? 21 : level == 1 ? 10 : 0; }
+
+template <int LEVEL>
+__global__ __launch_bounds__(kSelThreads) void kv4_select_long(Kv4 c, LongSel q, const float* __restrict__ w,
+                                                               int32_t* __restrict__ kept) {
+    __shared__ uint32_t hist[kBins];
+    __shared__ uint32_t scan[kSelWaves];
+    __shared__ uint32_t found[2];
+    __shared__ int cnt2[kSelWaves][2];
+    __shared__ int before[2];
+    const int row = blockIdx.x / q.n_seg, sg = blockIdx.x % q.n_seg, seq = row / c.n_kv;
+    bool bad;
+    const int len = seq_len(c, seq, &bad);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int32_t* kr = kept + (size_t)row * q.budget;
+    const int s0 = min(len, sg * q.seg), s1 = min(len, s0 + q.seg);
+    if (bad || len <= q.budget) {
+        if (LEVEL == 3) {
+            if (bad && tid == 0) raise_table();
+            for (int i = sg * kSelThreads + tid; i < q.budget; i += q.n_seg * kSelThreads) kr[i] = !bad && i < len ? i : -1;
+        }
+        return;
+    }
+    const int z = len - q.recent, segs = (len + q.seg - 1) / q.seg;
+    if (sg >= segs) return;
+    const float* wr = w + (size_t)row * c.max_pages * kPage;
+    uint32_t need = q.budget - q.sink - q.recent;
+    const bool choose = need > 0;
+    uint32_t* const h0 = q.hist + (size_t)row * 3 * kSegs * kBins;
+    uint32_t* const ab = q.above + (size_t)row * 2 * kSegs;
+    uint32_t cut = 0;                                    // the bits found so far
+    // levels before this launch's: add the segments up, find the bin in which
+    // the need-th largest lies
+    if (choose)
+#pragma unroll
+        for (int lv = 0; lv < LEVEL; lv++) {
+            constexpr int PB = kBins / kSelThreads;      // bins a thread adds up, highest first over the threads
+            const uint32_t* hl = h0 + (size_t)lv * kSegs * kBins;
+            const int hi = kBins - PB * (tid + 1);
+            uint32_t v[PB] = {};
+            for (int s = 0; s < segs; s++) {
+                const uint2 x = *(const uint2*)(hl + (size_t)s * kBins + hi);
+                v[0] += x.x;
+                v[1] += x.y;
+            }
+            static_assert(PB == 2, "bins a thread");
+            const uint32_t mine = v[0] + v[1];
+            uint32_t run = mine;                         // counts of this thread's bins and all higher ones
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t up = __shfl_up(run, o, kWave);
+                if (lane >= o) run += up;
+            }
+            __syncthreads();
+            if (lane == 63) scan[wave] = run;
+            __syncthreads();
+            for (int k = 0; k < wave; k++) run += scan[k];
+            const uint32_t higher = run - mine;
+            if (higher < need && run >= need) {          // one thread
+                const bool top = higher + v[1] >= need;
+                found[0] = top ? hi + 1 : hi;
+                found[1] = top ? higher : higher + v[1];
+            }
+            __syncthreads();
+            cut |= found[0] << bin_shift(lv);
+            need -= found[1];
+        }
+    if constexpr (LEVEL < 3) {
+        for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+        __syncthreads();
+        constexpr uint32_t known = LEVEL == 0 ? 0u : LEVEL == 1 ? ~0u << 21 : ~0u << 10;
+        constexpr uint32_t group = LEVEL <= 1 ? 0u : ~0u << 21;   // bits that the launch before knew
+        int over = 0;
+        for (int i0 = s0 + wave * 64; i0 < s1; i0 += kSelThreads) {
+            const int i = i0 + lane;
+            const bool cand = i < s1 && i >= q.sink && i < z && choose;
+            const uint32_t r = cand ? rank_of(wr[i]) : 0u;
+            if (cand && (r & known) == cut) atomicAdd(&hist[(r >> bin_shift(LEVEL)) & (kBins - 1) & (LEVEL == 2 ? 1023 : 2047)], 1u);
+            if (LEVEL > 0) over += __popcll(__ballot(cand && (r & known) > cut && (r & group) == (cut & group)));
+        }
+        if (LEVEL > 0 && lane == 0) cnt2[wave][0] = over;
+        __syncthreads();
+        uint32_t* ho = h0 + ((size_t)LEVEL * kSegs + sg) * kBins;
+        for (int i = tid; i < kBins; i += kSelThreads) ho[i] = hist[i];
+        if (LEVEL > 0 && tid == 0) {
+            int sum = 0;
+            for (int k = 0; k < kSelWaves; k++) sum += cnt2[k][0];
+            ab[(LEVEL - 1) * kSegs + sg] = sum;
+        }
+    } else {
+        // what the segments before this one keep: all outside [sink, z), the
+        // ranks above the cut, and the equal ones up to `need`
+        if (wave == 0) {
+            int sure = 0, eq = 0;
+            const uint32_t* hl = h0 + (size_t)2 * kSegs * kBins;
+            const uint32_t bin = cut & 1023;
+            for (int s = lane; choose && s < sg; s += 64) {
+                sure += ab[s] + ab[kSegs + s];
+                eq += hl[(size_t)s * kBins + bin];
+            }
+            sure = wave_isum_dpp(sure);
+            eq = wave_isum_dpp(eq);
+            if (lane == 0) {
+                before[0] = sure + min(s0, q.sink) + max(0, s0 - z);
+                before[1] = eq;
+            }
+        }
+        // the lowest level's ranks above the cut in those segments
+        const uint32_t* hl = h0 + (size_t)2 * kSegs * kBins;
+        int low_above = 0;
+        if (choose)
+            for (int s = 0; s < sg; s++)
+                for (int bn = tid; bn < 1024; bn += kSelThreads)
+                    if (bn > (int)(cut & 1023)) low_above += hl[(size_t)s * kBins + bn];
+        low_above = wave_isum_dpp(low_above);
+        if (lane == 0) scan[wave] = low_above;
+        // this segment: each wavefront its stretch
+        const int per = (q.seg + kSelWaves * 64 - 1) / (kSelWaves * 64) * 64;
+        const int a = s0 + wave * per, e = min(s1, a + per);
+        int above = 0, equal = 0;
+        for (int i0 = a; i0 < e; i0 += 64) {
+            const int i = i0 + lane;
+            const bool in = i < e, cand = in && i >= q.sink && i < z;
+            const uint32_t r = cand ? rank_of(wr[i]) : 0u;
+            above += __popcll(__ballot(in && (!cand || (choose && r > cut))));
+            equal += __popcll(__ballot(cand && choose && r == cut));
+        }
+        __syncthreads();
+        if (lane == 0) { cnt2[wave][0] = above; cnt2[wave][1] = equal; }
+        __syncthreads();
+        int at = before[0], eqs = before[1];
+        for (int k = 0; k < kSelWaves; k++) {
+            at += (int)scan[k];
+            if (k < wave) {
+                at += cnt2[k][0];
+                eqs += cnt2[k][1];
+            }
+        }
+        at += min(eqs, (int)need);
+        emit_kept(kr, a, e, q.sink, z, cut, choose, at, eqs, (int)need, lane,
+                  [&](int i, int, bool cand) { return cand ? rank_of(wr[i]) : 0u; });
+    }
+}
+
+// Moves the kept positions.  256 threads gather a page of the destination into
+// LDS and write it; a block has GROUPS such groups.  Not in place (GROUPS 1) a
+// block is one page.  In place a block takes all pages of its (KV head,
+// sequence) in order, GROUPS at a time: a kept position never lies before its
+// destination, so page p's sources are in pages >= p, and a page is written
+// only after it and the pages before it have been gathered.
+template <int GROUPS>
+__global__ __launch_bounds__(256 * GROUPS) void kv4_move(Kv4 src, Kv4 dst, const float* w_src, float* w_dst, int budget,
+                                                         const int32_t* __restrict__ kept) {
+    extern __shared__ __align__(16) uint8_t bufs[];      // GROUPS x 72 hd bytes
+    __shared__ int from[GROUPS][kPage];
+    __shared__ const uint8_t* page[GROUPS][kPage];       // the source's part of its page, null where there is none
+    const int hd = src.hd, hdg = hd / 64, tid = threadIdx.x & 255, grp = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    uint8_t* const buf = bufs + (size_t)grp * 72 * hd;
     int b = blockIdx.x;
-    const int p0 = serial ? 0 : b % dst.max_pages;
-    if (!serial) b /= dst.max_pages;
+    const int p0 = GROUPS > 1 ? 0 : b % dst.max_pages;
+    if (GROUPS == 1) b /= dst.max_pages;
     const int h = b % src.n_kv, seq = b / src.n_kv;
     const int32_t* kr = kept + ((size_t)seq * src.n_kv + h) * budget;
     const float* ws = w_src + ((size_t)seq * src.n_kv + h) * src.max_pages * kPage;
     float* wd = w_dst + ((size_t)seq * src.n_kv + h) * dst.max_pages * kPage;
-    if (tid == 0 && p0 == 0 && h == 0 && kr[0] < 0) dst.lens[seq] = 0;
-    const int p1 = serial ? dst.max_pages : p0 + 1;
-    for (int p = p0; p < p1; p++) {
-        __syncthreads();
+    const int p1 = GROUPS > 1 ? dst.max_pages : p0 + 1;
+    if (p0 == 0 && h == 0 && threadIdx.x == 0 && kr[0] < 0) dst.lens[seq] = 0;
+    for (int pb = p0; pb < p1; pb += GROUPS) {
+        const int p = pb + grp;
+        float wt = 0.f;
         if (tid < kPage) {
             const int i = p * kPage + tid;
-            const int f = i < budget ? kr[i] : -1;
-            from[tid] = f;
-            wt[tid] = f >= 0 ? ws[f] : 0.f;
-            if (h == 0 && f >= 0 && (i + 1 == budget || kr[i + 1] < 0)) dst.lens[seq] = i + 1;
+            const int f = p < p1 && i < budget ? kr[i] : -1;
+            const uint8_t* pg = nullptr;
+            if (f >= 0) {
+                pg = page_at(src, seq, f / kPage, h);
+                wt = ws[f];
+                if (!pg) raise_table();
+                if (h == 0 && (i + 1 == budget || kr[i + 1] < 0)) dst.lens[seq] = i + 1;
+            }
+            from[grp][tid] = f;
+            page[grp][tid] = pg;
         }
         __syncthreads();
-        if (from[0] >= 0) {
-            bool bad = false;
-            // keys: 8-byte pieces (position, 16 dims); pairs of both sides
-            for (int i = tid; i < kPage * hdg * 4; i += 256) {
-                const int t = i & 63, pc = i >> 6, f = from[t];
-                uint2 x = make_uint2(0u, 0u);
-                if (f >= 0) {
-                    const uint8_t* pg = page_at(src, seq, f / kPage, h);
-                    if (pg) x = *(const uint2*)(pg + key_off(f & 63, pc >> 2, pc & 3, hdg));
+        const bool some = from[grp][0] >= 0;
+        if (some) {
+            // keys: 16 bytes of a chunk hold 16 dims of positions 32 u + n and 32 u + 16 + n
+            for (int i = tid; i < 128 * hdg; i += 256) {
+                const int ln = i & 63, g = (i >> 6) % hdg, u = (i >> 6) / hdg;
+                uint2 x[2];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const int t = 32 * u + 16 * k + (ln & 15);
+                    const uint8_t* pg = page[grp][t];
+                    x[k] = pg ? *(const uint2*)(pg + key_off(from[grp][t] & 63, g, ln >> 4, hdg)) : make_uint2(0u, 0u);
                 }
-                *(uint2*)(buf + key_off(t, pc >> 2, pc & 3, hdg)) = x;
+                *(uint4*)(buf + (u * hdg + g) * 1024 + ln * 16) = make_uint4(x[0].x, x[0].y, x[1].x, x[1].y);
             }
             for (int i = tid; i < kPage * hdg * 2; i += 256) {
-                const int t = i & 63, g = (i >> 6) % hdg, side = (i >> 6) / hdg, f = from[t];
+                const int t = i & 63, g = (i >> 6) % hdg, side = (i >> 6) / hdg, f = from[grp][t];
+                const uint8_t* pg = page[grp][t];
                 uint32_t x = 0;
-                if (f >= 0) {
-                    const uint8_t* pg = page_at(src, seq, f / kPage, h);
-                    bad |= !pg;
-                    x = pg ? ((const uint32_t*)(pg + (32 + 36 * side) * hd))[g * 64 + slot_of(f & 63)] : 0x7e007e00u;
-                }
+                if (f >= 0) x = pg ? ((const uint32_t*)(pg + (32 + 36 * side) * hd))[g * 64 + slot_of(f & 63)] : 0x7e007e00u;
                 ((uint32_t*)(buf + (32 + 36 * side) * hd))[g * 64 + slot_of(t)] = x;
             }
-            // values: a word of eight positions of one dim
-            for (int i = tid; i < hd * 8; i += 256) {
-                const int d = i % hd, r = i / hd;
-                uint32_t x = 0;
+            // values: a word holds eight positions of one dim; the positions
+            // are the same for a wavefront, whose lanes are 64 dims
+#pragma unroll
+            for (int rr = 0; rr < 2; rr++) {
+                const int r = wave + 4 * rr;
+                const uint8_t* base[8];
+                int shift[8];
+#pragma unroll
                 for (int k = 0; k < 8; k++) {
-                    const int t = 16 * (k >> 1) + 2 * r + (k & 1), f = from[t];
-                    if (f < 0) continue;
-                    const uint8_t* pg = page_at(src, seq, f / kPage, h);
-                    if (!pg) continue;
-                    const uint32_t cd = pg[36 * hd + val_off(d, (f & 15) >> 1) + ((f & 63) >> 4)] >> (4 * (f & 1)) & 15;
-                    x |= cd << (8 * (k >> 1) + 4 * (k & 1));
+                    const int t = 16 * (k >> 1) + 2 * r + (k & 1), f = __builtin_amdgcn_readfirstlane(from[grp][t]);
+                    const uint64_t pg = (uint64_t)page[grp][t];
+                    const uint64_t u = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)pg) |
+                                       (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(pg >> 32)) << 32;
+                    // position f's byte of dim 0
+                    base[k] = u ? (const uint8_t*)u + 36 * hd + val_off(0, (f & 15) >> 1) + ((f & 63) >> 4) : nullptr;
+                    shift[k] = 4 * (f & 1);
                 }
-                *(uint32_t*)(buf + 36 * hd + val_off(d, r)) = x;
+                for (int g = 0; g < hdg; g++) {
+                    const int d = 64 * g + lane;
+                    const unsigned off = val_off(d, 0);
+                    uint32_t x = 0;
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        if (base[k]) x |= ((uint32_t)base[k][off] >> shift[k] & 15u) << (8 * (k >> 1) + 4 * (k & 1));
+                    *(uint32_t*)(buf + 36 * hd + val_off(d, r)) = x;
+                }
             }
-            if (bad) raise_table();
         }
         __syncthreads();
-        if (from[0] >= 0) {
+        if (some) {
             uint8_t* pg = page_at(dst, seq, p, h);
             if (pg) {
                 for (int i = tid; i < 72 * hd / 16; i += 256) ((uint4*)pg)[i] = ((const uint4*)buf)[i];
@@ -1069,7 +1276,8 @@ __global__ __launch_bounds__(256) void kv4_move(Kv4 src, Kv4 dst, const float* w
                 raise_table();
             }
         }
-        if (tid < kPage) wd[p * kPage + tid] = wt[tid];
+        if (tid < kPage && p < p1) wd[p * kPage + tid] = wt;
+        if (GROUPS > 1) __syncthreads();
     }
 }
 
@@ -1217,11 +1425,11 @@ extern "C" int ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float*
         return IBH_ERROR_PARAM;
     }
     const AttnPlan p = attn_plan(cache, n_heads, n_q, weights_out != nullptr);
-    if (!ws) {
+    if (!ws && p.bytes) {
         ws = ibh_workspace(p.bytes);
         ws_bytes = ws ? p.bytes : 0;
     }
-    if (!ws || ws_bytes < p.bytes || ((uintptr_t)ws & 15)) {
+    if (p.bytes && (!ws || ws_bytes < p.bytes || ((uintptr_t)ws & 15))) {
         ibh_set_error("ibh_kv4_attn: workspace of %zu bytes on 16 bytes needed", p.bytes);
         return IBH_ERROR_MEMORY;
     }
@@ -1246,8 +1454,16 @@ extern "C" int ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float*
     return IBH_OK;
 }
 
+static bool select_in_one(const ibh_kv4_cache* c) { return (int64_t)c->max_pages * kPage <= kSelMost; }
+
+extern "C" size_t ibh_kv4_evict_workspace_bytes(const ibh_kv4_cache* cache) {
+    if (!cache || cache->n_seq <= 0 || cache->n_kv <= 0 || cache->max_pages <= 0 || select_in_one(cache)) return 0;
+    return (size_t)cache->n_seq * cache->n_kv * kSegs * (3 * kBins + 2) * sizeof(uint32_t);
+}
+
 extern "C" int ibh_kv4_evict(const ibh_kv4_cache* src, const ibh_kv4_cache* dst, const float* weights_src,
-                             float* weights_dst, int budget, int sink, int recent, int32_t* kept, void* stream) {
+                             float* weights_dst, int budget, int sink, int recent, int32_t* kept, void* ws,
+                             size_t ws_bytes, void* stream) {
     if (!cache_ok(src, "ibh_kv4_evict (from)") || !cache_ok(dst, "ibh_kv4_evict (to)")) return IBH_ERROR_PARAM;
     if (!weights_src || !weights_dst || !kept || budget <= 0 || sink < 0 || recent < 0 || sink > budget ||
         recent > budget - sink || (size_t)budget > (size_t)dst->max_pages * kPage || src->n_seq != dst->n_seq ||
@@ -1264,14 +1480,45 @@ extern "C" int ibh_kv4_evict(const ibh_kv4_cache* src, const ibh_kv4_cache* dst,
                       "the pool differ");
         return IBH_ERROR_PARAM;
     }
+    const size_t need = ibh_kv4_evict_workspace_bytes(src);
+    if (!ws && need) {
+        ws = ibh_workspace(need);
+        ws_bytes = ws ? need : 0;
+    }
+    if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15))) {
+        ibh_set_error("ibh_kv4_evict: workspace of %zu bytes on 16 bytes needed", need);
+        return IBH_ERROR_MEMORY;
+    }
     const size_t heads = (size_t)src->n_seq * src->n_kv;
     const size_t blocks = heads * (in_place ? 1 : dst->max_pages);
-    if (!grid_ok(blocks, "ibh_kv4_evict")) return IBH_ERROR_PARAM;
+    if (!grid_ok(blocks, "ibh_kv4_evict") || !grid_ok(heads * kSegs, "ibh_kv4_evict")) return IBH_ERROR_PARAM;
     hipStream_t st = ibh_resolve_stream(stream);
-    kv4_select<<<(unsigned)heads, kSelThreads, 0, st>>>(device_of(src), weights_src, budget, sink, recent, kept);
+    const Kv4 s = device_of(src), d = device_of(dst);
+    if (!need) {
+        kv4_select<<<(unsigned)heads, kSelThreads, 0, st>>>(s, weights_src, budget, sink, recent, kept);
+    } else {
+        LongSel q;
+        q.hist = (uint32_t*)ws;
+        q.above = q.hist + heads * 3 * kSegs * kBins;
+        // at least 4096 positions a segment: shorter ones cost more in adding up counts than they save
+        q.seg = max(4096, ((src->max_pages + kSegs - 1) / kSegs) * kPage);
+        q.n_seg = (int)(((int64_t)src->max_pages * kPage + q.seg - 1) / q.seg);
+        q.budget = budget;
+        q.sink = sink;
+        q.recent = recent;
+        const unsigned grid = (unsigned)(heads * q.n_seg);
+        kv4_select_long<0><<<grid, kSelThreads, 0, st>>>(s, q, weights_src, kept);
+        kv4_select_long<1><<<grid, kSelThreads, 0, st>>>(s, q, weights_src, kept);
+        kv4_select_long<2><<<grid, kSelThreads, 0, st>>>(s, q, weights_src, kept);
+        kv4_select_long<3><<<grid, kSelThreads, 0, st>>>(s, q, weights_src, kept);
+    }
     IBH_CHECK_LAUNCH("ibh_kv4_evict (select)");
-    kv4_move<<<(unsigned)blocks, 256, 72 * src->head_dim, st>>>(device_of(src), device_of(dst), weights_src,
-                                                                weights_dst, budget, kept, in_place ? 1 : 0);
+    if (in_place && src->head_dim > 192)                 // as many groups as 64 KB of LDS hold
+        kv4_move<2><<<(unsigned)blocks, 512, 2 * 72 * src->head_dim, st>>>(s, d, weights_src, weights_dst, budget, kept);
+    else if (in_place)
+        kv4_move<4><<<(unsigned)blocks, 1024, 4 * 72 * src->head_dim, st>>>(s, d, weights_src, weights_dst, budget, kept);
+    else
+        kv4_move<1><<<(unsigned)blocks, 256, 72 * src->head_dim, st>>>(s, d, weights_src, weights_dst, budget, kept);
     IBH_CHECK_LAUNCH("ibh_kv4_evict (move)");
     return IBH_OK;
 }

@@ -198,19 +198,24 @@ def kv4_attn(out, q, cache: Kv4Cache, n_heads: int, weights_in=None, weights_out
         wi, wo = (cache._on(w, torch.float32, size) for w in (weights_in, weights_out))
     if ws is None:
         need = lib().ibh_kv4_attn_workspace_bytes(cache.ref, n_heads, n_q, wi is not None)
-        ws = torch.empty(need, dtype=torch.uint8, device=cache.device)
-    cache._call("ibh_kv4_attn", cache.ref, po, pq, n_heads, n_q, sq, wi, wo, cache._on(ws), ws.numel())
+        ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+    cache._call("ibh_kv4_attn", cache.ref, po, pq, n_heads, n_q, sq, wi, wo, None if ws is None else cache._on(ws),
+                0 if ws is None else ws.numel())
 
 
 def kv4_evict(src: Kv4Cache, dst: Kv4Cache, weights_src, weights_dst, budget: int, sink: int, recent: int,
-              kept) -> None:
+              kept, ws=None) -> None:
     """Cuts every sequence to `budget` positions by accumulated weight: rows, weights and lengths into dst (src itself
     for in place), the kept positions into kept int32 [n_seq, n_kv, budget]."""
     n = src.n_seq * src.n_kv
+    if ws is None:
+        need = lib().ibh_kv4_evict_workspace_bytes(src.ref)
+        ws = torch.empty(need, dtype=torch.uint8, device=src.device) if need else None
     src._call("ibh_kv4_evict", src.ref, dst.ref,
               src._on(weights_src, torch.float32, n * src.max_pages * KV4_PAGE),
               src._on(weights_dst, torch.float32, n * dst.max_pages * KV4_PAGE), budget, sink, recent,
-              src._on(kept, torch.int32, n * budget))
+              src._on(kept, torch.int32, n * budget), None if ws is None else src._on(ws),
+              0 if ws is None else ws.numel())
 
 
 class PqDeviceTensor:

@@ -65,8 +65,8 @@ def test_bad_caches_are_refused(bad):
     refused("ibh_kv4_append", c, 4096, 4096, 1, 128, None)
     refused("ibh_kv4_read", c, 4096, 4096, 1, 128, None)
     refused("ibh_kv4_attn", c, 4096, 4096, 4, 1, 256, None, None, 4096, 1 << 30, None)
-    refused("ibh_kv4_evict", c, C.byref(desc(table=8192, lens=8192)), 4096, 8192, 64, 0, 0, 4096, None)
-    refused("ibh_kv4_evict", C.byref(desc(table=8192, lens=8192)), c, 4096, 8192, 64, 0, 0, 4096, None)
+    refused("ibh_kv4_evict", c, C.byref(desc(table=8192, lens=8192)), 4096, 8192, 64, 0, 0, 4096, None, 0, None)
+    refused("ibh_kv4_evict", C.byref(desc(table=8192, lens=8192)), c, 4096, 8192, 64, 0, 0, 4096, None, 0, None)
 
 
 def test_bad_arguments_are_refused():
@@ -79,11 +79,13 @@ def test_bad_arguments_are_refused():
     for bad in (dict(out=0), dict(q=0), dict(heads=0), dict(heads=3), dict(heads=-2), dict(n_q=0), dict(stride=255),
                 dict(wi=4096), dict(wo=4096)):
         refused("ibh_kv4_attn", *attn(**bad))
+    c = C.byref(desc(max_pages=64))                              # long enough for splits, so for a workspace
     refused("ibh_kv4_attn", *attn(size=1), code=-3)
     refused("ibh_kv4_attn", *attn(ws=4100), code=-3)
+    c = C.byref(desc())
     to = C.byref(desc(table=8192, lens=8192))
     evict = lambda src=c, dst=to, ws=4096, wd=8192, budget=64, sink=0, recent=0, kept=4096: (
-        src, dst, ws, wd, budget, sink, recent, kept, None)
+        src, dst, ws, wd, budget, sink, recent, kept, None, 0, None)
     for bad in (dict(ws=0), dict(wd=0), dict(kept=0), dict(budget=0), dict(budget=129), dict(sink=-1), dict(recent=-1),
                 dict(sink=65), dict(sink=33, recent=32), dict(dst=C.byref(desc(table=8192, lens=8192, n_kv=4))),
                 dict(dst=C.byref(desc(table=8192, lens=8192, head_dim=128))),
@@ -98,7 +100,12 @@ def test_sizes():
     assert L.ibh_kv4_page_bytes(8, 128) == 8 * 9216
     for kv, hd in ((0, 128), (8, 96), (8, 0), (-1, 64), (8, 320)):
         assert L.ibh_kv4_page_bytes(kv, hd) == 0
-    assert L.ibh_kv4_attn_workspace_bytes(C.byref(desc()), 4, 1, 0) > 0
+    assert L.ibh_kv4_attn_workspace_bytes(C.byref(desc(max_pages=64)), 4, 1, 0) > 0
+    assert L.ibh_kv4_evict_workspace_bytes(C.byref(desc())) == 0
+    assert L.ibh_kv4_evict_workspace_bytes(C.byref(desc(max_pages=257))) > 0
+    long = desc(max_pages=257), desc(max_pages=257, table=8192, lens=8192)
+    refused("ibh_kv4_evict", C.byref(long[0]), C.byref(long[1]), 4096, 8192, 64, 0, 0, 4096, 4096, 1, None, code=-3)
+    refused("ibh_kv4_evict", C.byref(long[0]), C.byref(long[1]), 4096, 8192, 64, 0, 0, 4096, 4100, 1 << 30, None, code=-3)
     assert L.ibh_kv4_attn_workspace_bytes(C.byref(desc()), 0, 1, 1) == 0
 
 

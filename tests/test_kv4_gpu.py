@@ -303,7 +303,8 @@ def test_attention_bad_pages_are_reported(ops):
 EVICT = [  # kv heads, head_dim, lengths, budget, sink, recent
     (1, 64, [1], 1, 0, 0), (2, 64, [65, 64, 0, 200], 64, 4, 20), (1, 128, [1000], 130, 0, 0), (2, 128, [700, 63], 65, 65, 0),
     (1, 192, [300], 100, 0, 100), (1, 256, [129, 500], 128, 7, 121), (3, 64, [3000, 100], 1025, 4, 300), (1, 64, [70], 1, 0, 0),
-    (2, 64, [2500], 2200, 1, 64),
+    (2, 64, [2500], 2200, 1, 64), (1, 64, [16385, 90], 64, 1, 7), (2, 64, [20000, 16384, 0], 4500, 4, 300),
+    (1, 64, [40000], 40000, 0, 0), (1, 64, [33000], 100, 60, 40),
 ]
 
 
