@@ -916,35 +916,51 @@ constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
 constexpr int kSelKeys = 16;                             // ranks a thread of the one-block selection holds
 constexpr int kSelMost = kSelThreads * kSelKeys;         // longest row of it
 
-// Emits the kept positions of a wavefront's stretch a .. e - 1 in order: those
-// not for choice (before sink, from z on), those above `cut`, and of those
-// equal to it the ones whose count among all equals is below `equals`.
-template <class Rank>
-__device__ __forceinline__ void emit_kept(int32_t* kr, int a, int e, int sink, int z, uint32_t cut, bool choose,
-                                          int at, int eqs, int equals, int lane, Rank rank) {
-    const unsigned long long low = (1ull << lane) - 1;
-    for (int i0 = a, j = 0; i0 < e; i0 += 64, j++) {
-        const int i = i0 + lane;
-        const bool in = i < e, cand = in && i >= sink && i < z;
-        const uint32_t r = rank(i, j, cand);
-        const bool eq = cand && choose && r == cut;
-        const unsigned long long be = __ballot(eq);
-        const bool keep = in && (!cand || (choose && r > cut) || (eq && eqs + __popcll(be & low) < equals));
-        const unsigned long long bk = __ballot(keep);
-        if (keep) kr[at + __popcll(bk & low)] = i;
-        at += __popcll(bk);
-        eqs += __popcll(be);
+constexpr int kBins = 2048;
+__device__ __forceinline__ int bin_shift(int level) { return level == 0 ? 21 : level == 1 ? 10 : 0; }
+__device__ __forceinline__ uint32_t bin_of(uint32_t rank, int level) {
+    return (rank >> bin_shift(level)) & (level == 2 ? 1023u : 2047u);
+}
+
+// The bin that holds the need-th largest: thread t brings the counts of bins
+// hi = 2046 - 2 t (lo) and hi + 1 (up).  Returns the bin and takes what lies
+// above it off `need`.  Two barriers before the result is read, none after.
+struct BinPick {
+    uint32_t scan[kSelWaves];
+    uint32_t found[2];
+};
+__device__ __forceinline__ uint32_t pick_bin(BinPick& sh, uint32_t lo, uint32_t up, uint32_t& need) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = kBins - 2 * (tid + 1);
+    uint32_t run = lo + up;                              // counts of this thread's bins and all higher ones
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t v = __shfl_up(run, o, kWave);
+        if (lane >= o) run += v;
     }
+    if (lane == 63) sh.scan[wave] = run;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSelWaves; k++) run += k < wave ? sh.scan[k] : 0u;
+    const uint32_t higher = run - (lo + up);
+    if (higher < need && run >= need) {                  // one thread
+        const bool top = higher + up >= need;
+        sh.found[0] = top ? hi + 1 : hi;
+        sh.found[1] = top ? higher : higher + up;
+    }
+    __syncthreads();
+    need -= sh.found[1];
+    return sh.found[0];
 }
 
 // Rows of up to 16384 positions: block (KV head, sequence), the ranks in
-// registers.  The need-th largest is built bit by bit from the top: a bit
-// stays set while at least `need` ranks are no smaller (a ballot a register, a
-// wave's count in LDS, one barrier a bit), which takes no atomics and the
-// same time for any distribution.
+// registers.  Their top 11, middle 11 and low 10 bits in turn are counted in
+// LDS among the ranks that share the bits found before, which gives the
+// need-th largest rank and how many of those equal to it are kept.  (Bit by
+// bit with ballots and a barrier a bit took 21 us at 4096 positions.)
 __global__ __launch_bounds__(kSelThreads) void kv4_select(Kv4 c, const float* __restrict__ w, int budget, int sink,
                                                           int recent, int32_t* __restrict__ kept) {
-    __shared__ int cnt[2][kSelWaves];
+    __shared__ __align__(16) uint32_t hist[kBins];
+    __shared__ BinPick bp;
     __shared__ int cnt2[kSelWaves][2];
     const int seq = blockIdx.x / c.n_kv;
     bool bad;
@@ -961,27 +977,29 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select(Kv4 c, const float* __
     const int need = budget - sink - recent;
     const int per = (len + kSelWaves * 64 - 1) / (kSelWaves * 64) * 64;   // positions of a wavefront
     const int a = wave * per, e = min(len, a + per);
-    uint32_t key[kSelKeys];                              // 0 where nothing is to choose: never counted, a bit is set in every trial
+    uint32_t key[kSelKeys];
 #pragma unroll
     for (int j = 0; j < kSelKeys; j++) {
         const int i = a + 64 * j + lane;
         key[j] = i < e && i >= sink && i < z ? rank_of(wr[i]) : 0u;
     }
-    uint32_t cut = 0;
+    uint32_t cut = 0, left = need;
     const bool choose = need > 0;
     if (choose)
-        for (int bit = 31; bit >= 0; bit--) {
-            const uint32_t trial = cut | (1u << bit);
-            int n = 0;
 #pragma unroll
-            for (int j = 0; j < kSelKeys; j++)
-                if (64 * j < per) n += __popcll(__ballot(key[j] >= trial));
-            if (lane == 0) cnt[bit & 1][wave] = n;
+        for (int lv = 0; lv < 3; lv++) {
+            for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
             __syncthreads();
-            int sum = 0;
+            const uint32_t known = lv == 0 ? 0u : lv == 1 ? ~0u << 21 : ~0u << 10;
 #pragma unroll
-            for (int k = 0; k < kSelWaves; k++) sum += cnt[bit & 1][k];
-            if (sum >= need) cut = trial;
+            for (int j = 0; j < kSelKeys; j++) {
+                const int i = a + 64 * j + lane;
+                if (64 * j < per && i < e && i >= sink && i < z && (key[j] & known) == cut)
+                    atomicAdd(&hist[bin_of(key[j], lv)], 1u);
+            }
+            __syncthreads();
+            const uint2 v = *(const uint2*)&hist[kBins - 2 * (tid + 1)];
+            cut |= pick_bin(bp, v.x, v.y, left) << bin_shift(lv);
         }
     int above = 0, equal = 0;
 #pragma unroll
@@ -1021,28 +1039,26 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select(Kv4 c, const float* __
 }
 
 // Longer rows: up to 32 blocks a row, each with its own segment, in four
-// launches.  Launch 0, 1, 2 count the segment's ranks by their top 11, middle
-// 11 and low 10 bits, among those whose higher bits are the cut's; every block
-// of the next launch adds up the segments' counts and finds the next bits of
-// the cut for itself.  Launch 3 counts what the segments before its own keep
-// from the same counts, and emits.
-constexpr int kSegs = 32, kBins = 2048;
+// launches.  Launches 0, 1, 2 count a segment's ranks by their top 11, middle
+// 11 and low 10 bits, among those that share the bits found before; every
+// block of the next launch adds up the segments' counts and so finds the next
+// bits for itself.  Launch 3 takes what the segments before its own keep from
+// the same counts, and emits.
+constexpr int kSegs = 32;
 struct LongSel {
-    uint32_t* hist;                                      // [row][launch 0..2][segment][kBins]
-    uint32_t* above;                                     // [row][launch 1, 2][segment] ranks above the cut's bits so far, in its group
+    uint32_t* hist;                                      // [row][launch 0, 1, 2][segment][kBins]
+    uint32_t* above;                                     // [row][launch 1, 2][segment] ranks that the bits found last put above the cut
+    uint32_t* state;                                     // [row][launch 1, 2][2] cut and need behind that launch
     int seg, n_seg;                                      // positions of a segment, segments of a row
     int budget, sink, recent;
 };
-__device__ __forceinline__ int bin_shift(int level) { return level == 0 ? 21 : level == 1 ? 10 : 0; }
 
 template <int LEVEL>
 __global__ __launch_bounds__(kSelThreads) void kv4_select_long(Kv4 c, LongSel q, const float* __restrict__ w,
                                                                int32_t* __restrict__ kept) {
-    __shared__ uint32_t hist[kBins];
-    __shared__ uint32_t scan[kSelWaves];
-    __shared__ uint32_t found[2];
-    __shared__ int cnt2[kSelWaves][2];
-    __shared__ int before[2];
+    __shared__ __align__(16) uint32_t hist[LEVEL < 3 ? kBins : 4];
+    __shared__ BinPick bp;
+    __shared__ int cnt2[kSelWaves][3];
     const int row = blockIdx.x / q.n_seg, sg = blockIdx.x % q.n_seg, seq = row / c.n_kv;
     bool bad;
     const int len = seq_len(c, seq, &bad);
@@ -1059,58 +1075,50 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_long(Kv4 c, LongSel q,
     const int z = len - q.recent, segs = (len + q.seg - 1) / q.seg;
     if (sg >= segs) return;
     const float* wr = w + (size_t)row * c.max_pages * kPage;
-    uint32_t need = q.budget - q.sink - q.recent;
+    uint32_t need = q.budget - q.sink - q.recent, cut = 0;
     const bool choose = need > 0;
     uint32_t* const h0 = q.hist + (size_t)row * 3 * kSegs * kBins;
     uint32_t* const ab = q.above + (size_t)row * 2 * kSegs;
-    uint32_t cut = 0;                                    // the bits found so far
-    // levels before this launch's: add the segments up, find the bin in which
-    // the need-th largest lies
-    if (choose)
-#pragma unroll
-        for (int lv = 0; lv < LEVEL; lv++) {
-            constexpr int PB = kBins / kSelThreads;      // bins a thread adds up, highest first over the threads
-            const uint32_t* hl = h0 + (size_t)lv * kSegs * kBins;
-            const int hi = kBins - PB * (tid + 1);
-            uint32_t v[PB] = {};
-            for (int s = 0; s < segs; s++) {
-                const uint2 x = *(const uint2*)(hl + (size_t)s * kBins + hi);
-                v[0] += x.x;
-                v[1] += x.y;
-            }
-            static_assert(PB == 2, "bins a thread");
-            const uint32_t mine = v[0] + v[1];
-            uint32_t run = mine;                         // counts of this thread's bins and all higher ones
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const uint32_t up = __shfl_up(run, o, kWave);
-                if (lane >= o) run += up;
-            }
-            __syncthreads();
-            if (lane == 63) scan[wave] = run;
-            __syncthreads();
-            for (int k = 0; k < wave; k++) run += scan[k];
-            const uint32_t higher = run - mine;
-            if (higher < need && run >= need) {          // one thread
-                const bool top = higher + v[1] >= need;
-                found[0] = top ? hi + 1 : hi;
-                found[1] = top ? higher : higher + v[1];
-            }
-            __syncthreads();
-            cut |= found[0] << bin_shift(lv);
-            need -= found[1];
+    uint32_t* const st = q.state + (size_t)row * 4;
+    int low_before = 0;                                  // ranks of earlier segments that the low bits put above the cut
+    if (LEVEL > 0 && choose) {
+        if (LEVEL > 1) {
+            cut = st[2 * (LEVEL - 2)];
+            need = st[2 * (LEVEL - 2) + 1];
         }
+        const int hi = kBins - 2 * (tid + 1);
+        const uint32_t* hl = h0 + (size_t)(LEVEL - 1) * kSegs * kBins + hi;
+        uint32_t lo = 0, up = 0, lo_b = 0, up_b = 0;
+#pragma unroll 8
+        for (int s = 0; s < segs; s++) {
+            const uint2 x = *(const uint2*)(hl + (size_t)s * kBins);
+            lo += x.x;
+            up += x.y;
+            if (LEVEL == 3 && s < sg) {
+                lo_b += x.x;
+                up_b += x.y;
+            }
+        }
+        const uint32_t bin = pick_bin(bp, lo, up, need);
+        cut |= bin << bin_shift(LEVEL - 1);
+        if (LEVEL == 3) low_before = (hi > (int)bin ? lo_b : 0u) + (hi + 1 > (int)bin ? up_b : 0u);
+        else if (sg == 0 && tid == 0) {
+            st[2 * (LEVEL - 1)] = cut;
+            st[2 * (LEVEL - 1) + 1] = need;
+        }
+    }
     if constexpr (LEVEL < 3) {
         for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
         __syncthreads();
         constexpr uint32_t known = LEVEL == 0 ? 0u : LEVEL == 1 ? ~0u << 21 : ~0u << 10;
         constexpr uint32_t group = LEVEL <= 1 ? 0u : ~0u << 21;   // bits that the launch before knew
         int over = 0;
+#pragma unroll 4
         for (int i0 = s0 + wave * 64; i0 < s1; i0 += kSelThreads) {
             const int i = i0 + lane;
             const bool cand = i < s1 && i >= q.sink && i < z && choose;
             const uint32_t r = cand ? rank_of(wr[i]) : 0u;
-            if (cand && (r & known) == cut) atomicAdd(&hist[(r >> bin_shift(LEVEL)) & (kBins - 1) & (LEVEL == 2 ? 1023 : 2047)], 1u);
+            if (cand && (r & known) == cut) atomicAdd(&hist[bin_of(r, LEVEL)], 1u);
             if (LEVEL > 0) over += __popcll(__ballot(cand && (r & known) > cut && (r & group) == (cut & group)));
         }
         if (LEVEL > 0 && lane == 0) cnt2[wave][0] = over;
@@ -1125,34 +1133,18 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_long(Kv4 c, LongSel q,
     } else {
         // what the segments before this one keep: all outside [sink, z), the
         // ranks above the cut, and the equal ones up to `need`
-        if (wave == 0) {
-            int sure = 0, eq = 0;
-            const uint32_t* hl = h0 + (size_t)2 * kSegs * kBins;
-            const uint32_t bin = cut & 1023;
-            for (int s = lane; choose && s < sg; s += 64) {
-                sure += ab[s] + ab[kSegs + s];
-                eq += hl[(size_t)s * kBins + bin];
-            }
-            sure = wave_isum_dpp(sure);
-            eq = wave_isum_dpp(eq);
-            if (lane == 0) {
-                before[0] = sure + min(s0, q.sink) + max(0, s0 - z);
-                before[1] = eq;
-            }
+        int sure = 0, eqs = 0;
+        if (lane < sg && choose) {                       // kSegs <= 64: every wavefront for itself
+            sure = ab[lane] + ab[kSegs + lane];
+            eqs = h0[((size_t)2 * kSegs + lane) * kBins + (cut & 1023)];
         }
-        // the lowest level's ranks above the cut in those segments
-        const uint32_t* hl = h0 + (size_t)2 * kSegs * kBins;
-        int low_above = 0;
-        if (choose)
-            for (int s = 0; s < sg; s++)
-                for (int bn = tid; bn < 1024; bn += kSelThreads)
-                    if (bn > (int)(cut & 1023)) low_above += hl[(size_t)s * kBins + bn];
-        low_above = wave_isum_dpp(low_above);
-        if (lane == 0) scan[wave] = low_above;
+        sure = wave_isum_dpp(sure);
+        eqs = wave_isum_dpp(eqs);
         // this segment: each wavefront its stretch
         const int per = (q.seg + kSelWaves * 64 - 1) / (kSelWaves * 64) * 64;
         const int a = s0 + wave * per, e = min(s1, a + per);
         int above = 0, equal = 0;
+#pragma unroll 4
         for (int i0 = a; i0 < e; i0 += 64) {
             const int i = i0 + lane;
             const bool in = i < e, cand = in && i >= q.sink && i < z;
@@ -1160,20 +1152,36 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_long(Kv4 c, LongSel q,
             above += __popcll(__ballot(in && (!cand || (choose && r > cut))));
             equal += __popcll(__ballot(cand && choose && r == cut));
         }
+        low_before = wave_isum_dpp(low_before);
+        if (lane == 0) {
+            cnt2[wave][0] = above;
+            cnt2[wave][1] = equal;
+            cnt2[wave][2] = low_before;
+        }
         __syncthreads();
-        if (lane == 0) { cnt2[wave][0] = above; cnt2[wave][1] = equal; }
-        __syncthreads();
-        int at = before[0], eqs = before[1];
+        int at = sure + min(s0, q.sink) + max(0, s0 - z);
         for (int k = 0; k < kSelWaves; k++) {
-            at += (int)scan[k];
+            at += cnt2[k][2];
             if (k < wave) {
                 at += cnt2[k][0];
                 eqs += cnt2[k][1];
             }
         }
         at += min(eqs, (int)need);
-        emit_kept(kr, a, e, q.sink, z, cut, choose, at, eqs, (int)need, lane,
-                  [&](int i, int, bool cand) { return cand ? rank_of(wr[i]) : 0u; });
+        const unsigned long long low = (1ull << lane) - 1;
+#pragma unroll 4
+        for (int i0 = a; i0 < e; i0 += 64) {
+            const int i = i0 + lane;
+            const bool in = i < e, cand = in && i >= q.sink && i < z;
+            const uint32_t r = cand ? rank_of(wr[i]) : 0u;
+            const bool eq = cand && choose && r == cut;
+            const unsigned long long be = __ballot(eq);
+            const bool keep = in && (!cand || (choose && r > cut) || (eq && eqs + __popcll(be & low) < (int)need));
+            const unsigned long long bk = __ballot(keep);
+            if (keep) kr[at + __popcll(bk & low)] = i;
+            at += __popcll(bk);
+            eqs += __popcll(be);
+        }
     }
 }
 
@@ -1183,13 +1191,14 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_long(Kv4 c, LongSel q,
 // sequence) in order, GROUPS at a time: a kept position never lies before its
 // destination, so page p's sources are in pages >= p, and a page is written
 // only after it and the pages before it have been gathered.
-template <int GROUPS>
+template <int GROUPS, int HDG>
 __global__ __launch_bounds__(256 * GROUPS) void kv4_move(Kv4 src, Kv4 dst, const float* w_src, float* w_dst, int budget,
                                                          const int32_t* __restrict__ kept) {
     extern __shared__ __align__(16) uint8_t bufs[];      // GROUPS x 72 hd bytes
     __shared__ int from[GROUPS][kPage];
     __shared__ const uint8_t* page[GROUPS][kPage];       // the source's part of its page, null where there is none
-    const int hd = src.hd, hdg = hd / 64, tid = threadIdx.x & 255, grp = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    constexpr int hd = 64 * HDG, hdg = HDG;
+    const int tid = threadIdx.x & 255, grp = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     uint8_t* const buf = bufs + (size_t)grp * 72 * hd;
     int b = blockIdx.x;
@@ -1220,52 +1229,66 @@ __global__ __launch_bounds__(256 * GROUPS) void kv4_move(Kv4 src, Kv4 dst, const
         __syncthreads();
         const bool some = from[grp][0] >= 0;
         if (some) {
-            // keys: 16 bytes of a chunk hold 16 dims of positions 32 u + n and 32 u + 16 + n
-            for (int i = tid; i < 128 * hdg; i += 256) {
-                const int ln = i & 63, g = (i >> 6) % hdg, u = (i >> 6) / hdg;
-                uint2 x[2];
+            // every load of the page first, then LDS.  Values: a word holds
+            // eight positions of one dim; the positions are the same for a
+            // wavefront, whose lanes are 64 dims.  A position that is not
+            // there reads the pool's first bytes and counts as zero.
+            uint8_t vb[2][8][HDG];
+            uint32_t vm[2][8];
+            int sh[2][8];
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const int t = 32 * u + 16 * k + (ln & 15);
-                    const uint8_t* pg = page[grp][t];
-                    x[k] = pg ? *(const uint2*)(pg + key_off(from[grp][t] & 63, g, ln >> 4, hdg)) : make_uint2(0u, 0u);
-                }
-                *(uint4*)(buf + (u * hdg + g) * 1024 + ln * 16) = make_uint4(x[0].x, x[0].y, x[1].x, x[1].y);
-            }
-            for (int i = tid; i < kPage * hdg * 2; i += 256) {
-                const int t = i & 63, g = (i >> 6) % hdg, side = (i >> 6) / hdg, f = from[grp][t];
-                const uint8_t* pg = page[grp][t];
-                uint32_t x = 0;
-                if (f >= 0) x = pg ? ((const uint32_t*)(pg + (32 + 36 * side) * hd))[g * 64 + slot_of(f & 63)] : 0x7e007e00u;
-                ((uint32_t*)(buf + (32 + 36 * side) * hd))[g * 64 + slot_of(t)] = x;
-            }
-            // values: a word holds eight positions of one dim; the positions
-            // are the same for a wavefront, whose lanes are 64 dims
-#pragma unroll
-            for (int rr = 0; rr < 2; rr++) {
-                const int r = wave + 4 * rr;
-                const uint8_t* base[8];
-                int shift[8];
+            for (int rr = 0; rr < 2; rr++)
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
-                    const int t = 16 * (k >> 1) + 2 * r + (k & 1), f = __builtin_amdgcn_readfirstlane(from[grp][t]);
+                    const int r = wave + 4 * rr, t = 16 * (k >> 1) + 2 * r + (k & 1);
+                    const int f = __builtin_amdgcn_readfirstlane(from[grp][t]);
                     const uint64_t pg = (uint64_t)page[grp][t];
                     const uint64_t u = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)pg) |
                                        (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(pg >> 32)) << 32;
                     // position f's byte of dim 0
-                    base[k] = u ? (const uint8_t*)u + 36 * hd + val_off(0, (f & 15) >> 1) + ((f & 63) >> 4) : nullptr;
-                    shift[k] = 4 * (f & 1);
+                    const uint8_t* base = u ? (const uint8_t*)u + 36 * hd + val_off(0, (f & 15) >> 1) + ((f & 63) >> 4) : src.pool;
+                    vm[rr][k] = u ? 15u : 0u;
+                    sh[rr][k] = 4 * (f & 1);
+#pragma unroll
+                    for (int g = 0; g < HDG; g++) vb[rr][k][g] = base[(unsigned)(u ? val_off(64 * g + lane, 0) : 0)];
                 }
-                for (int g = 0; g < hdg; g++) {
-                    const int d = 64 * g + lane;
-                    const unsigned off = val_off(d, 0);
+            // keys: 16 bytes of a chunk hold 16 dims of positions 32 u + n and 32 u + 16 + n
+            constexpr int KI = (128 * HDG + 255) / 256;
+            uint2 kx[KI][2];
+            uint32_t px[KI];
+#pragma unroll
+            for (int j = 0; j < KI; j++) {
+                const int i = tid + 256 * j, ln = i & 63, g = (i >> 6) % hdg, u = (i >> 6) / hdg;
+                kx[j][0] = kx[j][1] = make_uint2(0u, 0u);
+                px[j] = 0;
+                if (i >= 128 * HDG) continue;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const int t = 32 * u + 16 * k + (ln & 15);
+                    const uint8_t* pg = page[grp][t];
+                    if (pg) kx[j][k] = *(const uint2*)(pg + key_off(from[grp][t] & 63, g, ln >> 4, hdg));
+                }
+                const int t = ln, side = u, f = from[grp][t];   // pairs of both sides: the same indexes
+                const uint8_t* pg = page[grp][t];
+                if (f >= 0) px[j] = pg ? ((const uint32_t*)(pg + (32 + 36 * side) * hd))[g * 64 + slot_of(f & 63)] : 0x7e007e00u;
+            }
+#pragma unroll
+            for (int j = 0; j < KI; j++) {
+                const int i = tid + 256 * j, ln = i & 63, g = (i >> 6) % hdg, u = (i >> 6) / hdg;
+                if (i >= 128 * HDG) continue;
+                *(uint4*)(buf + (u * hdg + g) * 1024 + ln * 16) = make_uint4(kx[j][0].x, kx[j][0].y, kx[j][1].x, kx[j][1].y);
+                ((uint32_t*)(buf + (32 + 36 * u) * hd))[g * 64 + slot_of(ln)] = px[j];
+            }
+#pragma unroll
+            for (int rr = 0; rr < 2; rr++)
+#pragma unroll
+                for (int g = 0; g < HDG; g++) {
                     uint32_t x = 0;
 #pragma unroll
                     for (int k = 0; k < 8; k++)
-                        if (base[k]) x |= ((uint32_t)base[k][off] >> shift[k] & 15u) << (8 * (k >> 1) + 4 * (k & 1));
-                    *(uint32_t*)(buf + 36 * hd + val_off(d, r)) = x;
+                        x |= ((uint32_t)vb[rr][k][g] >> sh[rr][k] & vm[rr][k]) << (8 * (k >> 1) + 4 * (k & 1));
+                    *(uint32_t*)(buf + 36 * hd + val_off(64 * g + lane, wave + 4 * rr)) = x;
                 }
-            }
         }
         __syncthreads();
         if (some) {
@@ -1454,11 +1477,18 @@ extern "C" int ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float*
     return IBH_OK;
 }
 
+template <int HDG>
+static void launch_move(const Kv4& s, const Kv4& d, const float* ws, float* wd, int budget, const int32_t* kept,
+                        bool in_place, size_t blocks, hipStream_t st) {
+    constexpr int G = HDG > 3 ? 2 : 4;                   // as many groups as 64 KB of LDS hold
+    if (in_place) kv4_move<G, HDG><<<(unsigned)blocks, 256 * G, G * 72 * 64 * HDG, st>>>(s, d, ws, wd, budget, kept);
+    else kv4_move<1, HDG><<<(unsigned)blocks, 256, 72 * 64 * HDG, st>>>(s, d, ws, wd, budget, kept);
+}
 static bool select_in_one(const ibh_kv4_cache* c) { return (int64_t)c->max_pages * kPage <= kSelMost; }
 
 extern "C" size_t ibh_kv4_evict_workspace_bytes(const ibh_kv4_cache* cache) {
     if (!cache || cache->n_seq <= 0 || cache->n_kv <= 0 || cache->max_pages <= 0 || select_in_one(cache)) return 0;
-    return (size_t)cache->n_seq * cache->n_kv * kSegs * (3 * kBins + 2) * sizeof(uint32_t);
+    return (size_t)cache->n_seq * cache->n_kv * (kSegs * (3 * kBins + 2) + 4) * sizeof(uint32_t);
 }
 
 extern "C" int ibh_kv4_evict(const ibh_kv4_cache* src, const ibh_kv4_cache* dst, const float* weights_src,
@@ -1500,6 +1530,7 @@ extern "C" int ibh_kv4_evict(const ibh_kv4_cache* src, const ibh_kv4_cache* dst,
         LongSel q;
         q.hist = (uint32_t*)ws;
         q.above = q.hist + heads * 3 * kSegs * kBins;
+        q.state = q.above + heads * 2 * kSegs;
         // at least 4096 positions a segment: shorter ones cost more in adding up counts than they save
         q.seg = max(4096, ((src->max_pages + kSegs - 1) / kSegs) * kPage);
         q.n_seg = (int)(((int64_t)src->max_pages * kPage + q.seg - 1) / q.seg);
@@ -1513,12 +1544,12 @@ extern "C" int ibh_kv4_evict(const ibh_kv4_cache* src, const ibh_kv4_cache* dst,
         kv4_select_long<3><<<grid, kSelThreads, 0, st>>>(s, q, weights_src, kept);
     }
     IBH_CHECK_LAUNCH("ibh_kv4_evict (select)");
-    if (in_place && src->head_dim > 192)                 // as many groups as 64 KB of LDS hold
-        kv4_move<2><<<(unsigned)blocks, 512, 2 * 72 * src->head_dim, st>>>(s, d, weights_src, weights_dst, budget, kept);
-    else if (in_place)
-        kv4_move<4><<<(unsigned)blocks, 1024, 4 * 72 * src->head_dim, st>>>(s, d, weights_src, weights_dst, budget, kept);
-    else
-        kv4_move<1><<<(unsigned)blocks, 256, 72 * src->head_dim, st>>>(s, d, weights_src, weights_dst, budget, kept);
+    switch (src->head_dim / 64) {
+        case 1: launch_move<1>(s, d, weights_src, weights_dst, budget, kept, in_place, blocks, st); break;
+        case 2: launch_move<2>(s, d, weights_src, weights_dst, budget, kept, in_place, blocks, st); break;
+        case 3: launch_move<3>(s, d, weights_src, weights_dst, budget, kept, in_place, blocks, st); break;
+        default: launch_move<4>(s, d, weights_src, weights_dst, budget, kept, in_place, blocks, st); break;
+    }
     IBH_CHECK_LAUNCH("ibh_kv4_evict (move)");
     return IBH_OK;
 }
