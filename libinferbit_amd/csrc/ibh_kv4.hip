@@ -913,8 +913,7 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
 }
 
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
-constexpr int kSelKeys = 16;                             // ranks a thread of the one-block selection holds
-constexpr int kSelMost = kSelThreads * kSelKeys;         // longest row of it
+constexpr int kSelMost = kSelThreads * 16;               // longest row of the one-block selection: 16 ranks a thread
 
 constexpr int kBins = 2048;
 __device__ __forceinline__ int bin_shift(int level) { return level == 0 ? 21 : level == 1 ? 10 : 0; }
@@ -957,9 +956,10 @@ __device__ __forceinline__ uint32_t pick_bin(BinPick& sh, uint32_t lo, uint32_t 
 // LDS among the ranks that share the bits found before, which gives the
 // need-th largest rank and how many of those equal to it are kept.  (Bit by
 // bit with ballots and a barrier a bit took 21 us at 4096 positions.)
+template <int KEYS>
 __global__ __launch_bounds__(kSelThreads) void kv4_select(Kv4 c, const float* __restrict__ w, int budget, int sink,
                                                           int recent, int32_t* __restrict__ kept) {
-    __shared__ __align__(16) uint32_t hist[kBins];
+    __shared__ __align__(16) uint32_t hist[3][kBins];
     __shared__ BinPick bp;
     __shared__ int cnt2[kSelWaves][2];
     const int seq = blockIdx.x / c.n_kv;
@@ -977,33 +977,33 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select(Kv4 c, const float* __
     const int need = budget - sink - recent;
     const int per = (len + kSelWaves * 64 - 1) / (kSelWaves * 64) * 64;   // positions of a wavefront
     const int a = wave * per, e = min(len, a + per);
-    uint32_t key[kSelKeys];
+    uint32_t key[KEYS];
 #pragma unroll
-    for (int j = 0; j < kSelKeys; j++) {
+    for (int j = 0; j < KEYS; j++) {
         const int i = a + 64 * j + lane;
         key[j] = i < e && i >= sink && i < z ? rank_of(wr[i]) : 0u;
     }
+    for (int i = tid; i < 3 * kBins / 4; i += kSelThreads) ((uint4*)&hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
+    __syncthreads();
     uint32_t cut = 0, left = need;
     const bool choose = need > 0;
     if (choose)
 #pragma unroll
         for (int lv = 0; lv < 3; lv++) {
-            for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
-            __syncthreads();
             const uint32_t known = lv == 0 ? 0u : lv == 1 ? ~0u << 21 : ~0u << 10;
 #pragma unroll
-            for (int j = 0; j < kSelKeys; j++) {
+            for (int j = 0; j < KEYS; j++) {
                 const int i = a + 64 * j + lane;
                 if (64 * j < per && i < e && i >= sink && i < z && (key[j] & known) == cut)
-                    atomicAdd(&hist[bin_of(key[j], lv)], 1u);
+                    atomicAdd(&hist[lv][bin_of(key[j], lv)], 1u);
             }
             __syncthreads();
-            const uint2 v = *(const uint2*)&hist[kBins - 2 * (tid + 1)];
+            const uint2 v = *(const uint2*)&hist[lv][kBins - 2 * (tid + 1)];
             cut |= pick_bin(bp, v.x, v.y, left) << bin_shift(lv);
         }
     int above = 0, equal = 0;
 #pragma unroll
-    for (int j = 0; j < kSelKeys; j++)
+    for (int j = 0; j < KEYS; j++)
         if (64 * j < per) {
             const int i = a + 64 * j + lane;
             const bool in = i < e, cand = in && i >= sink && i < z;
@@ -1025,7 +1025,7 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select(Kv4 c, const float* __
     at += min(eqs, equals);
     const unsigned long long low = (1ull << lane) - 1;
 #pragma unroll
-    for (int j = 0; j < kSelKeys; j++)
+    for (int j = 0; j < KEYS; j++)
         if (64 * j < per) {
             const int i = a + 64 * j + lane;
             const bool in = i < e, cand = in && i >= sink && i < z, eq = cand && choose && key[j] == cut;
@@ -1185,22 +1185,36 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_long(Kv4 c, LongSel q,
     }
 }
 
-// Moves the kept positions.  256 threads gather a page of the destination into
-// LDS and write it; a block has GROUPS such groups.  Not in place (GROUPS 1) a
-// block is one page.  In place a block takes all pages of its (KV head,
-// sequence) in order, GROUPS at a time: a kept position never lies before its
-// destination, so page p's sources are in pages >= p, and a page is written
-// only after it and the pages before it have been gathered.
+// Moves the kept positions.  A group of 128 HDG threads gathers a page of the
+// destination into registers, 16 bytes of keys, one pair and 16 bytes of values
+// a thread, and writes them; a block has GROUPS such groups.  Not in place
+// (GROUPS 1) a block is one page.  In place a block takes all pages of its (KV
+// head, sequence) in order, GROUPS at a time: a kept position never lies
+// before its destination, so page p's sources are in pages >= p, and a page is
+// written only after it and the pages before it have been gathered.
+//
+// Values: a lane's 16 bytes hold 16 positions of two dims, so they come from up
+// to 16 places.  A load takes 16 lanes of each of four positions (those of one
+// half of a word, 16 apart), 256 contiguous bytes each, of which one nibble a
+// dim is used; the lanes then hand each other their nibbles (each half, then
+// each quarter of the lanes keeps its share) and end with what they write.
+// (Gathered byte by byte into LDS the page took 39 us where this takes 15: 16
+// sequences of 8 heads cut to 2000 positions.)
 template <int GROUPS, int HDG>
-__global__ __launch_bounds__(256 * GROUPS) void kv4_move(Kv4 src, Kv4 dst, const float* w_src, float* w_dst, int budget,
-                                                         const int32_t* __restrict__ kept) {
-    extern __shared__ __align__(16) uint8_t bufs[];      // GROUPS x 72 hd bytes
-    __shared__ int from[GROUPS][kPage];
-    __shared__ const uint8_t* page[GROUPS][kPage];       // the source's part of its page, null where there is none
-    constexpr int hd = 64 * HDG, hdg = HDG;
-    const int tid = threadIdx.x & 255, grp = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
-    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    uint8_t* const buf = bufs + (size_t)grp * 72 * hd;
+__global__ __launch_bounds__(128 * HDG * GROUPS) void kv4_move(Kv4 src, Kv4 dst, const float* w_src, float* w_dst,
+                                                               int budget, const int32_t* __restrict__ kept) {
+    constexpr int hd = 64 * HDG, TG = 128 * HDG;
+    // of a position: where the pool holds its 16 dims 0 .. of keys, its pair
+    // of dims 0 .., its quarter of the values' first chunk; and the mask and
+    // place of its nibble in the 8 bytes of a dim (word, shift).  A position
+    // that is not there reads the pool's first bytes, masked away, so that no
+    // load stands behind a branch.
+    __shared__ int64_t koff[GROUPS][kPage], poff[GROUPS][kPage], voff[GROUPS][kPage];
+    __shared__ uint32_t there[GROUPS][kPage], lost[GROUPS][kPage], nib[GROUPS][kPage];
+    __shared__ int first[GROUPS];
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int grp = wv / (2 * HDG), wave = wv % (2 * HDG), lane = threadIdx.x & 63, tid = wave * 64 + lane;
+    const int li = lane & 15, lq = lane >> 4;
     int b = blockIdx.x;
     const int p0 = GROUPS > 1 ? 0 : b % dst.max_pages;
     if (GROUPS == 1) b /= dst.max_pages;
@@ -1213,6 +1227,7 @@ __global__ __launch_bounds__(256 * GROUPS) void kv4_move(Kv4 src, Kv4 dst, const
     for (int pb = p0; pb < p1; pb += GROUPS) {
         const int p = pb + grp;
         float wt = 0.f;
+        uint8_t* const to = p < p1 ? page_at(dst, seq, p, h) : nullptr;
         if (tid < kPage) {
             const int i = p * kPage + tid;
             const int f = p < p1 && i < budget ? kr[i] : -1;
@@ -1220,84 +1235,86 @@ __global__ __launch_bounds__(256 * GROUPS) void kv4_move(Kv4 src, Kv4 dst, const
             if (f >= 0) {
                 pg = page_at(src, seq, f / kPage, h);
                 wt = ws[f];
-                if (!pg) raise_table();
+                if (!pg || !to) raise_table();
                 if (h == 0 && (i + 1 == budget || kr[i + 1] < 0)) dst.lens[seq] = i + 1;
             }
-            from[grp][tid] = f;
-            page[grp][tid] = pg;
+            const int s = f & 63;
+            const int64_t at = pg ? pg - src.pool : 0;
+            koff[grp][tid] = pg ? at + key_off(s, 0, 0, HDG) : 0;
+            poff[grp][tid] = pg ? at + 32 * hd + 4 * slot_of(s) : 0;
+            voff[grp][tid] = pg ? at + 36 * hd + (s & 15) / 4 * 256 : 0;
+            there[grp][tid] = pg ? ~0u : 0u;
+            lost[grp][tid] = f >= 0 && !pg ? 0x7e007e00u : 0u;
+            nib[grp][tid] = ((s >> 1) & 1) * 32 + 8 * (s >> 4) + 4 * (s & 1);
+            if (tid == 0) first[grp] = f;
         }
         __syncthreads();
-        const bool some = from[grp][0] >= 0;
+        const bool some = first[grp] >= 0;
+        uint4 kx = make_uint4(0u, 0u, 0u, 0u), vx = kx;
+        uint32_t px = 0;
         if (some) {
-            // every load of the page first, then LDS.  Values: a word holds
-            // eight positions of one dim; the positions are the same for a
-            // wavefront, whose lanes are 64 dims.  A position that is not
-            // there reads the pool's first bytes and counts as zero.
-            uint8_t vb[2][8][HDG];
-            uint32_t vm[2][8];
-            int sh[2][8];
+            // values of dims 32 wave ..: positions 16 lq + 2 r + hl of word r, half hl
+            u32x4_t x[8][2];
 #pragma unroll
-            for (int rr = 0; rr < 2; rr++)
+            for (int r = 0; r < 8; r++)
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const int r = wave + 4 * rr, t = 16 * (k >> 1) + 2 * r + (k & 1);
-                    const int f = __builtin_amdgcn_readfirstlane(from[grp][t]);
-                    const uint64_t pg = (uint64_t)page[grp][t];
-                    const uint64_t u = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)pg) |
-                                       (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(pg >> 32)) << 32;
-                    // position f's byte of dim 0
-                    const uint8_t* base = u ? (const uint8_t*)u + 36 * hd + val_off(0, (f & 15) >> 1) + ((f & 63) >> 4) : src.pool;
-                    vm[rr][k] = u ? 15u : 0u;
-                    sh[rr][k] = 4 * (f & 1);
+                for (int hl = 0; hl < 2; hl++)
+                    x[r][hl] = *(const u32x4_t*)(src.pool + voff[grp][16 * lq + 2 * r + hl] + (there[grp][16 * lq + 2 * r + hl] & (wave * 1024 + li * 16)));
+            // keys: 16 dims of positions 32 u + li and 32 u + 16 + li; pairs of side u
+            const int g = wave % HDG, u = wave / HDG;
+            uint2 y[2];
+            uint32_t my[2];
 #pragma unroll
-                    for (int g = 0; g < HDG; g++) vb[rr][k][g] = base[(unsigned)(u ? val_off(64 * g + lane, 0) : 0)];
-                }
-            // keys: 16 bytes of a chunk hold 16 dims of positions 32 u + n and 32 u + 16 + n
-            constexpr int KI = (128 * HDG + 255) / 256;
-            uint2 kx[KI][2];
-            uint32_t px[KI];
-#pragma unroll
-            for (int j = 0; j < KI; j++) {
-                const int i = tid + 256 * j, ln = i & 63, g = (i >> 6) % hdg, u = (i >> 6) / hdg;
-                kx[j][0] = kx[j][1] = make_uint2(0u, 0u);
-                px[j] = 0;
-                if (i >= 128 * HDG) continue;
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const int t = 32 * u + 16 * k + (ln & 15);
-                    const uint8_t* pg = page[grp][t];
-                    if (pg) kx[j][k] = *(const uint2*)(pg + key_off(from[grp][t] & 63, g, ln >> 4, hdg));
-                }
-                const int t = ln, side = u, f = from[grp][t];   // pairs of both sides: the same indexes
-                const uint8_t* pg = page[grp][t];
-                if (f >= 0) px[j] = pg ? ((const uint32_t*)(pg + (32 + 36 * side) * hd))[g * 64 + slot_of(f & 63)] : 0x7e007e00u;
+            for (int k = 0; k < 2; k++) {
+                const int t = 32 * u + 16 * k + li;
+                my[k] = there[grp][t];
+                y[k] = *(const uint2*)(src.pool + koff[grp][t] + (my[k] & (g * 1024 + lq * 256)));
             }
+            const uint32_t mp = there[grp][lane];
+            const uint32_t pr = *(const uint32_t*)(src.pool + poff[grp][lane] + (mp & (36 * hd * u + g * 256)));
+            // every load above is on its way before the first is used: the
+            // compiler would otherwise take each apart, and wait, at once
 #pragma unroll
-            for (int j = 0; j < KI; j++) {
-                const int i = tid + 256 * j, ln = i & 63, g = (i >> 6) % hdg, u = (i >> 6) / hdg;
-                if (i >= 128 * HDG) continue;
-                *(uint4*)(buf + (u * hdg + g) * 1024 + ln * 16) = make_uint4(kx[j][0].x, kx[j][0].y, kx[j][1].x, kx[j][1].y);
-                ((uint32_t*)(buf + (32 + 36 * u) * hd))[g * 64 + slot_of(ln)] = px[j];
-            }
+            for (int r = 0; r < 8; r++)
 #pragma unroll
-            for (int rr = 0; rr < 2; rr++)
+                for (int hl = 0; hl < 2; hl++) asm volatile("" : "+v"(x[r][hl]));
+            kx = make_uint4(y[0].x & my[0], y[0].y & my[0], y[1].x & my[1], y[1].y & my[1]);
+            px = (pr & mp) | lost[grp][lane];
+            // word r of the lane's dims li and 16 + li, byte lq
+            uint32_t w0[8], w1[8];
 #pragma unroll
-                for (int g = 0; g < HDG; g++) {
-                    uint32_t x = 0;
+            for (int r = 0; r < 8; r++) {
+                w0[r] = w1[r] = 0;
 #pragma unroll
-                    for (int k = 0; k < 8; k++)
-                        x |= ((uint32_t)vb[rr][k][g] >> sh[rr][k] & vm[rr][k]) << (8 * (k >> 1) + 4 * (k & 1));
-                    *(uint32_t*)(buf + 36 * hd + val_off(64 * g + lane, wave + 4 * rr)) = x;
+                for (int hl = 0; hl < 2; hl++) {
+                    const uint32_t s = nib[grp][16 * lq + 2 * r + hl], m = there[grp][16 * lq + 2 * r + hl] & 15u;
+                    w0[r] |= (((s & 32) ? x[r][hl].y : x[r][hl].x) >> (s & 31) & m) << (8 * lq + 4 * hl);
+                    w1[r] |= (((s & 32) ? x[r][hl].w : x[r][hl].z) >> (s & 31) & m) << (8 * lq + 4 * hl);
                 }
+            }
+            // lanes 0 - 31 keep words 0 - 3, the others 4 - 7; then each 16 their two
+            uint32_t a0[4], a1[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const bool up = lq >= 2;
+                a0[i] = (up ? w0[4 + i] : w0[i]) | __shfl_xor(up ? w0[i] : w0[4 + i], 32, kWave);
+                a1[i] = (up ? w1[4 + i] : w1[i]) | __shfl_xor(up ? w1[i] : w1[4 + i], 32, kWave);
+            }
+            uint32_t c0[2], c1[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const bool up = lq & 1;
+                c0[i] = (up ? a0[2 + i] : a0[i]) | __shfl_xor(up ? a0[i] : a0[2 + i], 16, kWave);
+                c1[i] = (up ? a1[2 + i] : a1[i]) | __shfl_xor(up ? a1[i] : a1[2 + i], 16, kWave);
+            }
+            vx = make_uint4(c0[0], c0[1], c1[0], c1[1]);
         }
         __syncthreads();
-        if (some) {
-            uint8_t* pg = page_at(dst, seq, p, h);
-            if (pg) {
-                for (int i = tid; i < 72 * hd / 16; i += 256) ((uint4*)pg)[i] = ((const uint4*)buf)[i];
-            } else if (tid == 0) {
-                raise_table();
-            }
+        if (some && to) {
+            const int g = wave % HDG, u = wave / HDG;
+            *(uint4*)(to + wave * 1024 + lane * 16) = kx;      // chunk (u, g) is number u HDG + g
+            *(uint4*)(to + 36 * hd + wave * 1024 + lane * 16) = vx;
+            ((uint32_t*)(to + (32 + 36 * u) * hd))[g * 64 + slot_of(lane)] = px;
         }
         if (tid < kPage && p < p1) wd[p * kPage + tid] = wt;
         if (GROUPS > 1) __syncthreads();
@@ -1480,9 +1497,9 @@ extern "C" int ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float*
 template <int HDG>
 static void launch_move(const Kv4& s, const Kv4& d, const float* ws, float* wd, int budget, const int32_t* kept,
                         bool in_place, size_t blocks, hipStream_t st) {
-    constexpr int G = HDG > 3 ? 2 : 4;                   // as many groups as 64 KB of LDS hold
-    if (in_place) kv4_move<G, HDG><<<(unsigned)blocks, 256 * G, G * 72 * 64 * HDG, st>>>(s, d, ws, wd, budget, kept);
-    else kv4_move<1, HDG><<<(unsigned)blocks, 256, 72 * 64 * HDG, st>>>(s, d, ws, wd, budget, kept);
+    constexpr int G = 1024 / (128 * HDG);
+    if (in_place) kv4_move<G, HDG><<<(unsigned)blocks, 128 * HDG * G, 0, st>>>(s, d, ws, wd, budget, kept);
+    else kv4_move<1, HDG><<<(unsigned)blocks, 128 * HDG, 0, st>>>(s, d, ws, wd, budget, kept);
 }
 static bool select_in_one(const ibh_kv4_cache* c) { return (int64_t)c->max_pages * kPage <= kSelMost; }
 
@@ -1525,7 +1542,10 @@ extern "C" int ibh_kv4_evict(const ibh_kv4_cache* src, const ibh_kv4_cache* dst,
     hipStream_t st = ibh_resolve_stream(stream);
     const Kv4 s = device_of(src), d = device_of(dst);
     if (!need) {
-        kv4_select<<<(unsigned)heads, kSelThreads, 0, st>>>(s, weights_src, budget, sink, recent, kept);
+        if (src->max_pages * kPage <= 4 * kSelThreads)
+            kv4_select<4><<<(unsigned)heads, kSelThreads, 0, st>>>(s, weights_src, budget, sink, recent, kept);
+        else
+            kv4_select<16><<<(unsigned)heads, kSelThreads, 0, st>>>(s, weights_src, budget, sink, recent, kept);
     } else {
         LongSel q;
         q.hist = (uint32_t*)ws;
