@@ -1201,7 +1201,7 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_long(Kv4 c, LongSel q,
 // (Gathered byte by byte into LDS the page took 39 us where this takes 15: 16
 // sequences of 8 heads cut to 2000 positions.)
 template <int GROUPS, int HDG>
-__global__ __launch_bounds__(128 * HDG * GROUPS) void kv4_move(Kv4 src, Kv4 dst, const float* w_src, float* w_dst,
+__global__ __launch_bounds__(128 * HDG * GROUPS, GROUPS == 1 ? 5 : 4) void kv4_move(Kv4 src, Kv4 dst, const float* w_src, float* w_dst,
                                                                int budget, const int32_t* __restrict__ kept) {
     constexpr int hd = 64 * HDG, TG = 128 * HDG;
     // of a position: where the pool holds its 16 dims 0 .. of keys, its pair
