@@ -79,38 +79,43 @@ __device__ __forceinline__ int val_off(int d, int r) {
 
 // ── append ───────────────────────────────────────────────────────────────────
 // Block (64 dims, side, head, page, sequence), 4 threads a position: thread
-// (t, c) holds dims 16 i + 4 c .. + 3.  The group's ends give scale =
-// f16((hi - lo) / 15) and mid = f16(lo + 8 scale); a code is the fp32 quotient
-// rounded, then put right against the exact borders mid + (c +- 1/2) scale
-// (fp64 holds both sides), so the codes are those of the exact quotient.
+// (t, cq) holds dims 16 i + 4 cq .. + 3.  The group's ends give scale =
+// f16((hi - lo) / 15) and mid = f16(lo + 8 scale).  A code is the quotient (x -
+// mid) / scale by the reciprocal, which is at most 2^-19 off (three roundings
+// of 2^-24 of at most 9), rounded; where it comes within 2^-17 of a border
+// the wavefront compares x - mid with the exact borders (c +- 1/2) scale in
+// fp64, so the codes are those of the exact quotient.  (Dividing and comparing
+// for every element took 23 us where this takes 12: 4099 positions of 8 heads
+// of 128, 43 MB.)
+__device__ __forceinline__ void touched(const Kv4& c, int n, int n_touch, int& g, int& side, int& h, int& seq, int& pi) {
+    int b = blockIdx.x;
+    g = b % (c.hd / 64); b /= c.hd / 64;
+    side = b & 1; b >>= 1;
+    h = b % c.n_kv; b /= c.n_kv;
+    pi = b % n_touch;
+    seq = b / n_touch;
+}
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4 c, const float* __restrict__ k,
                                                          const float* __restrict__ v, int n_new, int stride,
                                                          int n_touch, int vec) {
-    __shared__ uint8_t code[kPage][68];
+    __shared__ __align__(16) uint8_t code[kPage][68];    // values: a code a byte
+    __shared__ __align__(16) uint8_t words[2048];        // keys: as they lie in the page
     const int hdg = c.hd / 64;
-    int b = blockIdx.x;
-    const int g = b % hdg; b /= hdg;
-    const int side = b & 1; b >>= 1;
-    const int h = b % c.n_kv; b /= c.n_kv;
-    const int seq = b / n_touch;
+    int g, side, h, seq, pi;
+    touched(c, n_new, n_touch, g, side, h, seq, pi);
     bool bad;
     const int len = seq_len(c, seq, &bad);
     const int first = len - n_new;                       // position of row 0
-    const int p = max(first, 0) / kPage + b % n_touch;
+    const int p = max(first, 0) / kPage + pi;
     if (bad) {
         if (threadIdx.x == 0) raise_table();
         return;
     }
     if (p * kPage >= len) return;
-    uint8_t* const pg = page_at(c, seq, p, h);
-    if (!pg) {
-        if (threadIdx.x == 0) raise_table();
-        return;
-    }
-    uint8_t* const part = pg + side * 36 * c.hd;
     const int tid = threadIdx.x, t = tid >> 2, cq = tid & 3;
     const int pos = p * kPage + t;
     const bool is_new = pos >= first && pos < len;
+    const bool whole = p * kPage >= first && p * kPage + kPage <= len;
     float x[16];
     if (is_new) {
         const float* src = (side ? v : k) + ((size_t)seq * n_new + (pos - first)) * (size_t)stride + h * c.hd + 64 * g + 4 * cq;
@@ -128,14 +133,28 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4 c, const float* __r
 #pragma unroll
         for (int i = 0; i < 16; i++) x[i] = 0.f;
     }
+    uint8_t* const pg = page_at(c, seq, p, h);
+    if (!pg) {
+        if (tid == 0) raise_table();
+        return;
+    }
+    uint8_t* const part = pg + side * 36 * c.hd;
+    // values: thread's two words of dim 32 j + 16 d1 + n, positions of quarter cv
+    const int vd = 32 * (tid >> 7) + 16 * (tid & 1) + ((tid >> 1) & 15), cv = (tid >> 5) & 3;
+    uint8_t* const vdst = part + (2 * g + (tid >> 7)) * 1024 + (cv * 16 + ((tid >> 1) & 15)) * 16 + (tid & 1) * 8;
+    uint2 old = make_uint2(0u, 0u);
+    if (side && !whole) old = *(const uint2*)vdst;       // what a page that is not all new keeps
     float lo = INFINITY, hi = -INFINITY;
     bool nan = false;
 #pragma unroll
     for (int i = 0; i < 16; i++) {
         nan |= x[i] != x[i];
-        x[i] = fminf(fmaxf(x[i], -65504.f), 65504.f);
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
+        x[i] = __builtin_amdgcn_fmed3f(x[i], -65504.f, 65504.f);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+        lo = fminf(fminf(x[i], x[i + 1]), lo);
+        hi = fmaxf(fmaxf(x[i], x[i + 1]), hi);
     }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
@@ -148,22 +167,41 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4 c, const float* __r
     const uint32_t mb = nan ? 0x7e00u : f2h(lo + 8.0f * sc);
     const float mid = h2f(mb);
     if (is_new && cq == 0) ((uint32_t*)(part + 32 * c.hd))[g * 64 + slot_of(t)] = sb | (mb << 16);
+    // a quotient held to -8 .. 7 plus 1.5 * 2^23 + 8 is rounded by the addition
+    // (to nearest, ties to even) and has the code in its low byte
+    constexpr float magic = 12582912.f + 8.f;
+    const bool some = sc > 0.f;                          // codes 8 where the scale is 0 or NaN
+    const float inv = some ? 1.0f / sc : 0.f, off = some ? mid : 0.f;
     uint32_t word[4];                                    // four codes, a byte each
+    float far = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        word[i] = 0;
+        uint32_t cd[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            float q = 0.f;
-            if (sc > 0.f) {
-                q = fminf(fmaxf(rintf((x[4 * i + j] - mid) / sc), -8.f), 7.f);
-                const double d = (double)x[4 * i + j] - (double)mid;
-                const double up = (double)((q + 0.5f) * sc), dn = (double)((q - 0.5f) * sc);
-                const bool odd = ((int)q & 1) != 0;      // a tie goes to the even neighbour
-                if (q < 7.f && (d > up || (d == up && odd))) q += 1.f;
-                else if (q > -8.f && (d < dn || (d == dn && odd))) q -= 1.f;
+            const float q = __builtin_amdgcn_fmed3f((x[4 * i + j] - off) * inv, -8.f, 7.f), r = q + magic;
+            far = fmaxf(far, fabsf(q - (r - magic)));
+            cd[j] = __builtin_bit_cast(uint32_t, r);
+        }
+        word[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(cd[3], cd[2], 0x0c0c0400), __builtin_amdgcn_perm(cd[1], cd[0], 0x0c0c0400), 0x05040100);
+    }
+    if (__any(some && far > 0.5f - 0x1p-17f)) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            word[i] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float q = 0.f;
+                if (sc > 0.f) {
+                    q = fminf(fmaxf(rintf((x[4 * i + j] - mid) * inv), -8.f), 7.f);
+                    const double d = (double)x[4 * i + j] - (double)mid;
+                    const double up = (double)((q + 0.5f) * sc), dn = (double)((q - 0.5f) * sc);
+                    const bool odd = ((int)q & 1) != 0;  // a tie goes to the even neighbour
+                    if (q < 7.f && (d > up || (d == up && odd))) q += 1.f;
+                    else if (q > -8.f && (d < dn || (d == dn && odd))) q -= 1.f;
+                }
+                word[i] |= (uint32_t)((int)q + 8) << (8 * j);
             }
-            word[i] |= (uint32_t)((int)q + 8) << (8 * j);
         }
     }
     if (side == 0) {
@@ -171,69 +209,91 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4 c, const float* __r
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint32_t o = __shfl_xor(word[i], 1, kWave);
-            if (is_new && !(cq & 1)) *(uint32_t*)(part + key_off(t, g, i, hdg) + (cq >> 1) * 4) = word[i] | (o << 4);
+            const uint32_t w = word[i] | (o << 4);
+            if (cq & 1) continue;
+            if (whole) *(uint32_t*)(words + (t >> 5) * 1024 + (i * 16 + (t & 15)) * 16 + ((t >> 4) & 1) * 8 + (cq >> 1) * 4) = w;
+            else if (is_new) *(uint32_t*)(part + key_off(t, g, i, hdg) + (cq >> 1) * 4) = w;
         }
+        if (!whole) return;
+        __syncthreads();
+        if (tid < 128) *(uint4*)(part + ((tid >> 6) * hdg + g) * 1024 + (tid & 63) * 16) = *(const uint4*)(words + tid * 16);
         return;
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) *(uint32_t*)&code[t][16 * i + 4 * cq] = word[i];
     __syncthreads();
     // a word of values holds eight positions of one dim: those that are not
-    // new keep their nibbles (no other block writes this word)
+    // new keep their nibbles (no other block writes these words)
+    uint32_t w[2], m[2];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-        const int d = tid & 63, r = (tid >> 6) + 4 * u;
-        uint32_t w = 0, m = 0;
+        const int r = 2 * cv + u;
+        w[u] = m[u] = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int hl = 0; hl < 2; hl++) {
                 const int tt = 16 * i + 2 * r + hl, ps = p * kPage + tt;
-                w |= (uint32_t)code[tt][d] << (8 * i + 4 * hl);
-                if (ps >= first && ps < len) m |= 0xfu << (8 * i + 4 * hl);
+                w[u] |= (uint32_t)code[tt][vd] << (8 * i + 4 * hl);
+                if (ps >= first && ps < len) m[u] |= 0xfu << (8 * i + 4 * hl);
             }
-        if (!m) continue;
-        uint32_t* dst = (uint32_t*)(part + val_off(64 * g + d, r));
-        *dst = m == 0xffffffffu ? w : ((w & m) | (*dst & ~m));
     }
+    if (m[0] | m[1]) *(uint2*)vdst = make_uint2((w[0] & m[0]) | (old.x & ~m[0]), (w[1] & m[1]) | (old.y & ~m[1]));
 }
 
 // ── read ─────────────────────────────────────────────────────────────────────
-// The values of a sequence's last n positions: block as above.
+// The values of a sequence's last n positions: blocks and threads as above, a
+// head's 64 dims of a page in LDS first.
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4 c, float* __restrict__ k, float* __restrict__ v, int n,
-                                                       int stride, int n_touch) {
+                                                       int stride, int n_touch, int vec) {
+    __shared__ __align__(16) uint8_t words[2048];
     const int hdg = c.hd / 64;
-    int b = blockIdx.x;
-    const int g = b % hdg; b /= hdg;
-    const int side = b & 1; b >>= 1;
-    const int h = b % c.n_kv; b /= c.n_kv;
-    const int seq = b / n_touch;
+    int g, side, h, seq, pi;
+    touched(c, n, n_touch, g, side, h, seq, pi);
     bool bad;
     const int len = seq_len(c, seq, &bad);
     const int first = len - n;
-    const int p = max(first, 0) / kPage + b % n_touch;
+    const int p = max(first, 0) / kPage + pi;
     if (bad && threadIdx.x == 0) raise_table();
     if (p * kPage >= len) return;
     const uint8_t* const pg = page_at(c, seq, p, h);
     if (!pg && threadIdx.x == 0) raise_table();
-    const int tid = threadIdx.x, d = tid & 63;
-    for (int t = tid >> 6; t < kPage; t += 4) {
-        const int pos = p * kPage + t;
-        if (pos < first || pos >= len) continue;
-        float y = NAN;
-        if (pg && !bad) {
-            const uint8_t* part = pg + side * 36 * c.hd;
-            const uint32_t pr = ((const uint32_t*)(part + 32 * c.hd))[g * 64 + slot_of(t)];
-            int cd;
-            if (side == 0) {
-                const int e = d & 15;
-                cd = part[key_off(t, g, d >> 4, hdg) + (e >> 3) * 4 + (e & 3)] >> (e & 4) & 15;
-            } else {
-                cd = part[val_off(64 * g + d, (t & 15) >> 1) + (t >> 4)] >> (4 * (t & 1)) & 15;
-            }
-            y = fmaf(h2f(pr), (float)(cd - 8), h2f(pr >> 16));
+    const int tid = threadIdx.x, t = tid >> 2, cq = tid & 3, pos = p * kPage + t;
+    const uint8_t* const part = pg ? pg + side * 36 * c.hd : nullptr;
+    uint32_t pr = 0x7e007e00u;
+    if (pg && !bad) {
+        if (tid < 128) {
+            const int at = side ? (2 * g + (tid >> 6)) * 1024 : ((tid >> 6) * hdg + g) * 1024;
+            *(uint4*)(words + tid * 16) = *(const uint4*)(part + at + (tid & 63) * 16);
         }
-        (side ? v : k)[((size_t)seq * n + (pos - first)) * (size_t)stride + h * c.hd + 64 * g + d] = y;
+        pr = ((const uint32_t*)(part + 32 * c.hd))[g * 64 + slot_of(t)];
+    }
+    __syncthreads();
+    if (pos < first || pos >= len) return;
+    const float sc = h2f(pr), mid = h2f(pr >> 16);
+    float* dst = (side ? v : k) + ((size_t)seq * n + (pos - first)) * (size_t)stride + h * c.hd + 64 * g + 4 * cq;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float y[4];
+        if (side == 0) {
+            const uint32_t w = *(const uint32_t*)(words + (t >> 5) * 1024 + (i * 16 + (t & 15)) * 16 + ((t >> 4) & 1) * 8 + (cq >> 1) * 4) >> (4 * (cq & 1));
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[j] = (float)((int)(w >> (8 * j) & 15u) - 8);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int d = 16 * i + 4 * cq + j;
+                y[j] = (float)((int)(words[val_off(d, (t & 15) >> 1) + (t >> 4)] >> (4 * (t & 1)) & 15) - 8);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) y[j] = fmaf(sc, y[j], mid);
+        if (vec) {
+            *(float4*)(dst + 16 * i) = make_float4(y[0], y[1], y[2], y[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) dst[16 * i + j] = y[j];
+        }
     }
 }
 
@@ -1389,8 +1449,9 @@ extern "C" int ibh_kv4_read(const ibh_kv4_cache* cache, float* k, float* v, int 
     const int n_touch = min((n + kPage - 2) / kPage + 1, cache->max_pages);
     const size_t blocks = (size_t)cache->n_seq * n_touch * cache->n_kv * 2 * (cache->head_dim / 64);
     if (!grid_ok(blocks, "ibh_kv4_read")) return IBH_ERROR_PARAM;
+    const int vec = (((uintptr_t)k | (uintptr_t)v) & 15) == 0 && kv_stride % 4 == 0;
     kv4_read_kernel<<<(unsigned)blocks, 256, 0, ibh_resolve_stream(stream)>>>(device_of(cache), k, v, n, kv_stride,
-                                                                              n_touch);
+                                                                              n_touch, vec);
     IBH_CHECK_LAUNCH("ibh_kv4_read");
     return IBH_OK;
 }
