@@ -390,16 +390,16 @@ struct AttnArgs {
 constexpr int attn_waves(int hdg, int rt) { return hdg * rt == 1 ? 4 : hdg * rt == 2 ? 3 : hdg * rt >= 8 && hdg > 2 ? 1 : 2; }
 
 // Block: `chunk` pages of one (sequence, KV head), RT tiles of 4 query rows,
-// four wavefronts that take the block's pages in turn, each with its own
-// running maximum and sums, joined at the end.
-template <int HDG, int RT, bool SCORES>
-__global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 c, AttnArgs a) {
+// NW wavefronts that take the block's pages in turn, each with its own running
+// maximum and sums, joined at the end.
+template <int HDG, int RT, bool SCORES, int NW>
+__global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 c, AttnArgs a) {
     constexpr int HD = 64 * HDG, ROWS = 4 * RT;
     __shared__ __align__(16) int8_t digs[RT * HDG * 1024];   // [tile][group][16][64]
-    __shared__ __align__(16) int8_t turn[4][HDG][4 * 320];   // a wavefront's p * scale digits, 64 B a row, a query row on 320
+    __shared__ __align__(16) int8_t turn[NW][HDG][4 * 320];   // a wavefront's p * scale digits, 64 B a row, a query row on 320
     __shared__ float rc[ROWS][1 + HDG];
-    __shared__ float ob[4][4][HD];
-    __shared__ float mlw[4][4][2];
+    __shared__ float ob[NW][4][HD];
+    __shared__ float mlw[NW][4][2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lq = lane >> 4;
     // the KV head runs fastest over the blocks, so that blocks which share a
@@ -430,7 +430,7 @@ __global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 
     // a page no table entry names is left out of the sums (the block reports
     // it at its end and gives NaN): its wavefront goes on to its next page
     auto next_page = [&](int& p) -> const uint8_t* {
-        for (; p < p1; p += 4) {
+        for (; p < p1; p += NW) {
             const uint8_t* pg = page_of_wave(c, seq, p, h);
             if (pg) return pg;
             bad = true;
@@ -442,7 +442,7 @@ __global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 
     const uint8_t* pg = p < p1 ? page_by_id(c, id0, h) : nullptr;
     if (!pg && p < p1) {
         bad = true;
-        p += 4;
+        p += NW;
         pg = next_page(p);
     }
     if (pg) {
@@ -461,7 +461,7 @@ __global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 
     }
 
     // the query rows as digits
-    for (int r = wave; r < ROWS; r += 4) {
+    for (int r = wave; r < ROWS; r += NW) {
         const int row = min(row0 + r, n_rows - 1);
         const float* src = a.q + ((size_t)seq * a.n_q + row / grp) * (size_t)a.q_stride + (h * grp + row % grp) * HD;
         float x[HDG], mx = 0.f;
@@ -501,7 +501,7 @@ __global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 
         const size_t tiles = (n_rows + 3) / 4;
 #pragma unroll
         for (int t = 0; t < RT; t++)
-            if ((t & 3) == wave && row0 + 4 * t < n_rows) {
+            if (t % NW == wave && row0 + 4 * t < n_rows) {
 #pragma unroll
                 for (int g = 0; g < HDG; g++) a.digits[((sh * tiles + row0 / 4 + t) * HDG + g) * 64 + lane] = qa[t][g];
                 const int row = row0 + 4 * t + lq;
@@ -647,7 +647,7 @@ __global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 
     const int full = min(p1, (lim_min + 1) >> 6);
     auto run = [&](int end, auto masked) {
         while (pg && p < end) {
-            int pn = p + 4;
+            int pn = p + NW;
             const uint8_t* nx = next_page(pn);
             if (!nx) at = 0;
             step(p * kPage, nx ? nx : pg, masked);
@@ -658,7 +658,7 @@ __global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 
     run(full, std::false_type{});
     run(p1, std::true_type{});
 
-    // the four wavefronts' sums, a tile at a time
+    // the wavefronts' sums, a tile at a time
     const bool any_bad = __syncthreads_or(bad);
     if (any_bad && tid == 0) raise_table();
 #pragma unroll
@@ -676,11 +676,12 @@ __global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 
         }
         __syncthreads();
         const int r = wave, row = row0 + 4 * t + r;
-        if (row < n_rows) {
-            float mm = fmaxf(fmaxf(mlw[0][r][0], mlw[1][r][0]), fmaxf(mlw[2][r][0], mlw[3][r][0]));
-            float f[4], sum = 0.f;
+        if (r < 4 && row < n_rows) {
+            float mm = -INFINITY, f[NW], sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
+            for (int w = 0; w < NW; w++) mm = fmaxf(mm, mlw[w][r][0]);
+#pragma unroll
+            for (int w = 0; w < NW; w++) {
                 f[w] = mlw[w][r][0] == -INFINITY && mlw[w][r][1] == 0.f ? 0.f : exp2_(mlw[w][r][0] - mm);
                 sum = fmaf(f[w], mlw[w][r][1], sum);
             }
@@ -694,7 +695,7 @@ __global__ __launch_bounds__(256, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 
             for (int g = 0; g < HDG; g++) {
                 float y = 0.f;
 #pragma unroll
-                for (int w = 0; w < 4; w++) y = fmaf(f[w], ob[w][r][64 * g + lane], y);
+                for (int w = 0; w < NW; w++) y = fmaf(f[w], ob[w][r][64 * g + lane], y);
                 dst[64 * g + lane] = y * norm;
             }
             if (lane == 0) {
@@ -918,10 +919,9 @@ __global__ __launch_bounds__(256) void kv4_attn_finish(Kv4 c, AttnArgs a, unsign
 
 // Accumulated weights where the rows fill several tiles: block (KV head, page,
 // sequence), its wavefronts take the tiles in turn.
-constexpr int kWeightWaves = 8;
-template <int HDG>
-__global__ __launch_bounds__(64 * kWeightWaves) void kv4_attn_weights(Kv4 c, AttnArgs a, const float* win, float* wout) {
-    __shared__ float part[kWeightWaves][kPage];
+template <int HDG, int NW>
+__global__ __launch_bounds__(64 * NW) void kv4_attn_weights(Kv4 c, AttnArgs a, const float* win, float* wout) {
+    __shared__ float part[NW][kPage];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int b = blockIdx.x;
@@ -942,7 +942,7 @@ __global__ __launch_bounds__(64 * kWeightWaves) void kv4_attn_weights(Kv4 c, Att
         pw.load(pg, lane);
         // queries before the page's first position see nothing of it
         const int t0 = max(0, p * kPage - (len - a.n_q)) * grp / 4;
-        part[wave][lane] = pw.sum(a.digits + sh * tiles * HDG * 64, p * kPage, lane, t0 + wave, tiles, kWeightWaves,
+        part[wave][lane] = pw.sum(a.digits + sh * tiles * HDG * 64, p * kPage, lane, t0 + wave, tiles, NW,
             [&](int t, int lq, float& kf, float& lse, float* qs, int& lim) {
                 const int r = 4 * t + lq, row = min(r, n_rows - 1);
                 const float* rcp = a.rowc + (sh * n_rows + row) * (1 + HDG);
@@ -960,7 +960,7 @@ __global__ __launch_bounds__(64 * kWeightWaves) void kv4_attn_weights(Kv4 c, Att
     if (wave) return;
     float add = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWeightWaves; w++) add += part[w][lane];
+    for (int w = 0; w < NW; w++) add += part[w][lane];
     wout[at] = p * kPage + lane < len ? win[at] + add : 0.f;
 }
 
@@ -1458,7 +1458,7 @@ extern "C" int ibh_kv4_read(const ibh_kv4_cache* cache, float* k, float* v, int 
 
 // How a call is cut: row tiles of 4 rt query rows, blocks of `chunk` pages.
 struct AttnPlan {
-    int rt, n_tile, chunk, n_split;
+    int rt, n_tile, chunk, n_split, nw;
     bool joint;                                          // the weights in the launch that joins the splits
     size_t part, part_ml, lse, digits, rowc, score, bytes;      // offsets into the workspace
 };
@@ -1472,6 +1472,11 @@ static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool wei
     size_t chunk = (work + want - 1) / want;
     chunk = max(chunk, ((size_t)c->max_pages + kMaxSplit - 1) / kMaxSplit);
     p.chunk = (int)((chunk + 3) / 4 * 4);
+    // up to 1024 positions a decode step is one launch: eight wavefronts take a
+    // head's pages, and nothing is left to join (600 positions of 32/4 heads:
+    // 7 us in one kernel, 7 + 3 in two)
+    p.nw = p.n_tile == 1 && p.rt <= 2 && (int)hdg * p.rt <= 6 && c->max_pages > 4 && c->max_pages <= 16 ? 8 : 4;
+    if (p.nw == 8) p.chunk = 16;
     p.n_split = (c->max_pages + p.chunk - 1) / p.chunk;
     p.joint = weights && p.n_tile == 1 && p.n_split > 1 && p.rt <= 2;
     size_t at = 0;
@@ -1499,13 +1504,18 @@ static void launch_attn_rt(const Kv4& c, const AttnArgs& a, const AttnPlan& p, s
     const size_t rows = p.n_split > 1 ? heads * a.n_q * (a.n_heads / c.n_kv) : 0;
     const unsigned blocks = (unsigned)(heads * p.n_tile * p.n_split);
     if constexpr (RT <= 2) {
-        if (p.joint) kv4_attn_kernel<HDG, RT, true><<<blocks, 256, 0, st>>>(c, a);
+        if (p.joint) kv4_attn_kernel<HDG, RT, true, 4><<<blocks, 256, 0, st>>>(c, a);
+        else if constexpr (HDG * RT <= 6) if (p.nw == 8) kv4_attn_kernel<HDG, RT, false, 8><<<blocks, 512, 0, st>>>(c, a);
     }
-    if (!p.joint) kv4_attn_kernel<HDG, RT, false><<<blocks, 256, 0, st>>>(c, a);
+    if (!p.joint && p.nw == 4) kv4_attn_kernel<HDG, RT, false, 4><<<blocks, 256, 0, st>>>(c, a);
     const size_t wb = p.joint ? heads * ((c.max_pages + 3) / 4) : 0;
     if (rows + wb) kv4_attn_finish<HDG, RT><<<(unsigned)(rows + wb), 256, 0, st>>>(c, a, (unsigned)rows, win, wout);
     if (wout && !p.joint)
-        kv4_attn_weights<HDG><<<(unsigned)(heads * c.max_pages), 64 * kWeightWaves, 0, st>>>(c, a, win, wout);
+{
+        // a wavefront a page where it has few rows, eight where they are many
+        if (a.n_q * (a.n_heads / c.n_kv) <= 16) kv4_attn_weights<HDG, 1><<<(unsigned)(heads * c.max_pages), 64, 0, st>>>(c, a, win, wout);
+        else kv4_attn_weights<HDG, 8><<<(unsigned)(heads * c.max_pages), 512, 0, st>>>(c, a, win, wout);
+    }
 }
 template <int HDG>
 static void launch_attn(const Kv4& c, const AttnArgs& a, const AttnPlan& p, size_t heads, const float* win,
