@@ -323,7 +323,7 @@ __device__ __forceinline__ i4_t unpack16(uint32_t a, uint32_t b) {
     return i4_t{(int)(a & M), (int)((a >> 4) & M), (int)(b & M), (int)((b >> 4) & M)};
 }
 __device__ __forceinline__ i4_t mfma16(i4_t a, i4_t b, i4_t c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ float join_digits(i4_t c) { return (float)((c[0] << 16) + ((c[1] << 8) + c[2])); }
+__device__ __forceinline__ float join_digits(i4_t c) { return (float)(int)((((uint32_t)c[0] << 8) + (uint32_t)c[1] << 8) + (uint32_t)c[2]); }
 // v_exp_f32: at most one unit in the last place off, results below 2^-126 are 0
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 // Largest value of the 16 lanes of a row, every lane getting it: v_max_f32
@@ -378,9 +378,11 @@ struct AttnArgs {
     int n_heads, n_q, q_stride;
     float scale;                                         // log2(e) / sqrt(head_dim)
     int chunk, n_split, n_tile;                          // pages of a block, blocks of a row tile, row tiles of a KV head
+    int tile_rows;                                       // query rows of a row tile
     float* part;                                         // [seq][KV head][row][split][head_dim], when n_split > 1
     float2* part_ml;                                     // [seq][KV head][row][split] maximum (log2) and sum
-    float* lse;                                          // [seq][KV head][row] log2 of the row's sum, when weights are wanted
+    float* lse;                                          // [seq][KV head][row, lse_pad of them] log2 of the row's sum, when weights are wanted
+    int lse_pad;
     i4_t* digits;                                        // [seq][KV head][4-row tile][group][lane]
     float* rowc;                                         // [seq][KV head][row][1 + groups] step * scale, sums of the query in steps
     float4* scores;                                      // [seq][KV head][page][tile][lane] scores (log2), -inf where not seen
@@ -611,8 +613,7 @@ __global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(
                     }
                 }
                 const float wm = row16_max(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])));
-                const float wt = fmaxf(wm, kTiny);
-                const float inv = kDigitMax * __builtin_amdgcn_rcpf(wt), ws = wt * (1.f / kDigitMax);
+                const float ws = fmaxf(wm, kTiny) * (1.f / kDigitMax), inv = __builtin_amdgcn_rcpf(ws);
                 uint32_t j[4];
 #pragma unroll
                 for (int s = 0; s < 4; s++) j[s] = (uint32_t)fmaf(w[s], inv, 32896.5f);
@@ -707,9 +708,475 @@ __global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(
     }
 }
 
+// ── attention of many rows ───────────────────────────────────────────────────
+// From 33 query rows of a KV head on the sums are the f16 matrix cores': a row
+// is one row of the MFMA, the query and p * scale are the sum of two fp16
+// numbers (22 bits of every element that is not 2^18 below its bound), the
+// codes are fp16 numbers -8 .. 7, and products are added in fp32.  That takes
+// as many MFMAs as three digits in four rows, but no joining of digits, and
+// the values' sums stay in the accumulators from page to page.  Block: 64 rows,
+// 16 a wavefront; the four take a page's codes apart together, into LDS, as
+// the matrix cores read them (a code word is a lane's 8 elements of one MFMA:
+// halves 0, 2, 4, 6, 1, 3, 5, 7 of its bytes' order).
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h8_alias __attribute__((ext_vector_type(8), may_alias));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+constexpr int kWideRows = 64;
+
+__device__ __forceinline__ f4_t mfma32(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+// A code word's eight numbers: 1024 + code as fp16 bits, less 1032.
+__device__ __forceinline__ h8_t unpack_half(uint32_t w) {
+    uint32_t r[4];
+    h8_t x;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        r[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u;
+        const h2_t y = __builtin_bit_cast(h2_t, r[i]) + h2_t{(_Float16)-1032.f, (_Float16)-1032.f};
+        x[2 * i] = y[0];
+        x[2 * i + 1] = y[1];
+    }
+    return x;
+}
+// x - the low (HI: high) half of h
+template <bool HI>
+__device__ __forceinline__ float less_half(float x, uint32_t h) {
+    float y;
+    if constexpr (HI) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(y) : "v"(h), "v"(x));
+    else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(y) : "v"(h), "v"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_rtz(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)); }
+
+// Rows' constants for the weights, each array padded to whole blocks of rows.
+struct WideRows {
+    h8_t* q;                                             // [seq][KV head][16-row tile][group][2][high, low][lane]
+    float *kf, *qsum, *lse;                              // [..][row], [..][group][row], [..][row]
+};
+__device__ __forceinline__ int wide_pad(int n_rows) { return (n_rows + kWideRows - 1) / kWideRows * kWideRows; }
+
+template <int HDG>
+__global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn_wide(Kv4 c, AttnArgs a, WideRows wr) {
+    constexpr int HD = 64 * HDG, PR = 72;                // halves of a row of p * scale in LDS: 64 and 8 for the banks
+    __shared__ __align__(16) uint8_t ops[16 * HDG * 1024];   // keys [position / 16][group][2], values [dim / 16][2]: a lane's 16 B
+    __shared__ __align__(16) uint16_t pw[4][2][16 * PR];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int li = lane & 15, lq = lane >> 4;
+    int b = blockIdx.x;
+    const int h = b % c.n_kv; b /= c.n_kv;
+    const int rt = a.n_tile - 1 - b % a.n_tile; b /= a.n_tile;
+    const int split = b % a.n_split, seq = b / a.n_split;
+    const int grp = a.n_heads / c.n_kv, n_rows = a.n_q * grp;
+    const int p0 = split * a.chunk;
+    const int id0 = ld_uniform(c.table + (size_t)seq * c.max_pages + min(p0, c.max_pages - 1));
+    bool bad;
+    const int len = seq_len(c, seq, &bad);
+    const int base = len - a.n_q;                        // the first query's position
+    const int lim_block = base + min(rt * kWideRows + kWideRows - 1, n_rows - 1) / grp;
+    const int pages = lim_block < 0 ? 0 : lim_block / kPage + 1;
+    const int p1 = min(p0 + a.chunk, pages);
+    if (split > 0 && p0 >= pages) return;
+    const int row0 = rt * kWideRows + wave * 16;
+    const bool active = row0 < n_rows;
+    const int lim_lo = base + min(row0, n_rows - 1) / grp, lim_hi = base + min(row0 + 15, n_rows - 1) / grp;
+    int lim[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) lim[r] = base + min(row0 + 4 * lq + r, n_rows - 1) / grp;
+    const size_t sh = (size_t)seq * c.n_kv + h;
+
+    // wavefronts 0, 1 take the keys apart (their halves u), 2, 3 the values
+    const int chunk0 = wave < 2 ? wave * HDG * 1024 : 2304 * HDG + (wave - 2) * HDG * 1024;
+    uint4 raw[HDG], kp[HDG], vp[HDG];
+    auto load = [&](const uint8_t* pg) {
+#pragma unroll
+        for (int g = 0; g < HDG; g++) {
+            raw[g] = *(const uint4*)(pg + chunk0 + g * 1024 + lane * 16);
+            kp[g] = *(const uint4*)(pg + 2048 * HDG + g * 256 + li * 16);
+            vp[g] = *(const uint4*)(pg + 4352 * HDG + g * 256 + li * 16);
+        }
+    };
+    int p = p0;
+    auto next_page = [&](int& p, int id) -> const uint8_t* {   // the same for every wavefront of the block
+        while (p < p1) {
+            const uint8_t* pg = page_by_id(c, id, h);
+            if (pg) return pg;
+            bad = true;
+            if (++p < p1) id = ld_uniform(c.table + (size_t)seq * c.max_pages + p);
+        }
+        return nullptr;
+    };
+    const uint8_t* pg = next_page(p, id0);
+    if (pg) load(pg);
+
+    // the wavefront's rows: lane (li, lq) holds dims 16 lq .. + 15 of every 64
+    h8_t qa[HDG][2][2];
+    float kf[4], qsum[4][HDG];
+    {
+        const int row = min(row0 + li, n_rows - 1);
+        const float* src = a.q + ((size_t)seq * a.n_q + row / grp) * (size_t)a.q_stride + (h * grp + row % grp) * HD + 16 * lq;
+        float x[HDG][16], mx = 0.f;
+#pragma unroll
+        for (int g = 0; g < HDG; g++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                x[g][i] = src[64 * g + i];
+                mx = fmaxf(mx, fabsf(x[g][i]));
+            }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+        // a power of two takes the largest element to 2^14 .. 2^15
+        const bool sane = mx > kTiny && mx < INFINITY;
+        const int k = sane ? 15 - __builtin_amdgcn_frexp_expf(mx) : 0;
+        float sum[HDG];
+#pragma unroll
+        for (int g = 0; g < HDG; g++) {
+            float t = 0.f;
+#pragma unroll
+            for (int kc = 0; kc < 2; kc++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int i = 8 * kc + (j < 4 ? 2 * j : 2 * j - 7);
+                    const float y = mx > kTiny || mx != mx ? ldexpf(x[g][i], k) : x[g][i] * 0.f;
+                    const _Float16 hi = (_Float16)y;
+                    qa[g][kc][0][j] = hi;
+                    qa[g][kc][1][j] = (_Float16)(y - (float)hi);
+                    t += y;
+                }
+            t += __shfl_xor(t, 16, kWave);
+            sum[g] = t + __shfl_xor(t, 32, kWave);
+        }
+        const float f = ldexpf(a.scale, -k);
+#pragma unroll
+        for (int r = 0; r < 4; r++) {                    // the rows of the results: 4 lq + r
+            kf[r] = __shfl(f, 4 * lq + r, kWave);
+#pragma unroll
+            for (int g = 0; g < HDG; g++) qsum[r][g] = __shfl(sum[g], 4 * lq + r, kWave);
+        }
+        if (wr.q && split == 0) {
+            const int pad = wide_pad(n_rows);
+            h8_t* to = wr.q + (sh * (pad / 16) + row0 / 16) * HDG * 256 + lane;
+#pragma unroll
+            for (int g = 0; g < HDG; g++)
+#pragma unroll
+                for (int kc = 0; kc < 2; kc++)
+#pragma unroll
+                    for (int hl = 0; hl < 2; hl++) to[((g * 2 + kc) * 2 + hl) * 64] = qa[g][kc][hl];
+            if (lq == 0) {
+                wr.kf[sh * pad + row0 + li] = f;
+#pragma unroll
+                for (int g = 0; g < HDG; g++) wr.qsum[(sh * HDG + g) * pad + row0 + li] = sum[g];
+                if (row0 + li >= n_rows) wr.lse[sh * pad + row0 + li] = INFINITY;   // adds nothing
+            }
+        }
+    }
+
+    float m[4], l[4], om[4][HDG], vf[HDG], vtop[HDG];
+    f4_t o[4 * HDG];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+#pragma unroll
+        for (int g = 0; g < HDG; g++) om[r][g] = 0.f;
+    }
+#pragma unroll
+    for (int g = 0; g < HDG; g++) {
+        vf[g] = 1.f;
+        vtop[g] = 0.f;
+    }
+#pragma unroll
+    for (int d = 0; d < 4 * HDG; d++) o[d] = f4_t{0.f, 0.f, 0.f, 0.f};
+    uint16_t* const ph = pw[wave][0];
+    uint16_t* const pl = pw[wave][1];
+
+    auto step = [&](const uint4 (&kq)[HDG], const uint4 (&vq)[HDG], int pos0, auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
+        float x[4][4];                                   // [row][position / 16]
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) x[r][s] = 0.f;
+#pragma unroll
+            for (int g = 0; g < HDG; g++) {
+                f4_t d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kc = 0; kc < 2; kc++) {
+                    const h8_t kb = *(const h8_alias*)(ops + ((s * HDG + g) * 2 + kc) * 1024 + lane * 16);
+                    d = mfma32(qa[g][kc][0], kb, d);
+                    d = mfma32(qa[g][kc][1], kb, d);
+                }
+                const uint32_t pr = part4(kq[g], s);
+#pragma unroll
+                for (int r = 0; r < 4; r++) x[r][s] = fmaf(h2f(pr), d[r], fmaf(h2f(pr >> 16), qsum[r][g], x[r][s]));
+            }
+            if constexpr (MASKED) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) x[r][s] = pos0 + 16 * s + li <= lim[r] ? x[r][s] : -INFINITY;
+            }
+        }
+        // the running maximum moves only when a score is over 2^8 times above
+        // it: p stays below 2^8, for which the values' factor leaves room
+        float top[4];
+        bool up = false;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            top[r] = row16_max(fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3]))) * kf[r];
+            up |= top[r] > m[r] + 8.f;
+        }
+        if (__any(up)) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float mn = fmaxf(m[r], top[r]);
+                const float al = mn == -INFINITY ? 1.f : exp2_(m[r] - mn);
+                m[r] = mn;
+                l[r] *= al;
+#pragma unroll
+                for (int d = 0; d < 4 * HDG; d++) o[d][r] *= al;
+#pragma unroll
+                for (int g = 0; g < HDG; g++) om[r][g] *= al;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const float mk = m[r] == -INFINITY ? 0.f : -m[r];
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                x[r][s] = exp2_(fmaf(x[r][s], kf[r], mk));
+                l[r] += x[r][s];
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < HDG; g++) {
+            // p * scale times a power of two that takes the largest scale so
+            // far to 2^6 .. 2^7
+            float vs[4], vm[4], vt = 0.f;
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const uint32_t pr = part4(vq[g], s);
+                vs[s] = h2f(pr);
+                vm[s] = h2f(pr >> 16);
+                if constexpr (MASKED) {                  // stale pairs may be anything
+                    const bool any = pos0 + 16 * s + li <= lim_hi;
+                    vs[s] = any ? vs[s] : 0.f;
+                    vm[s] = any ? vm[s] : 0.f;
+                }
+                vt = fmaxf(vt, vs[s]);
+            }
+            vt = row16_max(vt);
+            if (__any(vt > vtop[g])) {
+                vtop[g] = fmaxf(vt, vtop[g]);
+                const float nf = ldexpf(1.f, 7 - __builtin_amdgcn_frexp_expf(vtop[g])), al = nf / vf[g];
+                vf[g] = nf;
+#pragma unroll
+                for (int d = 0; d < 4; d++) o[4 * g + d] *= al;
+            }
+#pragma unroll
+            for (int s = 0; s < 4; s++) vs[s] *= vf[g];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                float w[4];
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    w[s] = x[r][s] * vs[s];
+                    if constexpr (MASKED) {              // a NaN that this row does not see
+                        const bool ok = pos0 + 16 * s + li <= lim[r];
+                        w[s] = ok ? w[s] : 0.f;
+                        om[r][g] += ok ? x[r][s] * vm[s] : 0.f;
+                    } else {
+                        om[r][g] = fmaf(x[r][s], vm[s], om[r][g]);
+                    }
+                }
+                // slots 4 li + s: quarter li / 4, half li / 2 % 2, then s = 0, 2 and s = 1, 3
+                const uint32_t h02 = pack_rtz(w[0], w[2]), h13 = pack_rtz(w[1], w[3]);
+                const uint32_t l02 = pack_rtz(less_half<false>(w[0], h02), less_half<true>(w[2], h02));
+                const uint32_t l13 = pack_rtz(less_half<false>(w[1], h13), less_half<true>(w[3], h13));
+                const int at = (4 * lq + r) * PR + (li >> 1) * 8 + (li & 1) * 2;
+                *(u32_alias*)(ph + at) = h02;
+                *(u32_alias*)(ph + at + 4) = h13;
+                *(u32_alias*)(pl + at) = l02;
+                *(u32_alias*)(pl + at + 4) = l13;
+            }
+            __builtin_amdgcn_wave_barrier();
+            h8_t wa[2][2];
+#pragma unroll
+            for (int kc = 0; kc < 2; kc++) {
+                wa[kc][0] = *(const h8_alias*)(ph + li * PR + lq * 16 + kc * 8);
+                wa[kc][1] = *(const h8_alias*)(pl + li * PR + lq * 16 + kc * 8);
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int d = 4 * g; d < 4 * g + 4; d++)
+#pragma unroll
+                for (int kc = 0; kc < 2; kc++) {
+                    const h8_t vb = *(const h8_alias*)(ops + (8 * HDG + d * 2 + kc) * 1024 + lane * 16);
+                    o[d] = mfma32(wa[kc][0], vb, o[d]);
+                    o[d] = mfma32(wa[kc][1], vb, o[d]);
+                }
+        }
+    };
+
+    while (pg) {
+        __syncthreads();                                 // the page before has been read
+        {
+            // chunk (u, g): operands (position / 16 = 2 u + i, g, half); value chunk j: (dim / 16 = 2 j + i, half)
+#pragma unroll
+            for (int g = 0; g < HDG; g++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int op = wave < 2 ? ((2 * wave + i) * HDG + g) * 2 : 8 * HDG + (2 * ((wave - 2) * HDG + g) + i) * 2;
+                    *(h8_alias*)(ops + op * 1024 + lane * 16) = unpack_half(i ? raw[g].z : raw[g].x);
+                    *(h8_alias*)(ops + (op + 1) * 1024 + lane * 16) = unpack_half(i ? raw[g].w : raw[g].y);
+                }
+        }
+        uint4 kq[HDG], vq[HDG];
+#pragma unroll
+        for (int g = 0; g < HDG; g++) {
+            kq[g] = kp[g];
+            vq[g] = vp[g];
+        }
+        int pn = p + 1;
+        const uint8_t* nx = pn < p1 ? next_page(pn, ld_uniform(c.table + (size_t)seq * c.max_pages + pn)) : nullptr;
+        if (nx) load(nx);
+        __syncthreads();
+        if (active && p * kPage <= lim_hi) {
+            if (p * kPage + kPage - 1 > lim_lo) step(kq, vq, p * kPage, std::true_type{});
+            else step(kq, vq, p * kPage, std::false_type{});
+        }
+        pg = nx;
+        p = pn;
+    }
+
+    if (bad && tid == 0) raise_table();
+    if (!active) return;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int row = row0 + 4 * lq + r;
+        float sum = row16_sum(l[r]);
+        if (bad) sum = NAN;
+        const size_t rr = sh * n_rows + row;
+        const bool in = row < n_rows;
+        float* dst = a.n_split > 1 ? a.part + (rr * a.n_split + split) * HD
+                                   : a.out + ((size_t)seq * a.n_q + row / grp) * (size_t)a.n_heads * HD + (h * grp + row % grp) * HD;
+        const float norm = a.n_split > 1 ? (bad ? NAN : 1.f) : (sum == 0.f ? 0.f : 1.f / sum);
+#pragma unroll
+        for (int g = 0; g < HDG; g++) {
+            const float mid = row16_sum(om[r][g]), back = 1.f / vf[g];
+#pragma unroll
+            for (int d = 0; d < 4; d++)
+                if (in) dst[64 * g + 16 * d + li] = fmaf(o[4 * g + d][r], back, mid) * norm;
+        }
+        if (in && li == 0) {
+            if (a.n_split > 1) a.part_ml[rr * a.n_split + split] = make_float2(m[r], sum);
+            else if (wr.lse) wr.lse[sh * wide_pad(n_rows) + row] = sum == 0.f ? INFINITY : m[r] + log2f(sum);
+        }
+    }
+}
+
+// Accumulated weights of many rows: block (KV head, page, sequence); every
+// wavefront holds the page's keys and takes 16-row tiles in turn.
+template <int HDG>
+__global__ __launch_bounds__(512) void kv4_weights_wide(Kv4 c, AttnArgs a, WideRows wr, const float* win, float* wout) {
+    constexpr int NW = 8;
+    __shared__ float part[NW][kPage];
+    const int lane = threadIdx.x & 63, li = lane & 15, lq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int b = blockIdx.x;
+    const int h = b % c.n_kv; b /= c.n_kv;
+    const int p = b % c.max_pages, seq = b / c.max_pages;
+    const int grp = a.n_heads / c.n_kv, n_rows = a.n_q * grp, pad = wide_pad(n_rows), tiles = (n_rows + 15) / 16;
+    bool bad;
+    const int len = seq_len(c, seq, &bad);
+    const size_t sh = (size_t)seq * c.n_kv + h;
+    const size_t at = (sh * c.max_pages + p) * kPage + lane;
+    if (p * kPage >= len) {
+        if (wave == 0) wout[at] = 0.f;
+        return;
+    }
+    const uint8_t* pg = page_of_wave(c, seq, p, h);
+    if (pg && !bad) {
+        h8_t kb[4][HDG][2];
+        uint4 kp[HDG];
+#pragma unroll
+        for (int g = 0; g < HDG; g++) {
+            kp[g] = key_pairs<HDG, false>(pg, g, 16 * lane);
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const uint4 x = key_codes<HDG, false>(pg, u, g, 16 * lane);
+                kb[2 * u][g][0] = unpack_half(x.x);
+                kb[2 * u][g][1] = unpack_half(x.y);
+                kb[2 * u + 1][g][0] = unpack_half(x.z);
+                kb[2 * u + 1][g][1] = unpack_half(x.w);
+            }
+        }
+        // queries before the page's first position see nothing of it
+        const int base = len - a.n_q, t0 = max(0, p * kPage - base) * grp / 16;
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int t = t0 + wave; t < tiles; t += NW) {
+            const h8_t* q = wr.q + (sh * (pad / 16) + t) * HDG * 256 + lane;
+            const int row = 16 * t + 4 * lq;
+            const f4_t kf = *(const f4_t*)(wr.kf + sh * pad + row), lse = *(const f4_t*)(wr.lse + sh * pad + row);
+            float x[4][4];
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int s = 0; s < 4; s++) x[r][s] = 0.f;
+#pragma unroll
+            for (int g = 0; g < HDG; g++) {
+                const f4_t qs = *(const f4_t*)(wr.qsum + (sh * HDG + g) * pad + row);
+                h8_t qa[2][2];
+#pragma unroll
+                for (int kc = 0; kc < 2; kc++)
+#pragma unroll
+                    for (int hl = 0; hl < 2; hl++) qa[kc][hl] = q[((g * 2 + kc) * 2 + hl) * 64];
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    f4_t d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int kc = 0; kc < 2; kc++) {
+                        d = mfma32(qa[kc][0], kb[s][g][kc], d);
+                        d = mfma32(qa[kc][1], kb[s][g][kc], d);
+                    }
+                    const uint32_t pr = part4(kp[g], s);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) x[r][s] = fmaf(h2f(pr), d[r], fmaf(h2f(pr >> 16), qs[r], x[r][s]));
+                }
+            }
+            if (p * kPage + kPage - 1 <= base + 16 * t / grp) {
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int s = 0; s < 4; s++) acc[s] += exp2_(fmaf(x[r][s], kf[r], -lse[r]));
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int lim = base + min(row + r, n_rows - 1) / grp;
+#pragma unroll
+                    for (int s = 0; s < 4; s++)
+                        acc[s] += p * kPage + 16 * s + li <= lim ? exp2_(fmaf(x[r][s], kf[r], -lse[r])) : 0.f;
+                }
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            acc[s] += __shfl_xor(acc[s], 16, kWave);
+            acc[s] += __shfl_xor(acc[s], 32, kWave);
+        }
+        part[wave][lane] = lq == 0 ? acc[0] : lq == 1 ? acc[1] : lq == 2 ? acc[2] : acc[3];
+    } else {
+        if (threadIdx.x == 0) raise_table();
+        part[wave][lane] = NAN;
+    }
+    __syncthreads();
+    if (wave) return;
+    float add = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; w++) add += part[w][lane];
+    wout[at] = p * kPage + lane < len ? win[at] + add : 0.f;
+}
+
 // Blocks of a row's tile that had work: as kv4_attn_kernel cut the pages.
-__device__ __forceinline__ int splits_of(const AttnArgs& a, int len, int row, int grp, int n_rows, int tile_rows) {
-    const int last = min(row / tile_rows * tile_rows + tile_rows, n_rows) - 1;
+__device__ __forceinline__ int splits_of(const AttnArgs& a, int len, int row, int grp, int n_rows) {
+    const int last = min(row / a.tile_rows * a.tile_rows + a.tile_rows, n_rows) - 1;
     const int lim = len - a.n_q + last / grp;
     return lim < 0 ? 1 : (lim / kPage + a.chunk) / a.chunk;
 }
@@ -828,7 +1295,7 @@ __global__ __launch_bounds__(256) void kv4_attn_finish(Kv4 c, AttnArgs a, unsign
         const size_t rr = blockIdx.x, sh = rr / n_rows;
         const int row = rr % n_rows, h = sh % c.n_kv, seq = sh / c.n_kv;
         const int len = seq_len(c, seq, &bad);
-        const int n = splits_of(a, len, row, grp, n_rows, 4 * RT);
+        const int n = splits_of(a, len, row, grp, n_rows);
         const float2* ml = a.part_ml + rr * a.n_split;
         const int td = tid % TD, cl = tid / TD;
         const float4* po = (const float4*)(a.part + rr * a.n_split * HD) + td;
@@ -876,7 +1343,7 @@ __global__ __launch_bounds__(256) void kv4_attn_finish(Kv4 c, AttnArgs a, unsign
             a.out[((size_t)seq * a.n_q + row / grp) * (size_t)a.n_heads * HD + (h * grp + row % grp) * HD + tid] =
                 sum == 0.f ? 0.f : y / sum;
         }
-        if (tid == 0 && a.lse) a.lse[rr] = sum == 0.f ? INFINITY : mm + log2f(sum);
+        if (tid == 0 && a.lse) a.lse[sh * a.lse_pad + row] = sum == 0.f ? INFINITY : mm + log2f(sum);
         return;
     }
     unsigned b = blockIdx.x - n_join;
@@ -895,7 +1362,7 @@ __global__ __launch_bounds__(256) void kv4_attn_finish(Kv4 c, AttnArgs a, unsign
     float4 x[RT];
 #pragma unroll
     for (int t = 0; t < RT; t++) x[t] = a.scores[((sh * c.max_pages + p) * RT + t) * 64 + lane];
-    const int n = splits_of(a, len, 0, grp, n_rows, 4 * RT);
+    const int n = splits_of(a, len, 0, grp, n_rows);
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
     const int lq = lane >> 4;
 #pragma unroll
@@ -1458,15 +1925,16 @@ extern "C" int ibh_kv4_read(const ibh_kv4_cache* cache, float* k, float* v, int 
 
 // How a call is cut: row tiles of 4 rt query rows, blocks of `chunk` pages.
 struct AttnPlan {
-    int rt, n_tile, chunk, n_split, nw;
+    int rt, n_tile, chunk, n_split, nw;                  // rt 16: kv4_attn_wide
     bool joint;                                          // the weights in the launch that joins the splits
-    size_t part, part_ml, lse, digits, rowc, score, bytes;      // offsets into the workspace
+    size_t part, part_ml, lse, digits, rowc, score, bytes;     // offsets into the workspace
 };
 static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool weights) {
     AttnPlan p;
     const size_t n_rows = (size_t)n_q * (n_heads / c->n_kv), hdg = c->head_dim / 64;
     const size_t heads = (size_t)c->n_seq * c->n_kv;
-    p.rt = n_rows <= 4 ? 1 : n_rows <= 8 || hdg > 2 ? 2 : 4;
+    const bool wide = n_rows > 32;
+    p.rt = wide ? kWideRows / 4 : n_rows <= 4 ? 1 : n_rows <= 8 || hdg > 2 ? 2 : 4;
     p.n_tile = (int)((n_rows + 4 * p.rt - 1) / (4 * p.rt));
     const size_t work = heads * p.n_tile * c->max_pages, want = p.rt <= 2 ? 2048 : 1024;
     size_t chunk = (work + want - 1) / want;
@@ -1483,9 +1951,11 @@ static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool wei
     auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
     p.part = take(p.n_split > 1 ? heads * n_rows * p.n_split * c->head_dim * sizeof(float) : 0);
     p.part_ml = take(p.n_split > 1 ? heads * n_rows * p.n_split * sizeof(float2) : 0);
-    p.lse = take(weights && !p.joint ? heads * n_rows * sizeof(float) : 0);
-    p.digits = take(weights && !p.joint ? heads * ((n_rows + 3) / 4) * hdg * 1024 : 0);
-    p.rowc = take(weights && !p.joint ? heads * n_rows * (1 + hdg) * sizeof(float) : 0);
+    const size_t pad = wide ? (n_rows + kWideRows - 1) / kWideRows * kWideRows : n_rows;
+    const size_t again = weights && !p.joint ? heads : 0;
+    p.lse = take(again * pad * sizeof(float));
+    p.digits = take(again * ((pad + 3) / 4) * hdg * 1024);
+    p.rowc = take(again * pad * (1 + hdg) * sizeof(float));
     p.score = take(p.joint ? heads * c->max_pages * p.rt * 1024 : 0);
     p.bytes = at;
     return p;
@@ -1520,7 +1990,13 @@ static void launch_attn_rt(const Kv4& c, const AttnArgs& a, const AttnPlan& p, s
 template <int HDG>
 static void launch_attn(const Kv4& c, const AttnArgs& a, const AttnPlan& p, size_t heads, const float* win,
                         float* wout, hipStream_t st) {
-    if (p.rt == 1) launch_attn_rt<HDG, 1>(c, a, p, heads, win, wout, st);
+    if (p.rt == kWideRows / 4) {
+        const size_t rows = heads * a.n_q * (a.n_heads / c.n_kv), pad = heads * p.n_tile * kWideRows;
+        const WideRows wr = wout ? WideRows{(h8_t*)a.digits, a.rowc, a.rowc + pad, a.lse} : WideRows{};
+        kv4_attn_wide<HDG><<<(unsigned)(heads * p.n_tile * p.n_split), 256, 0, st>>>(c, a, wr);
+        if (p.n_split > 1) kv4_attn_finish<HDG, 1><<<(unsigned)rows, 256, 0, st>>>(c, a, (unsigned)rows, win, wout);
+        if (wout) kv4_weights_wide<HDG><<<(unsigned)(heads * c.max_pages), 512, 0, st>>>(c, a, wr, win, wout);
+    } else if (p.rt == 1) launch_attn_rt<HDG, 1>(c, a, p, heads, win, wout, st);
     else if (p.rt == 2) launch_attn_rt<HDG, 2>(c, a, p, heads, win, wout, st);
     else if constexpr (HDG <= 2) launch_attn_rt<HDG, 4>(c, a, p, heads, win, wout, st);
 }
@@ -1550,8 +2026,9 @@ extern "C" int ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float*
         return IBH_ERROR_PARAM;
     char* w = (char*)ws;
     AttnArgs a{out, q, n_heads, n_q, q_stride, (float)(1.4426950408889634 / sqrt((double)cache->head_dim)), p.chunk,
-               p.n_split, p.n_tile, (float*)(w + p.part), (float2*)(w + p.part_ml),
+               p.n_split, p.n_tile, 4 * p.rt, (float*)(w + p.part), (float2*)(w + p.part_ml),
                weights_out && !p.joint ? (float*)(w + p.lse) : nullptr,
+               p.rt == kWideRows / 4 ? p.n_tile * kWideRows : n_q * (n_heads / cache->n_kv),
                weights_out && !p.joint ? (i4_t*)(w + p.digits) : nullptr, (float*)(w + p.rowc), (float4*)(w + p.score)};
     const Kv4 c = device_of(cache);
     hipStream_t st = ibh_resolve_stream(stream);

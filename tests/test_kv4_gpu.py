@@ -199,7 +199,7 @@ def test_attention_long_and_strided(ops):
     check_attention(ops, m, q, n_heads, n_q, out, wi, wo)
 
 
-@pytest.mark.parametrize("n_q", [1, 6])
+@pytest.mark.parametrize("n_q", [1, 6, 45])
 def test_attention_sharp_and_flat_scores(ops, n_q):
     """Queries that pick one position (scores of hundreds), and zero queries (every probability the same)."""
     rng = np.random.default_rng(3)
@@ -230,11 +230,12 @@ def test_attention_small_values_beside_large_scales(ops):
     check_attention(ops, m, q, n_heads, 1, out)
 
 
-def test_attention_not_finite(ops):
+@pytest.mark.parametrize("n_q", [4, 40])
+def test_attention_not_finite(ops, n_q):
     """A NaN key makes the rows that see it NaN, a NaN value its 64 dims; rows that do not see it, and what lies
     behind a length (NaN and infinite pairs there, see Made), stay clean."""
     rng = np.random.default_rng(8)
-    n_heads, n_kv, hd, n_q, t = 4, 2, 128, 4, 100
+    n_heads, n_kv, hd, t = 4, 2, 128, 100
     for side in ("k", "v", "q"):
         m = Made(ops, rng, [t, 30], n_kv, hd)
         q = torch.from_numpy(rng.standard_normal((2, n_q, n_heads * hd)).astype(np.float32)).cuda()
@@ -256,9 +257,9 @@ def test_attention_not_finite(ops):
         if side == "q":
             want[0, 1, 0] = True
         elif side == "k":
-            want[0, 2:, 2:] = True
+            want[0, n_q - 2:, 2:] = True
         else:
-            want[0, 2:, 2:, 64:] = True
+            want[0, n_q - 2:, 2:, 64:] = True
         np.testing.assert_array_equal(nan, want)
         assert torch.isfinite(wo[1]).all()
 
