@@ -727,12 +727,12 @@ constexpr int kWideRows = 64;
 __device__ __forceinline__ f4_t mfma32(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 // A code word's eight numbers: 1024 + code as fp16 bits, less 1032.
 __device__ __forceinline__ h8_t unpack_half(uint32_t w) {
-    uint32_t r[4];
+    constexpr uint32_t M = 0x000f000fu, X = 0x64006400u;
     h8_t x;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        r[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u;
-        const h2_t y = __builtin_bit_cast(h2_t, r[i]) + h2_t{(_Float16)-1032.f, (_Float16)-1032.f};
+        const uint32_t r = ((w >> (4 * i)) & M) | X;
+        const h2_t y = __builtin_bit_cast(h2_t, r) + h2_t{(_Float16)-1032.f, (_Float16)-1032.f};
         x[2 * i] = y[0];
         x[2 * i + 1] = y[1];
     }
@@ -760,6 +760,7 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
     constexpr int HD = 64 * HDG, PR = 72;                // halves of a row of p * scale in LDS: 64 and 8 for the banks
     __shared__ __align__(16) uint8_t ops[16 * HDG * 1024];   // keys [position / 16][group][2], values [dim / 16][2]: a lane's 16 B
     __shared__ __align__(16) uint16_t pw[4][2][16 * PR];
+    __shared__ __align__(16) uint32_t prs[2][HDG][64];   // the page's pairs, keys' then values'
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lq = lane >> 4;
     int b = blockIdx.x;
@@ -778,7 +779,7 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
     if (split > 0 && p0 >= pages) return;
     const int row0 = rt * kWideRows + wave * 16;
     const bool active = row0 < n_rows;
-    const int lim_lo = base + min(row0, n_rows - 1) / grp, lim_hi = base + min(row0 + 15, n_rows - 1) / grp;
+    const int lim_hi = base + min(row0 + 15, n_rows - 1) / grp;
     int lim[4];
 #pragma unroll
     for (int r = 0; r < 4; r++) lim[r] = base + min(row0 + 4 * lq + r, n_rows - 1) / grp;
@@ -786,13 +787,13 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
 
     // wavefronts 0, 1 take the keys apart (their halves u), 2, 3 the values
     const int chunk0 = wave < 2 ? wave * HDG * 1024 : 2304 * HDG + (wave - 2) * HDG * 1024;
-    uint4 raw[HDG], kp[HDG], vp[HDG];
+    uint4 raw[HDG];
+    uint32_t rawp[HDG];
     auto load = [&](const uint8_t* pg) {
 #pragma unroll
         for (int g = 0; g < HDG; g++) {
             raw[g] = *(const uint4*)(pg + chunk0 + g * 1024 + lane * 16);
-            kp[g] = *(const uint4*)(pg + 2048 * HDG + g * 256 + li * 16);
-            vp[g] = *(const uint4*)(pg + 4352 * HDG + g * 256 + li * 16);
+            rawp[g] = *(const uint32_t*)(pg + (wave < 2 ? 2048 : 4352) * HDG + g * 256 + lane * 4);
         }
     };
     int p = p0;
@@ -889,7 +890,7 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
     uint16_t* const ph = pw[wave][0];
     uint16_t* const pl = pw[wave][1];
 
-    auto step = [&](const uint4 (&kq)[HDG], const uint4 (&vq)[HDG], int pos0, auto masked) {
+    auto step = [&](int pos0, auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
         float x[4][4];                                   // [row][position / 16]
 #pragma unroll
@@ -905,14 +906,16 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
                     d = mfma32(qa[g][kc][0], kb, d);
                     d = mfma32(qa[g][kc][1], kb, d);
                 }
-                const uint32_t pr = part4(kq[g], s);
+                const uint32_t pr = part4(*(const uint4*)&prs[0][g][4 * li], s);
 #pragma unroll
                 for (int r = 0; r < 4; r++) x[r][s] = fmaf(h2f(pr), d[r], fmaf(h2f(pr >> 16), qsum[r][g], x[r][s]));
             }
-            if constexpr (MASKED) {
+        }
+        if constexpr (MASKED) {
+#pragma unroll
+            for (int s = 0; s < 4; s++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) x[r][s] = pos0 + 16 * s + li <= lim[r] ? x[r][s] : -INFINITY;
-            }
         }
         // the running maximum moves only when a score is over 2^8 times above
         // it: p stays below 2^8, for which the values' factor leaves room
@@ -952,7 +955,7 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
             float vs[4], vm[4], vt = 0.f;
 #pragma unroll
             for (int s = 0; s < 4; s++) {
-                const uint32_t pr = part4(vq[g], s);
+                const uint32_t pr = part4(*(const uint4*)&prs[1][g][4 * li], s);
                 vs[s] = h2f(pr);
                 vm[s] = h2f(pr >> 16);
                 if constexpr (MASKED) {                  // stale pairs may be anything
@@ -1005,17 +1008,22 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
             }
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int d = 4 * g; d < 4 * g + 4; d++)
+            for (int kc = 0; kc < 2; kc++) {
+                h8_t vb[4];
 #pragma unroll
-                for (int kc = 0; kc < 2; kc++) {
-                    const h8_t vb = *(const h8_alias*)(ops + (8 * HDG + d * 2 + kc) * 1024 + lane * 16);
-                    o[d] = mfma32(wa[kc][0], vb, o[d]);
-                    o[d] = mfma32(wa[kc][1], vb, o[d]);
-                }
+                for (int d = 0; d < 4; d++) vb[d] = *(const h8_alias*)(ops + (8 * HDG + (4 * g + d) * 2 + kc) * 1024 + lane * 16);
+#pragma unroll
+                for (int hl = 0; hl < 2; hl++)
+#pragma unroll
+                    for (int d = 0; d < 4; d++) o[4 * g + d] = mfma32(wa[kc][hl], vb[d], o[4 * g + d]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
-    while (pg) {
+    // pages that every row of the block sees, then the others
+    auto run = [&](int end, auto masked) {
+      while (pg && p < end) {
         __syncthreads();                                 // the page before has been read
         {
             // chunk (u, g): operands (position / 16 = 2 u + i, g, half); value chunk j: (dim / 16 = 2 j + i, half)
@@ -1027,24 +1035,22 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
                     *(h8_alias*)(ops + op * 1024 + lane * 16) = unpack_half(i ? raw[g].z : raw[g].x);
                     *(h8_alias*)(ops + (op + 1) * 1024 + lane * 16) = unpack_half(i ? raw[g].w : raw[g].y);
                 }
-        }
-        uint4 kq[HDG], vq[HDG];
+            if (!(wave & 1)) {
 #pragma unroll
-        for (int g = 0; g < HDG; g++) {
-            kq[g] = kp[g];
-            vq[g] = vp[g];
+                for (int g = 0; g < HDG; g++) prs[wave >> 1][g][lane] = rawp[g];
+            }
         }
         int pn = p + 1;
         const uint8_t* nx = pn < p1 ? next_page(pn, ld_uniform(c.table + (size_t)seq * c.max_pages + pn)) : nullptr;
         if (nx) load(nx);
         __syncthreads();
-        if (active && p * kPage <= lim_hi) {
-            if (p * kPage + kPage - 1 > lim_lo) step(kq, vq, p * kPage, std::true_type{});
-            else step(kq, vq, p * kPage, std::false_type{});
-        }
+        if (active && p * kPage <= lim_hi) step(p * kPage, masked);
         pg = nx;
         p = pn;
-    }
+      }
+    };
+    run(min(p1, (base + rt * kWideRows / grp + 1) >> 6), std::false_type{});
+    run(p1, std::true_type{});
 
     if (bad && tid == 0) raise_table();
     if (!active) return;
@@ -1260,6 +1266,37 @@ struct PageWeights {
         return lq == 0 ? acc[0] : lq == 1 ? acc[1] : lq == 2 ? acc[2] : acc[3];
     }
 };
+
+// Joins few splits of many rows: a wavefront a row, 64 HDG dims a lane's HDG.
+template <int HDG>
+__global__ __launch_bounds__(256) void kv4_attn_join(Kv4 c, AttnArgs a, size_t rows) {
+    constexpr int HD = 64 * HDG;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int grp = a.n_heads / c.n_kv, n_rows = a.n_q * grp;
+    const size_t rr = (size_t)blockIdx.x * 4 + wave;
+    if (rr >= rows) return;
+    const size_t sh = rr / n_rows;
+    const int row = rr % n_rows, h = sh % c.n_kv, seq = sh / c.n_kv;
+    bool bad;
+    const int n = splits_of(a, seq_len(c, seq, &bad), row, grp, n_rows);
+    const float2* ml = a.part_ml + rr * a.n_split;
+    const float* po = a.part + rr * a.n_split * HD + lane;
+    float mm = -INFINITY, sum = 0.f, y[HDG] = {};
+    for (int i = 0; i < n; i++) {
+        const float2 v = ml[i];
+        const float mn = fmaxf(mm, v.x);
+        const float f0 = mm == -INFINITY && sum == 0.f ? 0.f : exp2_(mm - mn), f1 = v.x == -INFINITY && v.y == 0.f ? 0.f : exp2_(v.x - mn);
+        mm = mn;
+        sum = fmaf(f1, v.y, sum * f0);
+#pragma unroll
+        for (int g = 0; g < HDG; g++) y[g] = fmaf(f1, po[(size_t)i * HD + 64 * g], y[g] * f0);
+    }
+    float* dst = a.out + ((size_t)seq * a.n_q + row / grp) * (size_t)a.n_heads * HD + (h * grp + row % grp) * HD + lane;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int g = 0; g < HDG; g++) dst[64 * g] = y[g] * inv;
+    if (lane == 0 && a.lse) a.lse[sh * a.lse_pad + row] = sum == 0.f ? INFINITY : mm + log2f(sum);
+}
 
 // log2 of a query row's sum over its splits, by the 16 lanes of a row.
 __device__ __forceinline__ float row_lse(const float2* ml, int n, int li) {
@@ -1994,7 +2031,8 @@ static void launch_attn(const Kv4& c, const AttnArgs& a, const AttnPlan& p, size
         const size_t rows = heads * a.n_q * (a.n_heads / c.n_kv), pad = heads * p.n_tile * kWideRows;
         const WideRows wr = wout ? WideRows{(h8_t*)a.digits, a.rowc, a.rowc + pad, a.lse} : WideRows{};
         kv4_attn_wide<HDG><<<(unsigned)(heads * p.n_tile * p.n_split), 256, 0, st>>>(c, a, wr);
-        if (p.n_split > 1) kv4_attn_finish<HDG, 1><<<(unsigned)rows, 256, 0, st>>>(c, a, (unsigned)rows, win, wout);
+        if (p.n_split > 8) kv4_attn_finish<HDG, 1><<<(unsigned)rows, 256, 0, st>>>(c, a, (unsigned)rows, win, wout);
+        else if (p.n_split > 1) kv4_attn_join<HDG><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(c, a, rows);
         if (wout) kv4_weights_wide<HDG><<<(unsigned)(heads * c.max_pages), 512, 0, st>>>(c, a, wr, win, wout);
     } else if (p.rt == 1) launch_attn_rt<HDG, 1>(c, a, p, heads, win, wout, st);
     else if (p.rt == 2) launch_attn_rt<HDG, 2>(c, a, p, heads, win, wout, st);
