@@ -212,13 +212,21 @@ int ibh_attn_exact_set_grouped(int on);
  *   pool   n_pages pages of ibh_kv4_page_bytes(n_kv, head_dim) bytes, on 16
  *          bytes;
  *   table  [n_seq][max_pages]: the page that holds positions 64 j .. 64 j + 63
- *          of a sequence.  Entries behind a sequence's last page are not read.
+ *          of a sequence.  Entries behind a sequence's last page are not used.
  *          Sequences may share full pages, not one that is appended to;
  *   lens   [n_seq] positions held, 0 .. 64 max_pages; 0 leaves a sequence out.
  * head_dim 64, 128, 192 or 256.  A page number outside the pool or a length
  * outside the row raises IBH_DEVERR_KV4_TABLE (ibh_device_errors): nothing is
- * stored for it, what would be computed from it is NaN, the other sequences
- * are served.  An element stands for mid + scale * (code - 8). */
+ * stored for it, what would be computed from it is NaN, an eviction keeps
+ * nothing of a sequence of such a length; the other sequences are served.
+ *
+ * An element stands for mid + scale * (code - 8).  For each KV head a page
+ * holds 72 head_dim bytes: key codes, the keys' pairs, value codes, the
+ * values' pairs.  Position t of a page has slot 4 (t % 16) + t / 16.  Key codes
+ * lie as [t / 32][dim / 64][dim / 16 % 4][t % 16][t / 16 % 2][16 dims], value
+ * codes as [dim / 32][slot / 16][dim % 16][dim / 16 % 2][16 slots]; 16 codes
+ * are two words, byte i of word w holding elements 8 w + i (low nibble) and
+ * 8 w + 4 + i (high).  Pairs of fp16 scale and mid lie as [dim / 64][slot]. */
 #define IBH_KV4_PAGE 64
 typedef struct {
     void* pool;

@@ -1902,8 +1902,10 @@ bool cache_ok(const ibh_kv4_cache* c, const char* who) {
 Kv4 device_of(const ibh_kv4_cache* c) {
     return {(uint8_t*)c->pool, c->table, c->lens, c->n_pages, c->n_seq, c->max_pages, c->n_kv, c->head_dim};
 }
+// No launch of this file has blocks of more than 1024 threads; one takes less
+// than 2^32 threads.
 bool grid_ok(size_t blocks, const char* who) {
-    if (blocks <= 0x7fffffffu) return true;
+    if (blocks < (size_t)1 << 22) return true;
     ibh_set_error("%s: %zu blocks of work are more than one launch takes", who, blocks);
     return false;
 }

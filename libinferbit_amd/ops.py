@@ -119,45 +119,56 @@ class Kv4Cache:
             raise ValueError("table must be [n_seq, max_pages] and lens [n_seq]")
         if table.dtype != torch.int32 or lens.dtype != torch.int32 or pool.dtype != torch.uint8:
             raise TypeError("a cache is a uint8 pool with an int32 table and int32 lens")
-        self.device = pool.device
+        self.device, self.index = pool.device, pool.get_device()
         self.pool, self.table, self.lens = pool, table, lens
         self.n_seq, self.max_pages = table.shape
         self.n_kv, self.head_dim = n_kv, head_dim
         size = lib().ibh_kv4_page_bytes(n_kv, head_dim)
         if not size or pool.numel() % size:
             raise ValueError(f"the pool is not whole pages of {n_kv} heads of {head_dim}")
-        self.desc = Kv4Desc(_ptr(pool), self._on(table), self._on(lens), pool.numel() // size, self.n_seq,
-                            self.max_pages, n_kv, head_dim)
+        self.desc = Kv4Desc(_ptr(pool), self._on(table, torch.int32, table.numel()),
+                            self._on(lens, torch.int32, self.n_seq), pool.numel() // size, self.n_seq, self.max_pages,
+                            n_kv, head_dim)
         self.ref = ctypes.byref(self.desc)
 
-    def _on(self, t, dtype=None, numel=None):
-        """t's address, if it is a contiguous tensor of this cache's GPU with the given type and size."""
-        if t.device != self.device:
+    def _on(self, t, dtype, numel):
+        """The address of t, a contiguous tensor of this cache's GPU with the given type and size."""
+        if t.get_device() != self.index:
             raise ValueError(f"operand on {t.device}, the cache is on {self.device}")
-        if dtype is not None and t.dtype != dtype:
+        if t.dtype != dtype:
             raise TypeError(f"operand must be {dtype}, got {t.dtype}")
-        if numel is not None and t.numel() != numel:
+        if t.numel() != numel:
             raise ValueError(f"operand must have {numel} elements, got {t.numel()}")
-        return _ptr(t)
+        if not t.is_contiguous():
+            raise ValueError("operand must be contiguous")
+        return t.data_ptr()
 
     def _rows(self, t, width: int):
         """(address, rows per sequence, floats between rows) of [n_seq, n, width] fp32 rows with unit inner stride."""
-        if t.device != self.device or not t.is_cuda:
+        if t.get_device() != self.index:
             raise ValueError(f"operand on {t.device}, the cache is on {self.device}")
         if t.dtype != torch.float32:
             raise TypeError(f"operand must be torch.float32, got {t.dtype}")
-        if t.dim() != 3 or t.shape[0] != self.n_seq or t.shape[2] != width:
-            raise ValueError(f"operand must be [{self.n_seq}, n, {width}], got {list(t.shape)}")
-        n = t.shape[1]
+        shape = t.shape
+        if len(shape) != 3 or shape[0] != self.n_seq or shape[2] != width:
+            raise ValueError(f"operand must be [{self.n_seq}, n, {width}], got {list(shape)}")
+        n = shape[1]
         s0, s1, s2 = t.stride()
         if n == 1:
             s1 = s0 if self.n_seq > 1 else width
-        if s2 != 1 or s1 < width or (self.n_seq > 1 and s0 != n * s1):
+        if s2 != 1 or s1 < width or s1 > 0x7fffffff or (self.n_seq > 1 and s0 != n * s1):
             raise ValueError("rows must be evenly spaced with contiguous elements")
         return t.data_ptr(), n, s1
 
+    def _workspace(self, need: int):
+        """(address, bytes, the tensor to keep) of `need` bytes of scratch memory of the current stream."""
+        if not need:
+            return None, 0, None
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        return ws.data_ptr(), need, ws
+
     def _call(self, name: str, *args) -> None:
-        index = self.device.index
+        index = self.index
         # the current stream's handle without the Python object around it: that takes 1.8 us of a call's 8
         stream = torch._C._cuda_getCurrentRawStream(index)
         if torch.cuda.current_device() == index:
@@ -189,7 +200,7 @@ def kv4_attn(out, q, cache: Kv4Cache, n_heads: int, weights_in=None, weights_out
     """Attention of the last q.shape[1] positions of every sequence: q [n_seq, n_q, n_heads * head_dim] (rows may be
     spaced), out the same, contiguous; weights fp32 [n_seq, n_kv, 64 * max_pages], accumulated from in to out."""
     pq, n_q, sq = cache._rows(q, n_heads * cache.head_dim)
-    po = cache._on(out, torch.float32, q.numel())
+    po = cache._on(out, torch.float32, cache.n_seq * n_q * n_heads * cache.head_dim)
     if (weights_in is None) != (weights_out is None):
         raise ValueError("weights_in and weights_out go together")
     wi = wo = None
@@ -197,25 +208,27 @@ def kv4_attn(out, q, cache: Kv4Cache, n_heads: int, weights_in=None, weights_out
         size = cache.n_seq * cache.n_kv * cache.max_pages * KV4_PAGE
         wi, wo = (cache._on(w, torch.float32, size) for w in (weights_in, weights_out))
     if ws is None:
-        need = lib().ibh_kv4_attn_workspace_bytes(cache.ref, n_heads, n_q, wi is not None)
-        ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
-    cache._call("ibh_kv4_attn", cache.ref, po, pq, n_heads, n_q, sq, wi, wo, None if ws is None else cache._on(ws),
-                0 if ws is None else ws.numel())
+        pw, nw, ws = cache._workspace(lib().ibh_kv4_attn_workspace_bytes(cache.ref, n_heads, n_q, wi is not None))
+    else:
+        pw, nw = cache._on(ws, torch.uint8, ws.numel()), ws.numel()
+    cache._call("ibh_kv4_attn", cache.ref, po, pq, n_heads, n_q, sq, wi, wo, pw, nw)
 
 
 def kv4_evict(src: Kv4Cache, dst: Kv4Cache, weights_src, weights_dst, budget: int, sink: int, recent: int,
               kept, ws=None) -> None:
     """Cuts every sequence to `budget` positions by accumulated weight: rows, weights and lengths into dst (src itself
     for in place), the kept positions into kept int32 [n_seq, n_kv, budget]."""
+    if dst.index != src.index:
+        raise ValueError(f"the caches are on {src.device} and {dst.device}")
     n = src.n_seq * src.n_kv
     if ws is None:
-        need = lib().ibh_kv4_evict_workspace_bytes(src.ref)
-        ws = torch.empty(need, dtype=torch.uint8, device=src.device) if need else None
+        pw, nw, ws = src._workspace(lib().ibh_kv4_evict_workspace_bytes(src.ref))
+    else:
+        pw, nw = src._on(ws, torch.uint8, ws.numel()), ws.numel()
     src._call("ibh_kv4_evict", src.ref, dst.ref,
               src._on(weights_src, torch.float32, n * src.max_pages * KV4_PAGE),
               src._on(weights_dst, torch.float32, n * dst.max_pages * KV4_PAGE), budget, sink, recent,
-              src._on(kept, torch.int32, n * budget), None if ws is None else src._on(ws),
-              0 if ws is None else ws.numel())
+              src._on(kept, torch.int32, n * budget), pw, nw)
 
 
 class PqDeviceTensor:

@@ -95,6 +95,16 @@ def test_bad_arguments_are_refused():
         refused("ibh_kv4_evict", *evict(**bad))
 
 
+def test_more_work_than_a_launch_takes_is_refused():
+    c = C.byref(desc(n_seq=1 << 20, n_kv=64, max_pages=1 << 10))
+    assert "launch" in refused("ibh_kv4_append", c, 4096, 4096, 1, 64 * 64, None)
+    assert "launch" in refused("ibh_kv4_read", c, 4096, 4096, 1, 64 * 64, None)
+    assert "launch" in refused("ibh_kv4_attn", c, 4096, 4096, 64, 1, 4096, None, None, 4096, (1 << 63) - 1, None)
+    to = C.byref(desc(n_seq=1 << 20, n_kv=64, max_pages=1 << 10, table=8192, lens=8192))
+    assert "launch" in refused("ibh_kv4_evict", c, to, 4096, 8192, 64, 0, 0, 4096, 4096, (1 << 63) - 1, None)
+    refused("ibh_kv4_attn", C.byref(desc()), 4096, 4096, 1 << 20, 1 << 20, (1 << 31) - 1, None, None, 4096, 1 << 62, None)
+
+
 def test_sizes():
     L = _lib.lib()
     assert L.ibh_kv4_page_bytes(8, 128) == 8 * 9216

@@ -185,10 +185,11 @@ def test_attention(ops, n_heads, n_kv, hd, n_q, lens, weights):
     assert device_errors() == 0
 
 
-def test_attention_long_and_strided(ops):
+@pytest.mark.parametrize("n_q", [2, 12])
+def test_attention_long_and_strided(ops, n_q):
     """Many pages for one head, q inside wider rows and off 16 bytes."""
     rng = np.random.default_rng(11)
-    n_heads, n_kv, hd, n_q = 4, 1, 128, 2
+    n_heads, n_kv, hd = 4, 1, 128
     m = Made(ops, rng, [9001, 4097], n_kv, hd)
     wide = torch.from_numpy(rng.standard_normal((2, n_q, n_heads * hd + 5)).astype(np.float32)).cuda()
     q = wide[:, :, 3:3 + n_heads * hd]
@@ -214,20 +215,21 @@ def test_attention_sharp_and_flat_scores(ops, n_q):
     check_attention(ops, m, q, n_heads, n_q, out, wi, wo)
 
 
-def test_attention_small_values_beside_large_scales(ops):
+@pytest.mark.parametrize("n_q", [1, 11])
+def test_attention_small_values_beside_large_scales(ops, n_q):
     """The heaviest position has values a thousandth of the others', as a sink position has."""
     rng = np.random.default_rng(4)
     n_heads, n_kv, hd, t = 4, 1, 64, 190
     m = Made(ops, rng, [t], n_kv, hd)
-    q = torch.from_numpy(rng.standard_normal((1, 1, n_heads * hd)).astype(np.float32)).cuda()
-    # a first position along every query
-    m.k[0][0] = q.cpu().numpy()[0, 0].reshape(n_heads, hd).sum(0) * 3
+    q = torch.from_numpy(rng.standard_normal((1, n_q, n_heads * hd)).astype(np.float32)).cuda()
+    # a first position along the last query's heads
+    m.k[0][0] = q.cpu().numpy()[0, -1].reshape(n_heads, hd).sum(0) * 3
     m.v[0][0] *= 1e-3
     m.v[0][5] *= 1e3
     ops.kv4_append(m.cache, torch.from_numpy(m.k[0][None]).cuda(), torch.from_numpy(m.v[0][None]).cuda())
     out = torch.empty_like(q)
     ops.kv4_attn(out, q, m.cache, n_heads)
-    check_attention(ops, m, q, n_heads, 1, out)
+    check_attention(ops, m, q, n_heads, n_q, out)
 
 
 @pytest.mark.parametrize("n_q", [4, 40])
@@ -348,14 +350,16 @@ def test_evict(ops, n_kv, hd, lens, budget, sink, recent, in_place):
             gw = tw[i, h].cpu().numpy()
             np.testing.assert_array_equal(gw[:new].view(np.uint32), w[i, h, f].view(np.uint32))
             assert (gw[new:] == 0).all()
-            for j, s in enumerate(f):
-                a = host[m.table[i, s // 64]].reshape(n_kv, -1)[h]
-                b = want[table[i, j // 64]].reshape(n_kv, -1)[h]
+            # the kept rows' codes and pairs, page by page of the destination
+            src = host[m.table[i]].reshape(-1, n_kv, 72 * hd)[:, h]
+            for p in range((new + 63) // 64):
+                g = f[64 * p:64 * p + 64]
+                b = want[table[i, p]].reshape(n_kv, -1)[h]
                 for at, shift, pair in R.places(hd):
-                    code = (a[at[s % 64]] >> shift[s % 64].astype(np.uint8)) & 15
-                    np.bitwise_or.at(b, at[j % 64], code << shift[j % 64].astype(np.uint8))
+                    code = (src[(g // 64)[:, None], at[g % 64]] >> shift[g % 64].astype(np.uint8)) & 15
+                    np.bitwise_or.at(b, at[:len(g)], code << shift[:len(g)].astype(np.uint8))
                     for o in (0, 1):
-                        b.view(np.uint16)[pair[j % 64] + o] = a.view(np.uint16)[pair[s % 64] + o]
+                        b.view(np.uint16)[pair[:len(g)] + o] = src.view(np.uint16)[(g // 64)[:, None], pair[g % 64] + o]
     np.testing.assert_array_equal(got, want)
     if not in_place:
         assert torch.equal(m.dpool, src_before) and m.dlens.tolist() == list(lens)
@@ -516,3 +520,7 @@ def test_python_refusals(ops):
         ops.kv4_attn(z(2, 1, 192), z(2, 1, 192), c, 3)
     with pytest.raises(TypeError):
         ops.kv4_evict(c, c, z(2, 2, 64), z(2, 2, 64), 5, 0, 0, z(2, 2, 5))
+    with pytest.raises(L.IbhError):                               # half in place
+        ops.kv4_evict(c, c, z(2, 2, 64), z(2, 2, 64), 5, 0, 0, z(2, 2, 5, dtype=torch.int32))
+    with pytest.raises(L.IbhError):
+        ops.kv4_attn(z(2, 1, 2048), z(2, 1, 2048), Made(ops, rng, [4100, 1], 2, 64).cache, 32, ws=z(8, dtype=torch.uint8))
