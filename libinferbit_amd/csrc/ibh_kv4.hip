@@ -711,18 +711,30 @@ __global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(
 // ── attention of many rows ───────────────────────────────────────────────────
 // From 33 query rows of a KV head on the sums are the f16 matrix cores': a row
 // is one row of the MFMA, the query and p * scale are the sum of two fp16
-// numbers (22 bits of every element that is not 2^18 below its bound), the
-// codes are fp16 numbers -8 .. 7, and products are added in fp32.  That takes
-// as many MFMAs as three digits in four rows, but no joining of digits, and
-// the values' sums stay in the accumulators from page to page.  Block: 64 rows,
-// 16 a wavefront; the four take a page's codes apart together, into LDS, as
-// the matrix cores read them (a code word is a lane's 8 elements of one MFMA:
+// numbers, the codes are fp16 numbers -8 .. 7, and products are added in fp32.
+// Such a sum has 22 bits, or steps of 2^-24 for numbers below 1/4: the query's
+// largest element is taken to 2^14 .. 2^15, a row's largest p * scale to 2^11
+// .. 2^16, so what is lost is below 2^-36 of the largest.  That takes as many
+// MFMAs as three digits in four rows, but no joining of digits, and the values'
+// sums stay in the accumulators from page to page.  Block: 64 rows, 16 a
+// wavefront; the four take a page's codes apart together, into LDS, as the
+// matrix cores read them (a code word is a lane's 8 elements of one MFMA:
 // halves 0, 2, 4, 6, 1, 3, 5, 7 of its bytes' order).
+//
+// 512 queries of 32 heads on 8 KV heads of 128 over 4100 positions: 130 us, 32
+// GFLOP at fp32's precision (the int8 kernel with 16 rows a block: 175 us).
+// The vector ALU is what it waits for most, busy 54% of the time at the two
+// wavefronts a SIMD that 220 registers leave: the exponentials, the rounding
+// of 64 p * scale a row and group into halves, and two barriers a page.  (Three
+// wavefronts a SIMD have 168 registers and spill.  A running maximum by 16-lane
+// reductions of every page's scores, as kv4_attn_kernel has it, and a factor of
+// p * scale for each row and group took 146 us.)
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 h8_alias __attribute__((ext_vector_type(8), may_alias));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 constexpr int kWideRows = 64;
+constexpr float kNoMax = -1e30f;                         // below every score
 
 __device__ __forceinline__ f4_t mfma32(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 // A code word's eight numbers: 1024 + code as fp16 bits, less 1032.
@@ -871,11 +883,12 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
         }
     }
 
+    // p is 2^(score - m); the values' sums o are those of p * scale * vf
     float m[4], l[4], om[4][HDG], vf[HDG], vtop[HDG];
     f4_t o[4 * HDG];
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-        m[r] = -INFINITY;
+        m[r] = kNoMax;
         l[r] = 0.f;
 #pragma unroll
         for (int g = 0; g < HDG; g++) om[r][g] = 0.f;
@@ -917,20 +930,58 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
 #pragma unroll
                 for (int r = 0; r < 4; r++) x[r][s] = pos0 + 16 * s + li <= lim[r] ? x[r][s] : -INFINITY;
         }
-        // the running maximum moves only when a score is over 2^8 times above
-        // it: p stays below 2^8, for which the values' factor leaves room
-        float top[4];
-        bool up = false;
+        // a power of two takes the largest of a group's scales so far to 2^11 .. 2^12
+        float vs[HDG][4], vsm[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            top[r] = row16_max(fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3]))) * kf[r];
-            up |= top[r] > m[r] + 8.f;
+        for (int g = 0; g < HDG; g++) {
+            float vt = 0.f;
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                vs[g][s] = h2f(part4(*(const uint4*)&prs[1][g][4 * li], s));
+                if constexpr (MASKED) vs[g][s] = pos0 + 16 * s + li <= lim_hi ? vs[g][s] : 0.f;   // stale pairs may be anything
+                vt = fmaxf(vt, vs[g][s]);
+            }
+            if (__any(vt > vtop[g])) {
+                vtop[g] = fmaxf(row16_max(vt), vtop[g]);
+                const float nf = ldexpf(1.f, 12 - __builtin_amdgcn_frexp_expf(vtop[g])), al = nf / vf[g];
+                vf[g] = nf;
+#pragma unroll
+                for (int d = 0; d < 4; d++) o[4 * g + d] *= al;
+            }
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                vs[g][s] *= vf[g];
+                vsm[s] = fmaxf(vsm[s], vs[g][s]);
+            }
         }
-        if (__any(up)) {
+        float e[4][4];
+        auto probs = [&]() {
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int s = 0; s < 4; s++) e[r][s] = exp2_(fmaf(x[r][s], kf[r], -m[r]));
+        };
+        probs();
+        // m moves only when a p * scale no longer fits fp16 or a p is above
+        // 2^60.  It is then set such that the page's largest p * scale is in
+        // 2^11 .. 2^12, or its largest p 2^40 where all that the row looks at
+        // have next to no scale.
+        float most = 0.f, high = 0.f;
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            const float pm = fmaxf(fmaxf(e[0][s], e[1][s]), fmaxf(e[2][s], e[3][s]));
+            high = fmaxf(high, pm);
+            most = fmaxf(most, pm * vsm[s]);
+        }
+        if (__any(most > 65504.f || high > 0x1p60f)) {
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const float mn = fmaxf(m[r], top[r]);
-                const float al = mn == -INFINITY ? 1.f : exp2_(m[r] - mn);
+                const float top = row16_max(fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3]))) * kf[r];
+                float w = 0.f;
+#pragma unroll
+                for (int s = 0; s < 4; s++) w = fmaxf(w, exp2_(fmaf(x[r][s], kf[r], -top)) * vsm[s]);
+                const float to = top - (float)min(12 - __builtin_amdgcn_frexp_expf(row16_max(w)), 40);
+                const float mn = top == -INFINITY ? m[r] : fmaxf(m[r], to), al = exp2_(m[r] - mn);
                 m[r] = mn;
                 l[r] *= al;
 #pragma unroll
@@ -938,55 +989,29 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
 #pragma unroll
                 for (int g = 0; g < HDG; g++) om[r][g] *= al;
             }
+            probs();
         }
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const float mk = m[r] == -INFINITY ? 0.f : -m[r];
+        for (int r = 0; r < 4; r++)
 #pragma unroll
-            for (int s = 0; s < 4; s++) {
-                x[r][s] = exp2_(fmaf(x[r][s], kf[r], mk));
-                l[r] += x[r][s];
-            }
-        }
+            for (int s = 0; s < 4; s++) l[r] += e[r][s];
 #pragma unroll
         for (int g = 0; g < HDG; g++) {
-            // p * scale times a power of two that takes the largest scale so
-            // far to 2^6 .. 2^7
-            float vs[4], vm[4], vt = 0.f;
+            float vm[4];
 #pragma unroll
-            for (int s = 0; s < 4; s++) {
-                const uint32_t pr = part4(*(const uint4*)&prs[1][g][4 * li], s);
-                vs[s] = h2f(pr);
-                vm[s] = h2f(pr >> 16);
-                if constexpr (MASKED) {                  // stale pairs may be anything
-                    const bool any = pos0 + 16 * s + li <= lim_hi;
-                    vs[s] = any ? vs[s] : 0.f;
-                    vm[s] = any ? vm[s] : 0.f;
-                }
-                vt = fmaxf(vt, vs[s]);
-            }
-            vt = row16_max(vt);
-            if (__any(vt > vtop[g])) {
-                vtop[g] = fmaxf(vt, vtop[g]);
-                const float nf = ldexpf(1.f, 7 - __builtin_amdgcn_frexp_expf(vtop[g])), al = nf / vf[g];
-                vf[g] = nf;
-#pragma unroll
-                for (int d = 0; d < 4; d++) o[4 * g + d] *= al;
-            }
-#pragma unroll
-            for (int s = 0; s < 4; s++) vs[s] *= vf[g];
+            for (int s = 0; s < 4; s++) vm[s] = h2f(part4(*(const uint4*)&prs[1][g][4 * li], s) >> 16);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 float w[4];
 #pragma unroll
                 for (int s = 0; s < 4; s++) {
-                    w[s] = x[r][s] * vs[s];
+                    w[s] = e[r][s] * vs[g][s];
                     if constexpr (MASKED) {              // a NaN that this row does not see
                         const bool ok = pos0 + 16 * s + li <= lim[r];
                         w[s] = ok ? w[s] : 0.f;
-                        om[r][g] += ok ? x[r][s] * vm[s] : 0.f;
+                        om[r][g] += ok ? e[r][s] * vm[s] : 0.f;
                     } else {
-                        om[r][g] = fmaf(x[r][s], vm[s], om[r][g]);
+                        om[r][g] = fmaf(e[r][s], vm[s], om[r][g]);
                     }
                 }
                 // slots 4 li + s: quarter li / 4, half li / 2 % 2, then s = 0, 2 and s = 1, 3

@@ -232,6 +232,29 @@ def test_attention_small_values_beside_large_scales(ops, n_q):
     check_attention(ops, m, q, n_heads, n_q, out)
 
 
+@pytest.mark.parametrize("hd", [64, 192])
+@pytest.mark.parametrize("n_q", [1, 3, 12])
+def test_attention_tiny_values_after_large_ones(ops, n_q, hd):
+    """Values of 2^10 that no query looks at, beside and before those of 2^-14 that all look at: the large ones get
+    probabilities below 2^-60, so the small ones alone decide the output."""
+    rng = np.random.default_rng(41 + hd)
+    n_heads, n_kv, t = 8, 2, 330
+    m = Made(ops, rng, [t], n_kv, hd)
+    u = rng.choice([-1.0, 1.0], hd)
+    seen = np.arange(t) % 64 > 40                             # the end of every page
+    seen[:70] = False                                         # and nothing of the first one
+    k = rng.standard_normal((t, n_kv, hd)) * 0.1 + np.where(seen, 3.0, -3.0)[:, None, None] * u
+    v = rng.standard_normal((t, n_kv, hd)) * np.where(seen, 2.0 ** -14, 2.0 ** 10)[:, None, None]
+    m.k[0], m.v[0] = (x.reshape(t, -1).astype(np.float32) for x in (k, v))
+    ops.kv4_append(m.cache, torch.from_numpy(m.k[0][None]).cuda(), torch.from_numpy(m.v[0][None]).cuda())
+    q = rng.standard_normal((1, n_q, n_heads, hd)) * 0.1 + 10 / np.sqrt(hd) * u
+    q = torch.from_numpy(q.reshape(1, n_q, n_heads * hd).astype(np.float32)).cuda()
+    out = torch.empty_like(q)
+    ops.kv4_attn(out, q, m.cache, n_heads)
+    assert out.abs().max() < 2.0 ** -10
+    check_attention(ops, m, q, n_heads, n_q, out)
+
+
 @pytest.mark.parametrize("n_q", [4, 40])
 def test_attention_not_finite(ops, n_q):
     """A NaN key makes the rows that see it NaN, a NaN value its 64 dims; rows that do not see it, and what lies
