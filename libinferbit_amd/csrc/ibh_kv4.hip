@@ -377,7 +377,9 @@ struct AttnArgs {
     const float* q;
     int n_heads, n_q, q_stride;
     float scale;                                         // log2(e) / sqrt(head_dim)
-    int chunk, n_split, n_tile;                          // pages of a block, blocks of a row tile, row tiles of a KV head
+    int n_split, n_tile;                                 // most blocks of a row tile, row tiles of a KV head
+    int chunk, quantum;                                  // pages of a block where a table row is full; a multiple of this
+    uint32_t per_split;                                  // 2^32 / n_split, rounded up
     int tile_rows;                                       // query rows of a row tile
     float* part;                                         // [seq][KV head][row][split][head_dim], when n_split > 1
     float2* part_ml;                                     // [seq][KV head][row][split] maximum (log2) and sum
@@ -387,6 +389,17 @@ struct AttnArgs {
     float* rowc;                                         // [seq][KV head][row][1 + groups] step * scale, sums of the query in steps
     float4* scores;                                      // [seq][KV head][page][tile][lane] scores (log2), -inf where not seen
 };
+
+// Pages of a block, for a sequence of `pages`: an equal share, whatever the
+// table could hold (32 sequences of 4096 positions in tables of 32768: 39 us,
+// 75 with blocks cut by the tables' size).
+__host__ __device__ __forceinline__ int chunk_of(int pages, int n_split, uint32_t per_split, int quantum) {
+    const uint32_t each = (uint32_t)(((uint64_t)(uint32_t)(pages + n_split - 1) * per_split) >> 32);
+    return max((int)((each + quantum - 1) & ~(uint32_t)(quantum - 1)), quantum);
+}
+__device__ __forceinline__ int chunk_of(const AttnArgs& a, int len) {
+    return a.n_split == 1 ? a.chunk : chunk_of((len + kPage - 1) / kPage, a.n_split, a.per_split, a.quantum);
+}
 
 // Wavefronts a SIMD holds: what the registers of a page and RT tiles leave.
 constexpr int attn_waves(int hdg, int rt) { return hdg * rt == 1 ? 4 : hdg * rt == 2 ? 3 : hdg * rt >= 8 && hdg > 2 ? 1 : 2; }
@@ -412,17 +425,19 @@ __global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(
     const int rt = a.n_tile - 1 - b % a.n_tile; b /= a.n_tile;
     const int split = b % a.n_split, seq = b / a.n_split;
     const int grp = a.n_heads / c.n_kv, n_rows = a.n_q * grp;
-    // the first page's number with the length, not behind it
-    const int p0 = split * a.chunk;
-    int p = p0 + wave;
-    const int id0 = ld_uniform(c.table + (size_t)seq * c.max_pages + min(p, c.max_pages - 1));
+    // the first page's number with the length, not behind it: that of a full row
+    const int32_t* const ids = c.table + (size_t)seq * c.max_pages;
+    int id0 = ld_uniform(ids + min(split * a.chunk + wave, c.max_pages - 1));
     bool bad;
-    const int len = seq_len(c, seq, &bad);
+    const int len = seq_len(c, seq, &bad), chunk = chunk_of(a, len);
+    const int p0 = split * chunk;
+    int p = p0 + wave;
+    if (chunk != a.chunk) id0 = ld_uniform(ids + min(p, c.max_pages - 1));
     const int row0 = rt * ROWS;
     // the last position that each row sees; rows past the last copy it
     const int lim_min = len - a.n_q + row0 / grp, lim_max = len - a.n_q + min(row0 + ROWS - 1, n_rows - 1) / grp;
     const int pages = lim_max < 0 ? 0 : lim_max / kPage + 1;
-    const int p1 = min(p0 + a.chunk, pages);
+    const int p1 = min(p0 + chunk, pages);
     if (split > 0 && p0 >= pages) return;
     int lim[RT];
 #pragma unroll
@@ -780,14 +795,16 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
     const int rt = a.n_tile - 1 - b % a.n_tile; b /= a.n_tile;
     const int split = b % a.n_split, seq = b / a.n_split;
     const int grp = a.n_heads / c.n_kv, n_rows = a.n_q * grp;
-    const int p0 = split * a.chunk;
-    const int id0 = ld_uniform(c.table + (size_t)seq * c.max_pages + min(p0, c.max_pages - 1));
+    const int32_t* const ids = c.table + (size_t)seq * c.max_pages;
+    int id0 = ld_uniform(ids + min(split * a.chunk, c.max_pages - 1));
     bool bad;
-    const int len = seq_len(c, seq, &bad);
+    const int len = seq_len(c, seq, &bad), chunk = chunk_of(a, len);
+    const int p0 = split * chunk;
+    if (chunk != a.chunk) id0 = ld_uniform(ids + min(p0, c.max_pages - 1));
     const int base = len - a.n_q;                        // the first query's position
     const int lim_block = base + min(rt * kWideRows + kWideRows - 1, n_rows - 1) / grp;
     const int pages = lim_block < 0 ? 0 : lim_block / kPage + 1;
-    const int p1 = min(p0 + a.chunk, pages);
+    const int p1 = min(p0 + chunk, pages);
     if (split > 0 && p0 >= pages) return;
     const int row0 = rt * kWideRows + wave * 16;
     const bool active = row0 < n_rows;
@@ -1209,7 +1226,8 @@ __global__ __launch_bounds__(512) void kv4_weights_wide(Kv4 c, AttnArgs a, WideR
 __device__ __forceinline__ int splits_of(const AttnArgs& a, int len, int row, int grp, int n_rows) {
     const int last = min(row / a.tile_rows * a.tile_rows + a.tile_rows, n_rows) - 1;
     const int lim = len - a.n_q + last / grp;
-    return lim < 0 ? 1 : (lim / kPage + a.chunk) / a.chunk;
+    const int chunk = chunk_of(a, len);
+    return lim < 0 ? 1 : (lim / kPage + chunk) / chunk;
 }
 
 // A page's keys, and 2^(score - lse) of its positions summed over the rows of
@@ -1989,7 +2007,8 @@ extern "C" int ibh_kv4_read(const ibh_kv4_cache* cache, float* k, float* v, int 
 
 // How a call is cut: row tiles of 4 rt query rows, blocks of `chunk` pages.
 struct AttnPlan {
-    int rt, n_tile, chunk, n_split, nw;                  // rt 16: kv4_attn_wide
+    int rt, n_tile, n_split, chunk, quantum, nw;         // rt 16: kv4_attn_wide
+    uint32_t per_split;
     bool joint;                                          // the weights in the launch that joins the splits
     size_t part, part_ml, lse, digits, rowc, score, bytes;     // offsets into the workspace
 };
@@ -2000,16 +2019,47 @@ static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool wei
     const bool wide = n_rows > 32;
     p.rt = wide ? kWideRows / 4 : n_rows <= 4 ? 1 : n_rows <= 8 || hdg > 2 ? 2 : 4;
     p.n_tile = (int)((n_rows + 4 * p.rt - 1) / (4 * p.rt));
-    const size_t work = heads * p.n_tile * c->max_pages, want = p.rt <= 2 ? 2048 : 1024;
-    size_t chunk = (work + want - 1) / want;
-    chunk = max(chunk, ((size_t)c->max_pages + kMaxSplit - 1) / kMaxSplit);
-    p.chunk = (int)((chunk + 3) / 4 * 4);
-    // up to 1024 positions a decode step is one launch: eight wavefronts take a
-    // head's pages, and nothing is left to join (600 positions of 32/4 heads:
-    // 7 us in one kernel, 7 + 3 in two)
-    p.nw = p.n_tile == 1 && p.rt <= 2 && (int)hdg * p.rt <= 6 && c->max_pages > 4 && c->max_pages <= 16 ? 8 : 4;
-    if (p.nw == 8) p.chunk = 16;
-    p.n_split = (c->max_pages + p.chunk - 1) / p.chunk;
+    const size_t base = heads * p.n_tile;
+    p.nw = 4;
+    p.quantum = 4;
+    size_t n = 1;
+    if (wide) {
+        // every block works at once, or in whole rounds: what a round takes in
+        // pages (and one for its start), and what the partial sums cost that
+        // are written and joined
+        p.quantum = 1;
+        const size_t slots = 256 * (hdg == 1 ? 3 : hdg == 2 ? 2 : 1);
+        double least = (double)((base + slots - 1) / slots) * (c->max_pages + 1);
+        for (size_t k = 1; k <= 4; k++) {
+            const size_t m = min(min(k * slots / base, (size_t)c->max_pages), (size_t)kMaxSplit);
+            if (m < 2) continue;
+            const double cost = (double)((base * m + slots - 1) / slots) * ((c->max_pages + m - 1) / m + 1) + base * m / 228.0 + 1.5;
+            if (cost < least) {
+                least = cost;
+                n = m;
+            }
+        }
+    } else {
+        const size_t work = base * c->max_pages, want = p.rt <= 2 ? 2048 : 1024;
+        size_t chunk = (work + want - 1) / want;
+        chunk = max(chunk, ((size_t)c->max_pages + kMaxSplit - 1) / kMaxSplit);
+        chunk = (chunk + 3) / 4 * 4;
+        // up to 1024 positions a decode step is one launch: eight wavefronts take a
+        // head's pages, and nothing is left to join (600 positions of 32/4 heads:
+        // 7 us in one kernel, 7 + 3 in two)
+        if (p.n_tile == 1 && p.rt <= 2 && (int)hdg * p.rt <= 6 && c->max_pages > 4 && c->max_pages <= 16) {
+            p.nw = 8;
+            chunk = 16;
+        }
+        n = (c->max_pages + chunk - 1) / chunk;
+        // two pages a wavefront where there are blocks enough (32 sequences of 128 .. 4096
+        // positions, 8 KV heads: 28.9 us, 30.4 with one), else one (4 sequences of 4096
+        // in tables of 131072: 15.8 us, 16.9 with two)
+        if (chunk >= 8 && base >= 128) p.quantum = 8;
+    }
+    p.n_split = (int)n;
+    p.per_split = n > 1 ? (uint32_t)((((uint64_t)1 << 32) + n - 1) / n) : 0;
+    p.chunk = n > 1 ? chunk_of(c->max_pages, p.n_split, p.per_split, p.quantum) : c->max_pages;
     p.joint = weights && p.n_tile == 1 && p.n_split > 1 && p.rt <= 2;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
@@ -2090,8 +2140,8 @@ extern "C" int ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float*
         !grid_ok(heads * n_q * (n_heads / cache->n_kv) + heads * cache->max_pages, "ibh_kv4_attn"))
         return IBH_ERROR_PARAM;
     char* w = (char*)ws;
-    AttnArgs a{out, q, n_heads, n_q, q_stride, (float)(1.4426950408889634 / sqrt((double)cache->head_dim)), p.chunk,
-               p.n_split, p.n_tile, 4 * p.rt, (float*)(w + p.part), (float2*)(w + p.part_ml),
+    AttnArgs a{out, q, n_heads, n_q, q_stride, (float)(1.4426950408889634 / sqrt((double)cache->head_dim)),
+               p.n_split, p.n_tile, p.chunk, p.quantum, p.per_split, 4 * p.rt, (float*)(w + p.part), (float2*)(w + p.part_ml),
                weights_out && !p.joint ? (float*)(w + p.lse) : nullptr,
                p.rt == kWideRows / 4 ? p.n_tile * kWideRows : n_q * (n_heads / cache->n_kv),
                weights_out && !p.joint ? (i4_t*)(w + p.digits) : nullptr, (float*)(w + p.rowc), (float4*)(w + p.score)};

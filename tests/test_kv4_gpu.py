@@ -185,6 +185,25 @@ def test_attention(ops, n_heads, n_kv, hd, n_q, lens, weights):
     assert device_errors() == 0
 
 
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("n_seq,n_heads,n_kv,hd,n_q,cap", [
+    (5, 8, 2, 64, 1, 40), (5, 8, 2, 128, 3, 333), (5, 8, 2, 64, 20, 41), (5, 4, 4, 256, 40, 40), (33, 8, 4, 64, 1, 100),
+    (33, 16, 4, 64, 2, 128)])
+def test_attention_in_tables_with_room(ops, n_seq, n_heads, n_kv, hd, n_q, cap, weights):
+    """Tables of many more pages than the sequences have: their pages are shared out over the blocks all the same."""
+    print(f"case room {n_seq} {n_heads}/{n_kv} hd={hd} n_q={n_q} cap={cap} weights={weights}", flush=True)
+    rng = np.random.default_rng(cap + n_q + hd)
+    lens = [int(t) for t in rng.permutation([0, 1, 64, 65, 700, *rng.integers(1, 500, n_seq)])[:n_seq]]
+    m = Made(ops, rng, lens, n_kv, hd, max_pages=cap)
+    q = torch.from_numpy(rng.standard_normal((n_seq, n_q, n_heads * hd)).astype(np.float32)).cuda()
+    out = torch.full_like(q, float("nan"))
+    wi = torch.from_numpy(rng.random((n_seq, n_kv, cap * 64)).astype(np.float32)).cuda() if weights else None
+    wo = torch.full_like(wi, float("nan")) if weights else None
+    ops.kv4_attn(out, q, m.cache, n_heads, **(dict(weights_in=wi, weights_out=wo) if weights else {}))
+    check_attention(ops, m, q, n_heads, n_q, out, wi, wo)
+    assert device_errors() == 0
+
+
 @pytest.mark.parametrize("n_q", [2, 12])
 def test_attention_long_and_strided(ops, n_q):
     """Many pages for one head, q inside wider rows and off 16 bytes."""
