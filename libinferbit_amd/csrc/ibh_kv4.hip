@@ -85,8 +85,10 @@ __device__ __forceinline__ int val_off(int d, int r) {
 // of 2^-24 of at most 9), rounded; where it comes within 2^-17 of a border
 // the wavefront compares x - mid with the exact borders (c +- 1/2) scale in
 // fp64, so the codes are those of the exact quotient.  (Dividing and comparing
-// for every element took 23 us where this takes 12: 4099 positions of 8 heads
-// of 128, 43 MB.)
+// every element took twice as long.)  4099 positions of 8 heads of 128: 38 MB
+// in 17 us, from cold caches.  What is left is one pass of loads, arithmetic,
+// LDS and stores a block: 2080 blocks are about one round, and the
+// chain of one block is what shows.
 __device__ __forceinline__ void touched(const Kv4& c, int n, int n_touch, int& g, int& side, int& h, int& seq, int& pi) {
     int b = blockIdx.x;
     g = b % (c.hd / 64); b /= c.hd / 64;
@@ -1310,7 +1312,9 @@ struct PageWeights {
     }
 };
 
-// Joins few splits of many rows: a wavefront a row, 64 HDG dims a lane's HDG.
+// Joins up to 8 splits of many rows: a wavefront a row (16384 rows of 128 dims
+// and 2 splits, 25 MB: 11 us; 29 by a block a row).
+constexpr int kFewSplits = 8;
 template <int HDG>
 __global__ __launch_bounds__(256) void kv4_attn_join(Kv4 c, AttnArgs a, size_t rows) {
     constexpr int HD = 64 * HDG;
@@ -1357,11 +1361,13 @@ __device__ __forceinline__ float row_lse(const float2* ml, int n, int li) {
 // What is left after the pages' blocks.  Blocks below n_join join the splits
 // of a query row: 16 HDG threads hold four dims each, the other threads take
 // other splits, so that all partial sums are in flight together.  The others,
-// where one row tile holds all rows, score a page a wavefront again for the
-// accumulated weights; they take lse from the splits' maxima and sums
-// themselves, so that they need not wait for the joining blocks.  (Scores kept
-// by the first kernel instead cost it 9 us of 26 at 32 sequences of up to 4096
-// positions: 1 KB stored a page, behind which its loads wait.)
+// where one row tile holds all rows, take a page a wavefront and turn the
+// scores that the first kernel kept into weights; they take lse from the
+// splits' maxima and sums themselves, so that they need not wait for the
+// joining blocks.  At 32 sequences of up to 4096 positions, 8 KV heads of 128,
+// this launch takes 10 us, and keeping the scores costs the first 1.2 us, by
+// nontemporal stores behind a page's loads (9 us by ordinary ones, which the
+// next loads wait for).  Scoring the pages again here took 20 us.
 template <int HDG, int RT>
 __global__ __launch_bounds__(256) void kv4_attn_finish(Kv4 c, AttnArgs a, unsigned n_join, const float* win, float* wout) {
     constexpr int HD = 64 * HDG, TD = HD / 4, CLS = 256 / TD;
@@ -1805,8 +1811,8 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_long(Kv4 c, LongSel q,
 // half of a word, 16 apart), 256 contiguous bytes each, of which one nibble a
 // dim is used; the lanes then hand each other their nibbles (each half, then
 // each quarter of the lanes keeps its share) and end with what they write.
-// (Gathered byte by byte into LDS the page took 39 us where this takes 15: 16
-// sequences of 8 heads cut to 2000 positions.)
+// (Gathered byte by byte into LDS the page took 61 us where this takes 31: 16
+// sequences of 8 heads of 128 cut to 2000 positions.)
 template <int GROUPS, int HDG>
 __global__ __launch_bounds__(128 * HDG * GROUPS, GROUPS == 1 ? 5 : 4) void kv4_move(Kv4 src, Kv4 dst, const float* w_src, float* w_dst,
                                                                int budget, const int32_t* __restrict__ kept) {
@@ -2016,6 +2022,12 @@ static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool wei
     AttnPlan p;
     const size_t n_rows = (size_t)n_q * (n_heads / c->n_kv), hdg = c->head_dim / 64;
     const size_t heads = (size_t)c->n_seq * c->n_kv;
+    // Few rows: the smallest tile that holds them, so that pages are read once.
+    // A tile of 16 rows and head_dim above 128 would leave one wavefront a SIMD
+    // and spills: two tiles of 8 instead.  From 33 rows on the f16 kernel: 8
+    // sequences of 4096 positions, 8 KV heads of 128, 32 rows 40 us here and 41
+    // there, 40 rows 54 and 43, 64 rows 67 and 46 (one sequence, where neither
+    // fills the card: 21 and 23, 22 and 26).
     const bool wide = n_rows > 32;
     p.rt = wide ? kWideRows / 4 : n_rows <= 4 ? 1 : n_rows <= 8 || hdg > 2 ? 2 : 4;
     p.n_tile = (int)((n_rows + 4 * p.rt - 1) / (4 * p.rt));
@@ -2040,7 +2052,11 @@ static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool wei
             }
         }
     } else {
-        const size_t work = base * c->max_pages, want = p.rt <= 2 ? 2048 : 1024;
+        // as many blocks as the card holds at once: each has its rows to set
+        // up and its sums to write and join (8 sequences of 4096 positions, 8
+        // KV heads of 128: 17 us with 4 rows, 40 with 32; 20 and 48 with 2048
+        // and 1024 blocks where 768 and 512 are held)
+        const size_t work = base * c->max_pages, want = 256 * attn_waves((int)hdg, p.rt);
         size_t chunk = (work + want - 1) / want;
         chunk = max(chunk, ((size_t)c->max_pages + kMaxSplit - 1) / kMaxSplit);
         chunk = (chunk + 3) / 4 * 4;
@@ -2052,10 +2068,6 @@ static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool wei
             chunk = 16;
         }
         n = (c->max_pages + chunk - 1) / chunk;
-        // two pages a wavefront where there are blocks enough (32 sequences of 128 .. 4096
-        // positions, 8 KV heads: 28.9 us, 30.4 with one), else one (4 sequences of 4096
-        // in tables of 131072: 15.8 us, 16.9 with two)
-        if (chunk >= 8 && base >= 128) p.quantum = 8;
     }
     p.n_split = (int)n;
     p.per_split = n > 1 ? (uint32_t)((((uint64_t)1 << 32) + n - 1) / n) : 0;
@@ -2094,10 +2106,10 @@ static void launch_attn_rt(const Kv4& c, const AttnArgs& a, const AttnPlan& p, s
     if (!p.joint && p.nw == 4) kv4_attn_kernel<HDG, RT, false, 4><<<blocks, 256, 0, st>>>(c, a);
     const size_t wb = p.joint ? heads * ((c.max_pages + 3) / 4) : 0;
     if (rows + wb) kv4_attn_finish<HDG, RT><<<(unsigned)(rows + wb), 256, 0, st>>>(c, a, (unsigned)rows, win, wout);
-    if (wout && !p.joint)
-{
-        // a wavefront a page where it has few rows, eight where they are many
-        if (a.n_q * (a.n_heads / c.n_kv) <= 16) kv4_attn_weights<HDG, 1><<<(unsigned)(heads * c.max_pages), 64, 0, st>>>(c, a, win, wout);
+    if (wout && !p.joint) {
+        // a wavefront a page where they fill the card, or have few rows; else
+        // eight (24 rows: 57 and 70 us with 4096 pages, 24 and 22 with 80)
+        if (heads * c.max_pages >= 2048 || a.n_q * (a.n_heads / c.n_kv) <= 16) kv4_attn_weights<HDG, 1><<<(unsigned)(heads * c.max_pages), 64, 0, st>>>(c, a, win, wout);
         else kv4_attn_weights<HDG, 8><<<(unsigned)(heads * c.max_pages), 512, 0, st>>>(c, a, win, wout);
     }
 }
@@ -2108,7 +2120,7 @@ static void launch_attn(const Kv4& c, const AttnArgs& a, const AttnPlan& p, size
         const size_t rows = heads * a.n_q * (a.n_heads / c.n_kv), pad = heads * p.n_tile * kWideRows;
         const WideRows wr = wout ? WideRows{(h8_t*)a.digits, a.rowc, a.rowc + pad, a.lse} : WideRows{};
         kv4_attn_wide<HDG><<<(unsigned)(heads * p.n_tile * p.n_split), 256, 0, st>>>(c, a, wr);
-        if (p.n_split > 8) kv4_attn_finish<HDG, 1><<<(unsigned)rows, 256, 0, st>>>(c, a, (unsigned)rows, win, wout);
+        if (p.n_split > kFewSplits) kv4_attn_finish<HDG, 1><<<(unsigned)rows, 256, 0, st>>>(c, a, (unsigned)rows, win, wout);
         else if (p.n_split > 1) kv4_attn_join<HDG><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(c, a, rows);
         if (wout) kv4_weights_wide<HDG><<<(unsigned)(heads * c.max_pages), 512, 0, st>>>(c, a, wr, win, wout);
     } else if (p.rt == 1) launch_attn_rt<HDG, 1>(c, a, p, heads, win, wout, st);
