@@ -1702,16 +1702,22 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_long(Kv4 c, LongSel q,
         const int hi = kBins - 2 * (tid + 1);
         const uint32_t* hl = h0 + (size_t)(LEVEL - 1) * kSegs * kBins + hi;
         uint32_t lo = 0, up = 0, lo_b = 0, up_b = 0;
-#pragma unroll 8
-        for (int s = 0; s < segs; s++) {
-            const uint2 x = *(const uint2*)(hl + (size_t)s * kBins);
-            lo += x.x;
-            up += x.y;
-            if (LEVEL == 3 && s < sg) {
-                lo_b += x.x;
-                up_b += x.y;
+        if (LEVEL < 3 || hi < 1024)                      // the low bits have 1024 bins
+            for (int s0 = 0; s0 < segs; s0 += 16) {      // slots behind the last segment are there, and not counted
+                uint2 x[16];
+#pragma unroll
+                for (int s = 0; s < 16; s++) x[s] = *(const uint2*)(hl + (size_t)(s0 + s) * kBins);
+#pragma unroll
+                for (int s = 0; s < 16; s++) {
+                    const bool in = s0 + s < segs, before = s0 + s < sg;
+                    lo += in ? x[s].x : 0u;
+                    up += in ? x[s].y : 0u;
+                    if (LEVEL == 3) {
+                        lo_b += before ? x[s].x : 0u;
+                        up_b += before ? x[s].y : 0u;
+                    }
+                }
             }
-        }
         const uint32_t bin = pick_bin(bp, lo, up, need);
         cut |= bin << bin_shift(LEVEL - 1);
         if (LEVEL == 3) low_before = (hi > (int)bin ? lo_b : 0u) + (hi + 1 > (int)bin ? up_b : 0u);
@@ -1737,7 +1743,7 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_long(Kv4 c, LongSel q,
         if (LEVEL > 0 && lane == 0) cnt2[wave][0] = over;
         __syncthreads();
         uint32_t* ho = h0 + ((size_t)LEVEL * kSegs + sg) * kBins;
-        for (int i = tid; i < kBins; i += kSelThreads) ho[i] = hist[i];
+        for (int i = tid; i < (LEVEL == 2 ? 1024 : kBins); i += kSelThreads) ho[i] = hist[i];
         if (LEVEL > 0 && tid == 0) {
             int sum = 0;
             for (int k = 0; k < kSelWaves; k++) sum += cnt2[k][0];
