@@ -212,7 +212,8 @@ int ibh_attn_exact_set_grouped(int on);
  *   pool   n_pages pages of ibh_kv4_page_bytes(n_kv, head_dim) bytes, on 16
  *          bytes;
  *   table  [n_seq][max_pages]: the page that holds positions 64 j .. 64 j + 63
- *          of a sequence.  Entries behind a sequence's last page are not used.
+ *          of a sequence.  Entries behind a sequence's last page are not used;
+ *          a table with room for more costs an attention next to nothing.
  *          Sequences may share full pages, not one that is appended to;
  *   lens   [n_seq] positions held, 0 .. 64 max_pages; 0 leaves a sequence out.
  * head_dim 64, 128, 192 or 256.  A page number outside the pool or a length
@@ -277,9 +278,9 @@ int    ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float* q, int 
  * [n_seq][n_kv][budget] the positions they had (-1 behind them).  The slots
  * behind the last kept one of a page are cleared; dst pages without a kept
  * position are left as they are.
- * In place: dst with src's pool, table, lens and weights.  Otherwise dst has
- * its own table, lens and weights, and pages that src does not use; src is
- * left as it was.  sink + recent <= budget <= 64 dst->max_pages.
+ * In place: dst with src's pool, table, lens and weights, and no page that two
+ * sequences share.  Otherwise dst has its own table, lens and weights, and
+ * pages that src does not use; src, which may share pages, is left as it was.  sink + recent <= budget <= 64 dst->max_pages.
  * `ws` >= ibh_kv4_evict_workspace_bytes(src) (0 for rows of up to 16384
  * positions) on 16 bytes, NULL = library workspace; calls that share one must
  * not overlap in time. */

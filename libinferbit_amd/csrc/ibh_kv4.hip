@@ -2111,7 +2111,7 @@ static void launch_attn_rt(const Kv4& c, const AttnArgs& a, const AttnPlan& p, s
     }
     if (!p.joint && p.nw == 4) kv4_attn_kernel<HDG, RT, false, 4><<<blocks, 256, 0, st>>>(c, a);
     const size_t wb = p.joint ? heads * ((c.max_pages + 3) / 4) : 0;
-    if (rows + wb) kv4_attn_finish<HDG, RT><<<(unsigned)(rows + wb), 256, 0, st>>>(c, a, (unsigned)rows, win, wout);
+    if (rows + wb) kv4_attn_finish<HDG, (RT <= 2 ? RT : 1)><<<(unsigned)(rows + wb), 256, 0, st>>>(c, a, (unsigned)rows, win, wout);
     if (wout && !p.joint) {
         // a wavefront a page where they fill the card, or have few rows; else
         // eight (24 rows: 57 and 70 us with 4096 pages, 24 and 22 with 80)

@@ -217,7 +217,7 @@ def kv4_attn(out, q, cache: Kv4Cache, n_heads: int, weights_in=None, weights_out
 def kv4_evict(src: Kv4Cache, dst: Kv4Cache, weights_src, weights_dst, budget: int, sink: int, recent: int,
               kept, ws=None) -> None:
     """Cuts every sequence to `budget` positions by accumulated weight: rows, weights and lengths into dst (src itself
-    for in place), the kept positions into kept int32 [n_seq, n_kv, budget]."""
+    for in place, where no page is shared), the kept positions into kept int32 [n_seq, n_kv, budget]."""
     if dst.index != src.index:
         raise ValueError(f"the caches are on {src.device} and {dst.device}")
     n = src.n_seq * src.n_kv
