@@ -221,7 +221,7 @@ int ibh_attn_exact_set_grouped(int on);
  * stored for it, what would be computed from it is NaN, an eviction keeps
  * nothing of a sequence of such a length; the other sequences are served.
  *
- * An element stands for mid + scale * (code - 8).  For each KV head a page
+ * An element stands for mid + scale * (code - 8), scale not negative.  For each KV head a page
  * holds 72 head_dim bytes: key codes, the keys' pairs, value codes, the
  * values' pairs.  Position t of a page has slot 4 (t % 16) + t / 16.  Key codes
  * lie as [t / 32][dim / 64][dim / 16 % 4][t % 16][t / 16 % 2][16 dims], value

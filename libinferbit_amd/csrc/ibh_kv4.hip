@@ -547,7 +547,7 @@ __global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(
     // one place of this page again (at = 0), which costs less than a branch.
     auto step = [&](int pos0, const uint8_t* nx, auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
-        float e[RT][4], y[RT][4];
+        float e[RT][4], y[RT][4];                        // y: scores to keep
         {
             i4_t kb[4][HDG];
 #pragma unroll
@@ -575,18 +575,19 @@ __global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(
                         x[s] = fmaf(h2f(pr), f, fmaf(h2f(pr >> 16), qsum[t][g], x[s]));
                     }
                 }
-                if constexpr (MASKED) {
+                // scores are rounded before the maximum is taken off: one fma
+                // for both would leave the product's rounding in the
+                // difference, which at scores of 2^31 is more than exp2 takes
 #pragma unroll
-                    for (int s = 0; s < 4; s++) x[s] = pos0 + 16 * s + li <= lim[t] ? x[s] : -INFINITY;
-                }
-                if constexpr (SCORES) {
-#pragma unroll
-                    for (int s = 0; s < 4; s++) y[t][s] = x[s] * kf[t];
+                for (int s = 0; s < 4; s++) {
+                    x[s] *= kf[t];
+                    if constexpr (MASKED) x[s] = pos0 + 16 * s + li <= lim[t] ? x[s] : -INFINITY;
+                    if constexpr (SCORES) y[t][s] = x[s];
                 }
                 const float top = row16_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
                 if (__any(top > m[t])) {
                     const float mn = fmaxf(m[t], top);
-                    const float al = mn == -INFINITY ? 1.f : exp2_((m[t] - mn) * kf[t]);
+                    const float al = mn == -INFINITY ? 1.f : exp2_(m[t] - mn);
                     m[t] = mn;
                     l[t] *= al;
 #pragma unroll
@@ -594,10 +595,10 @@ __global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(
 #pragma unroll
                     for (int g = 0; g < HDG; g++) om[t][g] *= al;
                 }
-                const float mk = m[t] == -INFINITY ? 0.f : -m[t] * kf[t];
+                const float mk = m[t] == -INFINITY ? 0.f : m[t];
 #pragma unroll
                 for (int s = 0; s < 4; s++) {
-                    e[t][s] = exp2_(fmaf(x[s], kf[t], mk));
+                    e[t][s] = exp2_(x[s] - mk);
                     l[t] += e[t][s];
                 }
             }
@@ -683,7 +684,7 @@ __global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(
     for (int t = 0; t < RT; t++) {
         const float ls = row16_sum(l[t]);
         if (li == 0) {
-            mlw[wave][lq][0] = m[t] == -INFINITY ? -INFINITY : m[t] * kf[t];
+            mlw[wave][lq][0] = m[t];
             mlw[wave][lq][1] = ls;
         }
 #pragma unroll
@@ -751,7 +752,7 @@ typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 h8_alias __attribute__((ext_vector_type(8), may_alias));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 constexpr int kWideRows = 64;
-constexpr float kNoMax = -1e30f;                         // below every score
+constexpr float kNoMax = -0x1.fffffep127f;               // no score is lower
 
 __device__ __forceinline__ f4_t mfma32(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 // A code word's eight numbers: 1024 + code as fp16 bits, less 1032.
@@ -943,12 +944,13 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
                 for (int r = 0; r < 4; r++) x[r][s] = fmaf(h2f(pr), d[r], fmaf(h2f(pr >> 16), qsum[r][g], x[r][s]));
             }
         }
-        if constexpr (MASKED) {
 #pragma unroll
-            for (int s = 0; s < 4; s++)
+        for (int s = 0; s < 4; s++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) x[r][s] = pos0 + 16 * s + li <= lim[r] ? x[r][s] : -INFINITY;
-        }
+            for (int r = 0; r < 4; r++) {
+                x[r][s] *= kf[r];                        // rounded before m is taken off, as above
+                if constexpr (MASKED) x[r][s] = pos0 + 16 * s + li <= lim[r] ? x[r][s] : -INFINITY;
+            }
         // a power of two takes the largest of a group's scales so far to 2^11 .. 2^12
         float vs[HDG][4], vsm[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -978,7 +980,7 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
-                for (int s = 0; s < 4; s++) e[r][s] = exp2_(fmaf(x[r][s], kf[r], -m[r]));
+                for (int s = 0; s < 4; s++) e[r][s] = exp2_(x[r][s] - m[r]);
         };
         probs();
         // m moves only when a p * scale no longer fits fp16 or a p is above
@@ -995,11 +997,13 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
         if (__any(most > 65504.f || high > 0x1p60f)) {
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const float top = row16_max(fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3]))) * kf[r];
+                const float top = row16_max(fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3])));
                 float w = 0.f;
 #pragma unroll
-                for (int s = 0; s < 4; s++) w = fmaxf(w, exp2_(fmaf(x[r][s], kf[r], -top)) * vsm[s]);
-                const float to = top - (float)min(12 - __builtin_amdgcn_frexp_expf(row16_max(w)), 40);
+                for (int s = 0; s < 4; s++) w = fmaxf(w, exp2_(x[r][s] - top) * vsm[s]);
+                // (from 2^22 on, where fp32 holds no such steps, the page's largest p is 1)
+                const int below = min(12 - __builtin_amdgcn_frexp_expf(row16_max(w)), 40);
+                const float to = fabsf(top) < 0x1p22f ? top - (float)below : top;
                 const float mn = top == -INFINITY ? m[r] : fmaxf(m[r], to), al = exp2_(m[r] - mn);
                 m[r] = mn;
                 l[r] *= al;
@@ -1123,10 +1127,11 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
 }
 
 // Accumulated weights of many rows: block (KV head, page, sequence); every
-// wavefront holds the page's keys and takes 16-row tiles in turn.
-template <int HDG>
-__global__ __launch_bounds__(512) void kv4_weights_wide(Kv4 c, AttnArgs a, WideRows wr, const float* win, float* wout) {
-    constexpr int NW = 8;
+// wavefront holds the page's keys and takes 16-row tiles in turn.  2048 rows
+// of 8 KV heads of 128 over 4100 positions: 51 us, in which every page reads
+// all rows' halves from L2, 8 KB a tile, 10 TB/s.
+template <int HDG, int NW>
+__global__ __launch_bounds__(64 * NW) void kv4_weights_wide(Kv4 c, AttnArgs a, WideRows wr, const float* win, float* wout) {
     __shared__ float part[NW][kPage];
     const int lane = threadIdx.x & 63, li = lane & 15, lq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1195,14 +1200,14 @@ __global__ __launch_bounds__(512) void kv4_weights_wide(Kv4 c, AttnArgs a, WideR
 #pragma unroll
                 for (int r = 0; r < 4; r++)
 #pragma unroll
-                    for (int s = 0; s < 4; s++) acc[s] += exp2_(fmaf(x[r][s], kf[r], -lse[r]));
+                    for (int s = 0; s < 4; s++) acc[s] += exp2_(x[r][s] * kf[r] - lse[r]);
             } else {
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int lim = base + min(row + r, n_rows - 1) / grp;
 #pragma unroll
                     for (int s = 0; s < 4; s++)
-                        acc[s] += p * kPage + 16 * s + li <= lim ? exp2_(fmaf(x[r][s], kf[r], -lse[r])) : 0.f;
+                        acc[s] += p * kPage + 16 * s + li <= lim ? exp2_(x[r][s] * kf[r] - lse[r]) : 0.f;
                 }
             }
         }
@@ -1293,7 +1298,7 @@ struct PageWeights {
                 }
             }
 #pragma unroll
-            for (int s = 0; s < 4; s++) acc[s] += pos0 + 16 * s + li <= lim ? exp2_(fmaf(x[s], kf, -lse)) : 0.f;
+            for (int s = 0; s < 4; s++) acc[s] += pos0 + 16 * s + li <= lim ? exp2_(x[s] * kf - lse) : 0.f;
             kf = kfn;
             lse = lsen;
             lim = limn;
@@ -2128,7 +2133,12 @@ static void launch_attn(const Kv4& c, const AttnArgs& a, const AttnPlan& p, size
         kv4_attn_wide<HDG><<<(unsigned)(heads * p.n_tile * p.n_split), 256, 0, st>>>(c, a, wr);
         if (p.n_split > kFewSplits) kv4_attn_finish<HDG, 1><<<(unsigned)rows, 256, 0, st>>>(c, a, (unsigned)rows, win, wout);
         else if (p.n_split > 1) kv4_attn_join<HDG><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(c, a, rows);
-        if (wout) kv4_weights_wide<HDG><<<(unsigned)(heads * c.max_pages), 512, 0, st>>>(c, a, wr, win, wout);
+        // four wavefronts a page, eight where there are few pages (2048 rows, 8
+        // KV heads of 128: 169 and 179 us with 512 pages, 81 and 68 with 80; 40
+        // rows, 4096 pages: 66 and 92; whole calls)
+        const unsigned pages = (unsigned)(heads * c.max_pages);
+        if (wout && pages >= 512) kv4_weights_wide<HDG, 4><<<pages, 256, 0, st>>>(c, a, wr, win, wout);
+        else if (wout) kv4_weights_wide<HDG, 8><<<pages, 512, 0, st>>>(c, a, wr, win, wout);
     } else if (p.rt == 1) launch_attn_rt<HDG, 1>(c, a, p, heads, win, wout, st);
     else if (p.rt == 2) launch_attn_rt<HDG, 2>(c, a, p, heads, win, wout, st);
     else if constexpr (HDG <= 2) launch_attn_rt<HDG, 4>(c, a, p, heads, win, wout, st);

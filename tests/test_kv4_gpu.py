@@ -274,6 +274,27 @@ def test_attention_tiny_values_after_large_ones(ops, n_q, hd):
     check_attention(ops, m, q, n_heads, n_q, out)
 
 
+@pytest.mark.parametrize("n_q,t", [(1, 150), (1, 1100), (3, 150), (9, 150), (9, 1100)])
+@pytest.mark.parametrize("size", [1e20, 1e33])
+def test_attention_huge_scores(ops, n_q, t, size):
+    """Queries so long that every score of a row is below -1e20, or -1e32: the largest position takes it all.  The
+    scores of two positions differ by far more than their roundings, so the output is that position's value."""
+    rng = np.random.default_rng(6)
+    n_heads, n_kv, hd = 8, 2, 64
+    m = Made(ops, rng, [t], n_kv, hd)
+    m.k[0] = (np.arange(t)[:, None] * 0.01 + 1 + np.zeros(n_kv * hd)).astype(np.float32)   # constant groups: scale 0
+    ops.kv4_append(m.cache, torch.from_numpy(m.k[0][None]).cuda(), torch.from_numpy(m.v[0][None]).cuda())
+    q = torch.full((1, n_q, n_heads * hd), -size, device="cuda")
+    out, w = torch.empty_like(q), torch.zeros(1, n_kv, m.table.shape[1] * 64, device="cuda")
+    ops.kv4_attn(out, q, m.cache, n_heads, weights_in=w, weights_out=w)
+    V = m.loaded(0)[1][:, 0]                                      # position 0 has the smallest key
+    assert (w[0, :, 1:] == 0).all() and (w[0, :, 0] == n_q * n_heads // n_kv).all()
+    got = out.cpu().numpy().reshape(n_q, n_heads, hd)
+    for h in range(n_heads):
+        want = V[h // (n_heads // n_kv)]
+        assert (np.abs(got[:, h] - want) <= 2.0 ** -21 * np.abs(want).max()).all()
+
+
 @pytest.mark.parametrize("n_q", [4, 40])
 def test_attention_not_finite(ops, n_q):
     """A NaN key makes the rows that see it NaN, a NaN value its 64 dims; rows that do not see it, and what lies
