@@ -406,9 +406,12 @@ __device__ __forceinline__ int chunk_of(const AttnArgs& a, int len) {
 // Wavefronts a SIMD holds: what the registers of a page and RT tiles leave.
 constexpr int attn_waves(int hdg, int rt) { return hdg * rt == 1 ? 4 : hdg * rt == 2 ? 3 : hdg * rt >= 8 && hdg > 2 ? 1 : 2; }
 
-// Block: `chunk` pages of one (sequence, KV head), RT tiles of 4 query rows,
-// NW wavefronts that take the block's pages in turn, each with its own running
-// maximum and sums, joined at the end.
+// Block: a share of the pages of one (sequence, KV head), RT tiles of 4 query
+// rows, NW wavefronts that take the block's pages in turn, each with its own
+// running maximum and sums, joined at the end.  4 sequences of 131071 positions,
+// 8 KV heads of 128, 4 rows each: 604 MB in 95 us, 6.3 TB/s, of which HBM is the
+// bound (7.0 by a kernel that only reads).  With 4096 positions it is the chain
+// of a block: length, page number, codes, products, sums: 6 us.
 template <int HDG, int RT, bool SCORES, int NW>
 __global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(Kv4 c, AttnArgs a) {
     constexpr int HD = 64 * HDG, ROWS = 4 * RT;
@@ -2034,8 +2037,8 @@ static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool wei
     const size_t n_rows = (size_t)n_q * (n_heads / c->n_kv), hdg = c->head_dim / 64;
     const size_t heads = (size_t)c->n_seq * c->n_kv;
     // Few rows: the smallest tile that holds them, so that pages are read once.
-    // A tile of 16 rows and head_dim above 128 would leave one wavefront a SIMD
-    // and spills: two tiles of 8 instead.  From 33 rows on the f16 kernel: 8
+    // A tile of 16 rows does not fit the registers with head_dim above 128: tiles
+    // of 8 there.  From 33 rows on the f16 kernel: 8
     // sequences of 4096 positions, 8 KV heads of 128, 32 rows 40 us here and 41
     // there, 40 rows 54 and 43, 64 rows 67 and 46 (one sequence, where neither
     // fills the card: 21 and 23, 22 and 26).
