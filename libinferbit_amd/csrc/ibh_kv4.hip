@@ -385,8 +385,8 @@ struct AttnArgs {
     int tile_rows;                                       // query rows of a row tile
     float* part;                                         // [seq][KV head][row][split][head_dim], when n_split > 1
     float2* part_ml;                                     // [seq][KV head][row][split] maximum (log2) and sum
-    float* lse;                                          // [seq][KV head][row, lse_pad of them] log2 of the row's sum, when weights are wanted
-    int lse_pad;
+    float2* stat;                                        // [seq][KV head][row, stat_pad of them] row_stat(), when weights are wanted
+    int stat_pad;
     i4_t* digits;                                        // [seq][KV head][4-row tile][group][lane]
     float* rowc;                                         // [seq][KV head][row][1 + groups] step * scale, sums of the query in steps
     float4* scores;                                      // [seq][KV head][page][tile][lane] scores (log2), -inf where not seen
@@ -401,6 +401,15 @@ __host__ __device__ __forceinline__ int chunk_of(int pages, int n_split, uint32_
 }
 __device__ __forceinline__ int chunk_of(const AttnArgs& a, int len) {
     return a.n_split == 1 ? a.chunk : chunk_of((len + kPage - 1) / kPage, a.n_split, a.per_split, a.quantum);
+}
+
+// A row's maximum (log2) and the inverse of its sum, from which the weights
+// are 2^(score - maximum) * inverse.  (Held as one number, maximum + log2(sum),
+// the sum's share is rounded in steps of the maximum's: two tied scores of 2^25
+// had weight 1 each, and a row at 10^4 weights that are all 3e-4 off.)  A row
+// that sees nothing gives nothing: no score is above its maximum.
+__device__ __forceinline__ float2 row_stat(float m, float sum) {
+    return sum == 0.f ? make_float2(INFINITY, 0.f) : make_float2(m, 1.f / sum);
 }
 
 // Wavefronts a SIMD holds: what the registers of a page and RT tiles leave.
@@ -722,7 +731,7 @@ __global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(
             }
             if (lane == 0) {
                 if (a.n_split > 1) a.part_ml[rr * a.n_split + split] = make_float2(mm, sum);
-                else if (a.lse) a.lse[rr] = sum == 0.f ? INFINITY : mm + log2f(sum);
+                else if (a.stat) a.stat[rr] = row_stat(mm, sum);
             }
         }
         __syncthreads();
@@ -784,7 +793,8 @@ __device__ __forceinline__ uint32_t pack_rtz(float a, float b) { return __builti
 // Rows' constants for the weights, each array padded to whole blocks of rows.
 struct WideRows {
     h8_t* q;                                             // [seq][KV head][16-row tile][group][2][high, low][lane]
-    float *kf, *qsum, *lse;                              // [..][row], [..][group][row], [..][row]
+    float *kf, *qsum;                                    // [..][row], [..][group][row]
+    float2* stat;                                        // [..][row]
 };
 __device__ __forceinline__ int wide_pad(int n_rows) { return (n_rows + kWideRows - 1) / kWideRows * kWideRows; }
 
@@ -901,7 +911,7 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
                 wr.kf[sh * pad + row0 + li] = f;
 #pragma unroll
                 for (int g = 0; g < HDG; g++) wr.qsum[(sh * HDG + g) * pad + row0 + li] = sum[g];
-                if (row0 + li >= n_rows) wr.lse[sh * pad + row0 + li] = INFINITY;   // adds nothing
+                if (row0 + li >= n_rows) wr.stat[sh * pad + row0 + li] = row_stat(0.f, 0.f);
             }
         }
     }
@@ -1124,7 +1134,7 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
         }
         if (in && li == 0) {
             if (a.n_split > 1) a.part_ml[rr * a.n_split + split] = make_float2(m[r], sum);
-            else if (wr.lse) wr.lse[sh * wide_pad(n_rows) + row] = sum == 0.f ? INFINITY : m[r] + log2f(sum);
+            else if (wr.stat) wr.stat[sh * wide_pad(n_rows) + row] = row_stat(m[r], sum);
         }
     }
 }
@@ -1172,7 +1182,10 @@ __global__ __launch_bounds__(64 * NW) void kv4_weights_wide(Kv4 c, AttnArgs a, W
         for (int t = t0 + wave; t < tiles; t += NW) {
             const h8_t* q = wr.q + (sh * (pad / 16) + t) * HDG * 256 + lane;
             const int row = 16 * t + 4 * lq;
-            const f4_t kf = *(const f4_t*)(wr.kf + sh * pad + row), lse = *(const f4_t*)(wr.lse + sh * pad + row);
+            const f4_t kf = *(const f4_t*)(wr.kf + sh * pad + row);
+            float2 st[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) st[r] = wr.stat[sh * pad + row + r];
             float x[4][4];
 #pragma unroll
             for (int r = 0; r < 4; r++)
@@ -1203,14 +1216,14 @@ __global__ __launch_bounds__(64 * NW) void kv4_weights_wide(Kv4 c, AttnArgs a, W
 #pragma unroll
                 for (int r = 0; r < 4; r++)
 #pragma unroll
-                    for (int s = 0; s < 4; s++) acc[s] += exp2_(x[r][s] * kf[r] - lse[r]);
+                    for (int s = 0; s < 4; s++) acc[s] = fmaf(exp2_(x[r][s] * kf[r] - st[r].x), st[r].y, acc[s]);
             } else {
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int lim = base + min(row + r, n_rows - 1) / grp;
 #pragma unroll
                     for (int s = 0; s < 4; s++)
-                        acc[s] += p * kPage + 16 * s + li <= lim ? exp2_(x[r][s] * kf[r] - lse[r]) : 0.f;
+                        acc[s] += p * kPage + 16 * s + li <= lim ? exp2_(x[r][s] * kf[r] - st[r].x) * st[r].y : 0.f;
                 }
             }
         }
@@ -1240,9 +1253,10 @@ __device__ __forceinline__ int splits_of(const AttnArgs& a, int len, int row, in
     return lim < 0 ? 1 : (lim / kPage + chunk) / chunk;
 }
 
-// A page's keys, and 2^(score - lse) of its positions summed over the rows of
+// A page's keys, and the probabilities of its positions summed over the rows of
 // tiles t0, t0 + dt, .. < t1: lane l of sum() returns position l's (the rows'
-// digits, step * scale, sums, lse and last positions as the callers give them).
+// digits, step * scale, sums, row_stat() and last positions as the callers give
+// them).
 template <int HDG>
 struct PageWeights {
     uint4 kc[2][HDG], kp[HDG];
@@ -1268,17 +1282,19 @@ struct PageWeights {
                 kb[2 * u + 1][g] = unpack16(kc[u][g].z, kc[u][g].w);
             }
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        float kf, lse, qs[HDG];
+        float kf, qs[HDG];
+        float2 st;
         int lim;                                         // the last position that the lane's row sees
         if (t0 < t1) {
 #pragma unroll
             for (int g = 0; g < HDG; g++) qa[g] = digits[((size_t)t0 * HDG + g) * 64 + lane];
-            rows(t0, lq, kf, lse, qs, lim);
+            rows(t0, lq, kf, st, qs, lim);
         }
         for (int t = t0; t < t1; t += dt) {
             // the next tile's rows are loaded while this one's are multiplied
             i4_t qn[HDG];
-            float kfn = 0.f, lsen = 0.f, qsn[HDG];
+            float kfn = 0.f, qsn[HDG];
+            float2 stn = make_float2(0.f, 0.f);
             int limn = -1;
 #pragma unroll
             for (int g = 0; g < HDG; g++) {
@@ -1288,7 +1304,7 @@ struct PageWeights {
             if (t + dt < t1) {
 #pragma unroll
                 for (int g = 0; g < HDG; g++) qn[g] = digits[((size_t)(t + dt) * HDG + g) * 64 + lane];
-                rows(t + dt, lq, kfn, lsen, qsn, limn);
+                rows(t + dt, lq, kfn, stn, qsn, limn);
             }
             float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -1301,9 +1317,9 @@ struct PageWeights {
                 }
             }
 #pragma unroll
-            for (int s = 0; s < 4; s++) acc[s] += pos0 + 16 * s + li <= lim ? exp2_(x[s] * kf - lse) : 0.f;
+            for (int s = 0; s < 4; s++) acc[s] += pos0 + 16 * s + li <= lim ? exp2_(x[s] * kf - st.x) * st.y : 0.f;
             kf = kfn;
-            lse = lsen;
+            st = stn;
             lim = limn;
 #pragma unroll
             for (int g = 0; g < HDG; g++) {
@@ -1350,11 +1366,11 @@ __global__ __launch_bounds__(256) void kv4_attn_join(Kv4 c, AttnArgs a, size_t r
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int g = 0; g < HDG; g++) dst[64 * g] = y[g] * inv;
-    if (lane == 0 && a.lse) a.lse[sh * a.lse_pad + row] = sum == 0.f ? INFINITY : mm + log2f(sum);
+    if (lane == 0 && a.stat) a.stat[sh * a.stat_pad + row] = row_stat(mm, sum);
 }
 
-// log2 of a query row's sum over its splits, by the 16 lanes of a row.
-__device__ __forceinline__ float row_lse(const float2* ml, int n, int li) {
+// A query row's row_stat() from its splits, by the 16 lanes of a row.
+__device__ __forceinline__ float2 joined_stat(const float2* ml, int n, int li) {
     float m = -INFINITY, s = 0.f;
     for (int i = li; i < n; i += 16) m = fmaxf(m, ml[i].x);
     m = row16_max(m);
@@ -1362,16 +1378,15 @@ __device__ __forceinline__ float row_lse(const float2* ml, int n, int li) {
         const float2 v = ml[i];
         s = fmaf(v.x == -INFINITY && v.y == 0.f ? 0.f : exp2_(v.x - m), v.y, s);
     }
-    s = row16_sum(s);
-    return s == 0.f ? INFINITY : m + log2f(s);
+    return row_stat(m, row16_sum(s));
 }
 
 // What is left after the pages' blocks.  Blocks below n_join join the splits
 // of a query row: 16 HDG threads hold four dims each, the other threads take
 // other splits, so that all partial sums are in flight together.  The others,
 // where one row tile holds all rows, take a page a wavefront and turn the
-// scores that the first kernel kept into weights; they take lse from the
-// splits' maxima and sums themselves, so that they need not wait for the
+// scores that the first kernel kept into weights; they take row_stat()
+// from the splits' maxima and sums themselves, so that they need not wait for the
 // joining blocks.  At 32 sequences of up to 4096 positions, 8 KV heads of 128,
 // this launch takes 10 us, and keeping the scores costs the first 1.2 us, by
 // nontemporal stores behind a page's loads (9 us by ordinary ones, which the
@@ -1437,7 +1452,7 @@ __global__ __launch_bounds__(256) void kv4_attn_finish(Kv4 c, AttnArgs a, unsign
             a.out[((size_t)seq * a.n_q + row / grp) * (size_t)a.n_heads * HD + (h * grp + row % grp) * HD + tid] =
                 sum == 0.f ? 0.f : y / sum;
         }
-        if (tid == 0 && a.lse) a.lse[sh * a.lse_pad + row] = sum == 0.f ? INFINITY : mm + log2f(sum);
+        if (tid == 0 && a.stat) a.stat[sh * a.stat_pad + row] = row_stat(mm, sum);
         return;
     }
     unsigned b = blockIdx.x - n_join;
@@ -1462,12 +1477,12 @@ __global__ __launch_bounds__(256) void kv4_attn_finish(Kv4 c, AttnArgs a, unsign
 #pragma unroll
     for (int t = 0; t < RT; t++) {
         const int r = 4 * t + lq;
-        float lse = row_lse(a.part_ml + (sh * n_rows + min(r, n_rows - 1)) * a.n_split, n, lane & 15);
-        if (r >= n_rows) lse = INFINITY;
-        acc[0] += exp2_(x[t].x - lse);
-        acc[1] += exp2_(x[t].y - lse);
-        acc[2] += exp2_(x[t].z - lse);
-        acc[3] += exp2_(x[t].w - lse);
+        float2 st = joined_stat(a.part_ml + (sh * n_rows + min(r, n_rows - 1)) * a.n_split, n, lane & 15);
+        if (r >= n_rows) st = row_stat(0.f, 0.f);
+        acc[0] = fmaf(exp2_(x[t].x - st.x), st.y, acc[0]);
+        acc[1] = fmaf(exp2_(x[t].y - st.x), st.y, acc[1]);
+        acc[2] = fmaf(exp2_(x[t].z - st.x), st.y, acc[2]);
+        acc[3] = fmaf(exp2_(x[t].w - st.x), st.y, acc[3]);
     }
 #pragma unroll
     for (int s = 0; s < 4; s++) {
@@ -1504,11 +1519,11 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_weights(Kv4 c, AttnArgs a, c
         // queries before the page's first position see nothing of it
         const int t0 = max(0, p * kPage - (len - a.n_q)) * grp / 4;
         part[wave][lane] = pw.sum(a.digits + sh * tiles * HDG * 64, p * kPage, lane, t0 + wave, tiles, NW,
-            [&](int t, int lq, float& kf, float& lse, float* qs, int& lim) {
+            [&](int t, int lq, float& kf, float2& st, float* qs, int& lim) {
                 const int r = 4 * t + lq, row = min(r, n_rows - 1);
                 const float* rcp = a.rowc + (sh * n_rows + row) * (1 + HDG);
                 kf = rcp[0];
-                lse = a.lse[sh * n_rows + row];
+                st = a.stat[sh * n_rows + row];
 #pragma unroll
                 for (int g = 0; g < HDG; g++) qs[g] = rcp[1 + g];
                 lim = r < n_rows ? len - a.n_q + row / grp : -1;
@@ -2030,7 +2045,7 @@ struct AttnPlan {
     int rt, n_tile, n_split, chunk, quantum, nw;         // rt 16: kv4_attn_wide
     uint32_t per_split;
     bool joint;                                          // the weights in the launch that joins the splits
-    size_t part, part_ml, lse, digits, rowc, score, bytes;     // offsets into the workspace
+    size_t part, part_ml, stat, digits, rowc, score, bytes;     // offsets into the workspace
 };
 static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool weights) {
     AttnPlan p;
@@ -2093,7 +2108,7 @@ static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool wei
     p.part_ml = take(p.n_split > 1 ? heads * n_rows * p.n_split * sizeof(float2) : 0);
     const size_t pad = wide ? (n_rows + kWideRows - 1) / kWideRows * kWideRows : n_rows;
     const size_t again = weights && !p.joint ? heads : 0;
-    p.lse = take(again * pad * sizeof(float));
+    p.stat = take(again * pad * sizeof(float2));
     p.digits = take(again * ((pad + 3) / 4) * hdg * 1024);
     p.rowc = take(again * pad * (1 + hdg) * sizeof(float));
     p.score = take(p.joint ? heads * c->max_pages * p.rt * 1024 : 0);
@@ -2132,7 +2147,7 @@ static void launch_attn(const Kv4& c, const AttnArgs& a, const AttnPlan& p, size
                         float* wout, hipStream_t st) {
     if (p.rt == kWideRows / 4) {
         const size_t rows = heads * a.n_q * (a.n_heads / c.n_kv), pad = heads * p.n_tile * kWideRows;
-        const WideRows wr = wout ? WideRows{(h8_t*)a.digits, a.rowc, a.rowc + pad, a.lse} : WideRows{};
+        const WideRows wr = wout ? WideRows{(h8_t*)a.digits, a.rowc, a.rowc + pad, a.stat} : WideRows{};
         kv4_attn_wide<HDG><<<(unsigned)(heads * p.n_tile * p.n_split), 256, 0, st>>>(c, a, wr);
         if (p.n_split > kFewSplits) kv4_attn_finish<HDG, 1><<<(unsigned)rows, 256, 0, st>>>(c, a, (unsigned)rows, win, wout);
         else if (p.n_split > 1) kv4_attn_join<HDG><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(c, a, rows);
@@ -2173,7 +2188,7 @@ extern "C" int ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float*
     char* w = (char*)ws;
     AttnArgs a{out, q, n_heads, n_q, q_stride, (float)(1.4426950408889634 / sqrt((double)cache->head_dim)),
                p.n_split, p.n_tile, p.chunk, p.quantum, p.per_split, 4 * p.rt, (float*)(w + p.part), (float2*)(w + p.part_ml),
-               weights_out && !p.joint ? (float*)(w + p.lse) : nullptr,
+               weights_out && !p.joint ? (float2*)(w + p.stat) : nullptr,
                p.rt == kWideRows / 4 ? p.n_tile * kWideRows : n_q * (n_heads / cache->n_kv),
                weights_out && !p.joint ? (i4_t*)(w + p.digits) : nullptr, (float*)(w + p.rowc), (float4*)(w + p.score)};
     const Kv4 c = device_of(cache);
