@@ -743,13 +743,16 @@ __global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(
 // is one row of the MFMA, the query and p * scale are the sum of two fp16
 // numbers, the codes are fp16 numbers -8 .. 7, and products are added in fp32.
 // Such a sum has 22 bits, or steps of 2^-24 for numbers below 1/4: the query's
-// largest element is taken to 2^14 .. 2^15, a row's largest p * scale to 2^11
-// .. 2^16, so what is lost is below 2^-36 of the largest.  That takes as many
-// MFMAs as three digits in four rows, but no joining of digits, and the values'
-// sums stay in the accumulators from page to page.  Block: 64 rows, 16 a
-// wavefront; the four take a page's codes apart together, into LDS, as the
-// matrix cores read them (a code word is a lane's 8 elements of one MFMA:
-// halves 0, 2, 4, 6, 1, 3, 5, 7 of its bytes' order).
+// largest element is taken to 2^14 .. 2^15, and p * scale by a factor of each
+// row and 64 dims, so that the largest which the row has met there is at 2^7 or
+// more, and what is lost is below 2^-31 of that, or 2^-84 of a p of 1.  (One
+// factor for all rows, and a maximum that makes up for it, left rows 7e-5 off
+// where values 2^24 times as large that they do not look at lie behind, or in
+// other dims.)  That takes as many MFMAs as three digits in four rows, but no
+// joining of digits, and the values' sums stay in the accumulators from page to
+// page.  Block: 64 rows, 16 a wavefront; the four take a page's codes apart
+// together, into LDS, as the matrix cores read them (a code word is a lane's 8
+// elements of one MFMA: halves 0, 2, 4, 6, 1, 3, 5, 7 of its bytes' order).
 //
 // 512 queries of 32 heads on 8 KV heads of 128 over 4100 positions: 130 us, 32
 // GFLOP at fp32's precision (the int8 kernel with 16 rows a block: 175 us).
@@ -765,6 +768,7 @@ typedef _Float16 h8_alias __attribute__((ext_vector_type(8), may_alias));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 constexpr int kWideRows = 64;
 constexpr float kNoMax = -0x1.fffffep127f;               // no score is lower
+constexpr float kMostFactor = 0x1p60f;                   // times a p of 2^60 it is still a number
 
 __device__ __forceinline__ f4_t mfma32(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 // A code word's eight numbers: 1024 + code as fp16 bits, less 1032.
@@ -916,21 +920,21 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
         }
     }
 
-    // p is 2^(score - m); the values' sums o are those of p * scale * vf
-    float m[4], l[4], om[4][HDG], vf[HDG], vtop[HDG];
+    // p is 2^(score - m); the values' sums o are those of p * scale * f
+    float m[4], l[4], om[4][HDG], f[4][HDG], fm[HDG];
     f4_t o[4 * HDG];
 #pragma unroll
     for (int r = 0; r < 4; r++) {
         m[r] = kNoMax;
         l[r] = 0.f;
 #pragma unroll
-        for (int g = 0; g < HDG; g++) om[r][g] = 0.f;
+        for (int g = 0; g < HDG; g++) {
+            om[r][g] = 0.f;
+            f[r][g] = kMostFactor;
+        }
     }
 #pragma unroll
-    for (int g = 0; g < HDG; g++) {
-        vf[g] = 1.f;
-        vtop[g] = 0.f;
-    }
+    for (int g = 0; g < HDG; g++) fm[g] = kMostFactor;
 #pragma unroll
     for (int d = 0; d < 4 * HDG; d++) o[d] = f4_t{0.f, 0.f, 0.f, 0.f};
     uint16_t* const ph = pw[wave][0];
@@ -964,68 +968,62 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
                 x[r][s] *= kf[r];                        // rounded before m is taken off, as above
                 if constexpr (MASKED) x[r][s] = pos0 + 16 * s + li <= lim[r] ? x[r][s] : -INFINITY;
             }
-        // a power of two takes the largest of a group's scales so far to 2^11 .. 2^12
-        float vs[HDG][4], vsm[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int g = 0; g < HDG; g++) {
-            float vt = 0.f;
-#pragma unroll
-            for (int s = 0; s < 4; s++) {
-                vs[g][s] = h2f(part4(*(const uint4*)&prs[1][g][4 * li], s));
-                if constexpr (MASKED) vs[g][s] = pos0 + 16 * s + li <= lim_hi ? vs[g][s] : 0.f;   // stale pairs may be anything
-                vt = fmaxf(vt, vs[g][s]);
-            }
-            if (__any(vt > vtop[g])) {
-                vtop[g] = fmaxf(row16_max(vt), vtop[g]);
-                const float nf = ldexpf(1.f, 12 - __builtin_amdgcn_frexp_expf(vtop[g])), al = nf / vf[g];
-                vf[g] = nf;
-#pragma unroll
-                for (int d = 0; d < 4; d++) o[4 * g + d] *= al;
-            }
-#pragma unroll
-            for (int s = 0; s < 4; s++) {
-                vs[g][s] *= vf[g];
-                vsm[s] = fmaxf(vsm[s], vs[g][s]);
-            }
-        }
         float e[4][4];
-        auto probs = [&]() {
 #pragma unroll
-            for (int r = 0; r < 4; r++)
+        for (int r = 0; r < 4; r++)
 #pragma unroll
-                for (int s = 0; s < 4; s++) e[r][s] = exp2_(x[r][s] - m[r]);
+            for (int s = 0; s < 4; s++) e[r][s] = exp2_(x[r][s] - m[r]);
+        auto scale = [&](int g, int s) {
+            const float v = h2f(part4(*(const uint4*)&prs[1][g][4 * li], s));
+            return !MASKED || pos0 + 16 * s + li <= lim_hi ? v : 0.f;   // stale pairs may be anything
         };
-        probs();
-        // m moves only when a p * scale no longer fits fp16 or a p is above
-        // 2^60.  It is then set such that the page's largest p * scale is in
-        // 2^11 .. 2^12, or its largest p 2^40 where all that the row looks at
-        // have next to no scale.
-        float most = 0.f, high = 0.f;
+        // m and f stay until a p is above 2^60 or a p * scale * f may not fit
+        // fp16 (by the largest p and factor of the lane's four rows)
+        float pm[4], high = 0.f, most = 0.f;
 #pragma unroll
         for (int s = 0; s < 4; s++) {
-            const float pm = fmaxf(fmaxf(e[0][s], e[1][s]), fmaxf(e[2][s], e[3][s]));
-            high = fmaxf(high, pm);
-            most = fmaxf(most, pm * vsm[s]);
+            pm[s] = fmaxf(fmaxf(e[0][s], e[1][s]), fmaxf(e[2][s], e[3][s]));
+            high = fmaxf(high, pm[s]);
+        }
+#pragma unroll
+        for (int g = 0; g < HDG; g++) {
+            float t = 0.f;
+#pragma unroll
+            for (int s = 0; s < 4; s++) t = fmaxf(t, pm[s] * scale(g, s));
+            most = fmaxf(most, t * fm[g]);
         }
         if (__any(most > 65504.f || high > 0x1p60f)) {
+            // m goes to the row's maximum.  A factor stays if the page's
+            // largest p * scale is at 2^7 .. 65504 with it; else it makes up for
+            // what p lost, or takes that largest to 2^8 .. 2^9.
+#pragma unroll
+            for (int g = 0; g < HDG; g++) fm[g] = 0.f;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const float top = row16_max(fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3])));
-                float w = 0.f;
-#pragma unroll
-                for (int s = 0; s < 4; s++) w = fmaxf(w, exp2_(x[r][s] - top) * vsm[s]);
-                // (from 2^22 on, where fp32 holds no such steps, the page's largest p is 1)
-                const int below = min(12 - __builtin_amdgcn_frexp_expf(row16_max(w)), 40);
-                const float to = fabsf(top) < 0x1p22f ? top - (float)below : top;
-                const float mn = top == -INFINITY ? m[r] : fmaxf(m[r], to), al = exp2_(m[r] - mn);
+                const float mn = fmaxf(m[r], row16_max(fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3]))));
+                const float al = exp2_(m[r] - mn), up = ldexpf(1.f, (int)fminf(mn - m[r], 122.f));
                 m[r] = mn;
                 l[r] *= al;
 #pragma unroll
-                for (int d = 0; d < 4 * HDG; d++) o[d][r] *= al;
+                for (int s = 0; s < 4; s++) e[r][s] = exp2_(x[r][s] - mn);
 #pragma unroll
-                for (int g = 0; g < HDG; g++) om[r][g] *= al;
+                for (int g = 0; g < HDG; g++) {
+                    float t = 0.f;
+#pragma unroll
+                    for (int s = 0; s < 4; s++) t = fmaxf(t, e[r][s] * scale(g, s));
+                    t = row16_max(t);
+                    const float old = f[r][g], raised = fminf(old * up, kMostFactor);
+                    float nf = raised;
+                    if (old * t <= 65504.f && old * t >= 128.f) nf = old;
+                    else if (raised * t > 65504.f) nf = ldexpf(1.f, 9 - __builtin_amdgcn_frexp_expf(t));
+                    f[r][g] = nf;
+                    fm[g] = fmaxf(fm[g], nf);
+                    om[r][g] *= al;
+                    const float of = ldexpf(al, __builtin_amdgcn_frexp_expf(nf) - __builtin_amdgcn_frexp_expf(old));
+#pragma unroll
+                    for (int d = 0; d < 4; d++) o[4 * g + d][r] *= of;
+                }
             }
-            probs();
         }
 #pragma unroll
         for (int r = 0; r < 4; r++)
@@ -1033,15 +1031,18 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
             for (int s = 0; s < 4; s++) l[r] += e[r][s];
 #pragma unroll
         for (int g = 0; g < HDG; g++) {
-            float vm[4];
+            float vs[4], vm[4];
 #pragma unroll
-            for (int s = 0; s < 4; s++) vm[s] = h2f(part4(*(const uint4*)&prs[1][g][4 * li], s) >> 16);
+            for (int s = 0; s < 4; s++) {
+                vs[s] = scale(g, s);
+                vm[s] = h2f(part4(*(const uint4*)&prs[1][g][4 * li], s) >> 16);
+            }
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 float w[4];
 #pragma unroll
                 for (int s = 0; s < 4; s++) {
-                    w[s] = e[r][s] * vs[g][s];
+                    w[s] = e[r][s] * f[r][g] * vs[s];
                     if constexpr (MASKED) {              // a NaN that this row does not see
                         const bool ok = pos0 + 16 * s + li <= lim[r];
                         w[s] = ok ? w[s] : 0.f;
@@ -1127,7 +1128,7 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
         const float norm = a.n_split > 1 ? (bad ? NAN : 1.f) : (sum == 0.f ? 0.f : 1.f / sum);
 #pragma unroll
         for (int g = 0; g < HDG; g++) {
-            const float mid = row16_sum(om[r][g]), back = 1.f / vf[g];
+            const float mid = row16_sum(om[r][g]), back = 1.f / f[r][g];
 #pragma unroll
             for (int d = 0; d < 4; d++)
                 if (in) dst[64 * g + 16 * d + li] = fmaf(o[4 * g + d][r], back, mid) * norm;

@@ -35,3 +35,55 @@ def test_weights_of_tied_scores(ops, n_q, t, size):
     got = w.cpu().numpy()[0]
     assert (np.abs(got[:, :t] - want) <= (4 + n_q * grp) * 2.0 ** -24 * want).all(), (got[:, 0], want[0])
     assert (got[:, t:] == 0).all()
+
+
+# ── values of uneven size ────────────────────────────────────────────────────
+def parts(m, i, q, n_q, n_heads):
+    """Row by row (query, head): the output's 64-dim groups in 64 bits, the sums of p |v| over each group, the largest
+    sum |q k| / sqrt(hd)."""
+    K, V = m.loaded(i)
+    hd, grp = m.hd, n_heads // m.n_kv
+    q = np.asarray(q, np.float64).reshape(n_q, n_heads, hd)
+    out, size, top = np.zeros((n_q, n_heads, hd // 64, 64)), np.zeros((n_q, n_heads, hd // 64)), 0.0
+    for a in range(n_q):
+        n = K.shape[1] - n_q + a + 1
+        for h in range(n_heads):
+            k, v = K[h // grp, :n], V[h // grp, :n].reshape(n, -1, 64)
+            s = k @ q[a, h] / np.sqrt(hd)
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            out[a, h] = np.tensordot(p, v, 1)
+            size[a, h] = p @ np.linalg.norm(v, axis=2)
+            top = max(top, float((np.abs(k) @ np.abs(q[a, h])).max() / np.sqrt(hd)))
+    return out, size, top
+
+
+@pytest.mark.parametrize("groups", [slice(0, 1), slice(0, None)])
+@pytest.mark.parametrize("n_heads,n_kv,n_q,t,hd", [
+    (8, 2, 1, 330, 64), (8, 2, 12, 330, 64), (8, 2, 12, 330, 128), (8, 2, 70, 1500, 128), (8, 2, 12, 330, 192),
+    (64, 64, 40, 130, 64), (64, 64, 40, 1600, 128), (64, 64, 34, 700, 256)])   # blocks of several pages: one split, and more
+def test_large_values_behind_small_ones(ops, n_heads, n_kv, n_q, t, hd, groups):
+    """The first page holds only values of 2^-14, which every query looks at; from the second page on there are others
+    of 2^10 (in the first 64 dims, or in all) that none looks at, with probabilities below 2^-60.  A score is off by
+    8 e S (S = sum |q k| / sqrt(hd)) and moves its probability by that share, and the normaliser by as much: 16 e
+    max(1, S) of sum p |v| of each 64 dims on their own."""
+    print(f"case behind {n_heads}/{n_kv} n_q={n_q} t={t} hd={hd} {groups}", flush=True)
+    rng = np.random.default_rng(43 + hd)
+    m = Made(ops, rng, [t], n_kv, hd)
+    u = rng.choice([-1.0, 1.0], hd)
+    seen = (np.arange(t) % 64 < 23) & (np.arange(t) < 250)
+    seen[:64] = True
+    k = rng.standard_normal((t, n_kv, hd)) * 0.1 + np.where(seen, 3.0, -3.0)[:, None, None] * u
+    v = rng.standard_normal((t, n_kv, hd)) * 2.0 ** -14
+    v.reshape(t, n_kv, -1, 64)[~seen, :, groups] *= 2.0 ** 24
+    m.k[0], m.v[0] = (x.reshape(t, -1).astype(np.float32) for x in (k, v))
+    ops.kv4_append(m.cache, torch.from_numpy(m.k[0][None]).cuda(), torch.from_numpy(m.v[0][None]).cuda())
+    q = rng.standard_normal((1, n_q, n_heads, hd)) * 0.1 + 10 / np.sqrt(hd) * u
+    q = torch.from_numpy(q.reshape(1, n_q, n_heads * hd).astype(np.float32)).cuda()
+    out = torch.empty_like(q)
+    ops.kv4_attn(out, q, m.cache, n_heads)
+    want, size, top = parts(m, 0, q[0].cpu().numpy(), n_q, n_heads)
+    err = np.linalg.norm(out.cpu().numpy().reshape(want.shape) - want, axis=-1)
+    tol = 16 * 2.0 ** -24 * max(1.0, top)
+    print("err / size", (err / size).max(), "tol", tol, flush=True)
+    assert (err <= tol * size).all()
