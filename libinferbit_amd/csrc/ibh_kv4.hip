@@ -745,7 +745,7 @@ __global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(
 // Such a sum has 22 bits, or steps of 2^-24 for numbers below 1/4: the query's
 // largest element is taken to 2^14 .. 2^15, and p * scale by a factor of each
 // row and 64 dims, so that the largest which the row has met there is at 2^7 or
-// more, and what is lost is below 2^-31 of that, or 2^-84 of a p of 1.  (One
+// more, and what is lost is below 2^-32 of that, or 2^-85 of a p of 1.  (One
 // factor for all rows, and a maximum that makes up for it, left rows 7e-5 off
 // where values 2^24 times as large that they do not look at lie behind, or in
 // other dims.)  That takes as many MFMAs as three digits in four rows, but no
@@ -792,7 +792,12 @@ __device__ __forceinline__ float less_half(float x, uint32_t h) {
     else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(y) : "v"(h), "v"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t pack_rtz(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)); }
+// Two fp16 numbers, rounded to nearest: halves that are cut off are all too
+// small, and the sum of the probabilities does not share that.
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+    typedef float f2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2_t{a, b}, h2_t));
+}
 
 // Rows' constants for the weights, each array padded to whole blocks of rows.
 struct WideRows {
@@ -1052,9 +1057,9 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
                     }
                 }
                 // slots 4 li + s: quarter li / 4, half li / 2 % 2, then s = 0, 2 and s = 1, 3
-                const uint32_t h02 = pack_rtz(w[0], w[2]), h13 = pack_rtz(w[1], w[3]);
-                const uint32_t l02 = pack_rtz(less_half<false>(w[0], h02), less_half<true>(w[2], h02));
-                const uint32_t l13 = pack_rtz(less_half<false>(w[1], h13), less_half<true>(w[3], h13));
+                const uint32_t h02 = pack_half(w[0], w[2]), h13 = pack_half(w[1], w[3]);
+                const uint32_t l02 = pack_half(less_half<false>(w[0], h02), less_half<true>(w[2], h02));
+                const uint32_t l13 = pack_half(less_half<false>(w[1], h13), less_half<true>(w[3], h13));
                 const int at = (4 * lq + r) * PR + (li >> 1) * 8 + (li & 1) * 2;
                 *(u32_alias*)(ph + at) = h02;
                 *(u32_alias*)(ph + at + 4) = h13;

@@ -87,3 +87,22 @@ def test_large_values_behind_small_ones(ops, n_heads, n_kv, n_q, t, hd, groups):
     tol = 16 * 2.0 ** -24 * max(1.0, top)
     print("err / size", (err / size).max(), "tol", tol, flush=True)
     assert (err <= tol * size).all()
+
+
+@pytest.mark.parametrize("n_heads,n_kv,n_q", [(16, 4, 64)])
+def test_probabilities_are_not_cut_short(ops, n_heads, n_kv, n_q):
+    """All positions hold one value vector, -2 in one dim of each 64 and 7/4 (scale 1/4, mid 0) in the others, so the
+    output is that vector whatever the probabilities are, and what it lacks is what p * scale lost.  Roundings to
+    nearest leave no mean: at most 4 e a row from its sums, and less than e in the mean over 64 rows and more."""
+    rng = np.random.default_rng(71)
+    hd, t = 64, 128
+    m = Made(ops, rng, [t], n_kv, hd)
+    v = np.where(np.arange(n_kv * hd) % 64 == 9, -2.0, 1.75)
+    m.v[0] = np.tile(v, (t, 1)).astype(np.float32)
+    ops.kv4_append(m.cache, torch.from_numpy(m.k[0][None]).cuda(), torch.from_numpy(m.v[0][None]).cuda())
+    q = torch.from_numpy(rng.standard_normal((1, n_q, n_heads * hd)).astype(np.float32)).cuda()
+    out = torch.empty_like(q)
+    ops.kv4_attn(out, q, m.cache, n_heads)
+    r = out.cpu().numpy().astype(np.float64).reshape(-1, 64) / v[:64] - 1
+    print("mean", r.mean(), "largest", np.abs(r).max(), flush=True)
+    assert abs(r.mean()) <= 2.0 ** -24
