@@ -301,31 +301,38 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4 c, float* __restrict_
 
 // ── attention ────────────────────────────────────────────────────────────────
 // The matrix cores multiply the codes as they lie.  The other operand of each
-// product is written in three signed base-256 digits, x = step * (65536 d0 +
-// 256 d1 + d2) with |x| <= 63.5 * 65536 step (22 bits below the largest element
-// of a query, or of a page's p * scale), so every product and sum is exact in
-// int32 and what is rounded is rounded as in fp32.  A tile is 4 query rows (a
-// row is one head of one query) as the 16 rows of the MFMA's first operand:
-// row 4 i + j is digit j of query row i, j < 3.  The result leaves lane l with
-// the digits' sums of query row l / 16 and column l % 16, so they are joined
-// in the lane.  Codes are 0 .. 15; a product with -8 in every place, used as
-// the accumulator, centres them.
+// product is written in four signed base-256 digits, x = step * (2^24 d0 + 2^16
+// d1 + 2^8 d2 + d3), step a power of two that takes the largest element of a
+// query, or of a page's p * scale, to 2^29 .. 2^30.  An element thus keeps its
+// 24 bits down to 2^-6 of the largest, and 2^-30 of the largest below that;
+// products and sums are exact in int32 and rounded where their digits are
+// joined.  (With three digits, 22 bits, a query that has one channel of 3000
+// among others of 1 left the output 4e-5 off.)  A tile is 4 query rows (a row
+// is one head of one query) as the 16 rows of the MFMA's first operand: row
+// 4 i + j is digit j of query row i.  The result leaves lane l with the digits'
+// sums of query row l / 16 and column l % 16, so they are joined in the lane.
+// Codes are 0 .. 15; a product with -8 in every place, used as the accumulator,
+// centres them.
 typedef int i4_t __attribute__((ext_vector_type(4)));
 typedef int i4_alias __attribute__((ext_vector_type(4), may_alias));
 typedef uint32_t u32_alias __attribute__((may_alias));
 
-// 63.5 * 65536: 64 products of such a number with -8 .. 7 fit 31 bits, so the
-// three digits' sums are joined as integers, by shifts
-constexpr float kDigitMax = 4161536.f;
+constexpr int kDigitBits = 30;                           // of the largest element: its highest digit is 64 or less
+constexpr uint32_t kDigitOff = 0x00808080u;              // takes the low three digits to 0 .. 255
 constexpr int kMaxSplit = 4096;                          // blocks of one row tile
-constexpr float kTiny = 1e-30f;                          // below this a query, or a page's p * scale, counts as zero
 
 __device__ __forceinline__ i4_t unpack16(uint32_t a, uint32_t b) {
     constexpr uint32_t M = 0x0f0f0f0fu;
     return i4_t{(int)(a & M), (int)((a >> 4) & M), (int)(b & M), (int)((b >> 4) & M)};
 }
 __device__ __forceinline__ i4_t mfma16(i4_t a, i4_t b, i4_t c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ float join_digits(i4_t c) { return (float)(int)((((uint32_t)c[0] << 8) + (uint32_t)c[1] << 8) + (uint32_t)c[2]); }
+// The upper and lower two digits' sums: 64 products of a pair with -8 .. 7 stay
+// below 2^25, so each half is rounded by 2^-24 of itself at most.
+__device__ __forceinline__ float upper_digits(i4_t c) { return (float)(c[0] * 256 + c[1]); }
+__device__ __forceinline__ float lower_digits(i4_t c) { return (float)(c[2] * 256 + c[3]); }
+__device__ __forceinline__ float join_digits(i4_t c) { return fmaf(upper_digits(c), 65536.f, lower_digits(c)); }
+// A row's elements are multiplied by 2^digit_shift(their largest).
+__device__ __forceinline__ int digit_shift(float most) { return kDigitBits - __builtin_amdgcn_frexp_expf(most); }
 // v_exp_f32: at most one unit in the last place off, results below 2^-126 are 0
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 // Largest value of the 16 lanes of a row, every lane getting it: v_max_f32
@@ -502,19 +509,20 @@ __global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(
             mx = fmaxf(mx, fabsf(x[g]));
         }
         mx = wave_max_dpp(mx);
-        const float step = mx > kTiny ? mx / kDigitMax : 1.f, inv = mx > kTiny ? kDigitMax / mx : 0.f;
+        const bool inf = mx == INFINITY;                 // a row of NaN
+        const int up = inf ? 0 : digit_shift(mx);
 #pragma unroll
         for (int g = 0; g < HDG; g++) {
-            const int j = (int)rintf(x[g] * inv) + 0x8080;   // the two low digits offset by 128 each
+            const uint32_t j = (inf ? 0u : (uint32_t)(int)rintf(ldexpf(x[g], up))) + kDigitOff;
             int8_t* d = digs + ((r >> 2) * HDG + g) * 1024 + (r & 3) * 256 + lane;
-            d[0] = (int8_t)(j >> 16);
-            d[64] = (int8_t)((j >> 8) ^ 0x80);
-            d[128] = (int8_t)(j ^ 0x80);
-            d[192] = 0;
-            const float sum = wave_sum_dpp(x[g]) / step;
-            if (lane == 0) rc[r][1 + g] = sum;
+            d[0] = (int8_t)(j >> 24);
+            d[64] = (int8_t)((j >> 16) ^ 0x80);
+            d[128] = (int8_t)((j >> 8) ^ 0x80);
+            d[192] = (int8_t)(j ^ 0x80);
+            const float sum = ldexpf(wave_sum_dpp(x[g]), up);
+            if (lane == 0) rc[r][1 + g] = inf ? NAN : sum;
         }
-        if (lane == 0) rc[r][0] = step * a.scale;
+        if (lane == 0) rc[r][0] = ldexpf(a.scale, -up);
     }
     __syncthreads();
     i4_t qa[RT][HDG];
@@ -643,24 +651,28 @@ __global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(
                     }
                 }
                 const float wm = row16_max(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])));
-                const float ws = fmaxf(wm, kTiny) * (1.f / kDigitMax), inv = __builtin_amdgcn_rcpf(ws);
+                const int up = digit_shift(wm);
+                const float ws = ldexpf(1.f, -up), wu = ldexpf(1.f, 16 - up);
                 uint32_t j[4];
 #pragma unroll
-                for (int s = 0; s < 4; s++) j[s] = (uint32_t)fmaf(w[s], inv, 32896.5f);
+                for (int s = 0; s < 4; s++) j[s] = (uint32_t)ldexpf(w[s], up) + kDigitOff;   // cut by 2^-30 of the largest
                 // bytes of the four slots 4 li + s, one word a digit
                 const uint32_t a01 = __builtin_amdgcn_perm(j[1], j[0], 0x05010400), a23 = __builtin_amdgcn_perm(j[3], j[2], 0x05010400);
-                const uint32_t b01 = __builtin_amdgcn_perm(j[1], j[0], 0x0c0c0602), b23 = __builtin_amdgcn_perm(j[3], j[2], 0x06020c0c);
+                const uint32_t b01 = __builtin_amdgcn_perm(j[1], j[0], 0x07030602), b23 = __builtin_amdgcn_perm(j[3], j[2], 0x07030602);
                 u32_alias* d = (u32_alias*)(tw + g * 1280 + lq * 320 + li * 4);
-                d[0] = b01 | b23;
-                d[16] = __builtin_amdgcn_perm(a23, a01, 0x07060302) ^ 0x80808080u;
-                d[32] = __builtin_amdgcn_perm(a23, a01, 0x05040100) ^ 0x80808080u;
+                d[0] = __builtin_amdgcn_perm(b23, b01, 0x07060302);
+                d[16] = __builtin_amdgcn_perm(b23, b01, 0x05040100) ^ 0x80808080u;
+                d[32] = __builtin_amdgcn_perm(a23, a01, 0x07060302) ^ 0x80808080u;
+                d[48] = __builtin_amdgcn_perm(a23, a01, 0x05040100) ^ 0x80808080u;
                 __builtin_amdgcn_wave_barrier();
                 const i4_t wa = *(const i4_alias*)(tw + g * 1280 + (li >> 2) * 320 + (li & 3) * 64 + lq * 16);
                 __builtin_amdgcn_wave_barrier();
                 const i4_t init = mfma16(wa, minus8, zero);
 #pragma unroll
-                for (int d4 = 0; d4 < 4; d4++)
-                    o[t][4 * g + d4] = fmaf(join_digits(mfma16(wa, vb[d4], init)), ws, o[t][4 * g + d4]);
+                for (int d4 = 0; d4 < 4; d4++) {
+                    const i4_t c = mfma16(wa, vb[d4], init);
+                    o[t][4 * g + d4] = fmaf(upper_digits(c), wu, fmaf(lower_digits(c), ws, o[t][4 * g + d4]));
+                }
             }
             vp[g] = val_pairs<HDG, RT <= 2>(nx, g, at);
         }
@@ -748,7 +760,7 @@ __global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(
 // more, and what is lost is below 2^-32 of that, or 2^-85 of a p of 1.  (One
 // factor for all rows, and a maximum that makes up for it, left rows 7e-5 off
 // where values 2^24 times as large that they do not look at lie behind, or in
-// other dims.)  That takes as many MFMAs as three digits in four rows, but no
+// other dims.)  That takes as many MFMAs as four digits in four rows, but no
 // joining of digits, and the values' sums stay in the accumulators from page to
 // page.  Block: 64 rows, 16 a wavefront; the four take a page's codes apart
 // together, into LDS, as the matrix cores read them (a code word is a lane's 8
@@ -767,6 +779,7 @@ typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 h8_alias __attribute__((ext_vector_type(8), may_alias));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 constexpr int kWideRows = 64;
+constexpr float kTiny = 1e-30f;                          // a query below this counts as zero
 constexpr float kNoMax = -0x1.fffffep127f;               // no score is lower
 constexpr float kMostFactor = 0x1p60f;                   // times a p of 2^60 it is still a number
 

@@ -89,7 +89,7 @@ def test_large_values_behind_small_ones(ops, n_heads, n_kv, n_q, t, hd, groups):
     assert (err <= tol * size).all()
 
 
-@pytest.mark.parametrize("n_heads,n_kv,n_q", [(16, 4, 64)])
+@pytest.mark.parametrize("n_heads,n_kv,n_q", [(64, 16, 1), (16, 4, 6), (16, 4, 64)])
 def test_probabilities_are_not_cut_short(ops, n_heads, n_kv, n_q):
     """All positions hold one value vector, -2 in one dim of each 64 and 7/4 (scale 1/4, mid 0) in the others, so the
     output is that vector whatever the probabilities are, and what it lacks is what p * scale lost.  Roundings to
@@ -106,3 +106,67 @@ def test_probabilities_are_not_cut_short(ops, n_heads, n_kv, n_q):
     r = out.cpu().numpy().astype(np.float64).reshape(-1, 64) / v[:64] - 1
     print("mean", r.mean(), "largest", np.abs(r).max(), flush=True)
     assert abs(r.mean()) <= 2.0 ** -24
+
+
+# ── queries with one large channel ───────────────────────────────────────────
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("n_heads,n_kv,hd,n_q,t", [(8, 2, 128, 1, 700), (8, 2, 128, 1, 4096), (8, 2, 64, 2, 1100), (8, 2, 128, 6, 700),
+                                                   (6, 2, 192, 5, 300), (4, 2, 256, 8, 300), (8, 2, 128, 9, 700)])
+@pytest.mark.parametrize("size", [30.0, 300.0, 3000.0])
+def test_query_with_an_outlier_channel(ops, n_heads, n_kv, hd, n_q, t, size, weights):
+    """One channel of the query is large, and the keys hold 0 there (scale 1/4, mid 0), so the others make the score.
+    A score is off by 8 e S (S = sum |q k| / sqrt(hd)): 16 e max(1, S) of sum p |v|."""
+    print(f"case outlier {n_heads}/{n_kv} hd={hd} n_q={n_q} t={t} size={size} weights={weights}", flush=True)
+    rng = np.random.default_rng(hd + n_q)
+    m = Made(ops, rng, [t], n_kv, hd)
+    k = np.clip(rng.standard_normal((t, n_kv, hd // 64, 64)), -2, 1.75)
+    k[..., 0], k[..., 1] = -2, 1.75
+    k[:, :, 0, 7] = 0
+    m.k[0] = k.reshape(t, -1).astype(np.float32)
+    ops.kv4_append(m.cache, torch.from_numpy(m.k[0][None]).cuda(), torch.from_numpy(m.v[0][None]).cuda())
+    q = rng.standard_normal((1, n_q, n_heads, hd))
+    q[..., 7] = size * rng.uniform(0.7, 1.4, q.shape[:-1])
+    q = torch.from_numpy(q.reshape(1, n_q, n_heads * hd).astype(np.float32)).cuda()
+    out, w = torch.empty_like(q), torch.zeros(1, n_kv, m.table.shape[1] * 64, device="cuda")
+    ops.kv4_attn(out, q, m.cache, n_heads, **(dict(weights_in=w, weights_out=w) if weights else {}))
+    want, size, top = parts(m, 0, q[0].cpu().numpy(), n_q, n_heads)
+    assert (m.loaded(0)[0][:, :, 7] == 0).all()
+    err = np.linalg.norm(out.cpu().numpy().reshape(want.shape) - want, axis=-1)
+    tol = 16 * 2.0 ** -24 * max(1.0, top)
+    print("err / size", (err / size).max(), "tol", tol, flush=True)
+    assert (err <= tol * size).all()
+    if weights:
+        p = R.attend(q[0].cpu().numpy(), *m.loaded(0), n_q)[1]
+        assert (np.abs(w[0, :, :t].cpu().numpy() - p) <= (tol + 2.0 ** -22) * p + 2.0 ** -120).all()
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,n_q,t", [(8, 2, 128, 1, 700), (8, 2, 64, 6, 300), (8, 2, 128, 9, 700)])
+@pytest.mark.parametrize("size", [30.0, 3000.0])
+def test_query_with_an_outlier_channel_beside_middles(ops, n_heads, n_kv, hd, n_q, t, size):
+    """The same where the keys' other channels lie around 3/2, so that 0 is -8 steps from a middle: a score is the sum
+    over its 64-dim groups of mid * sum q and scale * sum q (code - 8), which cancel.  Each is off by 8 e of its own
+    absolute sum, A = sum (|mid| sum |q| + scale sum |q (code - 8)|) / sqrt(hd): 16 e max(1, A) of sum p |v|."""
+    print(f"case beside middles {n_heads}/{n_kv} hd={hd} n_q={n_q} t={t} size={size}", flush=True)
+    rng = np.random.default_rng(hd + n_q)
+    m = Made(ops, rng, [t], n_kv, hd)
+    k = np.clip(rng.standard_normal((t, n_kv, hd)) * 0.5 + 1.5, 0.01, 3)
+    k[:, :, 7] = 0
+    m.k[0] = k.reshape(t, -1).astype(np.float32)
+    ops.kv4_append(m.cache, torch.from_numpy(m.k[0][None]).cuda(), torch.from_numpy(m.v[0][None]).cuda())
+    q = rng.standard_normal((1, n_q, n_heads, hd))
+    q[..., 7] = size * rng.uniform(0.7, 1.4, q.shape[:-1])
+    q = torch.from_numpy(q.reshape(1, n_q, n_heads * hd).astype(np.float32)).cuda()
+    out = torch.empty_like(q)
+    ops.kv4_attn(out, q, m.cache, n_heads)
+    want, sums, _ = parts(m, 0, q[0].cpu().numpy(), n_q, n_heads)
+    c, s, mid = (x.astype(np.float64) for x in R.quantise(m.k[0]))
+    aq = np.abs(q[0].cpu().numpy().astype(np.float64)).reshape(n_q, n_kv, -1, hd // 64, 64)
+    c, s, mid = c.reshape(t, n_kv, hd // 64, 64), s.reshape(t, n_kv, -1), mid.reshape(t, n_kv, -1)
+    top = 0.0
+    for h in range(n_kv):
+        a = np.einsum("tg,qrg->tqr", np.abs(mid[:, h]), aq[:, h].sum(-1)) + np.einsum("tg,tgd,qrgd->tqr", s[:, h], np.abs(c[:, h] - 8), aq[:, h])
+        top = max(top, a.max() / np.sqrt(hd))
+    err = np.linalg.norm(out.cpu().numpy().reshape(want.shape) - want, axis=-1)
+    tol = 16 * 2.0 ** -24 * max(1.0, top)
+    print("err / size", (err / sums).max(), "tol", tol, flush=True)
+    assert (err <= tol * sums).all()
