@@ -1999,10 +1999,9 @@ bool cache_ok(const ibh_kv4_cache* c, const char* who) {
 Kv4 device_of(const ibh_kv4_cache* c) {
     return {(uint8_t*)c->pool, c->table, c->lens, c->n_pages, c->n_seq, c->max_pages, c->n_kv, c->head_dim};
 }
-// No launch of this file has blocks of more than 1024 threads; one takes less
-// than 2^32 threads.
-bool grid_ok(size_t blocks, const char* who) {
-    if (blocks < (size_t)1 << 22) return true;
+// A launch takes less than 2^32 threads.
+bool grid_ok(size_t blocks, size_t threads, const char* who) {
+    if (blocks < ((size_t)1 << 32) / threads) return true;
     ibh_set_error("%s: %zu blocks of work are more than one launch takes", who, blocks);
     return false;
 }
@@ -2035,7 +2034,7 @@ extern "C" int ibh_kv4_append(const ibh_kv4_cache* cache, const float* k, const 
     }
     const int n_touch = min((n_new + kPage - 2) / kPage + 1, cache->max_pages);
     const size_t blocks = (size_t)cache->n_seq * n_touch * cache->n_kv * 2 * (cache->head_dim / 64);
-    if (!grid_ok(blocks, "ibh_kv4_append")) return IBH_ERROR_PARAM;
+    if (!grid_ok(blocks, 256, "ibh_kv4_append")) return IBH_ERROR_PARAM;
     const int vec = (((uintptr_t)k | (uintptr_t)v) & 15) == 0 && kv_stride % 4 == 0;
     kv4_append_kernel<<<(unsigned)blocks, 256, 0, ibh_resolve_stream(stream)>>>(device_of(cache), k, v, n_new,
                                                                                 kv_stride, n_touch, vec);
@@ -2051,7 +2050,7 @@ extern "C" int ibh_kv4_read(const ibh_kv4_cache* cache, float* k, float* v, int 
     }
     const int n_touch = min((n + kPage - 2) / kPage + 1, cache->max_pages);
     const size_t blocks = (size_t)cache->n_seq * n_touch * cache->n_kv * 2 * (cache->head_dim / 64);
-    if (!grid_ok(blocks, "ibh_kv4_read")) return IBH_ERROR_PARAM;
+    if (!grid_ok(blocks, 256, "ibh_kv4_read")) return IBH_ERROR_PARAM;
     const int vec = (((uintptr_t)k | (uintptr_t)v) & 15) == 0 && kv_stride % 4 == 0;
     kv4_read_kernel<<<(unsigned)blocks, 256, 0, ibh_resolve_stream(stream)>>>(device_of(cache), k, v, n, kv_stride,
                                                                               n_touch, vec);
@@ -2064,6 +2063,8 @@ struct AttnPlan {
     int rt, n_tile, n_split, chunk, quantum, nw;         // rt 16: kv4_attn_wide
     uint32_t per_split;
     bool joint;                                          // the weights in the launch that joins the splits
+    size_t blocks, joins, weighs;                        // blocks of the launches: attention, joining splits (and joint weights), weights
+    int weigh_nw;                                        // wavefronts of a block of the weights' launch
     size_t part, part_ml, stat, digits, rowc, score, bytes;     // offsets into the workspace
 };
 static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool weights) {
@@ -2121,6 +2122,18 @@ static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool wei
     p.per_split = n > 1 ? (uint32_t)((((uint64_t)1 << 32) + n - 1) / n) : 0;
     p.chunk = n > 1 ? chunk_of(c->max_pages, p.n_split, p.per_split, p.quantum) : c->max_pages;
     p.joint = weights && p.n_tile == 1 && p.n_split > 1 && p.rt <= 2;
+    p.blocks = base * p.n_split;
+    const size_t all = heads * n_rows;
+    p.joins = p.n_split == 1 ? 0 : wide && p.n_split <= kFewSplits ? (all + 3) / 4 : all;
+    if (p.joint) p.joins += heads * ((c->max_pages + 3) / 4);
+    p.weighs = weights && !p.joint ? heads * c->max_pages : 0;
+    // Wavefronts a page.  Many rows: four, eight where there are few pages
+    // (2048 rows, 8 KV heads of 128: 169 and 179 us with 512 pages, 81 and 68
+    // with 80; 40 rows, 4096 pages: 66 and 92; whole calls).  Up to 32: one
+    // where the pages fill the card or have few rows, else eight (24 rows: 57
+    // and 70 us with 4096 pages, 24 and 22 with 80).
+    if (wide) p.weigh_nw = p.weighs >= 512 ? 4 : 8;
+    else p.weigh_nw = p.weighs >= 2048 || n_rows <= 16 ? 1 : 8;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
     p.part = take(p.n_split > 1 ? heads * n_rows * p.n_split * c->head_dim * sizeof(float) : 0);
@@ -2145,21 +2158,16 @@ extern "C" size_t ibh_kv4_attn_workspace_bytes(const ibh_kv4_cache* cache, int n
 template <int HDG, int RT>
 static void launch_attn_rt(const Kv4& c, const AttnArgs& a, const AttnPlan& p, size_t heads, const float* win,
                            float* wout, hipStream_t st) {
-    const size_t rows = p.n_split > 1 ? heads * a.n_q * (a.n_heads / c.n_kv) : 0;
-    const unsigned blocks = (unsigned)(heads * p.n_tile * p.n_split);
+    const unsigned blocks = (unsigned)p.blocks, weighs = (unsigned)p.weighs;
     if constexpr (RT <= 2) {
         if (p.joint) kv4_attn_kernel<HDG, RT, true, 4><<<blocks, 256, 0, st>>>(c, a);
         else if constexpr (HDG * RT <= 6) if (p.nw == 8) kv4_attn_kernel<HDG, RT, false, 8><<<blocks, 512, 0, st>>>(c, a);
     }
     if (!p.joint && p.nw == 4) kv4_attn_kernel<HDG, RT, false, 4><<<blocks, 256, 0, st>>>(c, a);
-    const size_t wb = p.joint ? heads * ((c.max_pages + 3) / 4) : 0;
-    if (rows + wb) kv4_attn_finish<HDG, (RT <= 2 ? RT : 1)><<<(unsigned)(rows + wb), 256, 0, st>>>(c, a, (unsigned)rows, win, wout);
-    if (wout && !p.joint) {
-        // a wavefront a page where they fill the card, or have few rows; else
-        // eight (24 rows: 57 and 70 us with 4096 pages, 24 and 22 with 80)
-        if (heads * c.max_pages >= 2048 || a.n_q * (a.n_heads / c.n_kv) <= 16) kv4_attn_weights<HDG, 1><<<(unsigned)(heads * c.max_pages), 64, 0, st>>>(c, a, win, wout);
-        else kv4_attn_weights<HDG, 8><<<(unsigned)(heads * c.max_pages), 512, 0, st>>>(c, a, win, wout);
-    }
+    const unsigned rows = p.n_split > 1 ? (unsigned)(heads * a.n_q * (a.n_heads / c.n_kv)) : 0;
+    if (p.joins) kv4_attn_finish<HDG, (RT <= 2 ? RT : 1)><<<(unsigned)p.joins, 256, 0, st>>>(c, a, rows, win, wout);
+    if (weighs && p.weigh_nw == 1) kv4_attn_weights<HDG, 1><<<weighs, 64, 0, st>>>(c, a, win, wout);
+    else if (weighs) kv4_attn_weights<HDG, 8><<<weighs, 512, 0, st>>>(c, a, win, wout);
 }
 template <int HDG>
 static void launch_attn(const Kv4& c, const AttnArgs& a, const AttnPlan& p, size_t heads, const float* win,
@@ -2167,15 +2175,11 @@ static void launch_attn(const Kv4& c, const AttnArgs& a, const AttnPlan& p, size
     if (p.rt == kWideRows / 4) {
         const size_t rows = heads * a.n_q * (a.n_heads / c.n_kv), pad = heads * p.n_tile * kWideRows;
         const WideRows wr = wout ? WideRows{(h8_t*)a.digits, a.rowc, a.rowc + pad, a.stat} : WideRows{};
-        kv4_attn_wide<HDG><<<(unsigned)(heads * p.n_tile * p.n_split), 256, 0, st>>>(c, a, wr);
-        if (p.n_split > kFewSplits) kv4_attn_finish<HDG, 1><<<(unsigned)rows, 256, 0, st>>>(c, a, (unsigned)rows, win, wout);
-        else if (p.n_split > 1) kv4_attn_join<HDG><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(c, a, rows);
-        // four wavefronts a page, eight where there are few pages (2048 rows, 8
-        // KV heads of 128: 169 and 179 us with 512 pages, 81 and 68 with 80; 40
-        // rows, 4096 pages: 66 and 92; whole calls)
-        const unsigned pages = (unsigned)(heads * c.max_pages);
-        if (wout && pages >= 512) kv4_weights_wide<HDG, 4><<<pages, 256, 0, st>>>(c, a, wr, win, wout);
-        else if (wout) kv4_weights_wide<HDG, 8><<<pages, 512, 0, st>>>(c, a, wr, win, wout);
+        kv4_attn_wide<HDG><<<(unsigned)p.blocks, 256, 0, st>>>(c, a, wr);
+        if (p.n_split > kFewSplits) kv4_attn_finish<HDG, 1><<<(unsigned)p.joins, 256, 0, st>>>(c, a, (unsigned)rows, win, wout);
+        else if (p.joins) kv4_attn_join<HDG><<<(unsigned)p.joins, 256, 0, st>>>(c, a, rows);
+        if (p.weighs && p.weigh_nw == 4) kv4_weights_wide<HDG, 4><<<(unsigned)p.weighs, 256, 0, st>>>(c, a, wr, win, wout);
+        else if (p.weighs) kv4_weights_wide<HDG, 8><<<(unsigned)p.weighs, 512, 0, st>>>(c, a, wr, win, wout);
     } else if (p.rt == 1) launch_attn_rt<HDG, 1>(c, a, p, heads, win, wout, st);
     else if (p.rt == 2) launch_attn_rt<HDG, 2>(c, a, p, heads, win, wout, st);
     else if constexpr (HDG <= 2) launch_attn_rt<HDG, 4>(c, a, p, heads, win, wout, st);
@@ -2201,8 +2205,8 @@ extern "C" int ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float*
         return IBH_ERROR_MEMORY;
     }
     const size_t heads = (size_t)cache->n_seq * cache->n_kv;
-    if (!grid_ok(heads * p.n_tile * p.n_split, "ibh_kv4_attn") ||
-        !grid_ok(heads * n_q * (n_heads / cache->n_kv) + heads * cache->max_pages, "ibh_kv4_attn"))
+    if (!grid_ok(p.blocks, 64 * p.nw, "ibh_kv4_attn") || !grid_ok(p.joins, 256, "ibh_kv4_attn") ||
+        !grid_ok(p.weighs, 64 * p.weigh_nw, "ibh_kv4_attn"))
         return IBH_ERROR_PARAM;
     char* w = (char*)ws;
     AttnArgs a{out, q, n_heads, n_q, q_stride, (float)(1.4426950408889634 / sqrt((double)cache->head_dim)),
@@ -2266,7 +2270,9 @@ extern "C" int ibh_kv4_evict(const ibh_kv4_cache* src, const ibh_kv4_cache* dst,
     }
     const size_t heads = (size_t)src->n_seq * src->n_kv;
     const size_t blocks = heads * (in_place ? 1 : dst->max_pages);
-    if (!grid_ok(blocks, "ibh_kv4_evict") || !grid_ok(heads * kSegs, "ibh_kv4_evict")) return IBH_ERROR_PARAM;
+    if (!grid_ok(blocks, in_place ? 1024 : 2 * src->head_dim, "ibh_kv4_evict") ||
+        !grid_ok(heads * (need ? kSegs : 1), kSelThreads, "ibh_kv4_evict"))
+        return IBH_ERROR_PARAM;
     hipStream_t st = ibh_resolve_stream(stream);
     const Kv4 s = device_of(src), d = device_of(dst);
     if (!need) {

@@ -1,0 +1,113 @@
+"""The paged 4-bit cache at the limits of its calls: large batches and tables with
+room, the library's workspace, pages that sequences share, long evictions."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv4 as R
+from test_kv4_gpu import Made, check_attention, device_errors, ops  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def batch(ops, n_seq, n_kv, hd, max_pages, held):
+    """n_seq sequences in rows of max_pages pages; those of `held` {sequence: (K, V) rows} hold something, each one page."""
+    table = torch.zeros(n_seq, max_pages, dtype=torch.int32, device="cuda")
+    lens = torch.zeros(n_seq, dtype=torch.int32, device="cuda")
+    pool = torch.zeros(max(1, len(held)), n_kv * 72 * hd, dtype=torch.uint8)
+    for j, (i, (k, v)) in enumerate(held.items()):
+        R.store(pool.numpy(), [j], n_kv, hd, k, v, 0)
+        table[i, 0], lens[i] = j, len(k)
+    return ops.Kv4Cache(pool.cuda(), table, lens, n_kv, hd)
+
+
+def some(rng, where, n_kv, hd):
+    return {i: tuple(rng.standard_normal((2, n, n_kv * hd)).astype(np.float32)) for i, n in where.items()}
+
+
+@pytest.mark.parametrize("n_seq,n_kv,max_pages,weights", [(256, 8, 2048, False), (64, 8, 8192, False), (256, 8, 2048, True)])
+def test_attention_of_a_batch_in_long_tables(ops, n_seq, n_kv, max_pages, weights):
+    """2^22 pages of table: what a call launches goes by its blocks, not by its tables' room."""
+    print(f"case long tables {n_seq} {n_kv} {max_pages} {weights}", flush=True)
+    rng = np.random.default_rng(81)
+    hd, n_heads = 64, n_kv
+    held = some(rng, {0: 3, 17: 64, n_seq - 1: 1}, n_kv, hd)
+    c = batch(ops, n_seq, n_kv, hd, max_pages, held)
+    q = torch.from_numpy(rng.standard_normal((n_seq, 1, n_heads * hd)).astype(np.float32)).cuda()
+    out = torch.full_like(q, float("nan"))
+    w = torch.full((n_seq, n_kv, 64 * max_pages), 1.0, device="cuda") if weights else None
+    ops.kv4_attn(out, q, c, n_heads, **(dict(weights_in=w, weights_out=w) if weights else {}))
+    got = out.cpu().numpy()
+    for i in range(n_seq):
+        if i not in held:
+            assert (got[i] == 0).all()
+            continue
+        K, V = (R.held(x).reshape(-1, n_kv, hd).transpose(1, 0, 2) for x in held[i])
+        want, p, top = R.attend(q[i].cpu().numpy(), K, V, 1)
+        tol = 16 * 2.0 ** -24 * max(1.0, top)
+        assert np.linalg.norm(got[i] - want) <= tol * np.linalg.norm(want)
+        if weights:
+            n = K.shape[1]
+            assert (np.abs(w[i, :, :n].cpu().numpy() - 1 - p) <= tol * p + 2.0 ** -22 * (1 + p)).all()
+    if weights:
+        assert float(w.sum(dtype=torch.float64)) == pytest.approx(sum(n_kv * (len(k) + 1) for k, _ in held.values()), rel=1e-5)
+    assert device_errors() == 0
+
+
+def test_append_and_read_of_a_large_batch(ops):
+    """More than 2^22 blocks: 70000 sequences of 32 KV heads, all but two left out."""
+    rng = np.random.default_rng(82)
+    n_seq, n_kv, hd = 70000, 32, 64
+    table = torch.zeros(n_seq, 1, dtype=torch.int32, device="cuda")
+    lens = torch.zeros(n_seq, dtype=torch.int32, device="cuda")
+    lens[3], lens[n_seq - 1], table[n_seq - 1, 0] = 1, 1, 1
+    pool = torch.zeros(2, n_kv * 72 * hd, dtype=torch.uint8, device="cuda")
+    c = ops.Kv4Cache(pool, table, lens, n_kv, hd)
+    k, v = (torch.zeros(n_seq, 1, n_kv * hd, device="cuda") for _ in range(2))
+    rows = rng.standard_normal((2, 2, 1, n_kv * hd)).astype(np.float32)
+    for x, r in zip((k, v), rows):
+        x[3], x[n_seq - 1] = torch.from_numpy(r[0]).cuda(), torch.from_numpy(r[1]).cuda()
+    ops.kv4_append(c, k, v)
+    want = np.zeros((2, n_kv * 72 * hd), np.uint8)
+    for j in range(2):
+        R.store(want, [j], n_kv, hd, rows[0][j], rows[1][j], 0)
+    np.testing.assert_array_equal(pool.cpu().numpy(), want)
+    ops.kv4_read(c, k, v)
+    for x, r in zip((k, v), rows):
+        for i, y in ((3, r[0]), (n_seq - 1, r[1])):
+            np.testing.assert_array_equal(x[i].cpu().numpy(), R.held(y).astype(np.float32))
+        assert int((x != 0).any(-1).sum()) == 2
+    assert device_errors() == 0
+
+
+def test_evict_into_a_large_batch(ops):
+    """2^22 destination pages, nearly all of them without a kept position."""
+    rng = np.random.default_rng(83)
+    n_seq, n_kv, hd, budget = 256, 8, 64, 20
+    held = some(rng, {0: 3, 17: 64, n_seq - 1: 21}, n_kv, hd)
+    c = batch(ops, n_seq, n_kv, hd, 1, held)
+    table = torch.zeros(n_seq, 2048, dtype=torch.int32, device="cuda")
+    for j, i in enumerate(held):
+        table[i, 0] = j
+    to = ops.Kv4Cache(torch.zeros(3, n_kv * 72 * hd, dtype=torch.uint8, device="cuda"), table,
+                      torch.full((n_seq,), -1, dtype=torch.int32, device="cuda"), n_kv, hd)
+    w = torch.from_numpy(rng.random((n_seq, n_kv, 64)).astype(np.float32)).cuda()
+    dw = torch.full((n_seq, n_kv, 64 * 2048), 7.0, device="cuda")
+    kept = torch.empty(n_seq, n_kv, budget, dtype=torch.int32, device="cuda")
+    ops.kv4_evict(c, to, w, dw, budget, 2, 5, kept)
+    assert to.lens.tolist() == [min(budget, len(held[i][0])) if i in held else 0 for i in range(n_seq)]
+    k, v = (torch.zeros(n_seq, budget, n_kv * hd, device="cuda") for _ in range(2))
+    ops.kv4_read(to, k, v)
+    for i, kv in held.items():
+        n = len(kv[0])
+        for h in range(n_kv):
+            f = R.keep(w[i, h].cpu().numpy(), n, budget, 2, 5)
+            np.testing.assert_array_equal(kept[i, h, :len(f)].cpu().numpy(), f)
+            np.testing.assert_array_equal(dw[i, h, :len(f)].cpu().numpy(), w[i, h].cpu().numpy()[f])
+            for got, x in zip((k, v), kv):
+                want = R.held(x).astype(np.float32)[f][:, h * hd:(h + 1) * hd]
+                np.testing.assert_array_equal(got[i, budget - len(f):, h * hd:(h + 1) * hd].cpu().numpy(), want)
+    assert int((dw != 0).sum()) == sum(n_kv * min(budget, len(x[0])) for x in held.values())
+    assert device_errors() == 0
