@@ -212,9 +212,11 @@ int ibh_attn_exact_set_grouped(int on);
  *   pool   n_pages pages of ibh_kv4_page_bytes(n_kv, head_dim) bytes, on 16
  *          bytes;
  *   table  [n_seq][max_pages]: the page that holds positions 64 j .. 64 j + 63
- *          of a sequence.  Entries behind a sequence's last page are not used;
- *          a table with room for more costs an attention next to nothing.
- *          Sequences may share full pages, not one that is appended to;
+ *          of a sequence.  Entries behind a sequence's last page are not used.
+ *          Room for more pages costs an attention next to nothing without
+ *          weights; with weights every slot of weights_out is written, and the
+ *          workspace grows with the room.  Sequences may share full pages, not
+ *          one that is appended to;
  *   lens   [n_seq] positions held, 0 .. 64 max_pages; 0 leaves a sequence out.
  * head_dim 64, 128, 192 or 256.  A page number outside the pool or a length
  * outside the row raises IBH_DEVERR_KV4_TABLE (ibh_device_errors): nothing is
@@ -262,9 +264,11 @@ int ibh_kv4_read(const ibh_kv4_cache* cache, float* k, float* v, int n, int kv_s
  * weights_in + the softmax probabilities that the queries and heads of the KV
  * head gave each position; 0 behind a sequence's length.  The two may be the
  * same array.
- * `ws` >= ibh_kv4_attn_workspace_bytes (weights != 0: of a call with weights)
- * on 16 bytes, NULL = library workspace; calls that share one must not overlap
- * in time. */
+ * `ws` >= ibh_kv4_attn_workspace_bytes (weights != 0: of a call with weights,
+ * whose kept scores take up to 8 times the weights' own size) on 16 bytes.
+ * NULL = the library's workspace of 4 MiB: a call that needs more is refused
+ * (IBH_ERROR_MEMORY), and many do (several sequences, prompts, long contexts).
+ * Calls that share one must not overlap in time. */
 size_t ibh_kv4_attn_workspace_bytes(const ibh_kv4_cache* cache, int n_heads, int n_q, int weights);
 int    ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float* q, int n_heads, int n_q, int q_stride,
                     const float* weights_in, float* weights_out, void* ws, size_t ws_bytes, void* stream);
@@ -282,8 +286,9 @@ int    ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float* q, int 
  * sequences share.  Otherwise dst has its own table, lens and weights, and
  * pages that src does not use; src, which may share pages, is left as it was.  sink + recent <= budget <= 64 dst->max_pages.
  * `ws` >= ibh_kv4_evict_workspace_bytes(src) (0 for rows of up to 16384
- * positions) on 16 bytes, NULL = library workspace; calls that share one must
- * not overlap in time. */
+ * positions, else 0.75 MiB for each KV head of each sequence) on 16 bytes.
+ * NULL = the library's workspace of 4 MiB: a call that needs more is refused
+ * (IBH_ERROR_MEMORY).  Calls that share one must not overlap in time. */
 size_t ibh_kv4_evict_workspace_bytes(const ibh_kv4_cache* src);
 int    ibh_kv4_evict(const ibh_kv4_cache* src, const ibh_kv4_cache* dst, const float* weights_src, float* weights_dst,
                      int budget, int sink, int recent, int32_t* kept, void* ws, size_t ws_bytes, void* stream);

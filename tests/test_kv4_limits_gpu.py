@@ -111,3 +111,65 @@ def test_evict_into_a_large_batch(ops):
                 np.testing.assert_array_equal(got[i, budget - len(f):, h * hd:(h + 1) * hd].cpu().numpy(), want)
     assert int((dw != 0).sum()) == sum(n_kv * min(budget, len(x[0])) for x in held.values())
     assert device_errors() == 0
+
+
+# ── workspaces ───────────────────────────────────────────────────────────────
+def raw(name, *args):
+    import libinferbit_amd as L
+    rc = getattr(L.lib(), name)(*args)
+    msg = L.lib().ibh_last_error() if rc else b""
+    return rc, msg.decode()
+
+
+@pytest.mark.parametrize("n_q,lens,weights", [(1, [900], True), (1, [3000], False), (1, [3000], True), (12, [700], True)])
+def test_attention_in_the_library_workspace(ops, n_q, lens, weights):
+    """ws NULL: the same bits as in a workspace of the caller's."""
+    import libinferbit_amd as L
+    rng = np.random.default_rng(84)
+    n_heads, n_kv, hd = 8, 2, 64
+    m = Made(ops, rng, lens, n_kv, hd)
+    assert 0 <= L.lib().ibh_kv4_attn_workspace_bytes(m.cache.ref, n_heads, n_q, weights) <= 4 << 20
+    q = torch.randn(len(lens), n_q, n_heads * hd, device="cuda")
+    w = torch.rand(len(lens), n_kv, m.table.shape[1] * 64, device="cuda") if weights else None
+    out, own = torch.empty_like(q), torch.empty_like(q)
+    w2 = None if w is None else torch.empty_like(w)
+    w3 = None if w is None else torch.empty_like(w)
+    ptr = lambda t: None if t is None else t.data_ptr()
+    rc, msg = raw("ibh_kv4_attn", m.cache.ref, out.data_ptr(), q.data_ptr(), n_heads, n_q, n_heads * hd, ptr(w), ptr(w2),
+                  None, 0, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, msg
+    ops.kv4_attn(own, q, m.cache, n_heads, weights_in=w, weights_out=w3)
+    assert torch.equal(out, own) and (w is None or torch.equal(w2, w3))
+
+
+def test_calls_beyond_the_library_workspace_are_refused(ops):
+    import libinferbit_amd as L
+    rng = np.random.default_rng(85)
+    n_heads, n_kv, hd = 8, 2, 64
+    m = Made(ops, rng, [17000, 300], n_kv, hd)
+    stream = torch.cuda.current_stream().cuda_stream
+    q = torch.randn(2, 40, n_heads * hd, device="cuda")
+    out = torch.full_like(q, 3.5)
+    assert L.lib().ibh_kv4_attn_workspace_bytes(m.cache.ref, n_heads, 40, 0) > 4 << 20
+    rc, msg = raw("ibh_kv4_attn", m.cache.ref, out.data_ptr(), q.data_ptr(), n_heads, 40, n_heads * hd, None, None, None, 0, stream)
+    assert rc == -3 and "workspace" in msg
+    slots = m.table.shape[1] * 64
+    # an eviction's need goes by its KV heads: 4 rows fit, 8 do not
+    w = torch.rand(2, n_kv, slots, device="cuda")
+    assert L.lib().ibh_kv4_evict_workspace_bytes(m.cache.ref) <= 4 << 20
+    kept, want = (torch.empty(2, n_kv, 100, dtype=torch.int32, device="cuda") for _ in range(2))
+    table = torch.arange(4, dtype=torch.int32, device="cuda").view(2, 2)
+    to = lambda: ops.Kv4Cache(torch.zeros(4, n_kv * 72 * hd, dtype=torch.uint8, device="cuda"), table, torch.zeros(2, dtype=torch.int32, device="cuda"), n_kv, hd)
+    a, b, wa, wb = to(), to(), *(torch.zeros(2, n_kv, 128, device="cuda") for _ in range(2))
+    rc, msg = raw("ibh_kv4_evict", m.cache.ref, a.ref, w.data_ptr(), wa.data_ptr(), 100, 3, 7, kept.data_ptr(), None, 0, stream)
+    assert rc == 0, msg
+    ops.kv4_evict(m.cache, b, w, wb, 100, 3, 7, want)
+    assert torch.equal(kept, want) and torch.equal(a.pool, b.pool) and torch.equal(wa, wb)
+    both = ops.Kv4Cache(m.dpool, torch.cat([m.dtable] * 2), torch.cat([m.dlens] * 2), n_kv, hd)
+    big = ops.Kv4Cache(torch.zeros(8, n_kv * 72 * hd, dtype=torch.uint8, device="cuda"), torch.arange(8, dtype=torch.int32, device="cuda").view(4, 2),
+                       torch.full((4,), 9, dtype=torch.int32, device="cuda"), n_kv, hd)
+    w2, wd, k2 = torch.cat([w] * 2), torch.full((4, n_kv, 128), 3.5, device="cuda"), torch.full((4, n_kv, 100), -9, dtype=torch.int32, device="cuda")
+    rc, msg = raw("ibh_kv4_evict", both.ref, big.ref, w2.data_ptr(), wd.data_ptr(), 100, 3, 7, k2.data_ptr(), None, 0, stream)
+    assert rc == -3 and "workspace" in msg
+    torch.cuda.synchronize()
+    assert (out == 3.5).all() and (wd == 3.5).all() and (k2 == -9).all() and big.lens.tolist() == [9] * 4
