@@ -241,9 +241,13 @@ size_t ibh_kv4_page_bytes(int n_kv, int head_dim);
 
 /* Stores the last n_new positions of every sequence: lens already counts
  * them, so row i of k, v ([n_seq][n_new] rows of n_kv * head_dim floats,
- * kv_stride floats apart) goes to position lens - n_new + i; rows that would
- * lie before position 0 are left out, which serves sequences with fewer new
- * positions (their rows at the end).  Per 64 dims: lo, hi of the elements
+ * kv_stride floats apart) goes to position lens - n_new + i, over what that
+ * position held; rows that would lie before position 0 are left out.  n_new is
+ * the same for all sequences of a call: only one whose positions are all new
+ * may have fewer (its rows at the end).  A batch of unequal counts takes a call
+ * for each count, over a cache of those sequences' table rows and lengths and
+ * the same pool; so do its attention and its weights, since a row of padding
+ * would be a query like any other.  Per 64 dims: lo, hi of the elements
  * (held to +-65504), scale = fp16((hi - lo) / 15), mid = fp16(lo + 8 scale),
  * code = 8 + (x - mid) / scale rounded to nearest (ties to even) and held to
  * 0 .. 15, exactly; 8 where scale is 0.  A NaN makes its 64 dims NaN. */
@@ -263,7 +267,10 @@ int ibh_kv4_read(const ibh_kv4_cache* cache, float* k, float* v, int n, int kv_s
  * With weights (both or neither): weights_out[n_seq][n_kv][64 max_pages] =
  * weights_in + the softmax probabilities that the queries and heads of the KV
  * head gave each position; 0 behind a sequence's length.  The two may be the
- * same array.
+ * same array.  Positions that are taken back (lens lowered after a verify step)
+ * keep their weights until the next call, and new positions in their place
+ * would start with them: clear them.  What rejected queries gave to the other
+ * positions stays counted.
  * `ws` >= ibh_kv4_attn_workspace_bytes (weights != 0: of a call with weights,
  * whose kept scores take up to 8 times the weights' own size) on 16 bytes.
  * NULL = the library's workspace of 4 MiB: a call that needs more is refused

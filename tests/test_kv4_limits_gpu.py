@@ -173,3 +173,47 @@ def test_calls_beyond_the_library_workspace_are_refused(ops):
     assert rc == -3 and "workspace" in msg
     torch.cuda.synchronize()
     assert (out == 3.5).all() and (wd == 3.5).all() and (k2 == -9).all() and big.lens.tolist() == [9] * 4
+
+
+# ── unequal counts ───────────────────────────────────────────────────────────
+def test_a_batch_of_unequal_counts(ops):
+    """Decode steps, a verify step that is cut back, and a prompt chunk in one batch: a call for each count, over caches of
+    those sequences' rows and one pool, weights included."""
+    rng = np.random.default_rng(86)
+    n_heads, n_kv, hd, mp = 4, 2, 64, 4
+    start, new = [100, 63, 0, 70], [1, 5, 90, 1]
+    m = Made(ops, rng, start, n_kv, hd, max_pages=mp)
+    w = torch.from_numpy(rng.random((4, n_kv, mp * 64)).astype(np.float32)).cuda()
+    for i, t in enumerate(start):
+        w[i, :, t:] = 0
+    w0 = w.cpu().numpy()
+    lens = list(start)
+    probs, most = [np.zeros((n_kv, mp * 64)) for _ in start], 1.0
+    for step, counts in enumerate((new, [1, 1, 1, 1])):
+        for i, n in enumerate(counts):
+            lens[i] += n
+        m.dlens.copy_(torch.tensor(lens, dtype=torch.int32))
+        for n in sorted(set(counts)):
+            idx = torch.tensor([i for i, x in enumerate(counts) if x == n], device="cuda")
+            c = ops.Kv4Cache(m.dpool, m.dtable[idx], m.dlens[idx], n_kv, hd)
+            k, v = rng.standard_normal((2, len(idx), n, n_kv * hd)).astype(np.float32)
+            q = rng.standard_normal((len(idx), n, n_heads * hd)).astype(np.float32)
+            out, wi = torch.empty(len(idx), n, n_heads * hd, device="cuda"), w[idx]
+            ops.kv4_append(c, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda())
+            ops.kv4_attn(out, torch.from_numpy(q).cuda(), c, n_heads, weights_in=wi, weights_out=wi)
+            w[idx] = wi
+            for j, i in enumerate(idx.tolist()):
+                m.k[i], m.v[i] = np.concatenate([m.k[i], k[j]]), np.concatenate([m.v[i], v[j]])
+                want, p, top = R.attend(q[j], *m.loaded(i), n)
+                probs[i][:, :lens[i]] += p
+                most = max(most, top)
+                assert np.linalg.norm(out[j].cpu().numpy() - want) <= 16 * 2.0 ** -24 * max(1.0, top) * np.linalg.norm(want)
+        if step == 0:                                             # three of the five drafts are rejected
+            lens[1] -= 3
+            m.k[1], m.v[1] = m.k[1][:lens[1]], m.v[1][:lens[1]]
+            w[1, :, lens[1]:] = 0
+            probs[1][:, lens[1]:] = 0
+    for i in range(4):
+        want = w0[i] + probs[i]
+        assert (np.abs(w[i].cpu().numpy() - want) <= (16 * 2.0 ** -24 * most + 2 * 2.0 ** -22) * want + 2.0 ** -100).all()   # as above, and each call's sums
+    assert device_errors() == 0
