@@ -217,3 +217,99 @@ def test_a_batch_of_unequal_counts(ops):
         want = w0[i] + probs[i]
         assert (np.abs(w[i].cpu().numpy() - want) <= (16 * 2.0 ** -24 * most + 2 * 2.0 ** -22) * want + 2.0 ** -100).all()   # as above, and each call's sums
     assert device_errors() == 0
+
+
+# ── shared pages ─────────────────────────────────────────────────────────────
+@pytest.mark.parametrize("n_q,weights", [(1, False), (1, True), (5, True), (20, True)])
+def test_sequences_that_share_full_pages(ops, n_q, weights):
+    """Three sequences on one prompt's 5 full pages, one of them with nothing else: each as if the pages were its own, an
+    eviction into other pages too, and the shared pages unchanged."""
+    print(f"case shared n_q={n_q} weights={weights}", flush=True)
+    rng = np.random.default_rng(87)
+    n_heads, n_kv, hd, lens = 8, 2, 64, [400, 320, 377]
+    m = Made(ops, rng, lens, n_kv, hd)
+    for i in (1, 2):
+        m.k[i][:320], m.v[i][:320] = m.k[0][:320], m.v[0][:320]
+        m.table[i, :5] = m.table[0, :5]
+    m.dtable.copy_(torch.from_numpy(m.table))
+    for i in (0, 2):                                              # what lies behind the shared pages
+        one = ops.Kv4Cache(m.dpool, m.dtable[i:i + 1].contiguous(), m.dlens[i:i + 1].contiguous(), n_kv, hd)
+        ops.kv4_append(one, *(torch.from_numpy(x[i][None, 320:]).cuda() for x in (m.k, m.v)))
+    before = m.dpool.clone()
+    q = torch.from_numpy(rng.standard_normal((3, n_q, n_heads * hd)).astype(np.float32)).cuda()
+    out = torch.empty_like(q)
+    wi = torch.from_numpy(rng.random((3, n_kv, m.table.shape[1] * 64)).astype(np.float32)).cuda() if weights else None
+    wo = torch.empty_like(wi) if weights else None
+    ops.kv4_attn(out, q, m.cache, n_heads, **(dict(weights_in=wi, weights_out=wo) if weights else {}))
+    check_attention(ops, m, q, n_heads, n_q, out, wi, wo)
+    if weights:
+        budget, sink, recent = 200, 4, 50
+        to = ops.Kv4Cache(torch.zeros(12, n_kv * 72 * hd, dtype=torch.uint8, device="cuda"), torch.arange(12, dtype=torch.int32, device="cuda").view(3, 4),
+                          torch.zeros(3, dtype=torch.int32, device="cuda"), n_kv, hd)
+        wd, kept = torch.empty(3, n_kv, 256, device="cuda"), torch.empty(3, n_kv, budget, dtype=torch.int32, device="cuda")
+        ops.kv4_evict(m.cache, to, wo, wd, budget, sink, recent, kept)
+        k, v = (torch.empty(3, budget, n_kv * hd, device="cuda") for _ in range(2))
+        ops.kv4_read(to, k, v)
+        for i in range(3):
+            for h in range(n_kv):
+                f = R.keep(wo[i, h].cpu().numpy(), lens[i], budget, sink, recent)
+                np.testing.assert_array_equal(kept[i, h].cpu().numpy(), f)
+                for got, x in ((k, m.k), (v, m.v)):
+                    want = R.held(x[i]).astype(np.float32)[f][:, h * hd:(h + 1) * hd]
+                    np.testing.assert_array_equal(got[i, :, h * hd:(h + 1) * hd].cpu().numpy(), want)
+    assert torch.equal(m.dpool, before) and device_errors() == 0
+
+
+# ── evictions of long rows ───────────────────────────────────────────────────
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("lens,budget,sink,recent", [   # 17 to 32 segments of a row; segments of more than 4096 positions
+    ([70001, 300], 5000, 3, 1000), ([131071], 64, 1, 7), ([131072, 0, 65537], 66000, 0, 0), ([200000, 90], 150001, 4, 2000),
+    ([200000], 199999, 0, 0), ([262143, 131071], 8192, 16, 2048)])
+def test_evict_long_rows(ops, lens, budget, sink, recent, in_place):
+    print(f"case evict long {lens} {budget} {sink} {recent} in_place={in_place}", flush=True)
+    rng = np.random.default_rng(budget + len(lens))
+    n, n_kv, hd = len(lens), 1, 64
+    mp = (max(lens) + 63) // 64
+    pool = rng.integers(0, 256, (n * mp, 72 * hd), dtype=np.uint8)   # the bytes are moved, whatever they are
+    table = rng.permutation(n * mp).astype(np.int32).reshape(n, mp)
+    w = np.round(np.exp(rng.standard_normal((n, n_kv, mp * 64)) * 2) * 8).astype(np.float32) / 8   # ties in every segment
+    w[rng.random(w.shape) < 0.02] = np.nan
+    dev = lambda x: torch.from_numpy(x).cuda()
+    dpool, dw = dev(pool.copy()), dev(w)
+    src = ops.Kv4Cache(dpool, dev(table), torch.tensor(lens, dtype=torch.int32, device="cuda"), n_kv, hd)
+    to, tw, ttable, before = src, dw, table, pool
+    if not in_place:
+        dp = (budget + 63) // 64 + 1
+        ttable = rng.permutation(n * dp).astype(np.int32).reshape(n, dp)
+        before = rng.integers(0, 256, (n * dp, 72 * hd), dtype=np.uint8)
+        tw = torch.full((n, n_kv, dp * 64), 7.0, device="cuda")
+        to = ops.Kv4Cache(dev(before.copy()), dev(ttable), torch.full((n,), -3, dtype=torch.int32, device="cuda"), n_kv, hd)
+    kept = torch.full((n, n_kv, budget), -7, dtype=torch.int32, device="cuda")
+    ops.kv4_evict(src, to, dw, tw, budget, sink, recent, kept)
+    want = before.copy()
+    for i, t in enumerate(lens):
+        new = min(t, budget)
+        f = R.keep(w[i, 0], t, budget, sink, recent)
+        assert int(to.lens[i]) == new
+        g = kept[i, 0].cpu().numpy()
+        np.testing.assert_array_equal(g[:new], f)
+        gw = tw[i, 0].cpu().numpy()
+        np.testing.assert_array_equal(gw[:new].view(np.uint32), w[i, 0, f].view(np.uint32))
+        assert (g[new:] == -1).all() and (gw[new:] == 0).all()
+        rows = pool[table[i]]                                     # [page, byte]
+        half = rows.view(np.uint16)
+        pages = (new + 63) // 64
+        for at, shift, pair in R.places(hd):
+            code = np.zeros((pages * 64, hd), np.uint8)
+            code[:new] = (rows[(f // 64)[:, None], at[f % 64]] >> shift[f % 64].astype(np.uint8)) & 15
+            b = np.zeros((pages, 72 * hd), np.uint8)
+            for hi in (0, 4):                                     # each byte holds two codes
+                use = shift == hi
+                b[:, at[use]] |= code.reshape(pages, 64, hd)[:, use] << hi
+            pr = np.zeros((pages * 64, 2), np.uint16)
+            pr[:new] = half[(f // 64)[:, None], pair[f % 64][:, :1] + np.arange(2)]
+            b.view(np.uint16)[:, pair[:, :1] + np.arange(2)] = pr.reshape(pages, 64, 2)
+            lo = int(at.min())
+            want[ttable[i, :pages], lo:lo + 36 * hd] = b[:, lo:lo + 36 * hd]
+    np.testing.assert_array_equal(to.pool.cpu().numpy(), want)
+    assert device_errors() == 0
