@@ -1013,13 +1013,14 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
         if (__any(most > 65504.f || high > 0x1p60f)) {
             // m goes to the row's maximum.  A factor stays if the page's
             // largest p * scale is at 2^7 .. 65504 with it; else it makes up for
-            // what p lost, or takes that largest to 2^8 .. 2^9.
+            // what p lost (rounded up: a maximum may creep), or takes that largest
+            // to 2^8 .. 2^9.
 #pragma unroll
             for (int g = 0; g < HDG; g++) fm[g] = 0.f;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const float mn = fmaxf(m[r], row16_max(fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3]))));
-                const float al = exp2_(m[r] - mn), up = ldexpf(1.f, (int)fminf(mn - m[r], 122.f));
+                const float al = exp2_(m[r] - mn), up = ldexpf(1.f, (int)ceilf(fminf(mn - m[r], 122.f)));
                 m[r] = mn;
                 l[r] *= al;
 #pragma unroll

@@ -89,6 +89,40 @@ def test_large_values_behind_small_ones(ops, n_heads, n_kv, n_q, t, hd, groups):
     assert (err <= tol * size).all()
 
 
+def test_maxima_that_creep_up(ops):
+    """Scores of a row rise by 0.9 bits a page, while other rows of its wavefront jump by 8.7 bits on a page of their own;
+    the first 64 dims' values are 2^10 on the first page, all but out of sight at the end, and 2^-14 behind it.  One
+    split.  Bound as above."""
+    rng = np.random.default_rng(44)
+    n, n_kv, hd, n_q, pages = 64, 8, 128, 40, 32
+    t = pages * 64
+    m = Made(ops, rng, [t] + [1] * (n - 1), n_kv, hd)
+    page = np.arange(t) // 64
+    k = rng.integers(-8, 8, (t, n_kv, hd)).astype(np.float32)        # held exactly: scale 1, mid 0
+    for i in range(n_q):                                             # query i: a jump on pages 1 + i % 15 and 15 behind
+        k[:, :, i] = ((page >= 1 + i % 15) * 1 + (page >= 16 + i % 15) * 1)[:, None]
+    k[:, :, 15], k[:, :, 31] = 0, 0                                  # two rows that do not jump
+    k[:, :, 62], k[:, :, 63], k[:, :, 126], k[:, :, 127] = -8, 7, -8, 7
+    k[:, :, 64], k[:, :, 65] = (page % 16 - 8)[:, None], (page // 16)[:, None]
+    v = rng.standard_normal((t, n_kv, 2, 64))
+    v[:, :, 0] *= np.where(page == 0, 2.0 ** 10, 2.0 ** -14)[:, None, None]
+    m.k[0], m.v[0] = k.reshape(t, -1), v.reshape(t, -1).astype(np.float32)
+    one = ops.Kv4Cache(m.dpool, m.dtable[:1], m.dlens[:1], n_kv, hd)
+    ops.kv4_append(one, torch.from_numpy(m.k[0][None]).cuda(), torch.from_numpy(m.v[0][None]).cuda())
+    q = np.zeros((n, n_q, n_kv, hd), np.float32)
+    for i in range(n_q):
+        q[:, i, :, i] = 6 * np.sqrt(hd)
+    q[..., 64], q[..., 65] = 0.62 * np.sqrt(hd), 16 * 0.62 * np.sqrt(hd)
+    out = torch.empty(n, n_q, n_kv * hd, device="cuda")
+    ops.kv4_attn(out, torch.from_numpy(q.reshape(n, n_q, -1)).cuda(), m.cache, n_kv)
+    assert (m.loaded(0)[0] == k.transpose(1, 0, 2)).all()
+    want, size, top = parts(m, 0, q[0], n_q, n_kv)
+    err = np.linalg.norm(out[0].cpu().numpy().reshape(want.shape) - want, axis=-1)
+    tol = 12 * 2.0 ** -24 * max(1.0, top)
+    print("err / size", (err / size).max((1, 2)), "tol", tol, flush=True)
+    assert (err <= tol * size).all()
+
+
 @pytest.mark.parametrize("n_heads,n_kv,n_q", [(64, 16, 1), (16, 4, 6), (16, 4, 64)])
 def test_probabilities_are_not_cut_short(ops, n_heads, n_kv, n_q):
     """All positions hold one value vector, -2 in one dim of each 64 and 7/4 (scale 1/4, mid 0) in the others, so the
