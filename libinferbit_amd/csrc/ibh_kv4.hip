@@ -400,7 +400,7 @@ struct AttnArgs {
 };
 
 // Pages of a block, for a sequence of `pages`: an equal share, whatever the
-// table could hold (32 sequences of 4096 positions in tables of 32768: 39 us,
+// table could hold (32 sequences of 4096 positions in tables of 32768: 32 us,
 // 75 with blocks cut by the tables' size).
 __host__ __device__ __forceinline__ int chunk_of(int pages, int n_split, uint32_t per_split, int quantum) {
     const uint32_t each = (uint32_t)(((uint64_t)(uint32_t)(pages + n_split - 1) * per_split) >> 32);
@@ -425,7 +425,7 @@ constexpr int attn_waves(int hdg, int rt) { return hdg * rt == 1 ? 4 : hdg * rt 
 // Block: a share of the pages of one (sequence, KV head), RT tiles of 4 query
 // rows, NW wavefronts that take the block's pages in turn, each with its own
 // running maximum and sums, joined at the end.  4 sequences of 131071 positions,
-// 8 KV heads of 128, 4 rows each: 604 MB in 95 us, 6.3 TB/s, of which HBM is the
+// 8 KV heads of 128, 4 rows each: 604 MB in 96 us, 6.3 TB/s, of which HBM is the
 // bound (7.0 by a kernel that only reads).  With 4096 positions it is the chain
 // of a block: length, page number, codes, products, sums: 6 us.
 template <int HDG, int RT, bool SCORES, int NW>
@@ -766,14 +766,15 @@ __global__ __launch_bounds__(64 * NW, attn_waves(HDG, RT)) void kv4_attn_kernel(
 // together, into LDS, as the matrix cores read them (a code word is a lane's 8
 // elements of one MFMA: halves 0, 2, 4, 6, 1, 3, 5, 7 of its bytes' order).
 //
-// 512 queries of 32 heads on 8 KV heads of 128 over 4100 positions: 130 us, 32
-// GFLOP at fp32's precision (the int8 kernel with 16 rows a block: 175 us).
-// The vector ALU is what it waits for most, busy 54% of the time at the two
-// wavefronts a SIMD that 220 registers leave: the exponentials, the rounding
-// of 64 p * scale a row and group into halves, and two barriers a page.  (Three
-// wavefronts a SIMD have 168 registers and spill.  A running maximum by 16-lane
-// reductions of every page's scores, as kv4_attn_kernel has it, and a factor of
-// p * scale for each row and group took 146 us.)
+// 512 queries of 32 heads on 8 KV heads of 128 over 4100 positions: 129 us, 32
+// GFLOP at fp32's precision.  The vector ALU is what it waits for most, busy 62%
+// of the time at the two wavefronts a SIMD that 228 registers leave: the
+// exponentials, the rounding of 64 p * scale a row and group into halves, and two
+// barriers a page.  (Three wavefronts a SIMD have 168 registers and spill; they
+// serve 64 dims, with one register in scratch.  A running maximum by 16-lane
+// reductions of every page's scores, as kv4_attn_kernel has it, took 10% longer;
+// first factors that leave p * scale less room to grow, 2^11 .. 2^12 instead of
+// 2^8 .. 2^9, are set again more often and took 3% longer.)
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 h8_alias __attribute__((ext_vector_type(8), may_alias));
@@ -1161,7 +1162,7 @@ __global__ __launch_bounds__(256, HDG == 1 ? 3 : HDG == 2 ? 2 : 1) void kv4_attn
 
 // Accumulated weights of many rows: block (KV head, page, sequence); every
 // wavefront holds the page's keys and takes 16-row tiles in turn.  2048 rows
-// of 8 KV heads of 128 over 4100 positions: 51 us, in which every page reads
+// of 8 KV heads of 128 over 4100 positions: 55 us, in which every page reads
 // all rows' halves from L2, 8 KB a tile, 10 TB/s.
 template <int HDG, int NW>
 __global__ __launch_bounds__(64 * NW) void kv4_weights_wide(Kv4 c, AttnArgs a, WideRows wr, const float* win, float* wout) {
@@ -1356,8 +1357,11 @@ struct PageWeights {
     }
 };
 
-// Joins up to 8 splits of many rows: a wavefront a row (16384 rows of 128 dims
-// and 2 splits, 25 MB: 11 us; 29 by a block a row).
+// Joins up to 8 splits of many rows: a wavefront a row, where kv4_attn_finish has
+// a block a row.  Whole calls by the one and the other: 16384 rows of 128 dims
+// 131 and 150 us with 2 splits, 129 and 143 with 8, 148 and 161 with 16; 2560
+// rows 40 and 41 with 8, 57 and 55 with 24; 320 rows 28 and 27 with 8, 24 and 20
+// with 16.
 constexpr int kFewSplits = 8;
 template <int HDG>
 __global__ __launch_bounds__(256) void kv4_attn_join(Kv4 c, AttnArgs a, size_t rows) {
@@ -1410,7 +1414,9 @@ __device__ __forceinline__ float2 joined_stat(const float2* ml, int n, int li) {
 // joining blocks.  At 32 sequences of up to 4096 positions, 8 KV heads of 128,
 // this launch takes 10 us, and keeping the scores costs the first 1.2 us, by
 // nontemporal stores behind a page's loads (9 us by ordinary ones, which the
-// next loads wait for).  Scoring the pages again here took 20 us.
+// next loads wait for).  Scoring the pages again in a launch of their own takes
+// the call from 44 to 48 us where all are full, in tables of 32768 positions from
+// 66 to 68.
 template <int HDG, int RT>
 __global__ __launch_bounds__(256) void kv4_attn_finish(Kv4 c, AttnArgs a, unsigned n_join, const float* win, float* wout) {
     constexpr int HD = 64 * HDG, TD = HD / 4, CLS = 256 / TD;
@@ -2074,10 +2080,10 @@ static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool wei
     const size_t heads = (size_t)c->n_seq * c->n_kv;
     // Few rows: the smallest tile that holds them, so that pages are read once.
     // A tile of 16 rows does not fit the registers with head_dim above 128: tiles
-    // of 8 there.  From 33 rows on the f16 kernel: 8
-    // sequences of 4096 positions, 8 KV heads of 128, 32 rows 40 us here and 41
-    // there, 40 rows 54 and 43, 64 rows 67 and 46 (one sequence, where neither
-    // fills the card: 21 and 23, 22 and 26).
+    // of 8 there.  From 33 rows on the f16 kernel: 8 sequences of 4096
+    // positions, 8 KV heads of 128, 24 rows 34 us here and 37 there, 32 rows 37
+    // and 39, 40 rows 58 and 39, 64 rows 57 and 42.  (One sequence, where neither
+    // fills the card, is faster here: 40 rows 17 and 20, 64 rows 18 and 24.)
     const bool wide = n_rows > 32;
     p.rt = wide ? kWideRows / 4 : n_rows <= 4 ? 1 : n_rows <= 8 || hdg > 2 ? 2 : 4;
     p.n_tile = (int)((n_rows + 4 * p.rt - 1) / (4 * p.rt));
@@ -2088,7 +2094,13 @@ static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool wei
     if (wide) {
         // every block works at once, or in whole rounds: what a round takes in
         // pages (and one for its start), and what the partial sums cost that
-        // are written and joined
+        // are written and joined (228 blocks' as much as a page, a launch 1.5:
+        // fitted).  Times with no split, with the number that this takes and
+        // with the best of 1 to 256: 512 queries of 8 x 4 heads of 128 over 4100
+        // positions 163, 132, 127 us; 40 rows of 8 heads over 4096, one sequence
+        // 135, 21, 18, eight 138, 40, 40, 32 of 2048 78, 67, 67; 72 rows of 4
+        // heads of 64 in 8 sequences of 2049 47, 24, 22; 64 rows over 20000 676,
+        // 34, 34.
         p.quantum = 1;
         const size_t slots = 256 * (hdg == 1 ? 3 : hdg == 2 ? 2 : 1);
         double least = (double)((base + slots - 1) / slots) * (c->max_pages + 1);
@@ -2104,15 +2116,15 @@ static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool wei
     } else {
         // as many blocks as the card holds at once: each has its rows to set
         // up and its sums to write and join (8 sequences of 4096 positions, 8
-        // KV heads of 128: 17 us with 4 rows, 40 with 32; 20 and 48 with 2048
+        // KV heads of 128: 13 us with 4 rows, 37 with 32; 16 and 43 with 2048
         // and 1024 blocks where 768 and 512 are held)
         const size_t work = base * c->max_pages, want = 256 * attn_waves((int)hdg, p.rt);
         size_t chunk = (work + want - 1) / want;
         chunk = max(chunk, ((size_t)c->max_pages + kMaxSplit - 1) / kMaxSplit);
         chunk = (chunk + 3) / 4 * 4;
-        // up to 1024 positions a decode step is one launch: eight wavefronts take a
-        // head's pages, and nothing is left to join (600 positions of 32/4 heads:
-        // 7 us in one kernel, 7 + 3 in two)
+        // in tables of up to 1024 positions few rows are one launch: eight
+        // wavefronts take a head's pages, and nothing is left to join (600
+        // positions of 32/4 heads: 6.9 us, 8.5 by blocks of 4 pages and a join)
         if (p.n_tile == 1 && p.rt <= 2 && (int)hdg * p.rt <= 6 && c->max_pages > 4 && c->max_pages <= 16) {
             p.nw = 8;
             chunk = 16;
@@ -2129,10 +2141,10 @@ static AttnPlan attn_plan(const ibh_kv4_cache* c, int n_heads, int n_q, bool wei
     if (p.joint) p.joins += heads * ((c->max_pages + 3) / 4);
     p.weighs = weights && !p.joint ? heads * c->max_pages : 0;
     // Wavefronts a page.  Many rows: four, eight where there are few pages
-    // (2048 rows, 8 KV heads of 128: 169 and 179 us with 512 pages, 81 and 68
-    // with 80; 40 rows, 4096 pages: 66 and 92; whole calls).  Up to 32: one
-    // where the pages fill the card or have few rows, else eight (24 rows: 57
-    // and 70 us with 4096 pages, 24 and 22 with 80).
+    // (2048 rows, 8 KV heads of 128: 167 and 178 us with 512 pages, 81 and 65
+    // with 80; 40 rows, 4096 pages: 63 and 92; whole calls).  Up to 32: one
+    // where the pages fill the card or have few rows, else eight (24 rows: 46
+    // and 59 us with 4096 pages, 19 and 17 with 80; 12 rows: 32 and 44, 17 and 16).
     if (wide) p.weigh_nw = p.weighs >= 512 ? 4 : 8;
     else p.weigh_nw = p.weighs >= 2048 || n_rows <= 16 ? 1 : 8;
     size_t at = 0;
