@@ -313,3 +313,122 @@ def test_evict_long_rows(ops, lens, budget, sink, recent, in_place):
             want[ttable[i, :pages], lo:lo + 36 * hd] = b[:, lo:lo + 36 * hd]
     np.testing.assert_array_equal(to.pool.cpu().numpy(), want)
     assert device_errors() == 0
+
+
+# ── far pages, graphs, streams ───────────────────────────────────────────────
+def test_pages_beyond_four_gigabytes(ops):
+    """Pages at both ends of a pool of 5 GB: stored, read, attended to by few and by many rows, moved in place and away."""
+    rng = np.random.default_rng(90)
+    n_heads, n_kv, hd, lens = 8, 8, 128, [300, 130]
+    size = n_kv * 72 * hd
+    n_pages = (5 << 30) // size
+    pool = torch.empty(n_pages, size, dtype=torch.uint8, device="cuda")
+    table = np.array([[n_pages - 1, 0, n_pages - 2, n_pages // 2, n_pages - 7], [n_pages - 3, n_pages - 4, 1, 2, 3]], np.int32)
+    c = ops.Kv4Cache(pool, torch.from_numpy(table).cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), n_kv, hd)
+    k, v = rng.standard_normal((2, 2, 300, n_kv * hd)).astype(np.float32)
+    ops.kv4_append(c, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda())
+    rk, rv = (torch.empty(2, 300, n_kv * hd, device="cuda") for _ in range(2))
+    ops.kv4_read(c, rk, rv)
+    rows = [(k[i, 300 - t:], v[i, 300 - t:]) for i, t in enumerate(lens)]
+    for i, t in enumerate(lens):
+        for got, x in zip((rk, rv), rows[i]):
+            np.testing.assert_array_equal(got[i, 300 - t:].cpu().numpy(), R.held(x).astype(np.float32))
+    heads = lambda x: R.held(x).reshape(-1, n_kv, hd).transpose(1, 0, 2)
+    w = torch.zeros(2, n_kv, 5 * 64, device="cuda")
+    for n_q in (1, 40):
+        q = torch.from_numpy(rng.standard_normal((2, n_q, n_heads * hd)).astype(np.float32)).cuda()
+        out = torch.empty_like(q)
+        ops.kv4_attn(out, q, c, n_heads, weights_in=w, weights_out=w)
+        for i in range(2):
+            want, _, top = R.attend(q[i].cpu().numpy(), heads(rows[i][0]), heads(rows[i][1]), n_q)
+            assert np.linalg.norm(out[i].cpu().numpy() - want) <= 16 * 2.0 ** -24 * max(1.0, top) * np.linalg.norm(want)
+    before = w.cpu().numpy()
+    far = ops.Kv4Cache(pool, torch.tensor([[n_pages - 20, 20], [n_pages - 21, 21]], dtype=torch.int32, device="cuda"),
+                       torch.zeros(2, dtype=torch.int32, device="cuda"), n_kv, hd)
+    wd, kept = torch.empty(2, n_kv, 128, device="cuda"), torch.empty(2, n_kv, 100, dtype=torch.int32, device="cuda")
+    for dst, wt in ((far, wd), (c, w)):
+        ops.kv4_evict(c, dst, w, wt, 100, 2, 30, kept)
+        gk, gv = (torch.empty(2, 100, n_kv * hd, device="cuda") for _ in range(2))
+        ops.kv4_read(dst, gk, gv)
+        for i, t in enumerate(lens):
+            for h in range(n_kv):
+                f = R.keep(before[i, h], t, 100, 2, 30)
+                for got, x in zip((gk, gv), rows[i]):
+                    np.testing.assert_array_equal(got[i, :, h * hd:(h + 1) * hd].cpu().numpy(), R.held(x).astype(np.float32)[f][:, h * hd:(h + 1) * hd])
+    assert device_errors() == 0
+
+
+def captured(f):
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        f()
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        f()
+    return g
+
+
+@pytest.mark.parametrize("mp,in_place", [(6, False), (6, True), (300, False), (300, True)])
+def test_captured_evictions_follow_lens_and_weights(ops, mp, in_place):
+    """An eviction captured once (rows of one block, and long ones), replayed while lengths, weights and pages change."""
+    rng = np.random.default_rng(91)
+    n_kv, hd, budget = 2, 64, 150
+    m = Made(ops, rng, [mp * 64, 200], n_kv, hd, max_pages=mp)
+    w = torch.zeros(2, n_kv, mp * 64, device="cuda")
+    kept = torch.empty(2, n_kv, budget, dtype=torch.int32, device="cuda")
+    dpool, dlens, dw = torch.zeros(8, n_kv * 72 * hd, dtype=torch.uint8, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(2, n_kv, 256, device="cuda")
+    to = m.cache if in_place else ops.Kv4Cache(dpool, torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4), dlens, n_kv, hd)
+    tw = w if in_place else dw
+    pool0 = m.dpool.clone()
+    g = captured(lambda: ops.kv4_evict(m.cache, to, w, tw, budget, 3, 40, kept))
+    inputs = [([mp * 64, 200], 1), ([151, 0], 2), ([mp * 64 - 65, 150], 3), ([1, 383], 4)]
+    seen = {}
+    for mode in ("graph", "eager"):
+        for lens, seed in inputs:
+            m.dpool.copy_(pool0)
+            dpool.zero_(); dw.zero_(); dlens.zero_()
+            m.dlens.copy_(torch.tensor(lens, dtype=torch.int32))
+            w.copy_(torch.rand(w.shape, generator=torch.Generator().manual_seed(seed)))
+            g.replay() if mode == "graph" else ops.kv4_evict(m.cache, to, w, tw, budget, 3, 40, kept)
+            torch.cuda.synchronize()
+            got = [x.clone() for x in (kept, to.lens, tw, to.pool)]
+            if mode == "graph":
+                seen[seed] = got
+            else:
+                assert all(torch.equal(a, b) for a, b in zip(seen[seed], got)), lens
+                assert got[1].tolist() == [min(t, budget) for t in lens]
+    assert device_errors() == 0
+
+
+@pytest.mark.parametrize("n_heads,n_q", [(8, 1), (8, 6), (8, 30)])
+def test_two_streams_and_two_graphs_at_once(ops, n_heads, n_q):
+    """Calls with weights on two caches on two streams, and two captured ones replayed side by side, give what they give
+    one after the other."""
+    rng = np.random.default_rng(92)
+    n_kv, hd = 2, 128
+    made = [Made(ops, rng, lens, n_kv, hd) for lens in ([3000, 70], [500, 2900])]
+    qs = [torch.randn(2, n_q, n_heads * hd, device="cuda") for _ in made]
+    ws = [torch.rand(2, n_kv, m.table.shape[1] * 64, device="cuda") for m in made]
+    outs, wos = [torch.empty_like(q) for q in qs], [torch.empty_like(w) for w in ws]
+    call = lambda i: ops.kv4_attn(outs[i], qs[i], made[i].cache, n_heads, weights_in=ws[i], weights_out=wos[i])
+    want = []
+    for i in range(2):
+        call(i)
+        torch.cuda.synchronize()
+        want.append((outs[i].clone(), wos[i].clone()))
+    streams = [torch.cuda.Stream() for _ in made]
+    graphs = [captured(lambda i=i: call(i)) for i in range(2)]
+    for how in ("calls", "graphs"):
+        for x in outs + wos:
+            x.zero_()
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    call(i) if how == "calls" else graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(outs[i], want[i][0]) and torch.equal(wos[i], want[i][1]), how
+    assert device_errors() == 0
