@@ -126,7 +126,7 @@ def plain_norm(st):
     # the norm's factor cancels in a code, which is rounded from the quotient in 64 bits so that one next to a border
     # falls to its side; halves go away from zero
     part = 127.0 * p.double() / torch.where(top == 0, 1.0, top).double()
-    code = (torch.sign(part) * torch.floor(part.abs() + (0.5 + 2.0 ** -30))).float()
+    code = (torch.sign(part) * torch.floor(part.abs() + (0.5 + 2.0 ** -40))).float()
     tiny = top * r.unsqueeze(-1) < 1e-10
     code, scale = torch.where(tiny, 0.0, code), torch.where(tiny, 1e-10, scale)
     return out + [(code * scale).flatten(-2)[:, :n], scale.squeeze(-1)]
@@ -240,7 +240,7 @@ def exact(case, seed):
             step = part.abs().amax(1, keepdim=True) / 127
             steps = torch.where(step > 0, part.abs() / step, 0.0)
             low = torch.floor(steps)
-            code = (low + (steps - low >= 0.5 - 2.0 ** -30)) * torch.sign(part)
+            code = (low + (steps - low >= 0.5 - 2.0 ** -40)) * torch.sign(part)
             scale = step / root.unsqueeze(1)
             small = scale * 127 < 1e-10
             values[:, at:at + GROUP] = torch.where(small, 0.0, code * scale)
