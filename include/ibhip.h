@@ -69,6 +69,7 @@ int         ibh_memcpy_d2d(void* dst, const void* src, size_t bytes, void* strea
 #define IBH_DEVERR_TILE_WAIT 1   /* a bounded wait inside the tile GEMV expired */
 #define IBH_DEVERR_PQ_WS     2   /* a PQ workspace that ibh_pq_workspace_init did not prepare */
 #define IBH_DEVERR_KV4_TABLE 4   /* a 4-bit cache whose table names a page, or whose lens a length, that it has not */
+#define IBH_DEVERR_LORA      8   /* a row with an adapter, or an adapter with a rank, that the adapters have not */
 int         ibh_device_errors(int clear);
 
 /* ── quantized matvec, device pointers ─────────────────────── */
@@ -299,6 +300,75 @@ int    ibh_kv4_attn(const ibh_kv4_cache* cache, float* out, const float* q, int 
 size_t ibh_kv4_evict_workspace_bytes(const ibh_kv4_cache* src);
 int    ibh_kv4_evict(const ibh_kv4_cache* src, const ibh_kv4_cache* dst, const float* weights_src, float* weights_dst,
                      int budget, int sink, int recent, int32_t* kept, void* ws, size_t ws_bytes, void* stream);
+
+/* ── around a batch's projections, device pointers ─────────── */
+
+/* No counterparts in the reference, which runs one row at a time: what a batch
+ * of requests needs in front of, beside and behind the projections above.  B
+ * rows; B 0 does nothing.  Rows are the given numbers of floats apart (of no
+ * account for a single row), arrays without a stride are contiguous. */
+
+/* The residual's addition and the RMS norm of every row:
+ *   h = x + delta (rounded to fp32; x where delta is NULL),
+ *   p = h * weight (rounded to fp32), r = 1 / sqrt(sum h^2 / N + eps), y = p r.
+ * y [B][N] and / or the codes q [B][N] with their scales s [B][ceil(N / 128)],
+ * as ibh_matmul_w4a8_batch takes them; h [B][N] where it is not NULL.  For each
+ * 128 columns s = r max|p| / 127 and q = 127 p / max|p| rounded to nearest,
+ * halves away from zero, exactly: codes do not depend on r.  (The codes of
+ * ibh_quantize_act_g128 of y are the same but for quotients within its own
+ * rounding of a border.)  r max|p| < 1e-10 gives codes 0 and s 1e-10, as there.
+ * The sum is held in 64 bits.  A row that holds a NaN or an infinity is NaN in
+ * y and s, 128 columns of p that do in s; codes are 0 there.
+ * y or h may be x or delta themselves (rows of N floats); otherwise outputs
+ * overlap nothing. */
+int ibh_add_rmsnorm(float* y, int8_t* q, float* s, float* h, const float* x, const float* delta,
+                    const float* weight, float eps, int N, int B, int x_stride, int delta_stride, void* stream);
+
+/* Low-rank adapters of many requests beside a shared projection:
+ *   out[b] = base[b] + scales[i] * B_i (A_i x[b]),  i = ids[b]
+ * with fp32 sums of the adapters' 16-bit numbers and x as it is (no rounding in
+ * between but fp32's).  base NULL stands for zeros; base may be out.  A row of a
+ * negative id has no adapter: out = base.  Rows may come in any order; those of
+ * one adapter are served together.  ids, scales and ranks are read on the
+ * device, so a captured graph follows them.  An id of n or more, or a rank
+ * outside 0 .. rank, raises IBH_DEVERR_LORA (ibh_device_errors) and makes that
+ * row NaN.
+ * out overlaps nothing else.  `ws` >= ibh_lora_workspace_bytes on 16 bytes;
+ * NULL = the library's workspace of 4 MiB: a call that needs more is refused
+ * (IBH_ERROR_MEMORY).  Calls that share one must not overlap in time. */
+#define IBH_F16  0
+#define IBH_BF16 1
+#define IBH_LORA_MAX_RANK 256
+typedef struct {
+    const void* a;             /* [n][rank][N], of type kind */
+    const void* b;             /* [n][M][rank] */
+    const float* scales;       /* [n]; NULL: all 1 */
+    const int32_t* ranks;      /* [n], rows of a and columns of b that count: the others are not used.  NULL: rank */
+    int n, rank, N, M, kind;   /* IBH_F16 or IBH_BF16 */
+} ibh_lora_adapters;
+size_t ibh_lora_workspace_bytes(const ibh_lora_adapters* l, int B);
+int    ibh_lora(const ibh_lora_adapters* l, float* out, const float* base, const float* x, const int32_t* ids, int B,
+                int out_stride, int base_stride, int x_stride, void* ws, size_t ws_bytes, void* stream);
+
+/* Log-probabilities from rows of V logits, lse = log(sum exp z):
+ *   out[b][t] = z[tokens[b][t]] - lse for n_tokens given tokens a row (NaN for a
+ *     token outside 0 .. V - 1);
+ *   entropy[b] = -sum p log p;
+ *   top_ids, top_logprobs [b][k]: the k largest, from the largest down, equal
+ *     logits in the order of their places.
+ * n_tokens 0, entropy NULL or k 0 leave an output away.  A logit of -infinity has
+ * probability 0 and is never among the k; where fewer are left the rest is -1
+ * and -infinity.  A row without any finite logit but -infinity: log-probabilities
+ * -infinity, entropy 0.  A row that holds a NaN or +infinity: NaN, ids -1.
+ * Outputs overlap nothing.  `ws` >= ibh_logprobs_workspace_bytes (0 for many
+ * calls) on 16 bytes; NULL = the library's workspace of 4 MiB: a call that needs
+ * more is refused (IBH_ERROR_MEMORY).  Calls that share one must not overlap in
+ * time. */
+#define IBH_LOGPROBS_MAX_K 64
+size_t ibh_logprobs_workspace_bytes(int V, int B, int k);
+int    ibh_logprobs(float* out, float* entropy, int32_t* top_ids, float* top_logprobs, const float* logits,
+                    const int32_t* tokens, int V, int B, int stride, int n_tokens, int k, void* ws, size_t ws_bytes,
+                    void* stream);
 
 /* ── product-quantised LUT matvec, device pointers ─────────── */
 

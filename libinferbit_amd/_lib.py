@@ -50,6 +50,11 @@ SIGNATURES = {
     "ibh_kv4_attn": (I, [P, P, P, I, I, I, P, P, P, SZ, P]),
     "ibh_kv4_evict_workspace_bytes": (SZ, [P]),
     "ibh_kv4_evict": (I, [P, P, P, P, I, I, I, P, P, SZ, P]),
+    "ibh_add_rmsnorm": (I, [P, P, P, P, P, P, P, C.c_float, I, I, I, I, P]),
+    "ibh_lora_workspace_bytes": (SZ, [P, I]),
+    "ibh_lora": (I, [P, P, P, P, P, I, I, I, I, P, SZ, P]),
+    "ibh_logprobs_workspace_bytes": (SZ, [I, I, I]),
+    "ibh_logprobs": (I, [P, P, P, P, P, P, I, I, I, I, I, P, SZ, P]),
     "ibh_pq_workspace_bytes": (SZ, [P]),
     "ibh_pq_workspace_init": (I, [P, SZ, P]),
     "ibh_pq_matmul_fp32_host": (I, [P, P, P]),
@@ -170,6 +175,11 @@ class Kv4Desc(C.Structure):
     """ibh_kv4_cache (include/ibhip.h)."""
     _fields_ = [(n, P) for n in ("pool", "table", "lens")] + \
                [(n, I) for n in ("n_pages", "n_seq", "max_pages", "n_kv", "head_dim")]
+
+
+class LoraDesc(C.Structure):
+    """ibh_lora_adapters (include/ibhip.h)."""
+    _fields_ = [(n, P) for n in ("a", "b", "scales", "ranks")] + [(n, I) for n in ("n", "rank", "N", "M", "kind")]
 
 
 class PqPolicy(C.Structure):

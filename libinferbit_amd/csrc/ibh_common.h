@@ -30,6 +30,11 @@ hipStream_t ibh_resolve_stream(void* s);
         }                                                                       \
     } while (0)
 
+// Whether two ranges of device memory overlap (null pointers: none).
+inline bool ibh_overlap(const void* a, size_t na, const void* b, size_t nb) {
+    return a && b && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
 #define IBH_HIP(call, what)                                                     \
     do {                                                                        \
         hipError_t e_ = (call);                                                 \
@@ -46,6 +51,7 @@ hipStream_t ibh_resolve_stream(void* s);
 int ibh_tile_errors(bool clear);
 int ibh_pq_errors(bool clear);
 int ibh_kv4_errors(bool clear);
+int ibh_lora_errors(bool clear);
 
 // ── device helpers ─────────────────────────────────────────────────────────
 namespace ibh {

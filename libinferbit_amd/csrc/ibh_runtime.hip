@@ -33,12 +33,13 @@ extern "C" int ibh_device_errors(int clear) {
         ibh_set_error("ibh_device_errors: device synchronisation failed");
         return IBH_ERROR_INTERNAL;
     }
-    const int a = ibh_tile_errors(clear != 0), b = ibh_pq_errors(clear != 0), c = ibh_kv4_errors(clear != 0);
-    if (a < 0 || b < 0 || c < 0) {
+    const int a = ibh_tile_errors(clear != 0), b = ibh_pq_errors(clear != 0), c = ibh_kv4_errors(clear != 0),
+              d = ibh_lora_errors(clear != 0);
+    if (a < 0 || b < 0 || c < 0 || d < 0) {
         ibh_set_error("ibh_device_errors: cannot read the device error words");
         return IBH_ERROR_INTERNAL;
     }
-    return a | b | c;
+    return a | b | c | d;
 }
 
 extern "C" const char* ibh_version(void) { return "libinferbit_amd 0.1.0 (gfx950)"; }
