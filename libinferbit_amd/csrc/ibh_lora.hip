@@ -1,5 +1,12 @@
 // ibh_lora.hip -- low-rank adapters of many requests beside a shared
 // projection: out[b] = base[b] + scale * B (A x[b]) with the adapter of row b.
+//
+// Two products in a row, the first into t = scale * A x (a few numbers a row),
+// so two launches.  Every byte of x, base and out and of each adapter that some
+// row has is needed once: memory bounds both.  Sums are fp32 of exact products:
+// up to kFew rows on the vector units, beyond on the bf16 matrix cores, where
+// an fp32 number is three bf16 numbers (8 + 8 + 8 bits, exactly) and an fp16
+// one two.
 #include "ibh_common.h"
 
 namespace {
@@ -7,69 +14,549 @@ using namespace ibh;
 
 __device__ unsigned int ibh_lora_err;
 
+constexpr int kFew = 64;            // rows up to which a wavefront holds all ids, one a lane
+constexpr int kMaxAdapters = 8192;  // counters of the plan's block
+constexpr int kTile = 32;           // rows of one adapter that a block of the matrix kernels takes
+constexpr int kStep = 128;          // columns of x that it holds in LDS at a time
+constexpr int kMaxSplit = 16;       // blocks that share a tile's columns
+constexpr int kChunk = 512;         // outputs that a block of the second product takes
+
+typedef float f4_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u4h_t __attribute__((ext_vector_type(4), aligned(2)));
+
 struct Lora {
     const uint16_t *a, *b;
     const float* scales;
     const int32_t* ranks;
-    int n, R, N, M, kind;
+    int n, R, N, M;
     float* out;
     const float *base, *x;
     const int32_t* ids;
     int B;
     size_t os, bs, xs;
-    float* t;                                            // [B][R]: scale * A x
+    float* t;                       // [split][B][Rp]: scale * A x of each row; zeros behind its adapter's rank
+    int Rp;                         // R in whole eights
+    int S;                          // splits
+    int32_t* plan;                  // {tiles}, then Tile [tiles], then the rows in their order
+    int max_tiles;
+};
+struct Tile {
+    int32_t id, rank, start, count; // id -1: no adapter; rank -1: not in the table
 };
 
-__device__ __forceinline__ float widen(uint16_t h, int kind) {
-    return kind == IBH_F16 ? f16_to_f32(h) : __builtin_bit_cast(float, (uint32_t)h << 16);
+template <int KIND>
+__device__ __forceinline__ float widen(uint32_t h) {    // of the low half
+    if constexpr (KIND == IBH_F16) return f16_to_f32((uint16_t)h);
+    else return __uint_as_float(h << 16);
 }
-// The rank of adapter `id`; -1 where the table does not have it.
+// The rank of adapter `id`: 0 for none, -1 where the table does not have it.
 __device__ __forceinline__ int rank_of(const Lora& l, int id) {
+    if (id < 0) return 0;
     if (id >= l.n) return -1;
     const int r = l.ranks ? l.ranks[id] : l.R;
-    return r > l.R ? -1 : r < 0 ? -1 : r;
+    return r < 0 || r > l.R ? -1 : r;
+}
+__device__ __forceinline__ f4_t load4(const float* p, int j, int N) {
+    f4_t v = {0.f, 0.f, 0.f, 0.f};
+    if (j + 4 <= N) return *(const f4_t*)(p + j);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (j + i < N) v[i] = p[j + i];
+    return v;
+}
+__device__ __forceinline__ void store4(float* p, int j, int N, f4_t v) {
+    if (j + 4 <= N) {
+        *(f4_t*)(p + j) = v;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (j + i < N) p[j + i] = v[i];
+}
+// Eight 16-bit numbers from place j of n, zeros behind them.
+__device__ __forceinline__ u4_t load8h(const uint16_t* p, int j, int n) {
+    if (j + 8 <= n) return *(const u4h_t*)(p + j);
+    u4_t v = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (j + i < n) v[i / 2] |= (uint32_t)p[j + i] << (16 * (i % 2));
+    return v;
 }
 
-__global__ __launch_bounds__(256) void lora_shrink_kernel(Lora l) {
-    const int row = blockIdx.x;
-    const int id = l.ids[row];
-    if (id < 0) return;
-    const int rank = rank_of(l, id);
-    const float scale = rank > 0 && l.scales ? l.scales[id] : 1.f;
-    for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < rank; r += gridDim.y * 4) {
-        const uint16_t* a = l.a + ((size_t)id * l.R + r) * l.N;
-        const float* x = l.x + row * l.xs;
-        float s = 0;
-        for (int j = threadIdx.x & 63; j < l.N; j += 64) s = fmaf(widen(a[j], l.kind), x[j], s);
-        s = wave_sum(s);
-        if ((threadIdx.x & 63) == 0) l.t[(size_t)row * l.R + r] = s * scale;
+// ── up to kFew rows ──────────────────────────────────────────────────────────
+// Block x belongs to row x.  The rows of its adapter are served four at a time
+// by the blocks of its first, fifth, ... row: what they share is read from
+// memory once and from L2 by the others.
+struct Few {
+    int id, rank, rows;             // rows 0: this block has nothing to do
+    int row[4];
+};
+__device__ __forceinline__ Few few_of(const Lora& l) {
+    const int lane = threadIdx.x & 63, me = blockIdx.x;
+    const int mine = lane < l.B ? max(l.ids[lane], -1) : -2;
+    Few f;
+    f.id = __builtin_amdgcn_readlane(mine, me);
+    f.rank = rank_of(l, f.id);
+    uint64_t same = __ballot(mine == f.id);
+    f.rows = 0;
+    const int before = __popcll(same & ((1ull << me) - 1));
+    if (before % 4) return f;
+    same &= ~0ull << me;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        f.row[i] = same ? __ffsll((unsigned long long)same) - 1 : f.row[0];
+        f.rows += same != 0;
+        same &= same - 1;
+    }
+    return f;
+}
+
+// RR ranks of an adapter times NR rows: lanes take eights of columns.
+template <int KIND, int RR, int NR>
+__device__ __forceinline__ void shrink_rows(const Lora& l, const Few& f, int r0, float (*part)[4]) {
+    const int tid = threadIdx.x;
+    const uint16_t* a = l.a + ((size_t)f.id * l.R + r0) * l.N;
+    const int nr = min(RR, f.rank - r0);
+    float acc[RR][NR];
+#pragma unroll
+    for (int r = 0; r < RR; r++)
+#pragma unroll
+        for (int i = 0; i < NR; i++) acc[r][i] = 0.f;
+#pragma unroll 2
+    for (int j = tid * 8; j < l.N; j += 2048) {
+        u4_t w[RR];
+        f4_t v[NR][2];
+#pragma unroll
+        for (int r = 0; r < RR; r++) w[r] = r < nr ? load8h(a + (size_t)r * l.N, j, l.N) : u4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < NR; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) v[i][h] = load4(l.x + f.row[i] * l.xs, j + 4 * h, l.N);
+#pragma unroll
+        for (int r = 0; r < RR; r++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float we = widen<KIND>(e % 2 ? w[r][e / 2] >> 16 : w[r][e / 2] & 0xffffu);
+#pragma unroll
+                for (int i = 0; i < NR; i++) acc[r][i] = fmaf(we, v[i][e / 4][e % 4], acc[r][i]);
+            }
+    }
+#pragma unroll
+    for (int r = 0; r < RR; r++)
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+            const float s = wave_sum_dpp(acc[r][i]);
+            if ((tid & 63) == 0) part[r * NR + i][tid >> 6] = s;
+        }
+    __syncthreads();
+    if (tid < RR * NR) {
+        const int r = tid / NR, i = tid % NR;
+        const float s = (part[tid][0] + part[tid][1]) + (part[tid][2] + part[tid][3]);
+        if (i < f.rows && r0 + r < l.Rp)
+            l.t[(size_t)f.row[i] * l.Rp + r0 + r] = r < nr ? s * (l.scales ? l.scales[f.id] : 1.f) : 0.f;
     }
 }
 
-__global__ __launch_bounds__(256) void lora_expand_kernel(Lora l) {
-    const int row = blockIdx.x;
-    const int id = l.ids[row];
-    const int rank = id < 0 ? 0 : rank_of(l, id);
-    if (rank < 0 && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(&ibh_lora_err, IBH_DEVERR_LORA);
-    for (int m = blockIdx.y * 256 + threadIdx.x; m < l.M; m += gridDim.y * 256) {
-        float s = 0;
-        for (int r = 0; r < rank; r++)
-            s = fmaf(widen(l.b[((size_t)id * l.M + m) * l.R + r], l.kind), l.t[(size_t)row * l.R + r], s);
-        if (l.base) s += l.base[row * l.bs + m];
-        l.out[row * l.os + m] = rank < 0 ? __builtin_nanf("") : s;
+template <int KIND>
+__global__ __launch_bounds__(256) void lora_shrink_few(Lora l) {
+    __shared__ float part[16][4];
+    const Few f = few_of(l);
+    const int r0 = blockIdx.y * 4;
+    if (!f.rows || f.rank <= 0 || r0 >= (f.rank + 7) / 8 * 8) return;
+    if (f.rows == 1) shrink_rows<KIND, 4, 1>(l, f, r0, part);
+    else if (f.rows == 2) shrink_rows<KIND, 4, 2>(l, f, r0, part);
+    else shrink_rows<KIND, 4, 4>(l, f, r0, part);
+}
+
+// A row of b in `1 << lg` lanes, eight numbers each; kOut outputs a lane group.
+constexpr int kOut = 2;
+template <int KIND, int NR>
+__device__ __forceinline__ void expand_rows(const Lora& l, const Few& f, int lg) {
+    const int sub = threadIdx.x & ((1 << lg) - 1), per = 256 >> lg, r0 = 8 * sub;
+    const int m0 = blockIdx.y * per * kOut + (threadIdx.x >> lg);
+    const uint16_t* b = l.b + (size_t)f.id * l.M * l.R;
+    u4_t w[kOut];
+#pragma unroll
+    for (int o = 0; o < kOut; o++) {
+        const int m = m0 + o * per;
+        w[o] = m < l.M && r0 < f.rank ? load8h(b + (size_t)m * l.R, r0, f.rank) : u4_t{0, 0, 0, 0};
+    }
+    f4_t t[NR][2];
+    float y[kOut][NR];
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            t[i][h] = r0 < f.rank ? *(const f4_t*)(l.t + (size_t)f.row[i] * l.Rp + r0 + 4 * h) : f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int o = 0; o < kOut; o++) {
+            const int m = m0 + o * per;
+            y[o][i] = l.base && sub == 0 && m < l.M ? l.base[f.row[i] * l.bs + m] : 0.f;
+        }
+    }
+#pragma unroll
+    for (int o = 0; o < kOut; o++) {
+        float s[NR];
+#pragma unroll
+        for (int i = 0; i < NR; i++) s[i] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float we = widen<KIND>(e % 2 ? w[o][e / 2] >> 16 : w[o][e / 2] & 0xffffu);
+#pragma unroll
+            for (int i = 0; i < NR; i++) s[i] = fmaf(we, t[i][e / 4][e % 4], s[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+            for (int k = 0; k < lg; k++) s[i] += __shfl_xor(s[i], 1 << k, kWave);
+            const int m = m0 + o * per;
+            if (sub == 0 && m < l.M && i < f.rows) l.out[f.row[i] * l.os + m] = y[o][i] + s[i];
+        }
+    }
+}
+
+template <int KIND>
+__global__ __launch_bounds__(256) void lora_expand_few(Lora l, int lg) {
+    const Few f = few_of(l);
+    if (!f.rows) return;
+    if (f.rank <= 0) {                                   // no adapter: base; not in the table: NaN
+        if (f.rank < 0 && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(&ibh_lora_err, IBH_DEVERR_LORA);
+        if (f.rank == 0 && l.out == l.base) return;
+        const int span = (256 >> lg) * kOut, m0 = blockIdx.y * span;
+        for (int i = 0; i < f.rows; i++)
+            for (int m = m0 + threadIdx.x; m < min(m0 + span, l.M); m += 256)
+                l.out[f.row[i] * l.os + m] = f.rank < 0 ? __builtin_nanf("") : l.base ? l.base[f.row[i] * l.bs + m] : 0.f;
+        return;
+    }
+    if (f.rows == 1) expand_rows<KIND, 1>(l, f, lg);
+    else if (f.rows == 2) expand_rows<KIND, 2>(l, f, lg);
+    else expand_rows<KIND, 4>(l, f, lg);
+}
+
+// ── more rows: tiles of one adapter's rows on the matrix cores ───────────────
+// One block sorts the rows by adapter (counting; the order within one adapter
+// is left to chance and changes no result: a row's sums do not depend on its
+// place) and cuts each adapter's rows into tiles.
+__global__ __launch_bounds__(1024) void lora_plan(Lora l) {
+    __shared__ int32_t count[kMaxAdapters + 2];
+    __shared__ int32_t wave_rows[16], wave_tiles[16];
+    const int tid = threadIdx.x, keys = l.n + 2;         // n: no adapter; n + 1: not in the table
+    for (int i = tid; i < keys; i += 1024) count[i] = 0;
+    __syncthreads();
+    auto key_of = [&](int row) {
+        const int id = l.ids[row], rank = rank_of(l, id);
+        return rank < 0 ? l.n + 1 : rank == 0 ? l.n : id;
+    };
+    for (int i = tid; i < l.B; i += 1024) atomicAdd(&count[key_of(i)], 1);
+    __syncthreads();
+    // each thread's run of keys: rows and tiles in front of it
+    const int per = (keys + 1023) / 1024, k0 = min(tid * per, keys), k1 = min(k0 + per, keys);
+    int rows = 0, tiles = 0;
+    for (int k = k0; k < k1; k++) {
+        rows += count[k];
+        tiles += (count[k] + kTile - 1) / kTile;
+    }
+    int ir = rows, it = tiles;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int pr = __shfl_up(ir, o, 64), pt = __shfl_up(it, o, 64);
+        if ((tid & 63) >= o) ir += pr, it += pt;
+    }
+    if ((tid & 63) == 63) wave_rows[tid >> 6] = ir, wave_tiles[tid >> 6] = it;
+    __syncthreads();
+    ir -= rows;
+    it -= tiles;
+    for (int w = 0; w < (tid >> 6); w++) ir += wave_rows[w], it += wave_tiles[w];
+    if (tid == 1023) l.plan[0] = it + tiles;
+    Tile* out = (Tile*)(l.plan + 4);
+    for (int k = k0; k < k1; k++) {
+        const int c = count[k], rank = k < l.n ? (l.ranks ? l.ranks[k] : l.R) : l.n - k;
+        count[k] = ir;                                   // from here on: where its next row goes
+        for (int j = 0; j < c; j += kTile) out[it++] = {k < l.n ? k : -1, rank, ir + j, min(kTile, c - j)};
+        ir += c;
+    }
+    __syncthreads();
+    int32_t* order = l.plan + 4 + 4 * l.max_tiles;
+    for (int i = tid; i < l.B; i += 1024) order[atomicAdd(&count[key_of(i)], 1)] = i;
+}
+
+// fp32 numbers as bf16 numbers, upper halves cut off one after the other: 8
+// bits each, all 24 in three, nothing lost.
+__device__ __forceinline__ uint32_t upper(float a, float b) {
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+}
+__device__ __forceinline__ float below(float v) {
+    return v - __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+}
+// Eight 16-bit numbers of an adapter as bf16: one piece, or two for fp16 (8 and
+// 3 bits).
+template <int KIND>
+__device__ __forceinline__ void pieces(u4_t v, v8bf* p) {
+    if constexpr (KIND == IBH_BF16) p[0] = __builtin_bit_cast(v8bf, v);
+    else {
+        u4_t hi, lo;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float a = f16_to_f32((uint16_t)v[i]), b = f16_to_f32((uint16_t)(v[i] >> 16));
+            hi[i] = upper(a, b);
+            lo[i] = upper(below(a), below(b));
+        }
+        p[0] = __builtin_bit_cast(v8bf, hi);
+        p[1] = __builtin_bit_cast(v8bf, lo);
+    }
+}
+
+// t of a tile of rows and RT * 16 ranks over a share of the columns.  Four
+// wavefronts: 16 rows each, and half of each step's columns.
+template <int KIND, int RT>
+__global__ __launch_bounds__(256) void lora_shrink_tile(Lora l) {
+    constexpr int P = KIND == IBH_F16 ? 2 : 1, kRow = kStep + 8;   // 272 bytes: 16 rows on all banks
+    __shared__ __align__(16) uint16_t sx[3][kTile][kRow];
+    __shared__ __align__(16) uint16_t sa[P][RT * 16][kRow];
+    const int tile = blockIdx.x;
+    if (tile >= l.plan[0]) return;
+    const Tile tl = ((const Tile*)(l.plan + 4))[tile];
+    const int r0 = blockIdx.z * RT * 16;
+    if (r0 >= (tl.rank + 7) / 8 * 8) return;
+    const int32_t* order = l.plan + 4 + 4 * l.max_tiles + tl.start;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int steps = (l.N + kStep - 1) / kStep;
+    const int s0 = (int)((int64_t)steps * blockIdx.y / l.S), s1 = (int)((int64_t)steps * (blockIdx.y + 1) / l.S);
+
+    // loads: 32 lanes a row of x, 16 lanes a row of a
+    const float* xrow[4];
+    bool there[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = i * 8 + tid / 32;
+        there[i] = r < tl.count;
+        xrow[i] = l.x + order[there[i] ? r : 0] * l.xs;
+    }
+    const int xk = tid % 32 * 4, ak = tid % 16 * 8;
+    f4_t vx[4];
+    u4_t va[RT];
+    auto fetch = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) vx[i] = there[i] ? load4(xrow[i], s * kStep + xk, l.N) : f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+            const int r = r0 + i * 16 + tid / 16;
+            va[i] = r < tl.rank ? load8h(l.a + ((size_t)tl.id * l.R + r) * l.N, s * kStep + ak, l.N) : u4_t{0, 0, 0, 0};
+        }
+    };
+    v4f acc[RT];
+#pragma unroll
+    for (int i = 0; i < RT; i++) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+    if (s0 < s1) fetch(s0);
+    for (int s = s0; s < s1; s++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = i * 8 + tid / 32;
+            float v[4] = {vx[i][0], vx[i][1], vx[i][2], vx[i][3]};
+#pragma unroll
+            for (int p = 0; p < 3; p++) {
+                *(uint2*)&sx[p][r][xk] = make_uint2(upper(v[0], v[1]), upper(v[2], v[3]));
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = below(v[e]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+            v8bf p[2];
+            pieces<KIND>(va[i], p);
+#pragma unroll
+            for (int j = 0; j < P; j++) *(v8bf*)&sa[j][i * 16 + tid / 16][ak] = p[j];
+        }
+        __syncthreads();
+        if (s + 1 < s1) fetch(s + 1);
+        const int c = wave % 2 * 16 + lane % 16, k0 = wave / 2 * 64 + lane / 16 * 8;
+#pragma unroll
+        for (int k = 0; k < 64; k += 32) {
+            v8bf bx[3];
+#pragma unroll
+            for (int p = 0; p < 3; p++) bx[p] = *(const v8bf*)&sx[p][c][k0 + k];
+#pragma unroll
+            for (int i = 0; i < RT; i++)
+#pragma unroll
+                for (int j = 0; j < P; j++) {
+                    const v8bf ba = *(const v8bf*)&sa[j][i * 16 + lane % 16][k0 + k];
+#pragma unroll
+                    for (int p = 0; p < 3; p++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ba, bx[p], acc[i], 0, 0, 0);
+                }
+        }
+        __syncthreads();
+    }
+    // the second halves of the steps join the first; lane: row lane % 16 of the
+    // tile, ranks lane / 16 * 4 .. + 3
+    v4f* join = (v4f*)sx;
+    if (wave >= 2)
+#pragma unroll
+        for (int i = 0; i < RT; i++) join[((wave - 2) * RT + i) * 64 + lane] = acc[i];
+    __syncthreads();
+    const int c = wave * 16 + lane % 16;
+    if (wave >= 2 || c >= tl.count) return;
+    const float scale = l.scales ? l.scales[tl.id] : 1.f;
+    float* t = l.t + ((size_t)blockIdx.y * l.B + order[c]) * l.Rp;
+#pragma unroll
+    for (int i = 0; i < RT; i++) {
+        const int r = r0 + i * 16 + lane / 16 * 4;
+        if (r < l.Rp) *(v4f*)(t + r) = (acc[i] + join[(wave * RT + i) * 64 + lane]) * scale;
+    }
+}
+
+// out of a tile of rows and kChunk outputs.  t's splits are added up and cut
+// into pieces in LDS; a wavefront takes 64 outputs at a time, four matrix tiles
+// beside each other.
+template <int KIND>
+__global__ __launch_bounds__(256) void lora_expand_tile(Lora l) {
+    constexpr int P = KIND == IBH_F16 ? 2 : 1;
+    extern __shared__ __align__(16) uint16_t st[];       // [3][kTile][kr]
+    const int tile = blockIdx.x;
+    if (tile >= l.plan[0]) return;
+    const Tile tl = ((const Tile*)(l.plan + 4))[tile];
+    const int32_t* order = l.plan + 4 + 4 * l.max_tiles + tl.start;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int m_end = min((int)(blockIdx.y + 1) * kChunk, l.M);
+    if (tl.rank <= 0) {                                  // no adapter: base; not in the table: NaN
+        if (tl.rank < 0 && tid == 0 && blockIdx.y == 0) atomicOr(&ibh_lora_err, IBH_DEVERR_LORA);
+        if (tl.rank == 0 && l.out == l.base) return;
+        for (int i = wave; i < tl.count; i += 4) {
+            const int row = order[i];
+            for (int m = blockIdx.y * kChunk + lane * 4; m < m_end; m += 256) {
+                const float nan = __builtin_nanf("");
+                store4(l.out + row * l.os, m, l.M, tl.rank < 0 ? f4_t{nan, nan, nan, nan} :
+                       l.base ? load4(l.base + row * l.bs, m, l.M) : f4_t{0.f, 0.f, 0.f, 0.f});
+            }
+        }
+        return;
+    }
+    const int ks = (tl.rank + 31) / 32, kr = ks * 32 + 8;
+    for (int i = tid; i < kTile * ks * 8; i += 256) {
+        const int c = i / (ks * 8), r = i % (ks * 8) * 4;
+        v4f v = {0.f, 0.f, 0.f, 0.f};
+        if (c < tl.count && r < (tl.rank + 7) / 8 * 8)
+            for (int s = 0; s < l.S; s++) v += *(const v4f*)(l.t + ((size_t)s * l.B + order[c]) * l.Rp + r);
+        float e[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+        for (int p = 0; p < 3; p++) {
+            *(uint2*)&st[(p * kTile + c) * kr + r] = make_uint2(upper(e[0], e[1]), upper(e[2], e[3]));
+#pragma unroll
+            for (int q = 0; q < 4; q++) e[q] = below(e[q]);
+        }
+    }
+    __syncthreads();
+    const int c = lane % 16, q = lane / 16;
+    int row[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) row[h] = h * 16 + c < tl.count ? order[h * 16 + c] : -1;
+    const uint16_t* b = l.b + (size_t)tl.id * l.M * l.R;
+    for (int m0 = blockIdx.y * kChunk + wave * 64; m0 < m_end; m0 += 256) {
+        f4_t y[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                y[h][j] = l.base && row[h] >= 0 ? load4(l.base + row[h] * l.bs, m0 + 16 * j + 4 * q, l.M) : f4_t{0.f, 0.f, 0.f, 0.f};
+        v4f acc[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[h][j] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < ks; k++) {
+            const int r = k * 32 + q * 8;
+            u4_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int m = m0 + 16 * j + c;
+                w[j] = m < l.M && r < tl.rank ? load8h(b + (size_t)m * l.R, r, tl.rank) : u4_t{0, 0, 0, 0};
+            }
+            v8bf bt[2][3];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int p = 0; p < 3; p++) bt[h][p] = *(const v8bf*)&st[(p * kTile + h * 16 + c) * kr + r];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                v8bf bw[2];
+                pieces<KIND>(w[j], bw);
+#pragma unroll
+                for (int i = 0; i < P; i++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int p = 0; p < 3; p++)
+                            acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bw[i], bt[h][p], acc[h][j], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            if (row[h] >= 0)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    store4(l.out + row[h] * l.os, m0 + 16 * j + 4 * q, l.M, y[h][j] + acc[h][j]);
     }
 }
 
 bool adapters_ok(const ibh_lora_adapters* l, const char* who) {
-    if (!l || !l->a || !l->b || l->n <= 0 || l->rank <= 0 || l->rank > IBH_LORA_MAX_RANK || l->N <= 0 || l->M <= 0 ||
+    if (!l || !l->a || !l->b || l->n <= 0 || l->n > kMaxAdapters || l->rank <= 0 || l->rank > IBH_LORA_MAX_RANK || l->N <= 0 || l->M <= 0 ||
         l->N > (1 << 20) || l->M > (1 << 20) || (l->kind != IBH_F16 && l->kind != IBH_BF16)) {
         if (!l) ibh_set_error("%s: no adapters given", who);
         else
-            ibh_set_error("%s: invalid adapters (n=%d rank=%d N=%d M=%d kind=%d; rank up to %d, IBH_F16 or IBH_BF16)",
-                          who, l->n, l->rank, l->N, l->M, l->kind, IBH_LORA_MAX_RANK);
+            ibh_set_error("%s: invalid adapters (n=%d rank=%d N=%d M=%d kind=%d; up to %d adapters of rank "
+                          "up to %d, IBH_F16 or IBH_BF16)",
+                          who, l->n, l->rank, l->N, l->M, l->kind, kMaxAdapters, IBH_LORA_MAX_RANK);
         return false;
     }
     return true;
+}
+
+// How a call is cut.
+struct LoraPlan {
+    bool few;
+    int Rp, S, max_tiles;
+    size_t plan_bytes, bytes;
+};
+LoraPlan plan_of(const ibh_lora_adapters* l, int B) {
+    LoraPlan p;
+    p.few = B <= kFew;
+    p.Rp = (l->rank + 7) / 8 * 8;
+    p.S = 1;
+    p.max_tiles = 0;
+    p.plan_bytes = 0;
+    if (!p.few) {
+        const int groups = min(l->n + 2, B);
+        p.max_tiles = B / kTile + groups;
+        p.plan_bytes = (16 + 16 * (size_t)p.max_tiles + 4 * (size_t)B + 15) / 16 * 16;
+        const int tiles = (B + kTile - 1) / kTile + min(l->n, B) / 2;
+        p.S = max(1, min(min(kMaxSplit, (l->N + 511) / 512), 768 / tiles));
+    }
+    p.bytes = p.plan_bytes + (size_t)p.S * B * p.Rp * 4;
+    return p;
+}
+
+template <int KIND>
+int launch(const Lora& l, bool few, hipStream_t st) {
+    if (few) {
+        int lg = 0;
+        while (8 << lg < l.R) lg++;
+        const int span = (256 >> lg) * kOut;
+        lora_shrink_few<KIND><<<dim3(l.B, (l.Rp + 3) / 4), 256, 0, st>>>(l);
+        IBH_CHECK_LAUNCH("ibh_lora");
+        lora_expand_few<KIND><<<dim3(l.B, (l.M + span - 1) / span), 256, 0, st>>>(l, lg);
+        IBH_CHECK_LAUNCH("ibh_lora");
+        return IBH_OK;
+    }
+    lora_plan<<<1, 1024, 0, st>>>(l);
+    IBH_CHECK_LAUNCH("ibh_lora");
+    if (l.R <= 16) lora_shrink_tile<KIND, 1><<<dim3(l.max_tiles, l.S), 256, 0, st>>>(l);
+    else if (l.R <= 32) lora_shrink_tile<KIND, 2><<<dim3(l.max_tiles, l.S), 256, 0, st>>>(l);
+    else lora_shrink_tile<KIND, 4><<<dim3(l.max_tiles, l.S, (l.R + 63) / 64), 256, 0, st>>>(l);
+    IBH_CHECK_LAUNCH("ibh_lora");
+    lora_expand_tile<KIND><<<dim3(l.max_tiles, (l.M + kChunk - 1) / kChunk), 256,
+                             3 * kTile * ((l.R + 31) / 32 * 32 + 8) * 2, st>>>(l);
+    IBH_CHECK_LAUNCH("ibh_lora");
+    return IBH_OK;
 }
 
 }  // namespace
@@ -88,7 +575,7 @@ int ibh_lora_errors(bool clear) {
 
 extern "C" size_t ibh_lora_workspace_bytes(const ibh_lora_adapters* l, int B) {
     if (!adapters_ok(l, "ibh_lora_workspace_bytes") || B <= 0) return 0;
-    return (size_t)B * l->rank * 4;
+    return plan_of(l, B).bytes;
 }
 
 extern "C" int ibh_lora(const ibh_lora_adapters* l, float* out, const float* base, const float* x, const int32_t* ids,
@@ -109,22 +596,20 @@ extern "C" int ibh_lora(const ibh_lora_adapters* l, float* out, const float* bas
         ibh_set_error("ibh_lora: out overlaps another operand");
         return IBH_ERROR_PARAM;
     }
-    if (B >= (1 << 24)) {
+    const LoraPlan p = plan_of(l, B);
+    // a launch takes less than 2^32 threads
+    if (!p.few && (size_t)p.max_tiles * max((l->M + kChunk - 1) / kChunk, p.S * ((l->rank + 63) / 64)) >= (1 << 24)) {
         ibh_set_error("ibh_lora: %d rows are more than one launch takes", B);
         return IBH_ERROR_PARAM;
     }
-    const size_t need = ibh_lora_workspace_bytes(l, B);
-    float* t = (float*)(ws ? (ws_bytes >= need && !((uintptr_t)ws & 15) ? ws : nullptr) : ibh_workspace(need));
-    if (!t) {
-        ibh_set_error("ibh_lora: a workspace of %zu bytes on 16 bytes is needed", need);
+    uint8_t* w = (uint8_t*)(ws ? (ws_bytes >= p.bytes && !((uintptr_t)ws & 15) ? ws : nullptr) : ibh_workspace(p.bytes));
+    if (!w) {
+        ibh_set_error("ibh_lora: a workspace of %zu bytes on 16 bytes is needed", p.bytes);
         return IBH_ERROR_MEMORY;
     }
-    const Lora a{(const uint16_t*)l->a, (const uint16_t*)l->b, l->scales, l->ranks, l->n, l->rank, l->N, l->M, l->kind,
-                 out, base, x, ids, B, (size_t)out_stride, (size_t)base_stride, (size_t)x_stride, t};
+    const Lora a{(const uint16_t*)l->a, (const uint16_t*)l->b, l->scales, l->ranks, l->n, l->rank, l->N, l->M, out, base, x,
+                 ids, B, (size_t)out_stride, (size_t)base_stride, (size_t)x_stride, (float*)(w + p.plan_bytes), p.Rp, p.S,
+                 (int32_t*)w, p.max_tiles};
     hipStream_t st = ibh_resolve_stream(stream);
-    lora_shrink_kernel<<<dim3(B, B > 1024 ? 1 : (l->rank + 3) / 4), 256, 0, st>>>(a);
-    IBH_CHECK_LAUNCH("ibh_lora");
-    lora_expand_kernel<<<dim3(B, B > 1024 ? 1 : (l->M + 255) / 256), 256, 0, st>>>(a);
-    IBH_CHECK_LAUNCH("ibh_lora");
-    return IBH_OK;
+    return l->kind == IBH_F16 ? launch<IBH_F16>(a, p.few, st) : launch<IBH_BF16>(a, p.few, st);
 }
