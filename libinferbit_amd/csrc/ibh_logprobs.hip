@@ -1,11 +1,21 @@
 // ibh_logprobs.hip -- log-probabilities of given tokens, entropy and the best
 // alternatives of rows of logits.
+//
+// One pass over a row: every lane keeps the running maximum m, s = sum e^(z - m)
+// and e = sum e^(z - m) (z - m) of its logits, every wavefront the k best it has
+// seen.  log S = m + log s; entropy = log s - e / s.
 #include "ibh_common.h"
 
 namespace {
 using namespace ibh;
 
-constexpr int kT = 1024;
+constexpr int kWaves = 4;
+constexpr int kPiece = 1024;                             // logits that a wavefront takes at a time
+constexpr int kHeld = 256;                               // candidates that it holds
+constexpr int kMaxShares = 64;                          // blocks that share a row, at most
+constexpr float kLog2e = 1.44269504088896340736f;
+
+typedef float f4_t __attribute__((ext_vector_type(4), aligned(4)));
 
 struct LogArgs {
     float *out, *entropy, *top_lp;
@@ -14,78 +24,264 @@ struct LogArgs {
     const int32_t* tokens;
     int V, n_tok, k;
     size_t stride;
+    int S, seg;                                          // blocks that share a row, logits of each
+    float* part;                                         // [B][S]{m, s, e, -}
+    uint64_t* keys;                                      // [B][S][k], the best of each share, in no order, 0 behind them
 };
 
-// A logit and its place as one whole number: larger is better, of equal logits
-// the lower place.
-__device__ __forceinline__ uint64_t key_of(float z, int id) {
-    uint32_t b = __builtin_bit_cast(uint32_t, z + 0.f);  // -0 ties with 0
-    b = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return (uint64_t)b << 32 | (uint32_t)~id;
+// ── sums ─────────────────────────────────────────────────────────────────────
+struct Sums {
+    float m, s, e;                                       // s is NaN where a logit is NaN or +infinity
+};
+// What the sums of maximum `from` are multiplied by, and the distance, where
+// the maximum becomes `to`.  Masked logits (-infinity) and empty sums come out
+// as a factor of 0 beside a finite distance, so that no 0 * infinity arises.
+__device__ __forceinline__ float down(float from, float to, float* d) {
+    const float x = from - (to == -__builtin_inff() ? 0.f : to);
+    *d = fmaxf(x, -1e4f);
+    return __builtin_amdgcn_exp2f(x * kLog2e);
+}
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
+    Sums r;
+    r.m = fmaxf(a.m, b.m);
+    float da, db;
+    const float fa = down(a.m, r.m, &da), fb = down(b.m, r.m, &db);
+    r.s = a.s * fa + b.s * fb;
+    r.e = fa * (a.e + a.s * da) + fb * (b.e + b.s * db);
+    return r;
+}
+__device__ __forceinline__ Sums wave_join(Sums a) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        a = join(a, {__shfl_xor(a.m, o, kWave), __shfl_xor(a.s, o, kWave), __shfl_xor(a.e, o, kWave)});
+    return a;
 }
 
-__global__ __launch_bounds__(kT) void logprobs_kernel(LogArgs a) {
-    __shared__ float sm[kT / 64], ss[kT / 64], se[kT / 64];
-    __shared__ uint64_t sk[kT / 64];
-    const size_t row = blockIdx.x;
+// ── the k best ───────────────────────────────────────────────────────────────
+// A logit and its place as one whole number: larger is better, of equal logits
+// the lower place.
+__device__ __forceinline__ uint32_t order_of(float z) {
+    const uint32_t b = __float_as_uint(z + 0.f);         // -0 ties with 0
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t key_of(float z, int id) { return (uint64_t)order_of(z) << 32 | (uint32_t)~id; }
+constexpr uint64_t kNothing = 0x007fffffffffffffull;     // -infinity: what is to be held has to be above
+
+// A wavefront's candidates: at most kHeld keys, among them the k largest seen;
+// keys up to `bar` are known not to be among them.
+struct Best {
+    uint64_t* held;
+    int n, k;
+    uint64_t bar;
+
+    // Leaves the k largest: their smallest is found bit by bit.
+    __device__ __forceinline__ void cut() {
+        if (n <= k) return;
+        const int lane = threadIdx.x & 63;
+        uint64_t key[kHeld / 64];
+#pragma unroll
+        for (int i = 0; i < kHeld / 64; i++) key[i] = i * 64 + lane < n ? held[i * 64 + lane] : 0;
+        uint64_t t = 0;
+        for (int bit = 63; bit >= 0; bit--) {
+            const uint64_t c = t | 1ull << bit;
+            int above = 0;
+#pragma unroll
+            for (int i = 0; i < kHeld / 64; i++) above += __popcll(__ballot(key[i] >= c));
+            if (above >= k) t = c;
+            if (above == k) break;
+        }
+        int at = 0;
+#pragma unroll
+        for (int i = 0; i < kHeld / 64; i++) {
+            const uint64_t keep = __ballot(key[i] >= t);
+            if (key[i] >= t) held[at + __popcll(keep & ((1ull << lane) - 1))] = key[i];
+            at += __popcll(keep);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        n = at;
+        bar = t > bar ? t : bar;
+    }
+    __device__ __forceinline__ void offer(uint64_t key) {
+        uint64_t more = __ballot(key > bar);
+        if (!more) return;
+        if (n + __popcll(more) > kHeld) {
+            cut();
+            more = __ballot(key > bar);
+        }
+        const int lane = threadIdx.x & 63;
+        if (key > bar) held[n + __popcll(more & ((1ull << lane) - 1))] = key;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // other lanes read it
+        n += __popcll(more);
+    }
+    // A bar for the first piece: the k-th largest of the lanes' own largest
+    // logits (at least k logits are as large).
+    __device__ __forceinline__ void first(float largest) {
+        const uint32_t o = largest > -__builtin_inff() ? order_of(largest) : 0;
+        uint32_t t = 0;
+        for (int bit = 31; bit >= 0; bit--) {
+            const uint32_t c = t | 1u << bit;
+            const int above = __popcll(__ballot(o >= c));
+            if (above >= k) t = c;
+            if (above == k) break;
+        }
+        const uint64_t b = ((uint64_t)t << 32) - 1;
+        if (t && b > bar) bar = b;
+    }
+};
+
+// What the row's outputs are made of: by the first wavefront's candidates.
+__device__ __forceinline__ void finish(const LogArgs& a, size_t row, Sums t, Best& best) {
+    const int tid = threadIdx.x;
     const float* z = a.z + row * a.stride;
-    const int tid = threadIdx.x, wave = tid >> 6;
-    float m = -__builtin_inff();
-    bool nan = false;
-    for (int j = tid; j < a.V; j += kT) {
-        nan |= !(z[j] < __builtin_inff());
-        m = fmaxf(m, z[j]);
+    const bool bad = t.s != t.s, none = t.m == -__builtin_inff();
+    const float logs = logf(t.s), nanf = __builtin_nanf("");
+    for (int i = tid; i < a.n_tok; i += kWaves * 64) {
+        const int id = a.tokens[row * a.n_tok + i];
+        a.out[row * a.n_tok + i] = bad || id < 0 || id >= a.V ? nanf : none ? -__builtin_inff() : (z[id] - t.m) - logs;
     }
-    m = wave_max(nan ? __builtin_inff() : m);
-    if ((tid & 63) == 0) sm[wave] = m;
+    if (a.entropy && tid == 0) a.entropy[row] = bad ? nanf : none ? 0.f : logs - t.e / t.s;
+    if (!a.k || tid >= 64) return;
+    best.cut();
+    const uint64_t mine = tid < best.n ? best.held[tid] : 0;
+    int rank = 0;
+    for (int i = 0; i < best.n; i++) rank += best.held[i] > mine;
+    if (tid >= best.n) rank = tid;
+    if (rank < a.k) {
+        const int id = ~(uint32_t)mine;
+        const bool held = !bad && tid < best.n;
+        a.top_ids[row * a.k + rank] = held ? id : -1;
+        a.top_lp[row * a.k + rank] = bad ? nanf : held ? (z[id] - t.m) - logs : -__builtin_inff();
+    }
+}
+
+// The block's sums, and the other wavefronts' candidates to the first.
+__device__ __forceinline__ Sums gather(Sums t, Best& best, uint64_t (*held)[kHeld], int* counts, Sums* sums) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    t = wave_join(t);
+    if (best.k) best.cut();
+    if (lane == 0) sums[wave] = t, counts[wave] = best.n;
     __syncthreads();
-    for (int i = 0; i < kT / 64; i++) m = fmaxf(m, sm[i]);
-    float s = 0, e = 0;
-    for (int j = tid; j < a.V; j += kT) {
-        const float d = z[j] - m, p = expf(d);
-        if (z[j] > -__builtin_inff()) s += p, e += p * d;
-    }
-    s = wave_sum(s);
-    e = wave_sum(e);
-    if ((tid & 63) == 0) ss[wave] = s, se[wave] = e;
-    __syncthreads();
-    s = e = 0;
-    for (int i = 0; i < kT / 64; i++) s += ss[i], e += se[i];
-    const bool bad = m == __builtin_inff(), none = m == -__builtin_inff();
-    const float lse = logf(s), nanf = __builtin_nanf("");
-    for (int t = tid; t < a.n_tok; t += kT) {
-        const int id = a.tokens[row * a.n_tok + t];
-        a.out[row * a.n_tok + t] = bad || id < 0 || id >= a.V ? nanf : none ? -__builtin_inff() : (z[id] - m) - lse;
-    }
-    if (a.entropy && tid == 0) a.entropy[row] = bad ? nanf : none ? 0.f : lse - e / s;
-    uint64_t last = ~0ull;
-    for (int t = 0; t < a.k; t++) {
-        uint64_t best = 0;
-        if (!bad)
-            for (int j = tid; j < a.V; j += kT) {
-                const uint64_t key = key_of(z[j], j);
-                if (z[j] > -__builtin_inff() && key < last && key > best) best = key;
+    t = sums[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) t = join(t, sums[w]);
+    if (wave == 0 && best.k)
+        for (int w = 1; w < kWaves; w++) best.offer(lane < counts[w] ? held[w][lane] : 0);
+    return t;
+}
+
+__global__ __launch_bounds__(kWaves * 64) void logprobs_kernel(LogArgs a) {
+    __shared__ uint64_t held[kWaves][kHeld];
+    __shared__ int counts[kWaves];
+    __shared__ Sums sums[kWaves];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const size_t row = blockIdx.x / a.S;
+    const int share = blockIdx.x % a.S;
+    const float* z = a.z + row * a.stride;
+    const int v0 = share * a.seg, v1 = min(v0 + a.seg, a.V);
+    Sums t{-__builtin_inff(), 0.f, 0.f};
+    Best best{held[wave], 0, a.k, kNothing};
+    f4_t next[4];
+    auto fetch = [&](int at) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int j = at + q * 256 + lane * 4;
+            if (j + 4 <= v1) next[q] = *(const f4_t*)(z + j);
+            else
+#pragma unroll
+                for (int i = 0; i < 4; i++) next[q][i] = j + i < v1 ? z[j + i] : -__builtin_inff();
+        }
+    };
+    int at = v0 + wave * kPiece;
+    if (at < v1) fetch(at);
+    for (bool begin = true; at < v1; at += kWaves * kPiece, begin = false) {
+        f4_t v[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) v[q] = next[q];
+        if (at + kWaves * kPiece < v1) fetch(at + kWaves * kPiece);
+        float top = v[0][0];
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) top = fmaxf(top, v[q][i]);
+        float d;
+        const float m = fmaxf(t.m, top), f = down(t.m, m, &d);
+        Sums now{m, 0.f, 0.f};                           // apart, so that chains of additions stay short
+        t = {m, t.s * f, f * (t.e + t.s * d)};
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float p = down(v[q][i], m, &d);
+                now.s += p;
+                now.e = fmaf(p, d, now.e);
             }
-        for (int o = 32; o > 0; o >>= 1) {
-            const uint64_t other = __shfl_xor(best, o, 64);
-            best = other > best ? other : best;
-        }
-        if ((tid & 63) == 0) sk[wave] = best;
-        __syncthreads();
-        for (int i = 0; i < kT / 64; i++) best = sk[i] > best ? sk[i] : best;
-        __syncthreads();
-        const int id = ~(uint32_t)best;
-        if (tid == 0) {
-            a.top_ids[row * a.k + t] = best ? id : -1;
-            a.top_lp[row * a.k + t] = bad ? nanf : best ? (z[id] - m) - lse : -__builtin_inff();
-        }
-        last = best;
+        t.s += now.s;
+        t.e += now.e;
+        if (!a.k) continue;
+        if (begin) best.first(top);
+        if (!__ballot(order_of(top) > (uint32_t)(best.bar >> 32))) continue;
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) best.offer(key_of(v[q][i], at + q * 256 + lane * 4 + i));
     }
+    t = gather(t, best, held, counts, sums);
+    if (a.S == 1) {
+        finish(a, row, t, best);
+        return;
+    }
+    const size_t me = blockIdx.x;
+    if (threadIdx.x == 0) *(f4_t*)(a.part + me * 4) = f4_t{t.m, t.s, t.e, 0.f};
+    if (wave == 0 && a.k) {
+        best.cut();
+        if (lane < a.k) a.keys[me * a.k + lane] = lane < best.n ? held[0][lane] : 0;
+    }
+}
+
+// The shares of a row joined.
+__global__ __launch_bounds__(kWaves * 64) void logprobs_join(LogArgs a) {
+    __shared__ uint64_t held[kWaves][kHeld];
+    __shared__ int counts[kWaves];
+    __shared__ Sums sums[kWaves];
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const size_t row = blockIdx.x;
+    Sums t{-__builtin_inff(), 0.f, 0.f};
+    for (int i = tid; i < a.S; i += kWaves * 64) {
+        const f4_t v = *(const f4_t*)(a.part + (row * a.S + i) * 4);
+        t = join(t, {v[0], v[1], v[2]});
+    }
+    Best best{held[wave], 0, a.k, kNothing};
+    for (int i = 0; i < a.S * a.k; i += kWaves * 64) best.offer(i + tid < a.S * a.k ? a.keys[row * a.S * a.k + i + tid] : 0);
+    t = gather(t, best, held, counts, sums);
+    finish(a, row, t, best);
+}
+
+// How a call is cut: a row's shares are whole rounds of a block's pieces, as
+// many as fill the card.
+struct LogPlan {
+    int S, seg;
+    size_t part, bytes;
+};
+LogPlan plan_of(int V, int B, int k) {
+    LogPlan p;
+    const int round = kWaves * kPiece, rounds = (V + round - 1) / round;
+    const int want = max(1, min(min(rounds, kMaxShares), (1024 + B - 1) / B));
+    const int each = (rounds + want - 1) / want;
+    p.seg = each * round;
+    p.S = (rounds + each - 1) / each;
+    p.part = p.S > 1 ? (size_t)B * p.S * 16 : 0;
+    p.bytes = p.S > 1 ? p.part + (size_t)B * p.S * k * 8 : 0;
+    return p;
 }
 
 }  // namespace
 
-extern "C" size_t ibh_logprobs_workspace_bytes(int V, int B, int k) { return 0; }
+void* ibh_workspace(size_t bytes);
+
+extern "C" size_t ibh_logprobs_workspace_bytes(int V, int B, int k) {
+    if (V <= 0 || V > (1 << 30) || B <= 0 || k < 0 || k > IBH_LOGPROBS_MAX_K) return 0;
+    return plan_of(V, B, k).bytes;
+}
 
 extern "C" int ibh_logprobs(float* out, float* entropy, int32_t* top_ids, float* top_logprobs, const float* logits,
                             const int32_t* tokens, int V, int B, int stride, int n_tokens, int k, void* ws,
@@ -111,12 +307,27 @@ extern "C" int ibh_logprobs(float* out, float* entropy, int32_t* top_ids, float*
                 ibh_set_error("ibh_logprobs: an output overlaps another operand");
                 return IBH_ERROR_PARAM;
             }
-    if (B >= (1 << 22)) {
+    const LogPlan p = plan_of(V, B, k);
+    if ((size_t)B * p.S >= (1 << 24)) {                  // a launch takes less than 2^32 threads
         ibh_set_error("ibh_logprobs: %d rows are more than one launch takes", B);
         return IBH_ERROR_PARAM;
     }
-    const LogArgs a{out, entropy, top_logprobs, top_ids, logits, tokens, V, n_tokens, k, (size_t)stride};
-    logprobs_kernel<<<B, kT, 0, ibh_resolve_stream(stream)>>>(a);
+    uint8_t* w = nullptr;
+    if (p.bytes) {
+        w = (uint8_t*)(ws ? (ws_bytes >= p.bytes && !((uintptr_t)ws & 15) ? ws : nullptr) : ibh_workspace(p.bytes));
+        if (!w) {
+            ibh_set_error("ibh_logprobs: a workspace of %zu bytes on 16 bytes is needed", p.bytes);
+            return IBH_ERROR_MEMORY;
+        }
+    }
+    const LogArgs a{out, entropy, top_logprobs, top_ids, logits, tokens, V, n_tokens, k, (size_t)stride, p.S, p.seg,
+                    (float*)w, (uint64_t*)(w + p.part)};
+    hipStream_t st = ibh_resolve_stream(stream);
+    logprobs_kernel<<<B * p.S, kWaves * 64, 0, st>>>(a);
     IBH_CHECK_LAUNCH("ibh_logprobs");
+    if (p.S > 1) {
+        logprobs_join<<<B, kWaves * 64, 0, st>>>(a);
+        IBH_CHECK_LAUNCH("ibh_logprobs");
+    }
     return IBH_OK;
 }
