@@ -74,7 +74,20 @@ struct Best {
     int n, k;
     uint64_t bar;
 
-    // Leaves the k largest: their smallest is found bit by bit.
+    // Leaves the k largest, the largest first: each of up to 64 counts those
+    // above it.
+    __device__ __forceinline__ void sort() {
+        if (n > 64) cut();
+        const int lane = threadIdx.x & 63;
+        const uint64_t mine = lane < n ? held[lane] : 0;
+        int above = 0;
+#pragma unroll 8
+        for (int i = 0; i < n; i++) above += held[i] > mine;
+        if (lane < n) held[above] = mine;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        n = n < k ? n : k;
+    }
+    // Leaves the k largest in any order: their smallest is found bit by bit.
     __device__ __forceinline__ void cut() {
         if (n <= k) return;
         const int lane = threadIdx.x & 63;
@@ -113,14 +126,18 @@ struct Best {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // other lanes read it
         n += __popcll(more);
     }
-    // A bar for the first piece: the k-th largest of the lanes' own largest
-    // logits (at least k logits are as large).
-    __device__ __forceinline__ void first(float largest) {
-        const uint32_t o = largest > -__builtin_inff() ? order_of(largest) : 0;
+    // No logit below this one is above the bar, nor one of -infinity.
+    __device__ __forceinline__ float least() const {
+        const uint32_t o = (uint32_t)(bar >> 32);
+        return fmaxf(__uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o), -3.40282347e38f);
+    }
+    // A bar to begin with, from the upper half of each lane's largest key: the
+    // k-th largest of those (at least k keys are as large).
+    __device__ __forceinline__ void first(uint32_t upper) {
         uint32_t t = 0;
         for (int bit = 31; bit >= 0; bit--) {
             const uint32_t c = t | 1u << bit;
-            const int above = __popcll(__ballot(o >= c));
+            const int above = __popcll(__ballot(upper >= c));
             if (above >= k) t = c;
             if (above == k) break;
         }
@@ -129,8 +146,49 @@ struct Best {
     }
 };
 
-// What the row's outputs are made of: by the first wavefront's candidates.
-__device__ __forceinline__ void finish(const LogArgs& a, size_t row, Sums t, Best& best) {
+struct Shared {
+    uint64_t held[kWaves][kHeld];
+    int counts[kWaves];
+    Sums sums[kWaves];
+};
+
+// The block's sums in every thread, each wavefront's best sorted.
+__device__ __forceinline__ Sums gather(Sums t, Best& best, Shared& sh) {
+    const int wave = threadIdx.x >> 6;
+    t = wave_join(t);
+    if (best.k) best.sort();
+    if ((threadIdx.x & 63) == 0) sh.sums[wave] = t, sh.counts[wave] = best.n;
+    __syncthreads();
+    t = sh.sums[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) t = join(t, sh.sums[w]);
+    return t;
+}
+// A thread's own among the wavefronts' sorted best, and how many of the block's
+// are above it (k or more: not among the k best).  total: how many there are.
+__device__ __forceinline__ int rank_of(const Shared& sh, int k, uint64_t* key, int* total) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    *total = sh.counts[0] + sh.counts[1] + sh.counts[2] + sh.counts[3];
+    if (lane >= sh.counts[wave]) return k;
+    *key = sh.held[wave][lane];
+    int low[kWaves], high[kWaves];                       // of each list the keys above: found by halving, all at once
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) low[w] = 0, high[w] = sh.counts[w];
+#pragma unroll
+    for (int step = 0; step < 7; step++)                 // up to 64 keys
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            const int mid = (low[w] + high[w]) / 2;
+            const bool above = mid < high[w] && sh.held[w][mid] > *key;
+            low[w] = above ? mid + 1 : low[w];
+            high[w] = above ? high[w] : mid;
+        }
+    return low[0] + low[1] + low[2] + low[3];
+}
+
+// The row's outputs.
+__device__ __forceinline__ void finish(const LogArgs& a, size_t row, Sums t, const Shared& sh) {
+    static_assert(kWaves == 4, "rank_of");
     const int tid = threadIdx.x;
     const float* z = a.z + row * a.stride;
     const bool bad = t.s != t.s, none = t.m == -__builtin_inff();
@@ -140,55 +198,41 @@ __device__ __forceinline__ void finish(const LogArgs& a, size_t row, Sums t, Bes
         a.out[row * a.n_tok + i] = bad || id < 0 || id >= a.V ? nanf : none ? -__builtin_inff() : (z[id] - t.m) - logs;
     }
     if (a.entropy && tid == 0) a.entropy[row] = bad ? nanf : none ? 0.f : logs - t.e / t.s;
-    if (!a.k || tid >= 64) return;
-    best.cut();
-    const uint64_t mine = tid < best.n ? best.held[tid] : 0;
-    int rank = 0;
-    for (int i = 0; i < best.n; i++) rank += best.held[i] > mine;
-    if (tid >= best.n) rank = tid;
+    if (!a.k) return;
+    uint64_t key = 0;
+    int total;
+    const int rank = rank_of(sh, a.k, &key, &total);
     if (rank < a.k) {
-        const int id = ~(uint32_t)mine;
-        const bool held = !bad && tid < best.n;
-        a.top_ids[row * a.k + rank] = held ? id : -1;
-        a.top_lp[row * a.k + rank] = bad ? nanf : held ? (z[id] - t.m) - logs : -__builtin_inff();
+        const int id = ~(uint32_t)key;
+        a.top_ids[row * a.k + rank] = bad ? -1 : id;
+        a.top_lp[row * a.k + rank] = bad ? nanf : (z[id] - t.m) - logs;
+    }
+    if (tid >= total && tid < a.k) {                     // fewer than k are left
+        a.top_ids[row * a.k + tid] = -1;
+        a.top_lp[row * a.k + tid] = bad ? nanf : -__builtin_inff();
     }
 }
 
-// The block's sums, and the other wavefronts' candidates to the first.
-__device__ __forceinline__ Sums gather(Sums t, Best& best, uint64_t (*held)[kHeld], int* counts, Sums* sums) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    t = wave_join(t);
-    if (best.k) best.cut();
-    if (lane == 0) sums[wave] = t, counts[wave] = best.n;
-    __syncthreads();
-    t = sums[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; w++) t = join(t, sums[w]);
-    if (wave == 0 && best.k)
-        for (int w = 1; w < kWaves; w++) best.offer(lane < counts[w] ? held[w][lane] : 0);
-    return t;
-}
-
-__global__ __launch_bounds__(kWaves * 64) void logprobs_kernel(LogArgs a) {
-    __shared__ uint64_t held[kWaves][kHeld];
-    __shared__ int counts[kWaves];
-    __shared__ Sums sums[kWaves];
+__global__ __launch_bounds__(kWaves * 64, 8) void logprobs_kernel(LogArgs a) {
+    __shared__ Shared sh;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const size_t row = blockIdx.x / a.S;
     const int share = blockIdx.x % a.S;
     const float* z = a.z + row * a.stride;
-    const int v0 = share * a.seg, v1 = min(v0 + a.seg, a.V);
+    // pieces begin on 16 bytes, up to three logits in front of a row that does not
+    const int off = (int)((uintptr_t)z >> 2) & 3;
+    const int v0 = share * a.seg - off, v1 = min(v0 + a.seg, a.V);
     Sums t{-__builtin_inff(), 0.f, 0.f};
-    Best best{held[wave], 0, a.k, kNothing};
+    Best best{sh.held[wave], 0, a.k, kNothing};
     f4_t next[4];
     auto fetch = [&](int at) {
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             const int j = at + q * 256 + lane * 4;
-            if (j + 4 <= v1) next[q] = *(const f4_t*)(z + j);
+            if (j >= 0 && j + 4 <= v1) next[q] = *(const f4_t*)(z + j);
             else
 #pragma unroll
-                for (int i = 0; i < 4; i++) next[q][i] = j + i < v1 ? z[j + i] : -__builtin_inff();
+                for (int i = 0; i < 4; i++) next[q][i] = j + i >= 0 && j + i < v1 ? z[j + i] : -__builtin_inff();
         }
     };
     int at = v0 + wave * kPiece;
@@ -218,42 +262,73 @@ __global__ __launch_bounds__(kWaves * 64) void logprobs_kernel(LogArgs a) {
         t.s += now.s;
         t.e += now.e;
         if (!a.k) continue;
-        if (begin) best.first(top);
-        if (!__ballot(order_of(top) > (uint32_t)(best.bar >> 32))) continue;
+        const uint32_t o = order_of(top);
+        if (begin) best.first(top > -__builtin_inff() ? o : 0);
+        if (!__ballot(o > (uint32_t)(best.bar >> 32))) continue;
+        // each lane's own that may be above, one after the other (few: in
+        // registers they are picked by halving, not by an index)
+        const float least = best.least();
+        uint32_t may = 0;
 #pragma unroll
-        for (int q = 0; q < 4; q++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) best.offer(key_of(v[q][i], at + q * 256 + lane * 4 + i));
+        for (int e = 0; e < 16; e++) may |= (uint32_t)(v[e / 4][e % 4] >= least) << e;
+        for (; __ballot(may != 0); may &= may - 1) {
+            const int e = may ? __ffs(may) - 1 : 0;
+            const uint32_t s0 = -(uint32_t)(e & 1), s1 = -(uint32_t)(e >> 1 & 1), s2 = -(uint32_t)(e >> 2 & 1), s3 = -(uint32_t)(e >> 3);
+            auto pick = [](uint32_t a, uint32_t b, uint32_t second) { return (a & ~second) | (b & second); };
+            auto of4 = [&](f4_t w) {
+                return pick(pick(__float_as_uint(w[0]), __float_as_uint(w[1]), s0),
+                            pick(__float_as_uint(w[2]), __float_as_uint(w[3]), s0), s1);
+            };
+            const float x = __uint_as_float(pick(pick(of4(v[0]), of4(v[1]), s2), pick(of4(v[2]), of4(v[3]), s2), s3));
+            best.offer(may ? key_of(x, at + e / 4 * 256 + lane * 4 + e % 4) : 0);
+        }
     }
-    t = gather(t, best, held, counts, sums);
+    t = gather(t, best, sh);
     if (a.S == 1) {
-        finish(a, row, t, best);
+        finish(a, row, t, sh);
         return;
     }
     const size_t me = blockIdx.x;
     if (threadIdx.x == 0) *(f4_t*)(a.part + me * 4) = f4_t{t.m, t.s, t.e, 0.f};
-    if (wave == 0 && a.k) {
-        best.cut();
-        if (lane < a.k) a.keys[me * a.k + lane] = lane < best.n ? held[0][lane] : 0;
-    }
+    if (!a.k) return;
+    uint64_t key = 0;
+    int total;
+    const int rank = rank_of(sh, a.k, &key, &total);
+    if (rank < a.k) a.keys[me * a.k + rank] = key;
+    if ((int)threadIdx.x >= total && (int)threadIdx.x < a.k) a.keys[me * a.k + threadIdx.x] = 0;
 }
 
 // The shares of a row joined.
 __global__ __launch_bounds__(kWaves * 64) void logprobs_join(LogArgs a) {
-    __shared__ uint64_t held[kWaves][kHeld];
-    __shared__ int counts[kWaves];
-    __shared__ Sums sums[kWaves];
+    __shared__ Shared sh;
     const int tid = threadIdx.x, wave = tid >> 6;
     const size_t row = blockIdx.x;
-    Sums t{-__builtin_inff(), 0.f, 0.f};
-    for (int i = tid; i < a.S; i += kWaves * 64) {
-        const f4_t v = *(const f4_t*)(a.part + (row * a.S + i) * 4);
-        t = join(t, {v[0], v[1], v[2]});
+    const uint64_t* keys = a.keys + row * a.S * a.k;
+    const int n = a.S * a.k;
+    constexpr int kAll = kMaxShares * IBH_LOGPROBS_MAX_K / (kWaves * 64);
+    uint64_t key[kAll];
+#pragma unroll
+    for (int i = 0; i < kAll; i++) {
+        const int j = i * kWaves * 64 + tid;
+        key[i] = j < n ? keys[j] : 0;
     }
-    Best best{held[wave], 0, a.k, kNothing};
-    for (int i = 0; i < a.S * a.k; i += kWaves * 64) best.offer(i + tid < a.S * a.k ? a.keys[row * a.S * a.k + i + tid] : 0);
-    t = gather(t, best, held, counts, sums);
-    finish(a, row, t, best);
+    Sums t{-__builtin_inff(), 0.f, 0.f};
+    if (tid < a.S) {
+        const f4_t v = *(const f4_t*)(a.part + (row * a.S + tid) * 4);
+        t = {v[0], v[1], v[2]};
+    }
+    Best best{sh.held[wave], 0, a.k, kNothing};
+    if (a.k) {
+        uint64_t top = 0;
+#pragma unroll
+        for (int i = 0; i < kAll; i++) top = key[i] > top ? key[i] : top;
+        best.first((uint32_t)(top >> 32));
+#pragma unroll
+        for (int i = 0; i < kAll; i++)
+            if (i * kWaves * 64 < n) best.offer(key[i]);
+    }
+    t = gather(t, best, sh);
+    finish(a, row, t, sh);
 }
 
 // How a call is cut: a row's shares are whole rounds of a block's pieces, as
@@ -264,7 +339,7 @@ struct LogPlan {
 };
 LogPlan plan_of(int V, int B, int k) {
     LogPlan p;
-    const int round = kWaves * kPiece, rounds = (V + round - 1) / round;
+    const int round = kWaves * kPiece, rounds = (V + 3 + round - 1) / round;   // up to three in front of the row
     const int want = max(1, min(min(rounds, kMaxShares), (1024 + B - 1) / B));
     const int each = (rounds + want - 1) / want;
     p.seg = each * round;

@@ -92,7 +92,9 @@ __device__ __forceinline__ u4_t load8h(const uint16_t* p, int j, int n) {
 // memory once and from L2 by the others.
 struct Few {
     int id, rank, rows;             // rows 0: this block has nothing to do
-    int row[4];
+    int row[4];                     // by constants only: an array indexed by a variable would lie in LDS, and its place
+                                    // there be read off the dispatch packet in host memory, 10 us for 512 blocks
+    __device__ __forceinline__ int at(int i) const { return i == 0 ? row[0] : i == 1 ? row[1] : i == 2 ? row[2] : row[3]; }
 };
 __device__ __forceinline__ Few few_of(const Lora& l) {
     const int lane = threadIdx.x & 63, me = blockIdx.x;
@@ -156,7 +158,7 @@ __device__ __forceinline__ void shrink_rows(const Lora& l, const Few& f, int r0,
         const int r = tid / NR, i = tid % NR;
         const float s = (part[tid][0] + part[tid][1]) + (part[tid][2] + part[tid][3]);
         if (i < f.rows && r0 + r < l.Rp)
-            l.t[(size_t)f.row[i] * l.Rp + r0 + r] = r < nr ? s * (l.scales ? l.scales[f.id] : 1.f) : 0.f;
+            l.t[(size_t)f.at(i) * l.Rp + r0 + r] = r < nr ? s * (l.scales ? l.scales[f.id] : 1.f) : 0.f;
     }
 }
 
@@ -227,7 +229,7 @@ __global__ __launch_bounds__(256) void lora_expand_few(Lora l, int lg) {
         const int span = (256 >> lg) * kOut, m0 = blockIdx.y * span;
         for (int i = 0; i < f.rows; i++)
             for (int m = m0 + threadIdx.x; m < min(m0 + span, l.M); m += 256)
-                l.out[f.row[i] * l.os + m] = f.rank < 0 ? __builtin_nanf("") : l.base ? l.base[f.row[i] * l.bs + m] : 0.f;
+                l.out[f.at(i) * l.os + m] = f.rank < 0 ? __builtin_nanf("") : l.base ? l.base[f.at(i) * l.bs + m] : 0.f;
         return;
     }
     if (f.rows == 1) expand_rows<KIND, 1>(l, f, lg);
@@ -245,11 +247,38 @@ __global__ __launch_bounds__(1024) void lora_plan(Lora l) {
     const int tid = threadIdx.x, keys = l.n + 2;         // n: no adapter; n + 1: not in the table
     for (int i = tid; i < keys; i += 1024) count[i] = 0;
     __syncthreads();
-    auto key_of = [&](int row) {
-        const int id = l.ids[row], rank = rank_of(l, id);
+    auto key_of = [&](int id) {
+        const int rank = rank_of(l, id);
         return rank < 0 ? l.n + 1 : rank == 0 ? l.n : id;
     };
-    for (int i = tid; i < l.B; i += 1024) atomicAdd(&count[key_of(i)], 1);
+    // adds the wavefront's rows to the counters of their keys, -1 for none, and
+    // returns what each row found there: those that share the first row's key
+    // (packed prompts: all of them) in one addition
+    auto add = [&](int key) {
+        const int first = __builtin_amdgcn_readfirstlane(key), lane = tid & 63;
+        const uint64_t same = __ballot(key == first);
+        int got = 0;
+        if (key != first) {
+            if (key >= 0) got = atomicAdd(&count[key], 1);
+        } else if (first >= 0) {
+            if (lane == 0) got = atomicAdd(&count[first], __popcll(same));
+            got = __builtin_amdgcn_readfirstlane(got) + __popcll(same & ((1ull << lane) - 1));
+        }
+        return got;
+    };
+    // the first rows' keys stay in registers, their loads all under way at once
+    constexpr int kKept = 8;
+    int key[kKept];
+#pragma unroll
+    for (int u = 0; u < kKept; u++) key[u] = u * 1024 + tid < l.B ? l.ids[u * 1024 + tid] : 0;
+#pragma unroll
+    for (int u = 0; u < kKept; u++) key[u] = u * 1024 + tid < l.B ? key_of(key[u]) : -1;
+    const int later = kKept * 1024 + (tid & ~63);        // whole wavefronts go on together
+    auto late_key = [&](int i) { return i + (tid & 63) < l.B ? key_of(l.ids[i + (tid & 63)]) : -1; };
+#pragma unroll
+    for (int u = 0; u < kKept; u++)
+        if (u * 1024 < l.B) add(key[u]);
+    for (int i = later; i < l.B; i += 1024) add(late_key(i));
     __syncthreads();
     // each thread's run of keys: rows and tiles in front of it
     const int per = (keys + 1023) / 1024, k0 = min(tid * per, keys), k1 = min(k0 + per, keys);
@@ -278,7 +307,16 @@ __global__ __launch_bounds__(1024) void lora_plan(Lora l) {
     }
     __syncthreads();
     int32_t* order = l.plan + 4 + 4 * l.max_tiles;
-    for (int i = tid; i < l.B; i += 1024) order[atomicAdd(&count[key_of(i)], 1)] = i;
+#pragma unroll
+    for (int u = 0; u < kKept; u++)
+        if (u * 1024 < l.B) {
+            const int at = add(key[u]);
+            if (key[u] >= 0) order[at] = u * 1024 + tid;
+        }
+    for (int i = later; i < l.B; i += 1024) {
+        const int k = late_key(i), at = add(k);
+        if (k >= 0) order[at] = i + (tid & 63);
+    }
 }
 
 // fp32 numbers as bf16 numbers, upper halves cut off one after the other: 8
@@ -305,6 +343,13 @@ __device__ __forceinline__ void pieces(u4_t v, v8bf* p) {
         p[0] = __builtin_bit_cast(v8bf, hi);
         p[1] = __builtin_bit_cast(v8bf, lo);
     }
+}
+
+// A barrier that orders LDS alone: loads from memory stay under way across it.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // t of a tile of rows and RT * 16 ranks over a share of the columns.  Four
@@ -334,9 +379,7 @@ __global__ __launch_bounds__(256) void lora_shrink_tile(Lora l) {
         xrow[i] = l.x + order[there[i] ? r : 0] * l.xs;
     }
     const int xk = tid % 32 * 4, ak = tid % 16 * 8;
-    f4_t vx[4];
-    u4_t va[RT];
-    auto fetch = [&](int s) {
+    auto fetch = [&](int s, f4_t* vx, u4_t* va) {
 #pragma unroll
         for (int i = 0; i < 4; i++) vx[i] = there[i] ? load4(xrow[i], s * kStep + xk, l.N) : f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -348,8 +391,9 @@ __global__ __launch_bounds__(256) void lora_shrink_tile(Lora l) {
     v4f acc[RT];
 #pragma unroll
     for (int i = 0; i < RT; i++) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
-    if (s0 < s1) fetch(s0);
-    for (int s = s0; s < s1; s++) {
+    // a step's numbers go from registers to LDS, where those of the step after
+    // next take their place in the registers
+    auto step = [&](int s, f4_t* vx, u4_t* va) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int r = i * 8 + tid / 32;
@@ -368,8 +412,8 @@ __global__ __launch_bounds__(256) void lora_shrink_tile(Lora l) {
 #pragma unroll
             for (int j = 0; j < P; j++) *(v8bf*)&sa[j][i * 16 + tid / 16][ak] = p[j];
         }
-        __syncthreads();
-        if (s + 1 < s1) fetch(s + 1);
+        if (s + 2 < s1) fetch(s + 2, vx, va);
+        lds_barrier();
         const int c = wave % 2 * 16 + lane % 16, k0 = wave / 2 * 64 + lane / 16 * 8;
 #pragma unroll
         for (int k = 0; k < 64; k += 32) {
@@ -385,7 +429,15 @@ __global__ __launch_bounds__(256) void lora_shrink_tile(Lora l) {
                     for (int p = 0; p < 3; p++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ba, bx[p], acc[i], 0, 0, 0);
                 }
         }
-        __syncthreads();
+        lds_barrier();
+    };
+    f4_t x0[4], x1[4];
+    u4_t a0[RT], a1[RT];
+    if (s0 < s1) fetch(s0, x0, a0);
+    if (s0 + 1 < s1) fetch(s0 + 1, x1, a1);
+    for (int s = s0; s < s1; s += 2) {
+        step(s, x0, a0);
+        if (s + 1 < s1) step(s + 1, x1, a1);
     }
     // the second halves of the steps join the first; lane: row lane % 16 of the
     // tile, ranks lane / 16 * 4 .. + 3
@@ -409,7 +461,7 @@ __global__ __launch_bounds__(256) void lora_shrink_tile(Lora l) {
 // into pieces in LDS; a wavefront takes 64 outputs at a time, four matrix tiles
 // beside each other.
 template <int KIND>
-__global__ __launch_bounds__(256) void lora_expand_tile(Lora l) {
+__global__ __launch_bounds__(256, 3) void lora_expand_tile(Lora l) {
     constexpr int P = KIND == IBH_F16 ? 2 : 1;
     extern __shared__ __align__(16) uint16_t st[];       // [3][kTile][kr]
     const int tile = blockIdx.x;
@@ -446,18 +498,26 @@ __global__ __launch_bounds__(256) void lora_expand_tile(Lora l) {
         }
     }
     __syncthreads();
+    // Matrix tiles of 16 rows by 16 outputs, four beside each other: tile j holds
+    // outputs m0 + 4 c + j, so that a lane has four neighbouring ones of the rows
+    // 4 q + i, and 16 lanes read and write 256 bytes of a row.
     const int c = lane % 16, q = lane / 16;
-    int row[2];
+    int row[2][4];
 #pragma unroll
-    for (int h = 0; h < 2; h++) row[h] = h * 16 + c < tl.count ? order[h * 16 + c] : -1;
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int k = h * 16 + q * 4 + i;
+            row[h][i] = k < tl.count ? order[k] : -1;
+        }
     const uint16_t* b = l.b + (size_t)tl.id * l.M * l.R;
     for (int m0 = blockIdx.y * kChunk + wave * 64; m0 < m_end; m0 += 256) {
         f4_t y[2][4];
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                y[h][j] = l.base && row[h] >= 0 ? load4(l.base + row[h] * l.bs, m0 + 16 * j + 4 * q, l.M) : f4_t{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < 4; i++)
+                y[h][i] = l.base && row[h][i] >= 0 ? load4(l.base + row[h][i] * l.bs, m0 + 4 * c, l.M) : f4_t{0.f, 0.f, 0.f, 0.f};
         v4f acc[2][4];
 #pragma unroll
         for (int h = 0; h < 2; h++)
@@ -468,14 +528,14 @@ __global__ __launch_bounds__(256) void lora_expand_tile(Lora l) {
             u4_t w[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const int m = m0 + 16 * j + c;
+                const int m = m0 + 4 * c + j;
                 w[j] = m < l.M && r < tl.rank ? load8h(b + (size_t)m * l.R, r, tl.rank) : u4_t{0, 0, 0, 0};
             }
-            v8bf bt[2][3];
+            v8bf at[2][3];
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int p = 0; p < 3; p++) bt[h][p] = *(const v8bf*)&st[(p * kTile + h * 16 + c) * kr + r];
+                for (int p = 0; p < 3; p++) at[h][p] = *(const v8bf*)&st[(p * kTile + h * 16 + c) * kr + r];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 v8bf bw[2];
@@ -486,15 +546,16 @@ __global__ __launch_bounds__(256) void lora_expand_tile(Lora l) {
                     for (int h = 0; h < 2; h++)
 #pragma unroll
                         for (int p = 0; p < 3; p++)
-                            acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bw[i], bt[h][p], acc[h][j], 0, 0, 0);
+                            acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(at[h][p], bw[i], acc[h][j], 0, 0, 0);
             }
         }
 #pragma unroll
         for (int h = 0; h < 2; h++)
-            if (row[h] >= 0)
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    store4(l.out + row[h] * l.os, m0 + 16 * j + 4 * q, l.M, y[h][j] + acc[h][j]);
+            for (int i = 0; i < 4; i++)
+                if (row[h][i] >= 0)
+                    store4(l.out + row[h][i] * l.os, m0 + 4 * c, l.M,
+                           y[h][i] + f4_t{acc[h][0][i], acc[h][1][i], acc[h][2][i], acc[h][3][i]});
     }
 }
 
