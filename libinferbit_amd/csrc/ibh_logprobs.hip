@@ -224,24 +224,30 @@ __global__ __launch_bounds__(kWaves * 64, 8) void logprobs_kernel(LogArgs a) {
     const int v0 = share * a.seg - off, v1 = min(v0 + a.seg, a.V);
     Sums t{-__builtin_inff(), 0.f, 0.f};
     Best best{sh.held[wave], 0, a.k, kNothing};
+    // one piece ahead; a piece that is not whole reads single logits, -infinity
+    // for those outside the share
     f4_t next[4];
-    auto fetch = [&](int at) {
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const int j = at + q * 256 + lane * 4;
-            if (j >= 0 && j + 4 <= v1) next[q] = *(const f4_t*)(z + j);
-            else
-#pragma unroll
-                for (int i = 0; i < 4; i++) next[q][i] = j + i >= 0 && j + i < v1 ? z[j + i] : -__builtin_inff();
-        }
-    };
-    int at = v0 + wave * kPiece;
-    if (at < v1) fetch(at);
-    for (bool begin = true; at < v1; at += kWaves * kPiece, begin = false) {
+    bool begin = true;
+    auto from = [&](int j) { return (const char*)z + (uint32_t)(j * 4); };   // V is at most 2^30
+    for (int at = v0 + (wave - kWaves) * kPiece; at < v1; at += kWaves * kPiece) {
         f4_t v[4];
 #pragma unroll
         for (int q = 0; q < 4; q++) v[q] = next[q];
-        if (at + kWaves * kPiece < v1) fetch(at + kWaves * kPiece);
+        const int ahead = at + kWaves * kPiece;
+        if (ahead >= 0 && ahead + kPiece <= v1) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) next[q] = *(const f4_t*)(from(ahead + lane * 4) + q * 1024);
+        } else if (ahead < v1) {
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int j = ahead + q * 256 + lane * 4 + i;
+                    const float x = *(const float*)from(min(max(j, 0), v1 - 1));
+                    next[q][i] = j >= 0 && j < v1 ? x : -__builtin_inff();
+                }
+        }
+        if (at < v0) continue;
         float top = v[0][0];
 #pragma unroll
         for (int q = 0; q < 4; q++)
@@ -264,6 +270,7 @@ __global__ __launch_bounds__(kWaves * 64, 8) void logprobs_kernel(LogArgs a) {
         if (!a.k) continue;
         const uint32_t o = order_of(top);
         if (begin) best.first(top > -__builtin_inff() ? o : 0);
+        begin = false;
         if (!__ballot(o > (uint32_t)(best.bar >> 32))) continue;
         // each lane's own that may be above, one after the other (few: in
         // registers they are picked by halving, not by an index)

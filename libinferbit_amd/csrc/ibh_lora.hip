@@ -19,7 +19,6 @@ constexpr int kMaxAdapters = 8192;  // counters of the plan's block
 constexpr int kTile = 32;           // rows of one adapter that a block of the matrix kernels takes
 constexpr int kStep = 128;          // columns of x that it holds in LDS at a time
 constexpr int kMaxSplit = 16;       // blocks that share a tile's columns
-constexpr int kChunk = 512;         // outputs that a block of the second product takes
 
 typedef float f4_t __attribute__((ext_vector_type(4), aligned(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -40,11 +39,16 @@ struct Lora {
     float* t;                       // [split][B][Rp]: scale * A x of each row; zeros behind its adapter's rank
     int Rp;                         // R in whole eights
     int S;                          // splits
-    int32_t* plan;                  // {tiles}, then Tile [tiles], then the rows in their order
+    struct Tile* tiles;
     int max_tiles;
+    int chunk;                      // outputs that a block of the second product takes
 };
+// Rows of one adapter.  All that a block has to know in one place, so that it
+// waits for memory once before its first row.
 struct Tile {
-    int32_t id, rank, start, count; // id -1: no adapter; rank -1: not in the table
+    int32_t id, rank, count;        // rank -1: not in the table, 0: no adapter; count 0: no tile
+    float scale;
+    int32_t row[kTile];
 };
 
 template <int KIND>
@@ -59,30 +63,50 @@ __device__ __forceinline__ int rank_of(const Lora& l, int id) {
     const int r = l.ranks ? l.ranks[id] : l.R;
     return r < 0 || r > l.R ? -1 : r;
 }
+// Loads from place j of n, zeros behind n.  WHOLE: n is a multiple of what is
+// loaded, which leaves the code for a rest away (every line of code that a
+// small launch runs through is one more wait for memory).
+template <bool WHOLE>
 __device__ __forceinline__ f4_t load4(const float* p, int j, int N) {
     f4_t v = {0.f, 0.f, 0.f, 0.f};
-    if (j + 4 <= N) return *(const f4_t*)(p + j);
+    if (WHOLE ? j < N : j + 4 <= N) return *(const f4_t*)(p + j);
+    if constexpr (WHOLE) return v;
 #pragma unroll
     for (int i = 0; i < 4; i++)
         if (j + i < N) v[i] = p[j + i];
     return v;
 }
+template <bool WHOLE>
 __device__ __forceinline__ void store4(float* p, int j, int N, f4_t v) {
-    if (j + 4 <= N) {
+    if (WHOLE ? j < N : j + 4 <= N) {
         *(f4_t*)(p + j) = v;
         return;
     }
+    if constexpr (WHOLE) return;
 #pragma unroll
     for (int i = 0; i < 4; i++)
         if (j + i < N) p[j + i] = v[i];
 }
-// Eight 16-bit numbers from place j of n, zeros behind them.
+template <bool WHOLE>
 __device__ __forceinline__ u4_t load8h(const uint16_t* p, int j, int n) {
-    if (j + 8 <= n) return *(const u4h_t*)(p + j);
     u4_t v = {0, 0, 0, 0};
+    if (WHOLE ? j < n : j + 8 <= n) return *(const u4h_t*)(p + j);
+    if constexpr (WHOLE) return v;
 #pragma unroll
     for (int i = 0; i < 8; i++)
         if (j + i < n) v[i / 2] |= (uint32_t)p[j + i] << (16 * (i % 2));
+    return v;
+}
+// Numbers j .. j + 7 of a row of b, zeros from `rank` on.  WHOLE: the row is
+// whole eights, so all of them may be read.
+template <bool WHOLE>
+__device__ __forceinline__ u4_t load_rank(const uint16_t* p, int j, int rank) {
+    if constexpr (!WHOLE) return load8h<false>(p, j, rank);
+    u4_t v = {0, 0, 0, 0};
+    if (j < rank) v = *(const u4h_t*)(p + j);
+    if (j + 8 > rank)
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] &= (j + 2 * i < rank ? 0xffffu : 0) | (j + 2 * i + 1 < rank ? 0xffff0000u : 0);
     return v;
 }
 
@@ -117,7 +141,7 @@ __device__ __forceinline__ Few few_of(const Lora& l) {
 }
 
 // RR ranks of an adapter times NR rows: lanes take eights of columns.
-template <int KIND, int RR, int NR>
+template <int KIND, bool WHOLE, int RR, int NR>
 __device__ __forceinline__ void shrink_rows(const Lora& l, const Few& f, int r0, float (*part)[4]) {
     const int tid = threadIdx.x;
     const uint16_t* a = l.a + ((size_t)f.id * l.R + r0) * l.N;
@@ -132,11 +156,11 @@ __device__ __forceinline__ void shrink_rows(const Lora& l, const Few& f, int r0,
         u4_t w[RR];
         f4_t v[NR][2];
 #pragma unroll
-        for (int r = 0; r < RR; r++) w[r] = r < nr ? load8h(a + (size_t)r * l.N, j, l.N) : u4_t{0, 0, 0, 0};
+        for (int r = 0; r < RR; r++) w[r] = r < nr ? load8h<WHOLE>(a + (size_t)r * l.N, j, l.N) : u4_t{0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < NR; i++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) v[i][h] = load4(l.x + f.row[i] * l.xs, j + 4 * h, l.N);
+            for (int h = 0; h < 2; h++) v[i][h] = load4<WHOLE>(l.x + f.row[i] * l.xs, j + 4 * h, l.N);
 #pragma unroll
         for (int r = 0; r < RR; r++)
 #pragma unroll
@@ -162,20 +186,20 @@ __device__ __forceinline__ void shrink_rows(const Lora& l, const Few& f, int r0,
     }
 }
 
-template <int KIND>
+template <int KIND, bool WHOLE>
 __global__ __launch_bounds__(256) void lora_shrink_few(Lora l) {
     __shared__ float part[16][4];
     const Few f = few_of(l);
     const int r0 = blockIdx.y * 4;
     if (!f.rows || f.rank <= 0 || r0 >= (f.rank + 7) / 8 * 8) return;
-    if (f.rows == 1) shrink_rows<KIND, 4, 1>(l, f, r0, part);
-    else if (f.rows == 2) shrink_rows<KIND, 4, 2>(l, f, r0, part);
-    else shrink_rows<KIND, 4, 4>(l, f, r0, part);
+    if (f.rows == 1) shrink_rows<KIND, WHOLE, 4, 1>(l, f, r0, part);
+    else if (f.rows == 2) shrink_rows<KIND, WHOLE, 4, 2>(l, f, r0, part);
+    else shrink_rows<KIND, WHOLE, 4, 4>(l, f, r0, part);
 }
 
 // A row of b in `1 << lg` lanes, eight numbers each; kOut outputs a lane group.
 constexpr int kOut = 2;
-template <int KIND, int NR>
+template <int KIND, bool WHOLE, int NR>
 __device__ __forceinline__ void expand_rows(const Lora& l, const Few& f, int lg) {
     const int sub = threadIdx.x & ((1 << lg) - 1), per = 256 >> lg, r0 = 8 * sub;
     const int m0 = blockIdx.y * per * kOut + (threadIdx.x >> lg);
@@ -184,7 +208,7 @@ __device__ __forceinline__ void expand_rows(const Lora& l, const Few& f, int lg)
 #pragma unroll
     for (int o = 0; o < kOut; o++) {
         const int m = m0 + o * per;
-        w[o] = m < l.M && r0 < f.rank ? load8h(b + (size_t)m * l.R, r0, f.rank) : u4_t{0, 0, 0, 0};
+        w[o] = m < l.M ? load_rank<WHOLE>(b + (size_t)m * l.R, r0, f.rank) : u4_t{0, 0, 0, 0};
     }
     f4_t t[NR][2];
     float y[kOut][NR];
@@ -219,7 +243,7 @@ __device__ __forceinline__ void expand_rows(const Lora& l, const Few& f, int lg)
     }
 }
 
-template <int KIND>
+template <int KIND, bool WHOLE>
 __global__ __launch_bounds__(256) void lora_expand_few(Lora l, int lg) {
     const Few f = few_of(l);
     if (!f.rows) return;
@@ -232,9 +256,9 @@ __global__ __launch_bounds__(256) void lora_expand_few(Lora l, int lg) {
                 l.out[f.at(i) * l.os + m] = f.rank < 0 ? __builtin_nanf("") : l.base ? l.base[f.at(i) * l.bs + m] : 0.f;
         return;
     }
-    if (f.rows == 1) expand_rows<KIND, 1>(l, f, lg);
-    else if (f.rows == 2) expand_rows<KIND, 2>(l, f, lg);
-    else expand_rows<KIND, 4>(l, f, lg);
+    if (f.rows == 1) expand_rows<KIND, WHOLE, 1>(l, f, lg);
+    else if (f.rows == 2) expand_rows<KIND, WHOLE, 2>(l, f, lg);
+    else expand_rows<KIND, WHOLE, 4>(l, f, lg);
 }
 
 // ── more rows: tiles of one adapter's rows on the matrix cores ───────────────
@@ -243,7 +267,7 @@ __global__ __launch_bounds__(256) void lora_expand_few(Lora l, int lg) {
 // place) and cuts each adapter's rows into tiles.
 __global__ __launch_bounds__(1024) void lora_plan(Lora l) {
     __shared__ int32_t count[kMaxAdapters + 2];
-    __shared__ int32_t wave_rows[16], wave_tiles[16];
+    __shared__ int32_t wave_tiles[16];
     const int tid = threadIdx.x, keys = l.n + 2;         // n: no adapter; n + 1: not in the table
     for (int i = tid; i < keys; i += 1024) count[i] = 0;
     __syncthreads();
@@ -280,42 +304,45 @@ __global__ __launch_bounds__(1024) void lora_plan(Lora l) {
         if (u * 1024 < l.B) add(key[u]);
     for (int i = later; i < l.B; i += 1024) add(late_key(i));
     __syncthreads();
-    // each thread's run of keys: rows and tiles in front of it
+    // each thread's run of keys: tiles in front of it
     const int per = (keys + 1023) / 1024, k0 = min(tid * per, keys), k1 = min(k0 + per, keys);
-    int rows = 0, tiles = 0;
-    for (int k = k0; k < k1; k++) {
-        rows += count[k];
-        tiles += (count[k] + kTile - 1) / kTile;
-    }
-    int ir = rows, it = tiles;
+    int tiles = 0;
+    for (int k = k0; k < k1; k++) tiles += (count[k] + kTile - 1) / kTile;
+    int it = tiles;
     for (int o = 1; o < 64; o <<= 1) {
-        const int pr = __shfl_up(ir, o, 64), pt = __shfl_up(it, o, 64);
-        if ((tid & 63) >= o) ir += pr, it += pt;
+        const int p = __shfl_up(it, o, 64);
+        if ((tid & 63) >= o) it += p;
     }
-    if ((tid & 63) == 63) wave_rows[tid >> 6] = ir, wave_tiles[tid >> 6] = it;
+    if ((tid & 63) == 63) wave_tiles[tid >> 6] = it;
     __syncthreads();
-    ir -= rows;
     it -= tiles;
-    for (int w = 0; w < (tid >> 6); w++) ir += wave_rows[w], it += wave_tiles[w];
-    if (tid == 1023) l.plan[0] = it + tiles;
-    Tile* out = (Tile*)(l.plan + 4);
-    for (int k = k0; k < k1; k++) {
-        const int c = count[k], rank = k < l.n ? (l.ranks ? l.ranks[k] : l.R) : l.n - k;
-        count[k] = ir;                                   // from here on: where its next row goes
-        for (int j = 0; j < c; j += kTile) out[it++] = {k < l.n ? k : -1, rank, ir + j, min(kTile, c - j)};
-        ir += c;
+    int all = 0;
+    for (int w = 0; w < 16; w++) {
+        if (w == tid >> 6) it += all;
+        all += wave_tiles[w];
     }
+    for (int k = k0; k < k1; k++) {
+        const int c = count[k];
+        if (!c) continue;
+        const int rank = k < l.n ? (l.ranks ? l.ranks[k] : l.R) : l.n - k;
+        const float scale = k < l.n && l.scales ? l.scales[k] : 1.f;
+        count[k] = it * kTile;                           // from here on: the place of its next row
+        for (int j = 0; j < c; j += kTile, it++) {
+            Tile& t = l.tiles[it];
+            t.id = k, t.rank = rank, t.count = min(kTile, c - j), t.scale = scale;
+        }
+    }
+    for (int i = all + tid; i < l.max_tiles; i += 1024) l.tiles[i].count = 0;
     __syncthreads();
-    int32_t* order = l.plan + 4 + 4 * l.max_tiles;
 #pragma unroll
     for (int u = 0; u < kKept; u++)
         if (u * 1024 < l.B) {
             const int at = add(key[u]);
-            if (key[u] >= 0) order[at] = u * 1024 + tid;
+            if (key[u] >= 0) l.tiles[at / kTile].row[at % kTile] = u * 1024 + tid;
         }
     for (int i = later; i < l.B; i += 1024) {
         const int k = late_key(i), at = add(k);
-        if (k >= 0) order[at] = i + (tid & 63);
+        if (k >= 0) l.tiles[at / kTile].row[at % kTile] = i + (tid & 63);
     }
 }
 
@@ -354,18 +381,19 @@ __device__ __forceinline__ void lds_barrier() {
 
 // t of a tile of rows and RT * 16 ranks over a share of the columns.  Four
 // wavefronts: 16 rows each, and half of each step's columns.
-template <int KIND, int RT>
+template <int KIND, bool WHOLE, int RT>
 __global__ __launch_bounds__(256) void lora_shrink_tile(Lora l) {
     constexpr int P = KIND == IBH_F16 ? 2 : 1, kRow = kStep + 8;   // 272 bytes: 16 rows on all banks
     __shared__ __align__(16) uint16_t sx[3][kTile][kRow];
     __shared__ __align__(16) uint16_t sa[P][RT * 16][kRow];
-    const int tile = blockIdx.x;
-    if (tile >= l.plan[0]) return;
-    const Tile tl = ((const Tile*)(l.plan + 4))[tile];
-    const int r0 = blockIdx.z * RT * 16;
-    if (r0 >= (tl.rank + 7) / 8 * 8) return;
-    const int32_t* order = l.plan + 4 + 4 * l.max_tiles + tl.start;
+    const Tile& tl = l.tiles[blockIdx.x];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int rows[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) rows[i] = tl.row[i * 8 + tid / 32];
+    const int id = tl.id, rank = tl.rank, count = tl.count, r0 = blockIdx.z * RT * 16;
+    const float scale = tl.scale;
+    if (!count || r0 >= (rank + 7) / 8 * 8) return;
     const int steps = (l.N + kStep - 1) / kStep;
     const int s0 = (int)((int64_t)steps * blockIdx.y / l.S), s1 = (int)((int64_t)steps * (blockIdx.y + 1) / l.S);
 
@@ -374,18 +402,17 @@ __global__ __launch_bounds__(256) void lora_shrink_tile(Lora l) {
     bool there[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const int r = i * 8 + tid / 32;
-        there[i] = r < tl.count;
-        xrow[i] = l.x + order[there[i] ? r : 0] * l.xs;
+        there[i] = i * 8 + tid / 32 < count;
+        xrow[i] = l.x + (there[i] ? rows[i] : 0) * l.xs;
     }
     const int xk = tid % 32 * 4, ak = tid % 16 * 8;
     auto fetch = [&](int s, f4_t* vx, u4_t* va) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) vx[i] = there[i] ? load4(xrow[i], s * kStep + xk, l.N) : f4_t{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 4; i++) vx[i] = there[i] ? load4<WHOLE>(xrow[i], s * kStep + xk, l.N) : f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < RT; i++) {
             const int r = r0 + i * 16 + tid / 16;
-            va[i] = r < tl.rank ? load8h(l.a + ((size_t)tl.id * l.R + r) * l.N, s * kStep + ak, l.N) : u4_t{0, 0, 0, 0};
+            va[i] = r < rank ? load8h<WHOLE>(l.a + ((size_t)id * l.R + r) * l.N, s * kStep + ak, l.N) : u4_t{0, 0, 0, 0};
         }
     };
     v4f acc[RT];
@@ -447,9 +474,8 @@ __global__ __launch_bounds__(256) void lora_shrink_tile(Lora l) {
         for (int i = 0; i < RT; i++) join[((wave - 2) * RT + i) * 64 + lane] = acc[i];
     __syncthreads();
     const int c = wave * 16 + lane % 16;
-    if (wave >= 2 || c >= tl.count) return;
-    const float scale = l.scales ? l.scales[tl.id] : 1.f;
-    float* t = l.t + ((size_t)blockIdx.y * l.B + order[c]) * l.Rp;
+    if (wave >= 2 || c >= count) return;
+    float* t = l.t + ((size_t)blockIdx.y * l.B + tl.row[c]) * l.Rp;
 #pragma unroll
     for (int i = 0; i < RT; i++) {
         const int r = r0 + i * 16 + lane / 16 * 4;
@@ -457,42 +483,51 @@ __global__ __launch_bounds__(256) void lora_shrink_tile(Lora l) {
     }
 }
 
-// out of a tile of rows and kChunk outputs.  t's splits are added up and cut
+// out of a tile of rows and `chunk` outputs.  t's splits are added up and cut
 // into pieces in LDS; a wavefront takes 64 outputs at a time, four matrix tiles
 // beside each other.
-template <int KIND>
+template <int KIND, bool WHOLE>
 __global__ __launch_bounds__(256, 3) void lora_expand_tile(Lora l) {
     constexpr int P = KIND == IBH_F16 ? 2 : 1;
     extern __shared__ __align__(16) uint16_t st[];       // [3][kTile][kr]
-    const int tile = blockIdx.x;
-    if (tile >= l.plan[0]) return;
-    const Tile tl = ((const Tile*)(l.plan + 4))[tile];
-    const int32_t* order = l.plan + 4 + 4 * l.max_tiles + tl.start;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int m_end = min((int)(blockIdx.y + 1) * kChunk, l.M);
-    if (tl.rank <= 0) {                                  // no adapter: base; not in the table: NaN
-        if (tl.rank < 0 && tid == 0 && blockIdx.y == 0) atomicOr(&ibh_lora_err, IBH_DEVERR_LORA);
-        if (tl.rank == 0 && l.out == l.base) return;
-        for (int i = wave; i < tl.count; i += 4) {
-            const int row = order[i];
-            for (int m = blockIdx.y * kChunk + lane * 4; m < m_end; m += 256) {
+    const Tile& tl = l.tiles[blockIdx.x];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane % 16, q = lane / 16;
+    const int id = tl.id, rank = tl.rank, count = tl.count, m_begin = blockIdx.y * l.chunk, m_end = min(m_begin + l.chunk, l.M);
+    int row[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int k = h * 16 + q * 4 + i, at = tl.row[k];
+            row[h][i] = k < count ? at : -1;
+        }
+    if (!count) return;
+    if (rank <= 0) {                                     // no adapter: base; not in the table: NaN
+        if (rank < 0 && tid == 0 && blockIdx.y == 0) atomicOr(&ibh_lora_err, IBH_DEVERR_LORA);
+        if (rank == 0 && l.out == l.base) return;
+        for (int i = wave; i < count; i += 4) {
+            const size_t at = tl.row[i];
+            for (int m = m_begin + lane * 4; m < m_end; m += 256) {
                 const float nan = __builtin_nanf("");
-                store4(l.out + row * l.os, m, l.M, tl.rank < 0 ? f4_t{nan, nan, nan, nan} :
-                       l.base ? load4(l.base + row * l.bs, m, l.M) : f4_t{0.f, 0.f, 0.f, 0.f});
+                store4<WHOLE>(l.out + at * l.os, m, l.M, rank < 0 ? f4_t{nan, nan, nan, nan} :
+                              l.base ? load4<WHOLE>(l.base + at * l.bs, m, l.M) : f4_t{0.f, 0.f, 0.f, 0.f});
             }
         }
         return;
     }
-    const int ks = (tl.rank + 31) / 32, kr = ks * 32 + 8;
+    const int ks = (rank + 31) / 32, kr = ks * 32 + 8;
     for (int i = tid; i < kTile * ks * 8; i += 256) {
-        const int c = i / (ks * 8), r = i % (ks * 8) * 4;
+        const int k = i / (ks * 8), r = i % (ks * 8) * 4;
         v4f v = {0.f, 0.f, 0.f, 0.f};
-        if (c < tl.count && r < (tl.rank + 7) / 8 * 8)
-            for (int s = 0; s < l.S; s++) v += *(const v4f*)(l.t + ((size_t)s * l.B + order[c]) * l.Rp + r);
+        if (k < count && r < (rank + 7) / 8 * 8) {
+            const float* t = l.t + (size_t)tl.row[k] * l.Rp + r;
+#pragma unroll 4
+            for (int s = 0; s < l.S; s++) v += *(const v4f*)(t + (size_t)s * l.B * l.Rp);
+        }
         float e[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
         for (int p = 0; p < 3; p++) {
-            *(uint2*)&st[(p * kTile + c) * kr + r] = make_uint2(upper(e[0], e[1]), upper(e[2], e[3]));
+            *(uint2*)&st[(p * kTile + k) * kr + r] = make_uint2(upper(e[0], e[1]), upper(e[2], e[3]));
 #pragma unroll
             for (int q = 0; q < 4; q++) e[q] = below(e[q]);
         }
@@ -501,23 +536,14 @@ __global__ __launch_bounds__(256, 3) void lora_expand_tile(Lora l) {
     // Matrix tiles of 16 rows by 16 outputs, four beside each other: tile j holds
     // outputs m0 + 4 c + j, so that a lane has four neighbouring ones of the rows
     // 4 q + i, and 16 lanes read and write 256 bytes of a row.
-    const int c = lane % 16, q = lane / 16;
-    int row[2][4];
-#pragma unroll
-    for (int h = 0; h < 2; h++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int k = h * 16 + q * 4 + i;
-            row[h][i] = k < tl.count ? order[k] : -1;
-        }
-    const uint16_t* b = l.b + (size_t)tl.id * l.M * l.R;
-    for (int m0 = blockIdx.y * kChunk + wave * 64; m0 < m_end; m0 += 256) {
+    const uint16_t* b = l.b + (size_t)id * l.M * l.R;
+    for (int m0 = m_begin + wave * 64; m0 < m_end; m0 += 256) {
         f4_t y[2][4];
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                y[h][i] = l.base && row[h][i] >= 0 ? load4(l.base + row[h][i] * l.bs, m0 + 4 * c, l.M) : f4_t{0.f, 0.f, 0.f, 0.f};
+                y[h][i] = l.base && row[h][i] >= 0 ? load4<WHOLE>(l.base + row[h][i] * l.bs, m0 + 4 * c, l.M) : f4_t{0.f, 0.f, 0.f, 0.f};
         v4f acc[2][4];
 #pragma unroll
         for (int h = 0; h < 2; h++)
@@ -529,7 +555,7 @@ __global__ __launch_bounds__(256, 3) void lora_expand_tile(Lora l) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int m = m0 + 4 * c + j;
-                w[j] = m < l.M && r < tl.rank ? load8h(b + (size_t)m * l.R, r, tl.rank) : u4_t{0, 0, 0, 0};
+                w[j] = m < l.M ? load_rank<WHOLE>(b + (size_t)m * l.R, r, rank) : u4_t{0, 0, 0, 0};
             }
             v8bf at[2][3];
 #pragma unroll
@@ -554,7 +580,7 @@ __global__ __launch_bounds__(256, 3) void lora_expand_tile(Lora l) {
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 if (row[h][i] >= 0)
-                    store4(l.out + row[h][i] * l.os, m0 + 4 * c, l.M,
+                    store4<WHOLE>(l.out + row[h][i] * l.os, m0 + 4 * c, l.M,
                            y[h][i] + f4_t{acc[h][0][i], acc[h][1][i], acc[h][2][i], acc[h][3][i]});
     }
 }
@@ -575,7 +601,7 @@ bool adapters_ok(const ibh_lora_adapters* l, const char* who) {
 // How a call is cut.
 struct LoraPlan {
     bool few;
-    int Rp, S, max_tiles;
+    int Rp, S, max_tiles, chunk;
     size_t plan_bytes, bytes;
 };
 LoraPlan plan_of(const ibh_lora_adapters* l, int B) {
@@ -585,37 +611,49 @@ LoraPlan plan_of(const ibh_lora_adapters* l, int B) {
     p.S = 1;
     p.max_tiles = 0;
     p.plan_bytes = 0;
+    p.chunk = 0;
     if (!p.few) {
         const int groups = min(l->n + 2, B);
         p.max_tiles = B / kTile + groups;
-        p.plan_bytes = (16 + 16 * (size_t)p.max_tiles + 4 * (size_t)B + 15) / 16 * 16;
+        p.plan_bytes = sizeof(Tile) * (size_t)p.max_tiles;
         const int tiles = (B + kTile - 1) / kTile + min(l->n, B) / 2;
         p.S = max(1, min(min(kMaxSplit, (l->N + 511) / 512), 768 / tiles));
+        p.chunk = tiles * (l->M / 1024) >= 512 ? 1024 : tiles * (l->M / 512) >= 256 ? 512 : 256;
     }
     p.bytes = p.plan_bytes + (size_t)p.S * B * p.Rp * 4;
     return p;
 }
 
-template <int KIND>
-int launch(const Lora& l, bool few, hipStream_t st) {
+template <int KIND, bool WHOLE>
+void launch_shrink(const Lora& l, bool few, hipStream_t st) {
+    const dim3 grid(l.max_tiles, l.S, (l.R + 63) / 64);
+    if (few) lora_shrink_few<KIND, WHOLE><<<dim3(l.B, (l.Rp + 3) / 4), 256, 0, st>>>(l);
+    else if (l.R <= 16) lora_shrink_tile<KIND, WHOLE, 1><<<grid, 256, 0, st>>>(l);
+    else if (l.R <= 32) lora_shrink_tile<KIND, WHOLE, 2><<<grid, 256, 0, st>>>(l);
+    else lora_shrink_tile<KIND, WHOLE, 4><<<grid, 256, 0, st>>>(l);
+}
+template <int KIND, bool WHOLE>
+void launch_expand(const Lora& l, bool few, hipStream_t st) {
     if (few) {
         int lg = 0;
         while (8 << lg < l.R) lg++;
         const int span = (256 >> lg) * kOut;
-        lora_shrink_few<KIND><<<dim3(l.B, (l.Rp + 3) / 4), 256, 0, st>>>(l);
+        lora_expand_few<KIND, WHOLE><<<dim3(l.B, (l.M + span - 1) / span), 256, 0, st>>>(l, lg);
+    } else
+        lora_expand_tile<KIND, WHOLE><<<dim3(l.max_tiles, (l.M + l.chunk - 1) / l.chunk), 256,
+                                        3 * kTile * ((l.R + 31) / 32 * 32 + 8) * 2, st>>>(l);
+}
+template <int KIND>
+int launch(const Lora& l, bool few, hipStream_t st) {
+    if (!few) {
+        lora_plan<<<1, 1024, 0, st>>>(l);
         IBH_CHECK_LAUNCH("ibh_lora");
-        lora_expand_few<KIND><<<dim3(l.B, (l.M + span - 1) / span), 256, 0, st>>>(l, lg);
-        IBH_CHECK_LAUNCH("ibh_lora");
-        return IBH_OK;
     }
-    lora_plan<<<1, 1024, 0, st>>>(l);
+    if (l.N % 8 == 0) launch_shrink<KIND, true>(l, few, st);
+    else launch_shrink<KIND, false>(l, few, st);
     IBH_CHECK_LAUNCH("ibh_lora");
-    if (l.R <= 16) lora_shrink_tile<KIND, 1><<<dim3(l.max_tiles, l.S), 256, 0, st>>>(l);
-    else if (l.R <= 32) lora_shrink_tile<KIND, 2><<<dim3(l.max_tiles, l.S), 256, 0, st>>>(l);
-    else lora_shrink_tile<KIND, 4><<<dim3(l.max_tiles, l.S, (l.R + 63) / 64), 256, 0, st>>>(l);
-    IBH_CHECK_LAUNCH("ibh_lora");
-    lora_expand_tile<KIND><<<dim3(l.max_tiles, (l.M + kChunk - 1) / kChunk), 256,
-                             3 * kTile * ((l.R + 31) / 32 * 32 + 8) * 2, st>>>(l);
+    if (l.R % 8 == 0 && l.M % 4 == 0) launch_expand<KIND, true>(l, few, st);
+    else launch_expand<KIND, false>(l, few, st);
     IBH_CHECK_LAUNCH("ibh_lora");
     return IBH_OK;
 }
@@ -659,7 +697,7 @@ extern "C" int ibh_lora(const ibh_lora_adapters* l, float* out, const float* bas
     }
     const LoraPlan p = plan_of(l, B);
     // a launch takes less than 2^32 threads
-    if (!p.few && (size_t)p.max_tiles * max((l->M + kChunk - 1) / kChunk, p.S * ((l->rank + 63) / 64)) >= (1 << 24)) {
+    if (!p.few && (size_t)p.max_tiles * max((l->M + p.chunk - 1) / p.chunk, p.S * ((l->rank + 63) / 64)) >= (1 << 24)) {
         ibh_set_error("ibh_lora: %d rows are more than one launch takes", B);
         return IBH_ERROR_PARAM;
     }
@@ -670,7 +708,7 @@ extern "C" int ibh_lora(const ibh_lora_adapters* l, float* out, const float* bas
     }
     const Lora a{(const uint16_t*)l->a, (const uint16_t*)l->b, l->scales, l->ranks, l->n, l->rank, l->N, l->M, out, base, x,
                  ids, B, (size_t)out_stride, (size_t)base_stride, (size_t)x_stride, (float*)(w + p.plan_bytes), p.Rp, p.S,
-                 (int32_t*)w, p.max_tiles};
+                 (Tile*)w, p.max_tiles, p.chunk};
     hipStream_t st = ibh_resolve_stream(stream);
     return l->kind == IBH_F16 ? launch<IBH_F16>(a, p.few, st) : launch<IBH_BF16>(a, p.few, st);
 }
