@@ -17,7 +17,8 @@ __device__ unsigned int ibh_lora_err;
 constexpr int kFew = 64;            // rows up to which a wavefront holds all ids, one a lane
 constexpr int kMaxAdapters = 8192;  // counters of the plan's block
 constexpr int kTile = 32;           // rows of one adapter that a block of the matrix kernels takes
-constexpr int kStep = 128;          // columns of x that it holds in LDS at a time
+constexpr int kStep = 64;           // columns of x that a wavefront takes at a time
+constexpr int kSpan = 256;          // outputs that a block of the second product takes
 constexpr int kMaxSplit = 16;       // blocks that share a tile's columns
 
 typedef float f4_t __attribute__((ext_vector_type(4), aligned(4)));
@@ -41,7 +42,6 @@ struct Lora {
     int S;                          // splits
     struct Tile* tiles;
     int max_tiles;
-    int chunk;                      // outputs that a block of the second product takes
 };
 // Rows of one adapter.  All that a block has to know in one place, so that it
 // waits for memory once before its first row.
@@ -66,10 +66,11 @@ __device__ __forceinline__ int rank_of(const Lora& l, int id) {
 // Loads from place j of n, zeros behind n.  WHOLE: n is a multiple of what is
 // loaded, which leaves the code for a rest away (every line of code that a
 // small launch runs through is one more wait for memory).
+// x, base and out pass by once, past what the caches hold of the adapters.
 template <bool WHOLE>
 __device__ __forceinline__ f4_t load4(const float* p, int j, int N) {
     f4_t v = {0.f, 0.f, 0.f, 0.f};
-    if (WHOLE ? j < N : j + 4 <= N) return *(const f4_t*)(p + j);
+    if (WHOLE ? j < N : j + 4 <= N) return __builtin_nontemporal_load((const f4_t*)(p + j));
     if constexpr (WHOLE) return v;
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -379,140 +380,132 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// t of a tile of rows and RT * 16 ranks over a share of the columns.  Four
-// wavefronts: 16 rows each, and half of each step's columns.
+// t of a tile of rows and RT * 16 ranks over a share of the columns.  Each
+// wavefront takes 64 columns of all rows at a time, the next 64 under way: every
+// number of x is loaded, cut into pieces and multiplied by one lane, straight in
+// the matrix instructions' own order (16 rows, 32 columns in eights).
 template <int KIND, bool WHOLE, int RT>
-__global__ __launch_bounds__(256) void lora_shrink_tile(Lora l) {
-    constexpr int P = KIND == IBH_F16 ? 2 : 1, kRow = kStep + 8;   // 272 bytes: 16 rows on all banks
-    __shared__ __align__(16) uint16_t sx[3][kTile][kRow];
-    __shared__ __align__(16) uint16_t sa[P][RT * 16][kRow];
-    const Tile& tl = l.tiles[blockIdx.x];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int rows[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) rows[i] = tl.row[i * 8 + tid / 32];
+__global__ __launch_bounds__(256, RT <= 2 ? 3 : 2) void lora_shrink_tile(Lora l) {
+    constexpr int P = KIND == IBH_F16 ? 2 : 1;
+    __shared__ v4f join[4][2 * RT][64];
+    const Tile& tl = l.tiles[blockIdx.y];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane % 16, q = lane / 16;
+    int row[2] = {tl.row[c], tl.row[16 + c]};
     const int id = tl.id, rank = tl.rank, count = tl.count, r0 = blockIdx.z * RT * 16;
     const float scale = tl.scale;
     if (!count || r0 >= (rank + 7) / 8 * 8) return;
     const int steps = (l.N + kStep - 1) / kStep;
-    const int s0 = (int)((int64_t)steps * blockIdx.y / l.S), s1 = (int)((int64_t)steps * (blockIdx.y + 1) / l.S);
-
-    // loads: 32 lanes a row of x, 16 lanes a row of a
-    const float* xrow[4];
-    bool there[4];
+    const int s0 = (int)((int64_t)steps * blockIdx.x / l.S), s1 = (int)((int64_t)steps * (blockIdx.x + 1) / l.S);
+    // Places of the tile without a row, and ranks that the adapter has not, load
+    // another's: what comes of them is not stored.
+    const float* xp[2];
+    const uint16_t* ap[RT];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        there[i] = i * 8 + tid / 32 < count;
-        xrow[i] = l.x + (there[i] ? rows[i] : 0) * l.xs;
-    }
-    const int xk = tid % 32 * 4, ak = tid % 16 * 8;
-    auto fetch = [&](int s, f4_t* vx, u4_t* va) {
+    for (int h = 0; h < 2; h++) xp[h] = l.x + (h * 16 + c < count ? row[h] : tl.row[0]) * l.xs;
 #pragma unroll
-        for (int i = 0; i < 4; i++) vx[i] = there[i] ? load4<WHOLE>(xrow[i], s * kStep + xk, l.N) : f4_t{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < RT; i++) ap[i] = l.a + ((size_t)id * l.R + min(r0 + i * 16 + c, rank - 1)) * l.N;
+    struct Piece {
+        f4_t x[2][2][2];
+        u4_t a[RT][2];
+    };
+    auto fetch = [&](int s, Piece& p) {
+        const int k0 = s * kStep + q * 8;
 #pragma unroll
-        for (int i = 0; i < RT; i++) {
-            const int r = r0 + i * 16 + tid / 16;
-            va[i] = r < rank ? load8h<WHOLE>(l.a + ((size_t)id * l.R + r) * l.N, s * kStep + ak, l.N) : u4_t{0, 0, 0, 0};
+        for (int k = 0; k < 2; k++) {
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) p.x[h][k][e] = load4<WHOLE>(xp[h], k0 + 32 * k + 4 * e, l.N);
+#pragma unroll
+            for (int i = 0; i < RT; i++) p.a[i][k] = load8h<WHOLE>(ap[i], k0 + 32 * k, l.N);
         }
     };
-    v4f acc[RT];
-#pragma unroll
-    for (int i = 0; i < RT; i++) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
-    // a step's numbers go from registers to LDS, where those of the step after
-    // next take their place in the registers
-    auto step = [&](int s, f4_t* vx, u4_t* va) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = i * 8 + tid / 32;
-            float v[4] = {vx[i][0], vx[i][1], vx[i][2], vx[i][3]};
-#pragma unroll
-            for (int p = 0; p < 3; p++) {
-                *(uint2*)&sx[p][r][xk] = make_uint2(upper(v[0], v[1]), upper(v[2], v[3]));
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = below(v[e]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < RT; i++) {
-            v8bf p[2];
-            pieces<KIND>(va[i], p);
-#pragma unroll
-            for (int j = 0; j < P; j++) *(v8bf*)&sa[j][i * 16 + tid / 16][ak] = p[j];
-        }
-        if (s + 2 < s1) fetch(s + 2, vx, va);
-        lds_barrier();
-        const int c = wave % 2 * 16 + lane % 16, k0 = wave / 2 * 64 + lane / 16 * 8;
-#pragma unroll
-        for (int k = 0; k < 64; k += 32) {
-            v8bf bx[3];
-#pragma unroll
-            for (int p = 0; p < 3; p++) bx[p] = *(const v8bf*)&sx[p][c][k0 + k];
-#pragma unroll
-            for (int i = 0; i < RT; i++)
-#pragma unroll
-                for (int j = 0; j < P; j++) {
-                    const v8bf ba = *(const v8bf*)&sa[j][i * 16 + lane % 16][k0 + k];
-#pragma unroll
-                    for (int p = 0; p < 3; p++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ba, bx[p], acc[i], 0, 0, 0);
-                }
-        }
-        lds_barrier();
-    };
-    f4_t x0[4], x1[4];
-    u4_t a0[RT], a1[RT];
-    if (s0 < s1) fetch(s0, x0, a0);
-    if (s0 + 1 < s1) fetch(s0 + 1, x1, a1);
-    for (int s = s0; s < s1; s += 2) {
-        step(s, x0, a0);
-        if (s + 1 < s1) step(s + 1, x1, a1);
-    }
-    // the second halves of the steps join the first; lane: row lane % 16 of the
-    // tile, ranks lane / 16 * 4 .. + 3
-    v4f* join = (v4f*)sx;
-    if (wave >= 2)
-#pragma unroll
-        for (int i = 0; i < RT; i++) join[((wave - 2) * RT + i) * 64 + lane] = acc[i];
-    __syncthreads();
-    const int c = wave * 16 + lane % 16;
-    if (wave >= 2 || c >= count) return;
-    float* t = l.t + ((size_t)blockIdx.y * l.B + tl.row[c]) * l.Rp;
-#pragma unroll
-    for (int i = 0; i < RT; i++) {
-        const int r = r0 + i * 16 + lane / 16 * 4;
-        if (r < l.Rp) *(v4f*)(t + r) = (acc[i] + join[(wave * RT + i) * 64 + lane]) * scale;
-    }
-}
-
-// out of a tile of rows and `chunk` outputs.  t's splits are added up and cut
-// into pieces in LDS; a wavefront takes 64 outputs at a time, four matrix tiles
-// beside each other.
-template <int KIND, bool WHOLE>
-__global__ __launch_bounds__(256, 3) void lora_expand_tile(Lora l) {
-    constexpr int P = KIND == IBH_F16 ? 2 : 1;
-    extern __shared__ __align__(16) uint16_t st[];       // [3][kTile][kr]
-    const Tile& tl = l.tiles[blockIdx.x];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane % 16, q = lane / 16;
-    const int id = tl.id, rank = tl.rank, count = tl.count, m_begin = blockIdx.y * l.chunk, m_end = min(m_begin + l.chunk, l.M);
-    int row[2][4];
+    v4f acc[2][RT];
 #pragma unroll
     for (int h = 0; h < 2; h++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int k = h * 16 + q * 4 + i, at = tl.row[k];
-            row[h][i] = k < count ? at : -1;
-        }
-    if (!count) return;
-    if (rank <= 0) {                                     // no adapter: base; not in the table: NaN
-        if (rank < 0 && tid == 0 && blockIdx.y == 0) atomicOr(&ibh_lora_err, IBH_DEVERR_LORA);
-        if (rank == 0 && l.out == l.base) return;
-        for (int i = wave; i < count; i += 4) {
-            const size_t at = tl.row[i];
-            for (int m = m_begin + lane * 4; m < m_end; m += 256) {
-                const float nan = __builtin_nanf("");
-                store4<WHOLE>(l.out + at * l.os, m, l.M, rank < 0 ? f4_t{nan, nan, nan, nan} :
-                              l.base ? load4<WHOLE>(l.base + at * l.bs, m, l.M) : f4_t{0.f, 0.f, 0.f, 0.f});
+        for (int i = 0; i < RT; i++) acc[h][i] = v4f{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const Piece& p) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            v8bf ba[RT][2];
+#pragma unroll
+            for (int i = 0; i < RT; i++) pieces<KIND>(p.a[i][k], ba[i]);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = p.x[h][k][e / 4][e % 4];
+#pragma unroll
+                for (int w = 0; w < 3; w++) {
+                    u4_t u;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) u[e] = upper(v[2 * e], v[2 * e + 1]);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[e] = below(v[e]);
+#pragma unroll
+                    for (int i = 0; i < RT; i++)
+#pragma unroll
+                        for (int j = 0; j < P; j++)
+                            acc[h][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ba[i][j], __builtin_bit_cast(v8bf, u), acc[h][i], 0, 0, 0);
+                }
             }
         }
+    };
+    Piece p0, p1;
+    int s = s0 + wave;
+    if (s < s1) fetch(s, p0);
+    if (s + 4 < s1) fetch(s + 4, p1);
+    for (; s < s1; s += 8) {
+        multiply(p0);
+        if (s + 8 < s1) fetch(s + 8, p0);
+        if (s + 4 < s1) multiply(p1);
+        if (s + 12 < s1) fetch(s + 12, p1);
+    }
+    // the wavefronts' sums join; lane: row lane % 16 of 16, ranks lane / 16 * 4 .. + 3
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int i = 0; i < RT; i++) join[wave][h * RT + i][lane] = acc[h][i];
+    lds_barrier();
+    for (int w = wave; w < 2 * RT; w += 4) {
+        const int at = w / RT * 16 + c, r = r0 + w % RT * 16 + q * 4;
+        v4f v = ((join[0][w][lane] + join[1][w][lane]) + (join[2][w][lane] + join[3][w][lane])) * scale;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = r + e < rank ? v[e] : 0.f;
+        if (at < count && r < l.Rp) *(v4f*)(l.t + ((size_t)blockIdx.x * l.B + tl.row[at]) * l.Rp + r) = v;
+    }
+}
+
+// out of a tile of rows and kSpan outputs.  t's splits are added up and cut
+// into pieces in LDS.  A wavefront multiplies 64 outputs of all rows, four
+// matrix tiles beside each other (tile j holds outputs 4 c + j, so that a lane
+// has four neighbours); through LDS they come to wavefronts that add 256
+// outputs of a row to base at once, whole kilobytes of memory.
+template <int KIND, bool WHOLE>
+__global__ __launch_bounds__(256, 3) void lora_expand_tile(Lora l) {
+    constexpr int P = KIND == IBH_F16 ? 2 : 1;
+    __shared__ __align__(16) float so[kTile][kSpan + 4];
+    extern __shared__ __align__(16) uint16_t st[];       // [3][kTile][kr]
+    const Tile& tl = l.tiles[blockIdx.y];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane % 16, q = lane / 16;
+    const int id = tl.id, rank = tl.rank, count = tl.count, m0 = blockIdx.x * kSpan;
+    size_t row[8];                                       // this wavefront's to add and store
+#pragma unroll
+    for (int i = 0; i < 8; i++) row[i] = tl.row[wave * 8 + i];
+    const int mine = min(8, count - wave * 8);
+    if (!count) return;
+    if (rank < 0 && tid == 0 && blockIdx.x == 0) atomicOr(&ibh_lora_err, IBH_DEVERR_LORA);
+    if (rank == 0 && l.out == l.base) return;
+    f4_t y[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        y[i] = l.base && i < mine ? load4<WHOLE>(l.base + row[i] * l.bs, m0 + 4 * lane, l.M) : f4_t{0.f, 0.f, 0.f, 0.f};
+    if (rank <= 0) {                                     // no adapter: base; not in the table: NaN
+        const float nan = __builtin_nanf("");
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < mine) store4<WHOLE>(l.out + row[i] * l.os, m0 + 4 * lane, l.M, rank < 0 ? f4_t{nan, nan, nan, nan} : y[i]);
         return;
     }
     const int ks = (rank + 31) / 32, kr = ks * 32 + 8;
@@ -521,7 +514,7 @@ __global__ __launch_bounds__(256, 3) void lora_expand_tile(Lora l) {
         v4f v = {0.f, 0.f, 0.f, 0.f};
         if (k < count && r < (rank + 7) / 8 * 8) {
             const float* t = l.t + (size_t)tl.row[k] * l.Rp + r;
-#pragma unroll 4
+#pragma unroll 8
             for (int s = 0; s < l.S; s++) v += *(const v4f*)(t + (size_t)s * l.B * l.Rp);
         }
         float e[4] = {v[0], v[1], v[2], v[3]};
@@ -529,60 +522,52 @@ __global__ __launch_bounds__(256, 3) void lora_expand_tile(Lora l) {
         for (int p = 0; p < 3; p++) {
             *(uint2*)&st[(p * kTile + k) * kr + r] = make_uint2(upper(e[0], e[1]), upper(e[2], e[3]));
 #pragma unroll
-            for (int q = 0; q < 4; q++) e[q] = below(e[q]);
+            for (int w = 0; w < 4; w++) e[w] = below(e[w]);
         }
     }
-    __syncthreads();
-    // Matrix tiles of 16 rows by 16 outputs, four beside each other: tile j holds
-    // outputs m0 + 4 c + j, so that a lane has four neighbouring ones of the rows
-    // 4 q + i, and 16 lanes read and write 256 bytes of a row.
+    lds_barrier();
     const uint16_t* b = l.b + (size_t)id * l.M * l.R;
-    for (int m0 = m_begin + wave * 64; m0 < m_end; m0 += 256) {
-        f4_t y[2][4];
+    v4f acc[2][4];
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+    for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                y[h][i] = l.base && row[h][i] >= 0 ? load4<WHOLE>(l.base + row[h][i] * l.bs, m0 + 4 * c, l.M) : f4_t{0.f, 0.f, 0.f, 0.f};
-        v4f acc[2][4];
+        for (int j = 0; j < 4; j++) acc[h][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < ks; k++) {
+        const int r = k * 32 + q * 8;
+        u4_t w[4];
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) acc[h][j] = v4f{0.f, 0.f, 0.f, 0.f};
-        for (int k = 0; k < ks; k++) {
-            const int r = k * 32 + q * 8;
-            u4_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int m = m0 + 4 * c + j;
-                w[j] = m < l.M ? load_rank<WHOLE>(b + (size_t)m * l.R, r, rank) : u4_t{0, 0, 0, 0};
-            }
-            v8bf at[2][3];
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int p = 0; p < 3; p++) at[h][p] = *(const v8bf*)&st[(p * kTile + h * 16 + c) * kr + r];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                v8bf bw[2];
-                pieces<KIND>(w[j], bw);
-#pragma unroll
-                for (int i = 0; i < P; i++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-#pragma unroll
-                        for (int p = 0; p < 3; p++)
-                            acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(at[h][p], bw[i], acc[h][j], 0, 0, 0);
-            }
+        for (int j = 0; j < 4; j++) {
+            const int m = m0 + wave * 64 + 4 * c + j;
+            w[j] = load_rank<WHOLE>(b + (size_t)min(m, l.M - 1) * l.R, r, rank);
         }
+        v8bf at[2][3];
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (row[h][i] >= 0)
-                    store4<WHOLE>(l.out + row[h][i] * l.os, m0 + 4 * c, l.M,
-                           y[h][i] + f4_t{acc[h][0][i], acc[h][1][i], acc[h][2][i], acc[h][3][i]});
+            for (int p = 0; p < 3; p++) at[h][p] = *(const v8bf*)&st[(p * kTile + h * 16 + c) * kr + r];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            v8bf bw[2];
+            pieces<KIND>(w[j], bw);
+#pragma unroll
+            for (int i = 0; i < P; i++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int p = 0; p < 3; p++)
+                        acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(at[h][p], bw[i], acc[h][j], 0, 0, 0);
+        }
     }
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            *(v4f*)&so[h * 16 + 4 * q + i][wave * 64 + 4 * c] = v4f{acc[h][0][i], acc[h][1][i], acc[h][2][i], acc[h][3][i]};
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (i < mine)
+            store4<WHOLE>(l.out + row[i] * l.os, m0 + 4 * lane, l.M, y[i] + *(const f4_t*)&so[wave * 8 + i][4 * lane]);
 }
 
 bool adapters_ok(const ibh_lora_adapters* l, const char* who) {
@@ -601,7 +586,7 @@ bool adapters_ok(const ibh_lora_adapters* l, const char* who) {
 // How a call is cut.
 struct LoraPlan {
     bool few;
-    int Rp, S, max_tiles, chunk;
+    int Rp, S, max_tiles;
     size_t plan_bytes, bytes;
 };
 LoraPlan plan_of(const ibh_lora_adapters* l, int B) {
@@ -611,14 +596,13 @@ LoraPlan plan_of(const ibh_lora_adapters* l, int B) {
     p.S = 1;
     p.max_tiles = 0;
     p.plan_bytes = 0;
-    p.chunk = 0;
     if (!p.few) {
         const int groups = min(l->n + 2, B);
         p.max_tiles = B / kTile + groups;
         p.plan_bytes = sizeof(Tile) * (size_t)p.max_tiles;
-        const int tiles = (B + kTile - 1) / kTile + min(l->n, B) / 2;
-        p.S = max(1, min(min(kMaxSplit, (l->N + 511) / 512), 768 / tiles));
-        p.chunk = tiles * (l->M / 1024) >= 512 ? 1024 : tiles * (l->M / 512) >= 256 ? 512 : 256;
+        // the splits of a tile's columns: 512 columns a block, what its wavefronts
+        // have under way at once
+        p.S = min(kMaxSplit, (l->N + 511) / 512);
     }
     p.bytes = p.plan_bytes + (size_t)p.S * B * p.Rp * 4;
     return p;
@@ -626,7 +610,7 @@ LoraPlan plan_of(const ibh_lora_adapters* l, int B) {
 
 template <int KIND, bool WHOLE>
 void launch_shrink(const Lora& l, bool few, hipStream_t st) {
-    const dim3 grid(l.max_tiles, l.S, (l.R + 63) / 64);
+    const dim3 grid(l.S, l.max_tiles, (l.R + 63) / 64);  // a tile's splits beside each other
     if (few) lora_shrink_few<KIND, WHOLE><<<dim3(l.B, (l.Rp + 3) / 4), 256, 0, st>>>(l);
     else if (l.R <= 16) lora_shrink_tile<KIND, WHOLE, 1><<<grid, 256, 0, st>>>(l);
     else if (l.R <= 32) lora_shrink_tile<KIND, WHOLE, 2><<<grid, 256, 0, st>>>(l);
@@ -640,8 +624,8 @@ void launch_expand(const Lora& l, bool few, hipStream_t st) {
         const int span = (256 >> lg) * kOut;
         lora_expand_few<KIND, WHOLE><<<dim3(l.B, (l.M + span - 1) / span), 256, 0, st>>>(l, lg);
     } else
-        lora_expand_tile<KIND, WHOLE><<<dim3(l.max_tiles, (l.M + l.chunk - 1) / l.chunk), 256,
-                                        3 * kTile * ((l.R + 31) / 32 * 32 + 8) * 2, st>>>(l);
+        lora_expand_tile<KIND, WHOLE><<<dim3((l.M + kSpan - 1) / kSpan, l.max_tiles), 256,
+                                        3 * kTile * ((l.R + 31) / 32 * 32 + 8) * 2, st>>>(l);   // up to 50 KB beside 33
 }
 template <int KIND>
 int launch(const Lora& l, bool few, hipStream_t st) {
@@ -696,8 +680,9 @@ extern "C" int ibh_lora(const ibh_lora_adapters* l, float* out, const float* bas
         return IBH_ERROR_PARAM;
     }
     const LoraPlan p = plan_of(l, B);
-    // a launch takes less than 2^32 threads
-    if (!p.few && (size_t)p.max_tiles * max((l->M + p.chunk - 1) / p.chunk, p.S * ((l->rank + 63) / 64)) >= (1 << 24)) {
+    // a launch takes less than 2^32 threads, and 65535 tiles in its second dimension
+    if (!p.few && (p.max_tiles > 65535 ||
+                   (size_t)p.max_tiles * max((l->M + kSpan - 1) / kSpan, p.S * ((l->rank + 63) / 64)) >= (1 << 24))) {
         ibh_set_error("ibh_lora: %d rows are more than one launch takes", B);
         return IBH_ERROR_PARAM;
     }
@@ -708,7 +693,7 @@ extern "C" int ibh_lora(const ibh_lora_adapters* l, float* out, const float* bas
     }
     const Lora a{(const uint16_t*)l->a, (const uint16_t*)l->b, l->scales, l->ranks, l->n, l->rank, l->N, l->M, out, base, x,
                  ids, B, (size_t)out_stride, (size_t)base_stride, (size_t)x_stride, (float*)(w + p.plan_bytes), p.Rp, p.S,
-                 (Tile*)w, p.max_tiles, p.chunk};
+                 (Tile*)w, p.max_tiles};
     hipStream_t st = ibh_resolve_stream(stream);
     return l->kind == IBH_F16 ? launch<IBH_F16>(a, p.few, st) : launch<IBH_BF16>(a, p.few, st);
 }
