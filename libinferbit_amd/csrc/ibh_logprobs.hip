@@ -9,7 +9,7 @@
 namespace {
 using namespace ibh;
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 4, kManyWaves = 16;               // of a block
 constexpr int kPiece = 1024;                             // logits that a wavefront takes at a time
 constexpr int kHeld = 256;                               // candidates that it holds
 constexpr int kMaxShares = 64;                          // blocks that share a row, at most
@@ -146,75 +146,61 @@ struct Best {
     }
 };
 
+template <int W>
 struct Shared {
-    uint64_t held[kWaves][kHeld];
-    int counts[kWaves];
-    Sums sums[kWaves];
+    uint64_t held[W][kHeld];
+    int counts[W];
+    Sums sums[W];
 };
 
-// The block's sums in every thread, each wavefront's best sorted.
-__device__ __forceinline__ Sums gather(Sums t, Best& best, Shared& sh) {
-    const int wave = threadIdx.x >> 6;
+// The block's sums in every thread; its best, sorted, with the first wavefront.
+template <int W>
+__device__ __forceinline__ Sums gather(Sums t, Best& best, Shared<W>& sh) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     t = wave_join(t);
-    if (best.k) best.sort();
-    if ((threadIdx.x & 63) == 0) sh.sums[wave] = t, sh.counts[wave] = best.n;
+    if (best.n > 64) best.cut();
+    if (lane == 0) sh.sums[wave] = t, sh.counts[wave] = best.n;
     __syncthreads();
     t = sh.sums[0];
+    for (int w = 1; w < W; w++) t = join(t, sh.sums[w]);
+    if (wave || !best.k) return t;
+    uint64_t key[W], top = 0;
 #pragma unroll
-    for (int w = 1; w < kWaves; w++) t = join(t, sh.sums[w]);
+    for (int w = 0; w < W; w++) {
+        key[w] = lane < sh.counts[w] ? sh.held[w][lane] : 0;
+        top = key[w] > top ? key[w] : top;
+    }
+    best.n = 0;
+    best.bar = kNothing;
+    best.first((uint32_t)(top >> 32));
+#pragma unroll
+    for (int w = 0; w < W; w++) best.offer(key[w]);
+    best.sort();
     return t;
-}
-// A thread's own among the wavefronts' sorted best, and how many of the block's
-// are above it (k or more: not among the k best).  total: how many there are.
-__device__ __forceinline__ int rank_of(const Shared& sh, int k, uint64_t* key, int* total) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    *total = sh.counts[0] + sh.counts[1] + sh.counts[2] + sh.counts[3];
-    if (lane >= sh.counts[wave]) return k;
-    *key = sh.held[wave][lane];
-    int low[kWaves], high[kWaves];                       // of each list the keys above: found by halving, all at once
-#pragma unroll
-    for (int w = 0; w < kWaves; w++) low[w] = 0, high[w] = sh.counts[w];
-#pragma unroll
-    for (int step = 0; step < 7; step++)                 // up to 64 keys
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            const int mid = (low[w] + high[w]) / 2;
-            const bool above = mid < high[w] && sh.held[w][mid] > *key;
-            low[w] = above ? mid + 1 : low[w];
-            high[w] = above ? high[w] : mid;
-        }
-    return low[0] + low[1] + low[2] + low[3];
 }
 
 // The row's outputs.
-__device__ __forceinline__ void finish(const LogArgs& a, size_t row, Sums t, const Shared& sh) {
-    static_assert(kWaves == 4, "rank_of");
+template <int W>
+__device__ __forceinline__ void finish(const LogArgs& a, size_t row, Sums t, const Best& best) {
     const int tid = threadIdx.x;
     const float* z = a.z + row * a.stride;
     const bool bad = t.s != t.s, none = t.m == -__builtin_inff();
     const float logs = logf(t.s), nanf = __builtin_nanf("");
-    for (int i = tid; i < a.n_tok; i += kWaves * 64) {
+    for (int i = tid; i < a.n_tok; i += W * 64) {
         const int id = a.tokens[row * a.n_tok + i];
         a.out[row * a.n_tok + i] = bad || id < 0 || id >= a.V ? nanf : none ? -__builtin_inff() : (z[id] - t.m) - logs;
     }
     if (a.entropy && tid == 0) a.entropy[row] = bad ? nanf : none ? 0.f : logs - t.e / t.s;
-    if (!a.k) return;
-    uint64_t key = 0;
-    int total;
-    const int rank = rank_of(sh, a.k, &key, &total);
-    if (rank < a.k) {
-        const int id = ~(uint32_t)key;
-        a.top_ids[row * a.k + rank] = bad ? -1 : id;
-        a.top_lp[row * a.k + rank] = bad ? nanf : (z[id] - t.m) - logs;
-    }
-    if (tid >= total && tid < a.k) {                     // fewer than k are left
-        a.top_ids[row * a.k + tid] = -1;
-        a.top_lp[row * a.k + tid] = bad ? nanf : -__builtin_inff();
-    }
+    if (tid >= a.k) return;
+    const bool held = !bad && tid < best.n;              // fewer than k may be left
+    const int id = held ? (int)~(uint32_t)best.held[tid] : -1;
+    a.top_ids[row * a.k + tid] = id;
+    a.top_lp[row * a.k + tid] = bad ? nanf : held ? (z[id] - t.m) - logs : -__builtin_inff();
 }
 
-__global__ __launch_bounds__(kWaves * 64, 8) void logprobs_kernel(LogArgs a) {
-    __shared__ Shared sh;
+template <int W>
+__global__ __launch_bounds__(W * 64, W == kWaves ? 8 : 4) void logprobs_kernel(LogArgs a) {
+    __shared__ Shared<W> sh;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const size_t row = blockIdx.x / a.S;
     const int share = blockIdx.x % a.S;
@@ -229,11 +215,11 @@ __global__ __launch_bounds__(kWaves * 64, 8) void logprobs_kernel(LogArgs a) {
     f4_t next[4];
     bool begin = true;
     auto from = [&](int j) { return (const char*)z + (uint32_t)(j * 4); };   // V is at most 2^30
-    for (int at = v0 + (wave - kWaves) * kPiece; at < v1; at += kWaves * kPiece) {
+    for (int at = v0 + (wave - W) * kPiece; at < v1; at += W * kPiece) {
         f4_t v[4];
 #pragma unroll
         for (int q = 0; q < 4; q++) v[q] = next[q];
-        const int ahead = at + kWaves * kPiece;
+        const int ahead = at + W * kPiece;
         if (ahead >= 0 && ahead + kPiece <= v1) {
 #pragma unroll
             for (int q = 0; q < 4; q++) next[q] = *(const f4_t*)(from(ahead + lane * 4) + q * 1024);
@@ -292,22 +278,17 @@ __global__ __launch_bounds__(kWaves * 64, 8) void logprobs_kernel(LogArgs a) {
     }
     t = gather(t, best, sh);
     if (a.S == 1) {
-        finish(a, row, t, sh);
+        finish<W>(a, row, t, best);
         return;
     }
     const size_t me = blockIdx.x;
     if (threadIdx.x == 0) *(f4_t*)(a.part + me * 4) = f4_t{t.m, t.s, t.e, 0.f};
-    if (!a.k) return;
-    uint64_t key = 0;
-    int total;
-    const int rank = rank_of(sh, a.k, &key, &total);
-    if (rank < a.k) a.keys[me * a.k + rank] = key;
-    if ((int)threadIdx.x >= total && (int)threadIdx.x < a.k) a.keys[me * a.k + threadIdx.x] = 0;
+    if ((int)threadIdx.x < a.k) a.keys[me * a.k + threadIdx.x] = lane < best.n ? best.held[lane] : 0;
 }
 
 // The shares of a row joined.
 __global__ __launch_bounds__(kWaves * 64) void logprobs_join(LogArgs a) {
-    __shared__ Shared sh;
+    __shared__ Shared<kWaves> sh;
     const int tid = threadIdx.x, wave = tid >> 6;
     const size_t row = blockIdx.x;
     const uint64_t* keys = a.keys + row * a.S * a.k;
@@ -335,19 +316,26 @@ __global__ __launch_bounds__(kWaves * 64) void logprobs_join(LogArgs a) {
             if (i * kWaves * 64 < n) best.offer(key[i]);
     }
     t = gather(t, best, sh);
-    finish(a, row, t, sh);
+    finish<kWaves>(a, row, t, best);
 }
 
-// How a call is cut: a row's shares are whole rounds of a block's pieces, as
-// many as fill the card.
+// How a call is cut.  A row of one round of four wavefronts' pieces, or rows
+// that fill the card by themselves, take a block of four.  Few rows of up to two
+// rounds of sixteen take a block of those: one launch instead of two (1 x 32000,
+// 5 best: 10.3 us, 10.7 in two kernels and a launch; 255 rows, 20 best: 16 and
+// 20; but 1 x 64000 14 and 11, 1 x 4000 7.3 and 5.8 in one block of four).
+// Otherwise a row is shared by blocks, whole rounds each, as many as fill the
+// card, and the shares are joined.
 struct LogPlan {
-    int S, seg;
+    int W, S, seg;
     size_t part, bytes;
 };
 LogPlan plan_of(int V, int B, int k) {
     LogPlan p;
-    const int round = kWaves * kPiece, rounds = (V + 3 + round - 1) / round;   // up to three in front of the row
-    const int want = max(1, min(min(rounds, kMaxShares), (1024 + B - 1) / B));
+    const bool one = V + 3 <= kWaves * kPiece;           // up to three in front of the row
+    p.W = !one && B <= 256 && V + 3 <= 2 * kManyWaves * kPiece ? kManyWaves : kWaves;
+    const int round = p.W * kPiece, rounds = (V + 3 + round - 1) / round;
+    const int want = p.W == kManyWaves ? 1 : max(1, min(min(rounds, kMaxShares), (1024 + B - 1) / B));
     const int each = (rounds + want - 1) / want;
     p.seg = each * round;
     p.S = (rounds + each - 1) / each;
@@ -405,7 +393,8 @@ extern "C" int ibh_logprobs(float* out, float* entropy, int32_t* top_ids, float*
     const LogArgs a{out, entropy, top_logprobs, top_ids, logits, tokens, V, n_tokens, k, (size_t)stride, p.S, p.seg,
                     (float*)w, (uint64_t*)(w + p.part)};
     hipStream_t st = ibh_resolve_stream(stream);
-    logprobs_kernel<<<B * p.S, kWaves * 64, 0, st>>>(a);
+    if (p.W == kWaves) logprobs_kernel<kWaves><<<B * p.S, kWaves * 64, 0, st>>>(a);
+    else logprobs_kernel<kManyWaves><<<B * p.S, kManyWaves * 64, 0, st>>>(a);
     IBH_CHECK_LAUNCH("ibh_logprobs");
     if (p.S > 1) {
         logprobs_join<<<B, kWaves * 64, 0, st>>>(a);

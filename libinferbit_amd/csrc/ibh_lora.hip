@@ -15,7 +15,7 @@ using namespace ibh;
 __device__ unsigned int ibh_lora_err;
 
 constexpr int kFew = 64;            // rows up to which a wavefront holds all ids, one a lane
-constexpr int kMaxAdapters = 8192;  // counters of the plan's block
+constexpr int kMaxAdapters = 4096;  // counters of the plan's block
 constexpr int kTile = 32;           // rows of one adapter that a block of the matrix kernels takes
 constexpr int kStep = 64;           // columns of x that a wavefront takes at a time
 constexpr int kSpan = 256;          // outputs that a block of the second product takes
@@ -66,11 +66,10 @@ __device__ __forceinline__ int rank_of(const Lora& l, int id) {
 // Loads from place j of n, zeros behind n.  WHOLE: n is a multiple of what is
 // loaded, which leaves the code for a rest away (every line of code that a
 // small launch runs through is one more wait for memory).
-// x, base and out pass by once, past what the caches hold of the adapters.
 template <bool WHOLE>
 __device__ __forceinline__ f4_t load4(const float* p, int j, int N) {
     f4_t v = {0.f, 0.f, 0.f, 0.f};
-    if (WHOLE ? j < N : j + 4 <= N) return __builtin_nontemporal_load((const f4_t*)(p + j));
+    if (WHOLE ? j < N : j + 4 <= N) return *(const f4_t*)(p + j);
     if constexpr (WHOLE) return v;
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -105,7 +104,7 @@ __device__ __forceinline__ u4_t load_rank(const uint16_t* p, int j, int rank) {
     if constexpr (!WHOLE) return load8h<false>(p, j, rank);
     u4_t v = {0, 0, 0, 0};
     if (j < rank) v = *(const u4h_t*)(p + j);
-    if (j + 8 > rank)
+    if (rank % 8 && j + 8 > rank)                        // j is a multiple of 8
 #pragma unroll
         for (int i = 0; i < 4; i++) v[i] &= (j + 2 * i < rank ? 0xffffu : 0) | (j + 2 * i + 1 < rank ? 0xffff0000u : 0);
     return v;
@@ -267,54 +266,55 @@ __global__ __launch_bounds__(256) void lora_expand_few(Lora l, int lg) {
 // is left to chance and changes no result: a row's sums do not depend on its
 // place) and cuts each adapter's rows into tiles.
 __global__ __launch_bounds__(1024) void lora_plan(Lora l) {
-    __shared__ int32_t count[kMaxAdapters + 2];
+    constexpr int kKept = 8;                             // rows of a thread that stay in registers
+    __shared__ int32_t count[kMaxAdapters + 2], more[kMaxAdapters + 2];   // the keys' rows: those, the others
     __shared__ int32_t wave_tiles[16];
-    const int tid = threadIdx.x, keys = l.n + 2;         // n: no adapter; n + 1: not in the table
-    for (int i = tid; i < keys; i += 1024) count[i] = 0;
-    __syncthreads();
+    const int tid = threadIdx.x, lane = tid & 63, keys = l.n + 2;   // n: no adapter; n + 1: not in the table
+    int key[kKept], at[kKept];
+#pragma unroll
+    for (int u = 0; u < kKept; u++) key[u] = u * 1024 + tid < l.B ? l.ids[u * 1024 + tid] : 0;
+    const float scale0 = l.scales && tid < l.n ? l.scales[tid] : 1.f;   // of the first keys, under way with the ids
+    for (int i = tid; i < keys; i += 1024) count[i] = more[i] = 0;
     auto key_of = [&](int id) {
         const int rank = rank_of(l, id);
         return rank < 0 ? l.n + 1 : rank == 0 ? l.n : id;
     };
+#pragma unroll
+    for (int u = 0; u < kKept; u++) key[u] = u * 1024 + tid < l.B ? key_of(key[u]) : -1;
+    __syncthreads();
     // adds the wavefront's rows to the counters of their keys, -1 for none, and
     // returns what each row found there: those that share the first row's key
     // (packed prompts: all of them) in one addition
-    auto add = [&](int key) {
-        const int first = __builtin_amdgcn_readfirstlane(key), lane = tid & 63;
-        const uint64_t same = __ballot(key == first);
+    auto add = [&](int32_t* to, int k) {
+        const int first = __builtin_amdgcn_readfirstlane(k);
+        const uint64_t same = __ballot(k == first);
         int got = 0;
-        if (key != first) {
-            if (key >= 0) got = atomicAdd(&count[key], 1);
+        if (k != first) {
+            if (k >= 0) got = atomicAdd(&to[k], 1);
         } else if (first >= 0) {
-            if (lane == 0) got = atomicAdd(&count[first], __popcll(same));
+            if (lane == 0) got = atomicAdd(&to[first], __popcll(same));
             got = __builtin_amdgcn_readfirstlane(got) + __popcll(same & ((1ull << lane) - 1));
         }
         return got;
     };
-    // the first rows' keys stay in registers, their loads all under way at once
-    constexpr int kKept = 8;
-    int key[kKept];
-#pragma unroll
-    for (int u = 0; u < kKept; u++) key[u] = u * 1024 + tid < l.B ? l.ids[u * 1024 + tid] : 0;
-#pragma unroll
-    for (int u = 0; u < kKept; u++) key[u] = u * 1024 + tid < l.B ? key_of(key[u]) : -1;
-    const int later = kKept * 1024 + (tid & ~63);        // whole wavefronts go on together
-    auto late_key = [&](int i) { return i + (tid & 63) < l.B ? key_of(l.ids[i + (tid & 63)]) : -1; };
+    auto later = [&](auto&& f) {                         // whole wavefronts go on together
+        for (int i = kKept * 1024 + (tid & ~63); i < l.B; i += 1024) f(i + lane < l.B ? key_of(l.ids[i + lane]) : -1, i + lane);
+    };
 #pragma unroll
     for (int u = 0; u < kKept; u++)
-        if (u * 1024 < l.B) add(key[u]);
-    for (int i = later; i < l.B; i += 1024) add(late_key(i));
+        if (u * 1024 < l.B) at[u] = add(count, key[u]);
+    later([&](int k, int) { add(more, k); });
     __syncthreads();
     // each thread's run of keys: tiles in front of it
     const int per = (keys + 1023) / 1024, k0 = min(tid * per, keys), k1 = min(k0 + per, keys);
     int tiles = 0;
-    for (int k = k0; k < k1; k++) tiles += (count[k] + kTile - 1) / kTile;
+    for (int k = k0; k < k1; k++) tiles += (count[k] + more[k] + kTile - 1) / kTile;
     int it = tiles;
     for (int o = 1; o < 64; o <<= 1) {
         const int p = __shfl_up(it, o, 64);
-        if ((tid & 63) >= o) it += p;
+        if (lane >= o) it += p;
     }
-    if ((tid & 63) == 63) wave_tiles[tid >> 6] = it;
+    if (lane == 63) wave_tiles[tid >> 6] = it;
     __syncthreads();
     it -= tiles;
     int all = 0;
@@ -323,11 +323,12 @@ __global__ __launch_bounds__(1024) void lora_plan(Lora l) {
         all += wave_tiles[w];
     }
     for (int k = k0; k < k1; k++) {
-        const int c = count[k];
+        const int first = count[k], c = first + more[k];
         if (!c) continue;
         const int rank = k < l.n ? (l.ranks ? l.ranks[k] : l.R) : l.n - k;
-        const float scale = k < l.n && l.scales ? l.scales[k] : 1.f;
-        count[k] = it * kTile;                           // from here on: the place of its next row
+        const float scale = k >= l.n || !l.scales ? 1.f : per == 1 ? scale0 : l.scales[k];
+        count[k] = it * kTile;                           // from here on: the place of its first row,
+        more[k] = it * kTile + first;                    // and of its next one
         for (int j = 0; j < c; j += kTile, it++) {
             Tile& t = l.tiles[it];
             t.id = k, t.rank = rank, t.count = min(kTile, c - j), t.scale = scale;
@@ -335,16 +336,16 @@ __global__ __launch_bounds__(1024) void lora_plan(Lora l) {
     }
     for (int i = all + tid; i < l.max_tiles; i += 1024) l.tiles[i].count = 0;
     __syncthreads();
+    auto place = [&](int k, int row, int i) {
+        if (k >= 0) l.tiles[i / kTile].row[i % kTile] = row;
+    };
 #pragma unroll
     for (int u = 0; u < kKept; u++)
-        if (u * 1024 < l.B) {
-            const int at = add(key[u]);
-            if (key[u] >= 0) l.tiles[at / kTile].row[at % kTile] = u * 1024 + tid;
-        }
-    for (int i = later; i < l.B; i += 1024) {
-        const int k = late_key(i), at = add(k);
-        if (k >= 0) l.tiles[at / kTile].row[at % kTile] = i + (tid & 63);
-    }
+        if (u * 1024 < l.B) place(key[u], u * 1024 + tid, key[u] >= 0 ? count[key[u]] + at[u] : 0);
+    later([&](int k, int row) {
+        const int i = add(more, k);
+        place(k, row, i);
+    });
 }
 
 // fp32 numbers as bf16 numbers, upper halves cut off one after the other: 8
@@ -485,8 +486,8 @@ __global__ __launch_bounds__(256, RT <= 2 ? 3 : 2) void lora_shrink_tile(Lora l)
 template <int KIND, bool WHOLE>
 __global__ __launch_bounds__(256, 3) void lora_expand_tile(Lora l) {
     constexpr int P = KIND == IBH_F16 ? 2 : 1;
-    __shared__ __align__(16) float so[kTile][kSpan + 4];
-    extern __shared__ __align__(16) uint16_t st[];       // [3][kTile][kr]
+    extern __shared__ __align__(16) uint16_t st[];       // t [3][kTile][kr], then, in its place, outputs
+    float (*so)[kSpan + 4] = (float (*)[kSpan + 4])st;
     const Tile& tl = l.tiles[blockIdx.y];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane % 16, q = lane / 16;
     const int id = tl.id, rank = tl.rank, count = tl.count, m0 = blockIdx.x * kSpan;
@@ -508,6 +509,15 @@ __global__ __launch_bounds__(256, 3) void lora_expand_tile(Lora l) {
             if (i < mine) store4<WHOLE>(l.out + row[i] * l.os, m0 + 4 * lane, l.M, rank < 0 ? f4_t{nan, nan, nan, nan} : y[i]);
         return;
     }
+    const uint16_t* b[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) b[j] = l.b + ((size_t)id * l.M + min(m0 + wave * 64 + 4 * c + j, l.M - 1)) * l.R;
+    u4_t w[4];
+    auto fetch = [&](int k) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = load_rank<WHOLE>(b[j], k * 32 + q * 8, rank);
+    };
+    fetch(0);
     const int ks = (rank + 31) / 32, kr = ks * 32 + 8;
     for (int i = tid; i < kTile * ks * 8; i += 256) {
         const int k = i / (ks * 8), r = i % (ks * 8) * 4;
@@ -522,33 +532,29 @@ __global__ __launch_bounds__(256, 3) void lora_expand_tile(Lora l) {
         for (int p = 0; p < 3; p++) {
             *(uint2*)&st[(p * kTile + k) * kr + r] = make_uint2(upper(e[0], e[1]), upper(e[2], e[3]));
 #pragma unroll
-            for (int w = 0; w < 4; w++) e[w] = below(e[w]);
+            for (int u = 0; u < 4; u++) e[u] = below(e[u]);
         }
     }
     lds_barrier();
-    const uint16_t* b = l.b + (size_t)id * l.M * l.R;
     v4f acc[2][4];
 #pragma unroll
     for (int h = 0; h < 2; h++)
 #pragma unroll
         for (int j = 0; j < 4; j++) acc[h][j] = v4f{0.f, 0.f, 0.f, 0.f};
     for (int k = 0; k < ks; k++) {
-        const int r = k * 32 + q * 8;
-        u4_t w[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int m = m0 + wave * 64 + 4 * c + j;
-            w[j] = load_rank<WHOLE>(b + (size_t)min(m, l.M - 1) * l.R, r, rank);
-        }
         v8bf at[2][3];
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int p = 0; p < 3; p++) at[h][p] = *(const v8bf*)&st[(p * kTile + h * 16 + c) * kr + r];
+            for (int p = 0; p < 3; p++) at[h][p] = *(const v8bf*)&st[(p * kTile + h * 16 + c) * kr + k * 32 + q * 8];
+        u4_t now[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) now[j] = w[j];
+        if (k + 1 < ks) fetch(k + 1);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             v8bf bw[2];
-            pieces<KIND>(w[j], bw);
+            pieces<KIND>(now[j], bw);
 #pragma unroll
             for (int i = 0; i < P; i++)
 #pragma unroll
@@ -558,6 +564,7 @@ __global__ __launch_bounds__(256, 3) void lora_expand_tile(Lora l) {
                         acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(at[h][p], bw[i], acc[h][j], 0, 0, 0);
         }
     }
+    lds_barrier();
 #pragma unroll
     for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -625,7 +632,7 @@ void launch_expand(const Lora& l, bool few, hipStream_t st) {
         lora_expand_few<KIND, WHOLE><<<dim3(l.B, (l.M + span - 1) / span), 256, 0, st>>>(l, lg);
     } else
         lora_expand_tile<KIND, WHOLE><<<dim3((l.M + kSpan - 1) / kSpan, l.max_tiles), 256,
-                                        3 * kTile * ((l.R + 31) / 32 * 32 + 8) * 2, st>>>(l);   // up to 50 KB beside 33
+                                        max(3 * kTile * ((l.R + 31) / 32 * 32 + 8) * 2, kTile * (kSpan + 4) * 4), st>>>(l);
 }
 template <int KIND>
 int launch(const Lora& l, bool few, hipStream_t st) {

@@ -231,32 +231,36 @@ def kv4_evict(src: Kv4Cache, dst: Kv4Cache, weights_src, weights_dst, budget: in
               src._on(kept, torch.int32, n * budget), pw, nw)
 
 
+def _gpu(t) -> int:
+    """The GPU that t is on."""
+    index = t.get_device()
+    if index < 0:
+        raise ValueError("libinferbit_amd ops take GPU tensors")
+    return index
+
+
 def _on(t, index: int, dtype, shape):
-    """The address of t (None: none), a contiguous tensor of GPU `index` with the given type and shape."""
-    if t is None:
-        return None
-    if t.get_device() != index or index < 0:
-        raise ValueError(f"operand on {t.device}, expected a GPU tensor on cuda:{index}" if index >= 0 else
-                         "libinferbit_amd ops take GPU tensors")
-    if t.dtype != dtype:
+    """The address of t, a contiguous tensor of GPU `index` with the given type and shape."""
+    if t.get_device() == index and t.dtype is dtype and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
+    if t.get_device() != index:
+        raise ValueError(f"operand on {t.device}, another is on cuda:{index}")
+    if t.dtype is not dtype:
         raise TypeError(f"operand must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"operand must be {list(shape)}, got {list(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError("operand must be contiguous")
-    return t.data_ptr()
+    raise ValueError("operand must be contiguous")
 
 
 def _spaced(t, index: int, shape):
-    """(address, floats between rows) of t (None: none), fp32 rows [B, n] of contiguous elements on GPU `index`."""
-    if t is None:
-        return None, 0
-    if t.get_device() != index or index < 0:
-        raise ValueError(f"operand on {t.device}, expected a GPU tensor on cuda:{index}" if index >= 0 else
-                         "libinferbit_amd ops take GPU tensors")
-    if t.dtype != torch.float32:
+    """(address, floats between rows) of t, fp32 rows [B, n] of contiguous elements on GPU `index`."""
+    if t.get_device() == index and t.dtype is torch.float32 and t.shape == shape and t.is_contiguous():
+        return t.data_ptr(), shape[1]
+    if t.get_device() != index:
+        raise ValueError(f"operand on {t.device}, another is on cuda:{index}")
+    if t.dtype is not torch.float32:
         raise TypeError(f"operand must be torch.float32, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"operand must be {list(shape)}, got {list(t.shape)}")
     s0, s1 = t.stride()
     if shape[0] <= 1:
@@ -269,38 +273,40 @@ def _spaced(t, index: int, shape):
 def _call_on(index: int, name: str, *args) -> None:
     """A call on GPU `index`, on its current stream."""
     stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch.cuda.current_device() == index:
-        check(getattr(lib(), name)(*args, stream), name)
+    if torch._C._cuda_getDevice() == index:
+        rc = getattr(lib(), name)(*args, stream)
     else:
         with torch.cuda.device(index):
-            check(getattr(lib(), name)(*args, stream), name)
+            rc = getattr(lib(), name)(*args, stream)
+    if rc:
+        check(rc, name)
 
 
-def _scratch(ws, need: int, t):
-    """(address, bytes, the tensor to keep) of the given workspace, or of `need` bytes on t's GPU."""
+def _scratch(ws, need: int, index: int):
+    """(address, bytes, the tensor to keep) of the given workspace, or of `need` bytes on GPU `index`."""
     if ws is not None:
-        return _on(ws, t.get_device(), torch.uint8, tuple(ws.shape)), ws.numel(), ws
+        return _on(ws, index, torch.uint8, ws.shape), ws.numel(), ws
     if not need:
         return None, 0, None
-    ws = torch.empty(need, dtype=torch.uint8, device=t.device)
+    ws = torch.empty(need, dtype=torch.uint8, device=index)
     return ws.data_ptr(), need, ws
 
 
 def add_rmsnorm(y, x, weight, eps: float, delta=None, h=None, q=None, s=None) -> None:
     """The RMS norm of x + delta, rows [B, N] (which may be spaced): y fp32 [B, N] and / or the codes q int8 [B, N] with
     their scales s [B, ceil(N / 128)] for matmul_w4a8_batch; the sum itself into h.  y or h may be x or delta."""
-    if x.dim() != 2 or not x.shape[1]:
+    shape, index, f32 = x.shape, _gpu(x), torch.float32
+    if len(shape) != 2 or not shape[1]:
         raise ValueError("x must be [B, N] with N at least 1")
-    shape, index = tuple(x.shape), x.get_device()
-    B, N = shape
-    px, sx = _spaced(x, index, shape)
-    pd, sd = _spaced(delta, index, shape)
-    args = (_on(y, index, torch.float32, shape), _on(q, index, torch.int8, shape),
-            _on(s, index, torch.float32, (B, (N + 127) // 128)), _on(h, index, torch.float32, shape), px, pd,
-            _on(weight, index, torch.float32, (N,)))
     if (y is None and q is None) or (q is None) != (s is None):
         raise ValueError("y, or q with s, or all three are wanted")
-    _call_on(index, "ibh_add_rmsnorm", *args, eps, N, B, sx, sd)
+    B, N = shape
+    px, sx = _spaced(x, index, shape)
+    pd, sd = (None, 0) if delta is None else _spaced(delta, index, shape)
+    _call_on(index, "ibh_add_rmsnorm", None if y is None else _on(y, index, f32, shape),
+             None if q is None else _on(q, index, torch.int8, shape),
+             None if s is None else _on(s, index, f32, (B, (N + 127) // 128)),
+             None if h is None else _on(h, index, f32, shape), px, pd, _on(weight, index, f32, (N,)), eps, N, B, sx, sd)
 
 
 _LORA_KINDS = {torch.float16: 0, torch.bfloat16: 1}
@@ -310,47 +316,52 @@ def lora(out, x, a, b, ids, base=None, scales=None, ranks=None, ws=None) -> None
     """Adds to each row of base [B, M] (None: zeros; may be out) what its adapter makes of its row of x [B, N]:
     out[r] = base[r] + scales[i] * b[i] @ (a[i] @ x[r]), i = ids[r] (int32 [B]; negative: no adapter).  a [n, rank, N]
     and b [n, M, rank] in fp16 or bf16, scales fp32 [n], ranks int32 [n].  Rows of out, base and x may be spaced."""
-    if a.dim() != 3 or b.dim() != 3 or x.dim() != 2:
+    dtype, sa, sb = a.dtype, a.shape, b.shape
+    if len(sa) != 3 or len(sb) != 3 or x.dim() != 2:
         raise ValueError("a must be [n, rank, N], b [n, M, rank] and x [B, N]")
-    (n, R, N), B, M, index = a.shape, x.shape[0], b.shape[1], x.get_device()
-    kind = _LORA_KINDS.get(a.dtype)
+    (n, R, N), B, M = sa, x.shape[0], sb[1]
+    kind = _LORA_KINDS.get(dtype)
     if kind is None:
-        raise TypeError(f"adapters must be fp16 or bf16, got {a.dtype}")
-    desc = LoraDesc(_on(a, index, a.dtype, (n, R, N)), _on(b, index, a.dtype, (n, M, R)),
-                    _on(scales, index, torch.float32, (n,)), _on(ranks, index, torch.int32, (n,)), n, R, N, M, kind)
+        raise TypeError(f"adapters must be fp16 or bf16, got {dtype}")
+    index = _gpu(x)
+    ref = ctypes.byref(LoraDesc(_on(a, index, dtype, sa), _on(b, index, dtype, (n, M, R)),
+                                None if scales is None else _on(scales, index, torch.float32, (n,)),
+                                None if ranks is None else _on(ranks, index, torch.int32, (n,)), n, R, N, M, kind))
     po, so = _spaced(out, index, (B, M))
-    pb, sb = _spaced(base, index, (B, M))
+    pb, sb = (None, 0) if base is None else _spaced(base, index, (B, M))
     px, sx = _spaced(x, index, (B, N))
     pi = _on(ids, index, torch.int32, (B,))
-    ref = ctypes.byref(desc)
-    pw, nw, ws = _scratch(ws, lib().ibh_lora_workspace_bytes(ref, B) if ws is None else 0, x)
+    pw, nw, ws = _scratch(ws, 0 if ws is not None else lib().ibh_lora_workspace_bytes(ref, B), index)
     _call_on(index, "ibh_lora", ref, po, pb, px, pi, B, so, sb, sx, pw, nw)
 
 
 def logprobs(out, logits, tokens, entropy=None, top_ids=None, top_logprobs=None, ws=None) -> None:
     """From logits [B, V] (rows may be spaced): the log-probabilities of tokens (int32 [B] or [B, n]; None with out) into
     out of the same shape, the entropy into entropy [B], the k best into top_ids (int32) and top_logprobs [B, k]."""
-    if logits.dim() != 2 or not logits.shape[1]:
+    index, shape = _gpu(logits), logits.shape
+    if len(shape) != 2 or not shape[1]:
         raise ValueError("logits must be [B, V] with V at least 1")
-    (B, V), index = logits.shape, logits.get_device()
-    pz, sz = _spaced(logits, index, (B, V))
+    B, V = shape
+    pz, sz = _spaced(logits, index, shape)
     if (out is None) != (tokens is None) or (top_ids is None) != (top_logprobs is None):
         raise ValueError("out and tokens go together, and top_ids and top_logprobs")
     n = k = 0
+    po = pt = pi = pl = None
     if tokens is not None:
-        if tokens.dim() not in (1, 2) or tokens.shape[0] != B:
-            raise ValueError(f"tokens must be [{B}] or [{B}, n], got {list(tokens.shape)}")
-        n = 1 if tokens.dim() == 1 else tokens.shape[1]
-        out, tokens = (_on(out, index, torch.float32, tuple(tokens.shape)),
-                       _on(tokens, index, torch.int32, tuple(tokens.shape)))
+        st = tokens.shape
+        if len(st) not in (1, 2) or st[0] != B:
+            raise ValueError(f"tokens must be [{B}] or [{B}, n], got {list(st)}")
+        n = 1 if len(st) == 1 else st[1]
+        po, pt = _on(out, index, torch.float32, st), _on(tokens, index, torch.int32, st)
     if top_ids is not None:
-        if top_ids.dim() != 2:
+        sk = top_ids.shape
+        if len(sk) != 2 or sk[0] != B:
             raise ValueError("top_ids and top_logprobs must be [B, k]")
-        k = top_ids.shape[1]
-        top_ids, top_logprobs = (_on(top_ids, index, torch.int32, (B, k)), _on(top_logprobs, index, torch.float32, (B, k)))
-    pw, nw, ws = _scratch(ws, lib().ibh_logprobs_workspace_bytes(V, B, k) if ws is None else 0, logits)
-    _call_on(index, "ibh_logprobs", out, _on(entropy, index, torch.float32, (B,)), top_ids, top_logprobs, pz, tokens,
-             V, B, sz, n, k, pw, nw)
+        k = sk[1]
+        pi, pl = _on(top_ids, index, torch.int32, sk), _on(top_logprobs, index, torch.float32, sk)
+    pw, nw, ws = _scratch(ws, 0 if ws is not None else lib().ibh_logprobs_workspace_bytes(V, B, k), index)
+    _call_on(index, "ibh_logprobs", po, None if entropy is None else _on(entropy, index, torch.float32, (B,)), pi, pl, pz,
+             pt, V, B, sz, n, k, pw, nw)
 
 
 class PqDeviceTensor:
