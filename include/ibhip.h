@@ -328,13 +328,13 @@ int ibh_add_rmsnorm(float* y, int8_t* q, float* s, float* h, const float* x, con
  *   out[b] = base[b] + scales[i] * B_i (A_i x[b]),  i = ids[b]
  * with fp32 sums of the adapters' 16-bit numbers and x as it is (no rounding in
  * between but fp32's).  base NULL stands for zeros; base may be out.  A row of a
- * negative id has no adapter: out = base.  Rows may come in any order; those of
+ * negative id has no adapter: out = base.  Up to 4096 adapters.  Rows may come in any order; those of
  * one adapter are served together.  ids, scales and ranks are read on the
  * device, so a captured graph follows them.  An id of n or more, or a rank
  * outside 0 .. rank, raises IBH_DEVERR_LORA (ibh_device_errors) and makes that
  * row NaN.
- * out overlaps nothing else.  `ws` >= ibh_lora_workspace_bytes on 16 bytes;
- * NULL = the library's workspace of 4 MiB: a call that needs more is refused
+ * out overlaps nothing else.  `ws` >= ibh_lora_workspace_bytes (0 for few rows
+ * and small adapters) on 16 bytes; NULL = the library's workspace of 4 MiB: a call that needs more is refused
  * (IBH_ERROR_MEMORY).  Calls that share one must not overlap in time. */
 #define IBH_F16  0
 #define IBH_BF16 1

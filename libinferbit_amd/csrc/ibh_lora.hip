@@ -18,6 +18,10 @@ constexpr int kFew = 64;            // rows up to which a wavefront holds all id
 constexpr int kMaxAdapters = 4096;  // counters of the plan's block
 constexpr int kTile = 32;           // rows of one adapter that a block of the matrix kernels takes
 constexpr int kStep = 64;           // columns of x that a wavefront takes at a time
+constexpr int kOut = 2;             // outputs of a lane group in the second product of few rows
+constexpr int kBoth = 512;          // threads that do both products of few rows,
+constexpr int kBothOut = 4;         // the outputs of a lane group there,
+constexpr size_t kBothMost = 65536; // and the numbers of an adapter's a up to which they do
 constexpr int kSpan = 256;          // outputs that a block of the second product takes
 constexpr int kMaxSplit = 16;       // blocks that share a tile's columns
 
@@ -116,9 +120,13 @@ __device__ __forceinline__ u4_t load_rank(const uint16_t* p, int j, int rank) {
 // memory once and from L2 by the others.
 struct Few {
     int id, rank, rows;             // rows 0: this block has nothing to do
-    int row[4];                     // by constants only: an array indexed by a variable would lie in LDS, and its place
-                                    // there be read off the dispatch packet in host memory, 10 us for 512 blocks
-    __device__ __forceinline__ int at(int i) const { return i == 0 ? row[0] : i == 1 ? row[1] : i == 2 ? row[2] : row[3]; }
+    // Four numbers, all of them read to pick one: one of an array, or one of four
+    // places in the struct, would put it all into LDS, at a place read off the
+    // dispatch packet in host memory (10 us for 512 blocks).
+    int r0, r1, r2, r3;
+    __device__ __forceinline__ int row(int i) const {
+        return (r0 & -(i == 0)) | (r1 & -(i == 1)) | (r2 & -(i == 2)) | (r3 & -(i == 3));
+    }
 };
 __device__ __forceinline__ Few few_of(const Lora& l) {
     const int lane = threadIdx.x & 63, me = blockIdx.x;
@@ -131,18 +139,20 @@ __device__ __forceinline__ Few few_of(const Lora& l) {
     const int before = __popcll(same & ((1ull << me) - 1));
     if (before % 4) return f;
     same &= ~0ull << me;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        f.row[i] = same ? __ffsll((unsigned long long)same) - 1 : f.row[0];
-        f.rows += same != 0;
+    f.rows = min(4, __popcll(same));
+    auto next = [&] {
+        const int r = same ? __ffsll((unsigned long long)same) - 1 : me;
         same &= same - 1;
-    }
+        return r;
+    };
+    f.r0 = next(), f.r1 = next(), f.r2 = next(), f.r3 = next();
     return f;
 }
 
-// RR ranks of an adapter times NR rows: lanes take eights of columns.
-template <int KIND, bool WHOLE, int RR, int NR>
-__device__ __forceinline__ void shrink_rows(const Lora& l, const Few& f, int r0, float (*part)[4]) {
+// RR ranks of an adapter times NR rows by T threads, which take eights of
+// columns; to t, rows Rp apart, zeros behind the adapter's rank.
+template <int KIND, bool WHOLE, int T, int RR, int NR, class Store>
+__device__ __forceinline__ void shrink_rows(const Lora& l, const Few& f, int r0, float (*part)[T / 64], Store&& store) {
     const int tid = threadIdx.x;
     const uint16_t* a = l.a + ((size_t)f.id * l.R + r0) * l.N;
     const int nr = min(RR, f.rank - r0);
@@ -151,8 +161,7 @@ __device__ __forceinline__ void shrink_rows(const Lora& l, const Few& f, int r0,
     for (int r = 0; r < RR; r++)
 #pragma unroll
         for (int i = 0; i < NR; i++) acc[r][i] = 0.f;
-#pragma unroll 2
-    for (int j = tid * 8; j < l.N; j += 2048) {
+    for (int j = tid * 8; j < l.N; j += T * 8) {
         u4_t w[RR];
         f4_t v[NR][2];
 #pragma unroll
@@ -160,7 +169,7 @@ __device__ __forceinline__ void shrink_rows(const Lora& l, const Few& f, int r0,
 #pragma unroll
         for (int i = 0; i < NR; i++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) v[i][h] = load4<WHOLE>(l.x + f.row[i] * l.xs, j + 4 * h, l.N);
+            for (int h = 0; h < 2; h++) v[i][h] = load4<WHOLE>(l.x + f.row(i) * l.xs, j + 4 * h, l.N);
 #pragma unroll
         for (int r = 0; r < RR; r++)
 #pragma unroll
@@ -180,9 +189,10 @@ __device__ __forceinline__ void shrink_rows(const Lora& l, const Few& f, int r0,
     __syncthreads();
     if (tid < RR * NR) {
         const int r = tid / NR, i = tid % NR;
-        const float s = (part[tid][0] + part[tid][1]) + (part[tid][2] + part[tid][3]);
-        if (i < f.rows && r0 + r < l.Rp)
-            l.t[(size_t)f.at(i) * l.Rp + r0 + r] = r < nr ? s * (l.scales ? l.scales[f.id] : 1.f) : 0.f;
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < T / 64; w++) s += part[tid][w];
+        if (i < f.rows && r0 + r < l.Rp) store(i, r0 + r, r < nr ? s * (l.scales ? l.scales[f.id] : 1.f) : 0.f);
     }
 }
 
@@ -192,73 +202,109 @@ __global__ __launch_bounds__(256) void lora_shrink_few(Lora l) {
     const Few f = few_of(l);
     const int r0 = blockIdx.y * 4;
     if (!f.rows || f.rank <= 0 || r0 >= (f.rank + 7) / 8 * 8) return;
-    if (f.rows == 1) shrink_rows<KIND, WHOLE, 4, 1>(l, f, r0, part);
-    else if (f.rows == 2) shrink_rows<KIND, WHOLE, 4, 2>(l, f, r0, part);
-    else shrink_rows<KIND, WHOLE, 4, 4>(l, f, r0, part);
+    auto store = [&](int i, int r, float v) { l.t[(size_t)f.row(i) * l.Rp + r] = v; };
+    if (f.rows == 1) shrink_rows<KIND, WHOLE, 256, 4, 1>(l, f, r0, part, store);
+    else if (f.rows == 2) shrink_rows<KIND, WHOLE, 256, 4, 2>(l, f, r0, part, store);
+    else shrink_rows<KIND, WHOLE, 256, 4, 4>(l, f, r0, part, store);
 }
 
-// A row of b in `1 << lg` lanes, eight numbers each; kOut outputs a lane group.
-constexpr int kOut = 2;
+// Outputs of a block: a row of b in `1 << lg` lanes, eight numbers each; OUT
+// outputs a lane group.
+template <int KIND, bool WHOLE, int T, int OUT, int NR>
+struct Expand {
+    u4_t w[OUT];
+    float y[OUT][NR];
+    int sub, per, m0, lg;
+
+    // what does not need t
+    __device__ __forceinline__ Expand(const Lora& l, const Few& f, int lg_) : lg(lg_) {
+        sub = threadIdx.x & ((1 << lg) - 1), per = T >> lg;
+        m0 = blockIdx.y * per * OUT + (threadIdx.x >> lg);
+        const uint16_t* b = l.b + (size_t)f.id * l.M * l.R;
+#pragma unroll
+        for (int o = 0; o < OUT; o++) {
+            const int m = m0 + o * per;
+            w[o] = m < l.M ? load_rank<WHOLE>(b + (size_t)m * l.R, 8 * sub, f.rank) : u4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < NR; i++) y[o][i] = l.base && sub == 0 && m < l.M ? l.base[f.row(i) * l.bs + m] : 0.f;
+        }
+    }
+    template <class Load>
+    __device__ __forceinline__ void finish(const Lora& l, const Few& f, Load&& load) const {
+        f4_t t[NR][2];
+#pragma unroll
+        for (int i = 0; i < NR; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) t[i][h] = 8 * sub < f.rank ? load(i, 8 * sub + 4 * h) : f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int o = 0; o < OUT; o++) {
+            float s[NR];
+#pragma unroll
+            for (int i = 0; i < NR; i++) s[i] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float we = widen<KIND>(e % 2 ? w[o][e / 2] >> 16 : w[o][e / 2] & 0xffffu);
+#pragma unroll
+                for (int i = 0; i < NR; i++) s[i] = fmaf(we, t[i][e / 4][e % 4], s[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < NR; i++) {
+                for (int k = 0; k < lg; k++) s[i] += __shfl_xor(s[i], 1 << k, kWave);
+                const int m = m0 + o * per;
+                if (sub == 0 && m < l.M && i < f.rows) l.out[f.row(i) * l.os + m] = y[o][i] + s[i];
+            }
+        }
+    }
+};
+
+// Rows without an adapter: base; with one that is not in the table: NaN.
+__device__ __forceinline__ void few_without(const Lora& l, const Few& f, int span) {
+    if (f.rank < 0 && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(&ibh_lora_err, IBH_DEVERR_LORA);
+    if (f.rank == 0 && l.out == l.base) return;
+    const int m0 = blockIdx.y * span;
+    for (int i = 0; i < f.rows; i++)
+        for (int m = m0 + threadIdx.x; m < min(m0 + span, l.M); m += blockDim.x)
+            l.out[f.row(i) * l.os + m] = f.rank < 0 ? __builtin_nanf("") : l.base ? l.base[f.row(i) * l.bs + m] : 0.f;
+}
+
 template <int KIND, bool WHOLE, int NR>
 __device__ __forceinline__ void expand_rows(const Lora& l, const Few& f, int lg) {
-    const int sub = threadIdx.x & ((1 << lg) - 1), per = 256 >> lg, r0 = 8 * sub;
-    const int m0 = blockIdx.y * per * kOut + (threadIdx.x >> lg);
-    const uint16_t* b = l.b + (size_t)f.id * l.M * l.R;
-    u4_t w[kOut];
-#pragma unroll
-    for (int o = 0; o < kOut; o++) {
-        const int m = m0 + o * per;
-        w[o] = m < l.M ? load_rank<WHOLE>(b + (size_t)m * l.R, r0, f.rank) : u4_t{0, 0, 0, 0};
-    }
-    f4_t t[NR][2];
-    float y[kOut][NR];
-#pragma unroll
-    for (int i = 0; i < NR; i++) {
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-            t[i][h] = r0 < f.rank ? *(const f4_t*)(l.t + (size_t)f.row[i] * l.Rp + r0 + 4 * h) : f4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int o = 0; o < kOut; o++) {
-            const int m = m0 + o * per;
-            y[o][i] = l.base && sub == 0 && m < l.M ? l.base[f.row[i] * l.bs + m] : 0.f;
-        }
-    }
-#pragma unroll
-    for (int o = 0; o < kOut; o++) {
-        float s[NR];
-#pragma unroll
-        for (int i = 0; i < NR; i++) s[i] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float we = widen<KIND>(e % 2 ? w[o][e / 2] >> 16 : w[o][e / 2] & 0xffffu);
-#pragma unroll
-            for (int i = 0; i < NR; i++) s[i] = fmaf(we, t[i][e / 4][e % 4], s[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < NR; i++) {
-            for (int k = 0; k < lg; k++) s[i] += __shfl_xor(s[i], 1 << k, kWave);
-            const int m = m0 + o * per;
-            if (sub == 0 && m < l.M && i < f.rows) l.out[f.row[i] * l.os + m] = y[o][i] + s[i];
-        }
-    }
+    Expand<KIND, WHOLE, 256, kOut, NR>(l, f, lg).finish(l, f, [&](int i, int r) {
+        return *(const f4_t*)(l.t + (size_t)f.row(i) * l.Rp + r);
+    });
 }
-
 template <int KIND, bool WHOLE>
 __global__ __launch_bounds__(256) void lora_expand_few(Lora l, int lg) {
     const Few f = few_of(l);
     if (!f.rows) return;
-    if (f.rank <= 0) {                                   // no adapter: base; not in the table: NaN
-        if (f.rank < 0 && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(&ibh_lora_err, IBH_DEVERR_LORA);
-        if (f.rank == 0 && l.out == l.base) return;
-        const int span = (256 >> lg) * kOut, m0 = blockIdx.y * span;
-        for (int i = 0; i < f.rows; i++)
-            for (int m = m0 + threadIdx.x; m < min(m0 + span, l.M); m += 256)
-                l.out[f.at(i) * l.os + m] = f.rank < 0 ? __builtin_nanf("") : l.base ? l.base[f.at(i) * l.bs + m] : 0.f;
-        return;
-    }
-    if (f.rows == 1) expand_rows<KIND, WHOLE, 1>(l, f, lg);
+    if (f.rank <= 0) few_without(l, f, (256 >> lg) * kOut);
+    else if (f.rows == 1) expand_rows<KIND, WHOLE, 1>(l, f, lg);
     else if (f.rows == 2) expand_rows<KIND, WHOLE, 2>(l, f, lg);
     else expand_rows<KIND, WHOLE, 4>(l, f, lg);
+}
+
+// Both products in one launch where an adapter's a is small: every block that
+// takes outputs of some rows works their t out by itself.
+template <int KIND, bool WHOLE, int NR>
+__device__ __forceinline__ void both_rows(const Lora& l, const Few& f, int lg, float (*part)[kBoth / 64], float* t) {
+    const Expand<KIND, WHOLE, kBoth, kBothOut, NR> e(l, f, lg);
+    for (int r0 = 0; r0 < (f.rank + 7) / 8 * 8; r0 += 8) {
+        if (r0) __syncthreads();
+        shrink_rows<KIND, WHOLE, kBoth, 8, NR>(l, f, r0, part, [&](int i, int r, float v) { t[i * l.Rp + r] = v; });
+    }
+    __syncthreads();
+    e.finish(l, f, [&](int i, int r) { return *(const f4_t*)(t + min(i, f.rows - 1) * l.Rp + r); });
+}
+template <int KIND, bool WHOLE>
+__global__ __launch_bounds__(kBoth) void lora_both_few(Lora l, int lg) {
+    __shared__ float part[32][kBoth / 64];
+    __shared__ __align__(16) float t[4 * IBH_LORA_MAX_RANK];
+    const Few f = few_of(l);
+    if (!f.rows) return;
+    if (f.rank <= 0) few_without(l, f, (kBoth >> lg) * kBothOut);
+    else if (f.rows == 1) both_rows<KIND, WHOLE, 1>(l, f, lg, part, t);
+    else if (f.rows == 2) both_rows<KIND, WHOLE, 2>(l, f, lg, part, t);
+    else both_rows<KIND, WHOLE, 4>(l, f, lg, part, t);
 }
 
 // ── more rows: tiles of one adapter's rows on the matrix cores ───────────────
@@ -592,13 +638,23 @@ bool adapters_ok(const ibh_lora_adapters* l, const char* who) {
 
 // How a call is cut.
 struct LoraPlan {
-    bool few;
+    bool few, both;
+    int lg;                                              // lanes of a row of b, their logarithm
     int Rp, S, max_tiles;
     size_t plan_bytes, bytes;
 };
 LoraPlan plan_of(const ibh_lora_adapters* l, int B) {
     LoraPlan p;
     p.few = B <= kFew;
+    p.lg = 0;
+    while (8 << p.lg < l->rank) p.lg++;
+    // One launch where a is small and a block a CU holds all outputs: it reads a
+    // once for each block of outputs, but spares a launch and a workspace (kernels
+    // alone, one and two launches: 1 x 2048, rank 8: 4.5 and 6.1 us; 32 x 4096 of
+    // rank 16: 8.0 and 7.4, 10 and 14 with the call; M 14336 there: 15 and 9.8;
+    // 64 x 4096 of rank 32: 25 and 13).
+    const int span = (kBoth >> p.lg) * kBothOut;
+    p.both = p.few && (size_t)l->rank * l->N <= kBothMost && (size_t)B * ((l->M + span - 1) / span) <= 256;
     p.Rp = (l->rank + 7) / 8 * 8;
     p.S = 1;
     p.max_tiles = 0;
@@ -611,40 +667,47 @@ LoraPlan plan_of(const ibh_lora_adapters* l, int B) {
         // have under way at once
         p.S = min(kMaxSplit, (l->N + 511) / 512);
     }
-    p.bytes = p.plan_bytes + (size_t)p.S * B * p.Rp * 4;
+    p.bytes = p.both ? 0 : p.plan_bytes + (size_t)p.S * B * p.Rp * 4;
     return p;
 }
 
 template <int KIND, bool WHOLE>
-void launch_shrink(const Lora& l, bool few, hipStream_t st) {
+void launch_shrink(const Lora& l, const LoraPlan& p, hipStream_t st) {
     const dim3 grid(l.S, l.max_tiles, (l.R + 63) / 64);  // a tile's splits beside each other
-    if (few) lora_shrink_few<KIND, WHOLE><<<dim3(l.B, (l.Rp + 3) / 4), 256, 0, st>>>(l);
+    if (p.few) lora_shrink_few<KIND, WHOLE><<<dim3(l.B, (l.Rp + 3) / 4), 256, 0, st>>>(l);
     else if (l.R <= 16) lora_shrink_tile<KIND, WHOLE, 1><<<grid, 256, 0, st>>>(l);
     else if (l.R <= 32) lora_shrink_tile<KIND, WHOLE, 2><<<grid, 256, 0, st>>>(l);
     else lora_shrink_tile<KIND, WHOLE, 4><<<grid, 256, 0, st>>>(l);
 }
 template <int KIND, bool WHOLE>
-void launch_expand(const Lora& l, bool few, hipStream_t st) {
-    if (few) {
-        int lg = 0;
-        while (8 << lg < l.R) lg++;
-        const int span = (256 >> lg) * kOut;
-        lora_expand_few<KIND, WHOLE><<<dim3(l.B, (l.M + span - 1) / span), 256, 0, st>>>(l, lg);
-    } else
+void launch_expand(const Lora& l, const LoraPlan& p, int lg, hipStream_t st) {
+    const int span = (256 >> lg) * kOut;
+    if (p.few) lora_expand_few<KIND, WHOLE><<<dim3(l.B, (l.M + span - 1) / span), 256, 0, st>>>(l, lg);
+    else
         lora_expand_tile<KIND, WHOLE><<<dim3((l.M + kSpan - 1) / kSpan, l.max_tiles), 256,
                                         max(3 * kTile * ((l.R + 31) / 32 * 32 + 8) * 2, kTile * (kSpan + 4) * 4), st>>>(l);
 }
 template <int KIND>
-int launch(const Lora& l, bool few, hipStream_t st) {
-    if (!few) {
+int launch(const Lora& l, const LoraPlan& p, hipStream_t st) {
+    const int lg = p.lg;
+    const bool whole_a = l.N % 8 == 0, whole_b = l.R % 8 == 0 && l.M % 4 == 0;
+    if (p.both) {
+        const int span = (kBoth >> lg) * kBothOut;
+        const dim3 grid(l.B, (l.M + span - 1) / span);
+        if (whole_a && whole_b) lora_both_few<KIND, true><<<grid, kBoth, 0, st>>>(l, lg);
+        else lora_both_few<KIND, false><<<grid, kBoth, 0, st>>>(l, lg);
+        IBH_CHECK_LAUNCH("ibh_lora");
+        return IBH_OK;
+    }
+    if (!p.few) {
         lora_plan<<<1, 1024, 0, st>>>(l);
         IBH_CHECK_LAUNCH("ibh_lora");
     }
-    if (l.N % 8 == 0) launch_shrink<KIND, true>(l, few, st);
-    else launch_shrink<KIND, false>(l, few, st);
+    if (whole_a) launch_shrink<KIND, true>(l, p, st);
+    else launch_shrink<KIND, false>(l, p, st);
     IBH_CHECK_LAUNCH("ibh_lora");
-    if (l.R % 8 == 0 && l.M % 4 == 0) launch_expand<KIND, true>(l, few, st);
-    else launch_expand<KIND, false>(l, few, st);
+    if (whole_b) launch_expand<KIND, true>(l, p, lg, st);
+    else launch_expand<KIND, false>(l, p, lg, st);
     IBH_CHECK_LAUNCH("ibh_lora");
     return IBH_OK;
 }
@@ -693,14 +756,17 @@ extern "C" int ibh_lora(const ibh_lora_adapters* l, float* out, const float* bas
         ibh_set_error("ibh_lora: %d rows are more than one launch takes", B);
         return IBH_ERROR_PARAM;
     }
-    uint8_t* w = (uint8_t*)(ws ? (ws_bytes >= p.bytes && !((uintptr_t)ws & 15) ? ws : nullptr) : ibh_workspace(p.bytes));
-    if (!w) {
-        ibh_set_error("ibh_lora: a workspace of %zu bytes on 16 bytes is needed", p.bytes);
-        return IBH_ERROR_MEMORY;
+    uint8_t* w = nullptr;
+    if (p.bytes) {
+        w = (uint8_t*)(ws ? (ws_bytes >= p.bytes && !((uintptr_t)ws & 15) ? ws : nullptr) : ibh_workspace(p.bytes));
+        if (!w) {
+            ibh_set_error("ibh_lora: a workspace of %zu bytes on 16 bytes is needed", p.bytes);
+            return IBH_ERROR_MEMORY;
+        }
     }
     const Lora a{(const uint16_t*)l->a, (const uint16_t*)l->b, l->scales, l->ranks, l->n, l->rank, l->N, l->M, out, base, x,
                  ids, B, (size_t)out_stride, (size_t)base_stride, (size_t)x_stride, (float*)(w + p.plan_bytes), p.Rp, p.S,
                  (Tile*)w, p.max_tiles};
     hipStream_t st = ibh_resolve_stream(stream);
-    return l->kind == IBH_F16 ? launch<IBH_F16>(a, p.few, st) : launch<IBH_BF16>(a, p.few, st);
+    return l->kind == IBH_F16 ? launch<IBH_F16>(a, p, st) : launch<IBH_BF16>(a, p, st);
 }

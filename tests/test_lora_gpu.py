@@ -89,6 +89,13 @@ def test_rows(B, n):
     one(B, 256, 136, 16, n, "bf16", spread(B, n, B), seed=B)
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("B", [1, 7, 64])
+@pytest.mark.parametrize("rank,N", [(16, 4096), (16, 4104), (17, 4096), (128, 512), (128, 520), (1, 60000), (8, 9000), (64, 5000)])
+def test_one_launch_and_two(rank, N, B, kind):
+    one(B, N, 300, rank, 5, kind, spread(B, 5, rank), seed=rank + N)
+
+
 @pytest.mark.parametrize("B", [20, 150])
 def test_uneven_ranks(B):
     for kind in TYPES:
@@ -245,5 +252,6 @@ def test_wrappers_refuse():
                           (ValueError, (out[:1].expand(3, 32), x, a, b, ids), {}), (_lib.IbhError, (x[:, :32], x, a, b, ids), {})):
         with pytest.raises(err):
             ops.lora(*args, **kw)
+    a, b, s = (t.cuda() for t in adapters(2, 64, 4096, 32, "fp16", 0))
     with pytest.raises(_lib.IbhError):
-        ops.lora(out, x, a, b, ids, ws=torch.empty(4, dtype=torch.uint8, device="cuda"))
+        ops.lora(out, torch.zeros(3, 4096, device="cuda"), a, b, ids, ws=torch.empty(4, dtype=torch.uint8, device="cuda"))

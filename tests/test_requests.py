@@ -97,12 +97,20 @@ def test_lora_refuses_overlaps(bad):
 
 
 def test_lora_refuses_workspaces():
-    need = _lib.lib().ibh_lora_workspace_bytes(C.byref(lora_desc()), B)
+    big = lora_desc(rank=64, N=4096)
+    need = _lib.lib().ibh_lora_workspace_bytes(C.byref(big), B)
     assert need > 0
-    refused("ibh_lora", *lora_args(size=need - 1), code=-3)
-    refused("ibh_lora", *lora_args(ws=9 * GAP + 4), code=-3)
-    assert _lib.lib().ibh_lora_workspace_bytes(C.byref(lora_desc()), 0) == 0
+    refused("ibh_lora", *lora_args(big, xs=4096, size=need - 1), code=-3)
+    refused("ibh_lora", *lora_args(big, xs=4096, ws=9 * GAP + 4), code=-3)
+    assert _lib.lib().ibh_lora_workspace_bytes(C.byref(big), 0) == 0
     refused("ibh_lora", None, *lora_args()[1:])
+
+
+def test_more_rows_than_a_launch_takes_are_refused():
+    far = [k << 40 for k in range(1, 9)]
+    d = _lib.LoraDesc(far[0], far[1], far[2], far[3], 4, 16, 64, 64, 0)
+    assert "launch" in refused("ibh_lora", C.byref(d), far[4], None, far[5], far[6], 1 << 22, 64, 0, 64, far[7], 1 << 40, None)
+    assert "launch" in refused("ibh_logprobs", far[0], far[1], None, None, far[2], far[3], 100, 1 << 24, 100, 1, 0, None, 0, None)
 
 
 def log_args(**c):
