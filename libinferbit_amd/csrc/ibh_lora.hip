@@ -49,7 +49,7 @@ struct Lora {
 };
 // Rows of one adapter.  All that a block has to know in one place, so that it
 // waits for memory once before its first row.
-struct Tile {
+struct __align__(16) Tile {
     int32_t id, rank, count;        // rank -1: not in the table, 0: no adapter; count 0: no tile
     float scale;
     int32_t row[kTile];
@@ -375,10 +375,7 @@ __global__ __launch_bounds__(1024) void lora_plan(Lora l) {
         const float scale = k >= l.n || !l.scales ? 1.f : per == 1 ? scale0 : l.scales[k];
         count[k] = it * kTile;                           // from here on: the place of its first row,
         more[k] = it * kTile + first;                    // and of its next one
-        for (int j = 0; j < c; j += kTile, it++) {
-            Tile& t = l.tiles[it];
-            t.id = k, t.rank = rank, t.count = min(kTile, c - j), t.scale = scale;
-        }
+        for (int j = 0; j < c; j += kTile, it++) *(int4*)&l.tiles[it] = make_int4(k, rank, min(kTile, c - j), __float_as_int(scale));
     }
     for (int i = all + tid; i < l.max_tiles; i += 1024) l.tiles[i].count = 0;
     __syncthreads();
