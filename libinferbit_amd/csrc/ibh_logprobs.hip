@@ -12,6 +12,7 @@ using namespace ibh;
 constexpr int kWaves = 4, kManyWaves = 16;               // of a block
 constexpr int kPiece = 1024;                             // logits that a wavefront takes at a time
 constexpr int kHeld = 256;                               // candidates that it holds
+constexpr int kManyRows = 256;                           // that fill the card by themselves
 constexpr int kMaxShares = 64;                          // blocks that share a row, at most
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -214,7 +215,7 @@ __global__ __launch_bounds__(W * 64, W == kWaves ? 8 : 4) void logprobs_kernel(L
     // for those outside the share
     f4_t next[4];
     bool begin = true;
-    auto from = [&](int j) { return (const char*)z + (uint32_t)(j * 4); };   // V is at most 2^30
+    auto from = [&](int j) { return (const char*)z + (uint32_t)j * 4u; };    // V is at most 2^30
     for (int at = v0 + (wave - W) * kPiece; at < v1; at += W * kPiece) {
         f4_t v[4];
 #pragma unroll
@@ -319,13 +320,16 @@ __global__ __launch_bounds__(kWaves * 64) void logprobs_join(LogArgs a) {
     finish<kWaves>(a, row, t, best);
 }
 
-// How a call is cut.  A row of one round of four wavefronts' pieces, or rows
-// that fill the card by themselves, take a block of four.  Few rows of up to two
-// rounds of sixteen take a block of those: one launch instead of two (1 x 32000,
-// 5 best: 10.3 us, 10.7 in two kernels and a launch; 255 rows, 20 best: 16 and
-// 20; but 1 x 64000 14 and 11, 1 x 4000 7.3 and 5.8 in one block of four).
-// Otherwise a row is shared by blocks, whole rounds each, as many as fill the
-// card, and the shares are joined.
+// How a call is cut.  Rows that fill the card by themselves, and rows of one
+// round of four wavefronts' pieces, take a block of four (300 x 128000, 20 best:
+// 48 us, 45 and a launch where they are shared; 600 x 64000, 8 best: 39 and 44;
+// 60 and 52 in blocks of sixteen).  Fewer rows of up to two rounds of sixteen
+// take a block of those: one launch instead of two (1 x 32000, 5 best: 10.3 us,
+// 10.7 in two kernels and a launch; 255 rows, 20 best: 16 and 20; but 1 x 64000
+// 14 and 11, 1 x 4000 7.3 and 5.8 in one block of four).  Otherwise a row is
+// shared by blocks, whole rounds each, and the shares are joined (32 x 128000, 20
+// best, 256, 512, 1024 and 2048 blocks in all: 20, 18.2, 18.3 and 17.2 us; 8 x
+// 260000: 15.7, 14.5, 15 and 14.7).
 struct LogPlan {
     int W, S, seg;
     size_t part, bytes;
@@ -333,9 +337,9 @@ struct LogPlan {
 LogPlan plan_of(int V, int B, int k) {
     LogPlan p;
     const bool one = V + 3 <= kWaves * kPiece;           // up to three in front of the row
-    p.W = !one && B <= 256 && V + 3 <= 2 * kManyWaves * kPiece ? kManyWaves : kWaves;
+    p.W = !one && B < kManyRows && V + 3 <= 2 * kManyWaves * kPiece ? kManyWaves : kWaves;
     const int round = p.W * kPiece, rounds = (V + 3 + round - 1) / round;
-    const int want = p.W == kManyWaves ? 1 : max(1, min(min(rounds, kMaxShares), (1024 + B - 1) / B));
+    const int want = p.W == kManyWaves || B >= kManyRows ? 1 : min(min(rounds, kMaxShares), (512 + B - 1) / B);
     const int each = (rounds + want - 1) / want;
     p.seg = each * round;
     p.S = (rounds + each - 1) / each;

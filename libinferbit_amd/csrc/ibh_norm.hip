@@ -93,25 +93,32 @@ __device__ __forceinline__ double block_sum(double v, double* part) {
     return s;
 }
 
-// Columns j .. j + 3 of a row.  p = h * weight (rounded), y = p * r.  A code is
+// Columns j .. j + 3 of a row.  p = h * weight (rounded), y = p * r, r in 64
+// bits (beside subnormal numbers it is beyond fp32).  A code is
 // 127 p / max|p| of its 128 columns: r cancels, so codes do not depend on how
 // the squares were summed.  In lowest terms a quotient lies 2^-33 or more from
 // a border that it does not hit (p and max|p| have 24 bits, and the lowest
 // border is max|p| / 254, 8 bits down), the product here is within 2^-43: with
 // 2^-38 added before the fraction is cut off, halves go away from zero and
 // nothing else changes sides.
-__device__ __forceinline__ void emit4(const NormArgs& a, size_t row, int j, f4_t p, float r) {
-    if (a.y) store4(a.y + row * a.N, j, a.N, p * r);
+__device__ __forceinline__ void emit4(const NormArgs& a, size_t row, int j, f4_t p, double r) {
+    if (a.y) {
+        f4_t y;
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[i] = (float)((double)p[i] * r);
+        store4(a.y + row * a.N, j, a.N, y);
+    }
     if (!a.q) return;
     uint32_t bits = 0;                                   // of the largest |p|: as whole numbers a NaN is above all
 #pragma unroll
     for (int i = 0; i < 4; i++) bits = max(bits, __float_as_uint(p[i]) & 0x7fffffffu);
     bits = row_umax(bits);
     bits = max(bits, (uint32_t)__shfl_xor((int)bits, 16, 32));   // 32 lanes hold a group
-    const float m = __builtin_bit_cast(float, bits), top = m * r;
-    const bool sound = bits < 0x7f800000u && top == top, zero = !sound || top < 1e-10f;
+    const float m = __builtin_bit_cast(float, bits);
+    const double top = (double)m * r;
+    const bool sound = bits < 0x7f800000u && top == top, zero = !sound || top < 1e-10;
     if (j >= a.N) return;
-    if ((j & 127) == 0) a.s[row * a.G + j / 128] = !sound ? __builtin_nanf("") : zero ? 1e-10f : top / 127.0f;
+    if ((j & 127) == 0) a.s[row * a.G + j / 128] = !sound ? __builtin_nanf("") : zero ? 1e-10f : (float)(top * (1.0 / 127.0));
     const double k = 127.0 * rcp_f64((double)m);
     uint32_t packed = 0;
 #pragma unroll
@@ -158,7 +165,7 @@ __global__ __launch_bounds__(T) void norm_row_kernel(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; i++) sum = __builtin_fma((double)h[e][i], (double)h[e][i], sum);
     }
-    const float r = (float)rsqrt_f64(block_sum<T>(sum, part) / a.N + (double)a.eps);
+    const double r = rsqrt_f64(block_sum<T>(sum, part) / a.N + (double)a.eps);
 #pragma unroll
     for (int e = 0; e < E; e++) emit4(a, row, (e * T + threadIdx.x) * 4, h[e] * w[e], r);
 }
@@ -178,7 +185,7 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; i++) sum = __builtin_fma((double)v[i], (double)v[i], sum);
     }
-    const float r = (float)rsqrt_f64(block_sum<1024>(sum, part) / a.N + (double)a.eps);
+    const double r = rsqrt_f64(block_sum<1024>(sum, part) / a.N + (double)a.eps);
     // whole blocks of columns, so that all lanes of a group are there for its maximum
     for (int base = 0; base < a.N; base += 4096) {
         const int j = base + threadIdx.x * 4;
@@ -186,6 +193,11 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a) {
         if (d && !h) v += load4(d, j, a.N);
         emit4(a, row, j, v * load4(a.weight, j, a.N), r);
     }
+}
+
+template <int T, int E>
+void launch(const NormArgs& a, int B, hipStream_t st) {
+    norm_row_kernel<T, E><<<B, T, 0, st>>>(a);
 }
 
 }  // namespace
@@ -226,11 +238,19 @@ extern "C" int ibh_add_rmsnorm(float* y, int8_t* q, float* s, float* h, const fl
     }
     const NormArgs a{y, s, h, q, x, delta, weight, eps, N, G, (size_t)x_stride, (size_t)delta_stride};
     hipStream_t st = ibh_resolve_stream(stream);
-    if (N <= 1024) norm_row_kernel<256, 1><<<B, 256, 0, st>>>(a);
-    else if (N <= 2048) norm_row_kernel<256, 2><<<B, 256, 0, st>>>(a);
-    else if (N <= 4096) norm_row_kernel<256, 4><<<B, 256, 0, st>>>(a);
-    else if (N <= 8192) norm_row_kernel<512, 4><<<B, 512, 0, st>>>(a);
-    else if (N <= 16384) norm_row_kernel<1024, 4><<<B, 1024, 0, st>>>(a);
+    // Threads by quads of columns: the fewest that hold the row for short rows
+    // (6000 x 200 in 64 threads 6.2 us, in 256 9.7; 4000 x 1000 in 128 11.0, in 256
+    // 13.2); then, for few rows, wide blocks, whose loads are all under way sooner
+    // (1 x 4096 in 512 threads 3.0 us, in 256 3.9; 64 rows 3.9 and 4.8; 512 rows
+    // 8.3 and 8.6), for many small ones, of which a CU holds more (4099 x 4096 in
+    // 512 50.5 us, in 256 47.1; 4099 x 2048 in 512 27.0, in 64 22.5).
+    const bool few = B <= 1024;
+    if (N <= 256) launch<64, 1>(a, B, st);
+    else if (N <= 1024) launch<128, 2>(a, B, st);
+    else if (N <= 2048) few ? launch<512, 1>(a, B, st) : launch<64, 8>(a, B, st);
+    else if (N <= 4096) few ? launch<512, 2>(a, B, st) : launch<256, 4>(a, B, st);
+    else if (N <= 8192) few ? launch<1024, 2>(a, B, st) : launch<512, 4>(a, B, st);
+    else if (N <= 16384) launch<1024, 4>(a, B, st);
     else norm_long_kernel<<<B, 1024, 0, st>>>(a);
     IBH_CHECK_LAUNCH("ibh_add_rmsnorm");
     return IBH_OK;

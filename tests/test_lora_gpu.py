@@ -219,6 +219,31 @@ def test_two_streams_at_once():
         check(out.cpu().numpy(), None, x.numpy(), a, b, ids, s.numpy(), None)
 
 
+@pytest.mark.parametrize("B,rank", [(6, 64), (90, 16)])
+def test_two_graphs_at_once(B, rank):
+    """Each with a workspace of its own, replayed side by side on two streams."""
+    sets = [(adapters(4, rank, 2048, 256, "bf16", k), torch.randn(B, 2048), spread(B, 4, k)) for k in range(2)]
+    dev = [([t.cuda() for t in ab], x.cuda(), torch.tensor(ids, dtype=torch.int32, device="cuda")) for ab, x, ids in sets]
+    outs, graphs, streams = [torch.empty(B, 256, device="cuda") for _ in sets], [], [torch.cuda.Stream() for _ in sets]
+    for (ab, x, ids), out in zip(dev, outs):
+        ops.lora(out, x, ab[0], ab[1], ids, scales=ab[2])
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ops.lora(out, x, ab[0], ab[1], ids, scales=ab[2])
+        graphs.append(g)
+    for _ in range(10):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for ((a, b, s), x, ids), out in zip(sets, outs):
+            check(out.cpu().numpy(), None, x.numpy(), a, b, ids, s.numpy(), None)
+
+
 def test_no_rows():
     a, b, s = (t.cuda() for t in adapters(2, 8, 64, 32, "fp16", 0))
     ops.lora(torch.empty(0, 32, device="cuda"), torch.empty(0, 64, device="cuda"), a, b,

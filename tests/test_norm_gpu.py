@@ -81,6 +81,16 @@ def test_many_rows(B):
     check(run(x, d, w, 1e-5), x, d, w, 1e-5)
 
 
+@pytest.mark.parametrize("N", [200, 1000, 1026, 2048, 2051, 4096, 4100, 8190])
+def test_more_rows_than_wide_blocks_take(N):
+    """The many rows of a call are a few, again and again: equal rows come out equal, the first ones are right."""
+    x, d, w = inputs(3, N, N)
+    o = run(np.tile(x, (350, 1)), np.tile(d, (350, 1)), w, 1e-5)
+    check({k: v[:3] for k, v in o.items()}, x, d, w, 1e-5)
+    for k, v in o.items():
+        np.testing.assert_array_equal(v, np.tile(v[:3], (350, 1)), err_msg=k)
+
+
 def test_codes_at_borders():
     """Quotients of 127 p / max|p| at halves, and as near to them as floats come."""
     rng = np.random.default_rng(5)
@@ -114,6 +124,17 @@ def test_values_at_the_ends_of_the_range(N):
         q, s = R.codes(p[i], r[i, 0])
         np.testing.assert_array_equal(o["q"][i], q)
         np.testing.assert_array_equal(np.isnan(o["s"][i]), np.isnan(s))
+
+
+@pytest.mark.parametrize("N", [300, 4096, 17000])
+def test_rows_of_subnormal_numbers(N):
+    """Without eps the factor is beyond fp32, y and the scales are ordinary numbers."""
+    x, _, w = inputs(3, N, 4)
+    x[0] *= np.float32(1e-39)
+    x[1] *= np.float32(1e-42)
+    x[2] *= np.float32(1e-37)
+    check(run(x, None, w, 0.0, h=False), x, None, w, 0.0)
+    check(run(x, None, w, 1e-30, h=False), x, None, w, 1e-30)
 
 
 def test_a_row_of_zeros_without_eps():
