@@ -91,6 +91,14 @@ __device__ __forceinline__ void lds_only_barrier() {
     __builtin_amdgcn_s_barrier();
 }
 
+// The same with fences of LDS alone, which the compiler respects as well: no LDS
+// access moves across it, loads from memory stay under way.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // Butterfly sum over the 64 lanes of a wavefront (every lane gets the total).
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll

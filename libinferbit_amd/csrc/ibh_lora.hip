@@ -417,13 +417,6 @@ __device__ __forceinline__ void pieces(u4_t v, v8bf* p) {
     }
 }
 
-// A barrier that orders LDS alone: loads from memory stay under way across it.
-__device__ __forceinline__ void lds_barrier() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
 // t of a tile of rows and RT * 16 ranks over a share of the columns.  Each
 // wavefront takes 64 columns of all rows at a time, the next 64 under way: every
 // number of x is loaded, cut into pieces and multiplied by one lane, straight in
