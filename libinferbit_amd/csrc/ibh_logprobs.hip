@@ -287,37 +287,39 @@ __global__ __launch_bounds__(W * 64, W == kWaves ? 8 : 4) void logprobs_kernel(L
     if ((int)threadIdx.x < a.k) a.keys[me * a.k + threadIdx.x] = lane < best.n ? best.held[lane] : 0;
 }
 
-// The shares of a row joined.
-__global__ __launch_bounds__(kWaves * 64) void logprobs_join(LogArgs a) {
-    __shared__ Shared<kWaves> sh;
-    const int tid = threadIdx.x, wave = tid >> 6;
+// The shares of a row joined, by one wavefront: a few hundred keys, and all its
+// time is the code that it has to fetch.
+__global__ __launch_bounds__(64) void logprobs_join(LogArgs a) {
+    __shared__ uint64_t held[kHeld];
+    const int lane = threadIdx.x, n = a.S * a.k;
     const size_t row = blockIdx.x;
-    const uint64_t* keys = a.keys + row * a.S * a.k;
-    const int n = a.S * a.k;
-    constexpr int kAll = kMaxShares * IBH_LOGPROBS_MAX_K / (kWaves * 64);
-    uint64_t key[kAll];
+    const uint64_t* keys = a.keys + row * n;
+    constexpr int kEach = 16;                            // keys of a lane under way at once
+    uint64_t key[kEach];
+    auto fetch = [&](int at) {
 #pragma unroll
-    for (int i = 0; i < kAll; i++) {
-        const int j = i * kWaves * 64 + tid;
-        key[i] = j < n ? keys[j] : 0;
-    }
+        for (int i = 0; i < kEach; i++) key[i] = at + i * 64 + lane < n ? keys[at + i * 64 + lane] : 0;
+    };
+    fetch(0);
     Sums t{-__builtin_inff(), 0.f, 0.f};
-    if (tid < a.S) {
-        const f4_t v = *(const f4_t*)(a.part + (row * a.S + tid) * 4);
+    if (lane < a.S) {
+        const f4_t v = *(const f4_t*)(a.part + (row * a.S + lane) * 4);
         t = {v[0], v[1], v[2]};
     }
-    Best best{sh.held[wave], 0, a.k, kNothing};
-    if (a.k) {
+    t = wave_join(t);
+    Best best{held, 0, a.k, kNothing};
+    for (int at = 0; at < n; at += kEach * 64) {
+        if (at) fetch(at);
         uint64_t top = 0;
 #pragma unroll
-        for (int i = 0; i < kAll; i++) top = key[i] > top ? key[i] : top;
+        for (int i = 0; i < kEach; i++) top = key[i] > top ? key[i] : top;
         best.first((uint32_t)(top >> 32));
 #pragma unroll
-        for (int i = 0; i < kAll; i++)
-            if (i * kWaves * 64 < n) best.offer(key[i]);
+        for (int i = 0; i < kEach; i++)
+            if (at + i * 64 < n) best.offer(key[i]);
     }
-    t = gather(t, best, sh);
-    finish<kWaves>(a, row, t, best);
+    best.sort();
+    finish<1>(a, row, t, best);
 }
 
 // How a call is cut.  Rows that fill the card by themselves, and rows of one
@@ -401,7 +403,7 @@ extern "C" int ibh_logprobs(float* out, float* entropy, int32_t* top_ids, float*
     else logprobs_kernel<kManyWaves><<<B * p.S, kManyWaves * 64, 0, st>>>(a);
     IBH_CHECK_LAUNCH("ibh_logprobs");
     if (p.S > 1) {
-        logprobs_join<<<B, kWaves * 64, 0, st>>>(a);
+        logprobs_join<<<B, 64, 0, st>>>(a);
         IBH_CHECK_LAUNCH("ibh_logprobs");
     }
     return IBH_OK;
