@@ -4,6 +4,14 @@
 // One pass over a row: every lane keeps the running maximum m, s = sum e^(z - m)
 // and e = sum e^(z - m) (z - m) of its logits, every wavefront the k best it has
 // seen.  log S = m + log s; entropy = log s - e / s.
+//
+// Memory bounds long calls: 2047 rows of 32003, 262 MB, take 50 us without
+// alternatives (5.2 TB/s, as a copy does), 57 with the 8 best and 63 with 20:
+// the candidates' instructions (a wavefront's bar is the k-th best of its first
+// 1024 logits, so each later piece has about k).  Short calls are chains: of the
+// 11.5 us of 32 x 128000 with the 20 best, 3.2 pass until the first logits are
+// there, 1.3 over the candidates, 0.6 over the sums, 2.5 over the wavefronts'
+// lists, and 4.5 us go to the launch that joins the shares.
 #include "ibh_common.h"
 
 namespace {
@@ -330,8 +338,8 @@ __global__ __launch_bounds__(64) void logprobs_join(LogArgs a) {
 // 10.7 in two kernels and a launch; 255 rows, 20 best: 16 and 20; but 1 x 64000
 // 14 and 11, 1 x 4000 7.3 and 5.8 in one block of four).  Otherwise a row is
 // shared by blocks, whole rounds each, and the shares are joined (32 x 128000, 20
-// best, 256, 512, 1024 and 2048 blocks in all: 20, 18.2, 18.3 and 17.2 us; 8 x
-// 260000: 15.7, 14.5, 15 and 14.7).
+// best, 256, 512, 1024 and 2048 blocks in all, without the join: 14.4, 11.5, 11.8
+// and 10.5 us; 8 x 260000: 9.6, 7.7, 7.6 and 7.7).
 struct LogPlan {
     int W, S, seg;
     size_t part, bytes;
