@@ -46,6 +46,8 @@ struct Lora {
     int S;                          // splits
     struct Tile* tiles;
     int max_tiles;
+    const uint16_t *a_end, *b_end;  // behind the arrays
+    const float *x_end, *base_end;
 };
 // Rows of one adapter.  All that a block has to know in one place, so that it
 // waits for memory once before its first row.
@@ -67,45 +69,55 @@ __device__ __forceinline__ int rank_of(const Lora& l, int id) {
     const int r = l.ranks ? l.ranks[id] : l.R;
     return r < 0 || r > l.R ? -1 : r;
 }
-// Loads from place j of n, zeros behind n.  WHOLE: n is a multiple of what is
-// loaded, which leaves the code for a rest away (every line of code that a
-// small launch runs through is one more wait for memory).
+// Loads from place j of a row of n, zeros behind n.  WHOLE: n is a multiple of
+// what is loaded.  Otherwise what lies behind the row is read with it and
+// masked, one by one only where the array ends (`end`): every line of code that a
+// small launch runs through is one more wait for memory.
 template <bool WHOLE>
-__device__ __forceinline__ f4_t load4(const float* p, int j, int N) {
+__device__ __forceinline__ f4_t load4(const float* p, int j, int n, const float* end) {
     f4_t v = {0.f, 0.f, 0.f, 0.f};
-    if (WHOLE ? j < N : j + 4 <= N) return *(const f4_t*)(p + j);
-    if constexpr (WHOLE) return v;
+    if (j >= n) return v;
+    if (WHOLE || p + j + 4 <= end) v = *(const f4_t*)(p + j);
+    else
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (j + i < N) v[i] = p[j + i];
+        for (int i = 0; i < 4; i++)
+            if (p + j + i < end) v[i] = p[j + i];
+    if constexpr (!WHOLE)
+#pragma unroll
+        for (int i = 1; i < 4; i++) v[i] = j + i < n ? v[i] : 0.f;
     return v;
 }
 template <bool WHOLE>
-__device__ __forceinline__ void store4(float* p, int j, int N, f4_t v) {
-    if (WHOLE ? j < N : j + 4 <= N) {
+__device__ __forceinline__ void store4(float* p, int j, int n, f4_t v) {
+    if (WHOLE ? j < n : j + 4 <= n) {
         *(f4_t*)(p + j) = v;
         return;
     }
     if constexpr (WHOLE) return;
 #pragma unroll
     for (int i = 0; i < 4; i++)
-        if (j + i < N) p[j + i] = v[i];
+        if (j + i < n) p[j + i] = v[i];
 }
+// Eight 16-bit numbers, likewise.
 template <bool WHOLE>
-__device__ __forceinline__ u4_t load8h(const uint16_t* p, int j, int n) {
+__device__ __forceinline__ u4_t load8h(const uint16_t* p, int j, int n, const uint16_t* end) {
     u4_t v = {0, 0, 0, 0};
-    if (WHOLE ? j < n : j + 8 <= n) return *(const u4h_t*)(p + j);
-    if constexpr (WHOLE) return v;
+    if (j >= n) return v;
+    if (WHOLE || p + j + 8 <= end) v = *(const u4h_t*)(p + j);
+    else
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (j + i < n) v[i / 2] |= (uint32_t)p[j + i] << (16 * (i % 2));
+        for (int i = 0; i < 8; i++)
+            if (p + j + i < end) v[i / 2] |= (uint32_t)p[j + i] << (16 * (i % 2));
+    if (!WHOLE && j + 8 > n)
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] &= (j + 2 * i < n ? 0xffffu : 0) | (j + 2 * i + 1 < n ? 0xffff0000u : 0);
     return v;
 }
 // Numbers j .. j + 7 of a row of b, zeros from `rank` on.  WHOLE: the row is
 // whole eights, so all of them may be read.
 template <bool WHOLE>
-__device__ __forceinline__ u4_t load_rank(const uint16_t* p, int j, int rank) {
-    if constexpr (!WHOLE) return load8h<false>(p, j, rank);
+__device__ __forceinline__ u4_t load_rank(const Lora& l, const uint16_t* p, int j, int rank) {
+    if constexpr (!WHOLE) return load8h<false>(p, j, rank, l.b_end);
     u4_t v = {0, 0, 0, 0};
     if (j < rank) v = *(const u4h_t*)(p + j);
     if (rank % 8 && j + 8 > rank)                        // j is a multiple of 8
@@ -151,6 +163,41 @@ __device__ __forceinline__ Few few_of(const Lora& l) {
     return f;
 }
 
+// The wavefront's sums of K numbers (2 .. 32): each step gives half of them away
+// to the lane across and takes the other half's, 31 exchanges for 32 numbers where
+// one sum after the other would take 32 times six.  Returns whose sum a[0] is
+// then, -1 in the lanes that hold copies.
+template <int K>
+__device__ __forceinline__ int wave_sums(float* a) {
+    const int lane = threadIdx.x & 63;
+    auto across = [](float v, int s) {
+        const int b = (int)__float_as_uint(v);
+        return s == 0 ? __uint_as_float(__builtin_amdgcn_mov_dpp(b, 0xB1, 0xF, 0xF, false)) :     // lane ^ 1
+               s == 1 ? __uint_as_float(__builtin_amdgcn_mov_dpp(b, 0x4E, 0xF, 0xF, false)) :     // lane ^ 2
+               s == 2 ? __uint_as_float(__builtin_amdgcn_mov_dpp(b, 0x128, 0xF, 0xF, false)) :    // lane ^ 8
+                        __shfl_xor(v, s == 3 ? 16 : s == 4 ? 32 : 4, kWave);
+    };
+    constexpr int bit[6] = {1, 2, 8, 16, 32, 4};
+    int index = 0, copy = 0;
+#pragma unroll
+    for (int s = 0; s < 6; s++) {
+        const int half = K >> (s + 1);
+        const uint32_t up = lane & bit[s] ? ~0u : 0u;    // a mask: picked by one, the numbers would go to memory
+        if (half) {
+#pragma unroll
+            for (int i = 0; i < half; i++) {
+                const uint32_t x = __float_as_uint(a[i]), y = __float_as_uint(a[i + half]);
+                a[i] = __uint_as_float((y & up) | (x & ~up)) + across(__uint_as_float((x & up) | (y & ~up)), s);
+            }
+            index += half & up;
+        } else {
+            a[0] += across(a[0], s);
+            copy |= up;
+        }
+    }
+    return copy ? -1 : index;
+}
+
 // RR ranks of an adapter times NR rows by T threads, which take eights of
 // columns; to t, rows Rp apart, zeros behind the adapter's rank.
 template <int KIND, bool WHOLE, int T, int RR, int NR, class Store>
@@ -167,11 +214,11 @@ __device__ __forceinline__ void shrink_rows(const Lora& l, const Few& f, int r0,
         u4_t w[RR];
         f4_t v[NR][2];
 #pragma unroll
-        for (int r = 0; r < RR; r++) w[r] = r < nr ? load8h<WHOLE>(a + (size_t)r * l.N, j, l.N) : u4_t{0, 0, 0, 0};
+        for (int r = 0; r < RR; r++) w[r] = r < nr ? load8h<WHOLE>(a + (size_t)r * l.N, j, l.N, l.a_end) : u4_t{0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < NR; i++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) v[i][h] = load4<WHOLE>(l.x + f.row(i) * l.xs, j + 4 * h, l.N);
+            for (int h = 0; h < 2; h++) v[i][h] = load4<WHOLE>(l.x + f.row(i) * l.xs, j + 4 * h, l.N, l.x_end);
 #pragma unroll
         for (int r = 0; r < RR; r++)
 #pragma unroll
@@ -181,13 +228,8 @@ __device__ __forceinline__ void shrink_rows(const Lora& l, const Few& f, int r0,
                 for (int i = 0; i < NR; i++) acc[r][i] = fmaf(we, v[i][e / 4][e % 4], acc[r][i]);
             }
     }
-#pragma unroll
-    for (int r = 0; r < RR; r++)
-#pragma unroll
-        for (int i = 0; i < NR; i++) {
-            const float s = wave_sum_dpp(acc[r][i]);
-            if ((tid & 63) == 0) part[r * NR + i][tid >> 6] = s;
-        }
+    const int at = wave_sums<RR * NR>(&acc[0][0]);
+    if (at >= 0) part[at][tid >> 6] = acc[0][0];
     __syncthreads();
     if (tid < RR * NR) {
         const int r = tid / NR, i = tid % NR;
@@ -226,7 +268,7 @@ struct Expand {
 #pragma unroll
         for (int o = 0; o < OUT; o++) {
             const int m = m0 + o * per;
-            w[o] = m < l.M ? load_rank<WHOLE>(b + (size_t)m * l.R, 8 * sub, f.rank) : u4_t{0, 0, 0, 0};
+            w[o] = m < l.M ? load_rank<WHOLE>(l, b + (size_t)m * l.R, 8 * sub, f.rank) : u4_t{0, 0, 0, 0};
 #pragma unroll
             for (int i = 0; i < NR; i++) y[o][i] = l.base && sub == 0 && m < l.M ? l.base[f.row(i) * l.bs + m] : 0.f;
         }
@@ -433,7 +475,7 @@ __global__ __launch_bounds__(256, RT <= 2 ? 3 : 2) void lora_shrink_tile(Lora l)
     __shared__ v4f join[4][2 * RT][64];
     const Tile& tl = l.tiles[blockIdx.y];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane % 16, q = lane / 16;
-    int row[2] = {tl.row[c], tl.row[16 + c]};
+    const int row[2] = {tl.row[c], tl.row[16 + c]};
     const int id = tl.id, rank = tl.rank, count = tl.count, r0 = blockIdx.z * RT * 16;
     const float scale = tl.scale;
     if (!count || r0 >= (rank + 7) / 8 * 8) return;
@@ -458,9 +500,9 @@ __global__ __launch_bounds__(256, RT <= 2 ? 3 : 2) void lora_shrink_tile(Lora l)
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) p.x[h][k][e] = load4<WHOLE>(xp[h], k0 + 32 * k + 4 * e, l.N);
+                for (int e = 0; e < 2; e++) p.x[h][k][e] = load4<WHOLE>(xp[h], k0 + 32 * k + 4 * e, l.N, l.x_end);
 #pragma unroll
-            for (int i = 0; i < RT; i++) p.a[i][k] = load8h<WHOLE>(ap[i], k0 + 32 * k, l.N);
+            for (int i = 0; i < RT; i++) p.a[i][k] = load8h<WHOLE>(ap[i], k0 + 32 * k, l.N, l.a_end);
         }
     };
     v4f acc[2][RT];
@@ -545,7 +587,7 @@ __global__ __launch_bounds__(256, 3) void lora_expand_tile(Lora l) {
     f4_t y[8];
 #pragma unroll
     for (int i = 0; i < 8; i++)
-        y[i] = l.base && i < mine ? load4<WHOLE>(l.base + row[i] * l.bs, m0 + 4 * lane, l.M) : f4_t{0.f, 0.f, 0.f, 0.f};
+        y[i] = l.base && i < mine ? load4<WHOLE>(l.base + row[i] * l.bs, m0 + 4 * lane, l.M, l.base_end) : f4_t{0.f, 0.f, 0.f, 0.f};
     if (rank <= 0) {                                     // no adapter: base; not in the table: NaN
         const float nan = __builtin_nanf("");
 #pragma unroll
@@ -559,7 +601,7 @@ __global__ __launch_bounds__(256, 3) void lora_expand_tile(Lora l) {
     u4_t w[4];
     auto fetch = [&](int k) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) w[j] = load_rank<WHOLE>(b[j], k * 32 + q * 8, rank);
+        for (int j = 0; j < 4; j++) w[j] = load_rank<WHOLE>(l, b[j], k * 32 + q * 8, rank);
     };
     fetch(0);
     const int ks = (rank + 31) / 32, kr = ks * 32 + 8;
@@ -658,8 +700,7 @@ LoraPlan plan_of(const ibh_lora_adapters* l, int B) {
     p.max_tiles = 0;
     p.plan_bytes = 0;
     if (!p.few) {
-        const int groups = min(l->n + 2, B);
-        p.max_tiles = B / kTile + groups;
+        p.max_tiles = B / kTile + min(l->n + 2, B);
         p.plan_bytes = sizeof(Tile) * (size_t)p.max_tiles;
         // the splits of a tile's columns: 512 columns a block, what its wavefronts
         // have under way at once
@@ -764,7 +805,8 @@ extern "C" int ibh_lora(const ibh_lora_adapters* l, float* out, const float* bas
     }
     const Lora a{(const uint16_t*)l->a, (const uint16_t*)l->b, l->scales, l->ranks, l->n, l->rank, l->N, l->M, out, base, x,
                  ids, B, (size_t)out_stride, (size_t)base_stride, (size_t)x_stride, (float*)(w + p.plan_bytes), p.Rp, p.S,
-                 (Tile*)w, p.max_tiles};
+                 (Tile*)w, p.max_tiles, (const uint16_t*)l->a + n * l->rank * l->N,
+                 (const uint16_t*)l->b + n * l->rank * l->M, x + xb / 4, base ? base + bb / 4 : nullptr};
     hipStream_t st = ibh_resolve_stream(stream);
     return l->kind == IBH_F16 ? launch<IBH_F16>(a, p, st) : launch<IBH_BF16>(a, p, st);
 }
