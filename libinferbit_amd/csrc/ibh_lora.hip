@@ -280,23 +280,31 @@ struct Expand {
         for (int i = 0; i < NR; i++)
 #pragma unroll
             for (int h = 0; h < 2; h++) t[i][h] = 8 * sub < f.rank ? load(i, 8 * sub + 4 * h) : f4_t{0.f, 0.f, 0.f, 0.f};
+        float s[OUT][NR];
 #pragma unroll
         for (int o = 0; o < OUT; o++) {
-            float s[NR];
 #pragma unroll
-            for (int i = 0; i < NR; i++) s[i] = 0.f;
+            for (int i = 0; i < NR; i++) s[o][i] = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const float we = widen<KIND>(e % 2 ? w[o][e / 2] >> 16 : w[o][e / 2] & 0xffffu);
 #pragma unroll
-                for (int i = 0; i < NR; i++) s[i] = fmaf(we, t[i][e / 4][e % 4], s[i]);
+                for (int i = 0; i < NR; i++) s[o][i] = fmaf(we, t[i][e / 4][e % 4], s[o][i]);
             }
+        }
+        for (int k = 0; k < lg; k++)                     // the lanes of an output, all outputs side by side
 #pragma unroll
-            for (int i = 0; i < NR; i++) {
-                for (int k = 0; k < lg; k++) s[i] += __shfl_xor(s[i], 1 << k, kWave);
-                const int m = m0 + o * per;
-                if (sub == 0 && m < l.M && i < f.rows) l.out[f.row(i) * l.os + m] = y[o][i] + s[i];
-            }
+            for (int o = 0; o < OUT; o++)
+#pragma unroll
+                for (int i = 0; i < NR; i++) s[o][i] += __shfl_xor(s[o][i], 1 << k, kWave);
+        if (sub) return;
+#pragma unroll
+        for (int o = 0; o < OUT; o++) {
+            const int m = m0 + o * per;
+            if (m >= l.M) break;
+#pragma unroll
+            for (int i = 0; i < NR; i++)
+                if (i < f.rows) l.out[f.row(i) * l.os + m] = y[o][i] + s[o][i];
         }
     }
 };
