@@ -89,6 +89,14 @@ def test_rows(B, n):
     one(B, 256, 136, 16, n, "bf16", spread(B, n, B), seed=B)
 
 
+@pytest.mark.parametrize("B,n", [(8191, 3), (8192, 40), (8193, 1), (9001, 300), (20000, 2), (70, 1022), (300, 1023), (1000, 1500), (8500, 4096)])
+def test_many_rows_and_adapters(B, n):
+    """More rows than the sorting block keeps in registers, more adapters than it has threads."""
+    one(B, 64, 32, 8, n, "bf16", spread(B, n, B), seed=n)
+    one(B, 36, 20, 3, n, "fp16", np.random.default_rng(B).integers(-1, n, B).tolist(), seed=n)
+    one(B, 32, 32, 4, n, "bf16", sorted(spread(B, n, B + 1)), seed=n, ranks=np.random.default_rng(n).integers(-1, 6, n).tolist())
+
+
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("B", [1, 7, 64])
 @pytest.mark.parametrize("rank,N", [(16, 4096), (16, 4104), (17, 4096), (128, 512), (128, 520), (1, 60000), (8, 9000), (64, 5000)])
