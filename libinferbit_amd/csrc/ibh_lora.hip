@@ -131,7 +131,7 @@ __device__ __forceinline__ u4_t load_rank(const Lora& l, const uint16_t* p, int 
 // by the blocks of its first, fifth, ... row: what they share is read from
 // memory once and from L2 by the others.  A chain of waits bounds these: ids, an
 // adapter's rank, its numbers and x, sums over the block (32 rows of 4096, each
-// with an adapter of rank 16: 8.4 MB in 3.8 and 3.5 us, 8.0 in one launch).
+// with an adapter of rank 16: 8.4 MB in 4.2 and 3.3 us, 7.1 in one launch).
 struct Few {
     int id, rank, rows;             // rows 0: this block has nothing to do
     // Four numbers, all of them read to pick one: one of an array, or one of four
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(kBoth) void lora_both_few(Lora l, int lg) {
 // ── more rows: tiles of one adapter's rows on the matrix cores ───────────────
 // One block sorts the rows by adapter (counting; the order within one adapter
 // is left to chance and changes no result: a row's sums do not depend on its
-// place) and cuts each adapter's rows into tiles.  3.6 us for 120 rows, 5.7 for
+// place) and cuts each adapter's rows into tiles.  3.6 us for 120 rows, 5.8 for
 // 4099: 1.5 until ids are there, the rest code that is fetched once and LDS
 // atomics one behind the other.
 __global__ __launch_bounds__(1024) void lora_plan(Lora l) {
@@ -698,9 +698,9 @@ LoraPlan plan_of(const ibh_lora_adapters* l, int B) {
     while (8 << p.lg < l->rank) p.lg++;
     // One launch where a is small and a block a CU holds all outputs: it reads a
     // once for each block of outputs, but spares a launch and a workspace (kernels
-    // alone, one and two launches: 1 x 2048, rank 8: 4.5 and 6.1 us; 32 x 4096 of
-    // rank 16: 8.0 and 7.4, 10 and 14 with the call; M 14336 there: 15 and 9.8;
-    // 64 x 4096 of rank 32: 25 and 13).
+    // alone, one and two launches: 1 x 2048, rank 8: 4.3 and 5.8 us; 32 x 4096 of
+    // rank 16: 7.1 and 7.5, 10 and 14 with the call; M 14336 there: 13.1 and 9.3;
+    // 64 x 4096 of rank 32: 14.1 and 10.9).
     const int span = (kBoth >> p.lg) * kBothOut;
     p.both = p.few && (size_t)l->rank * l->N <= kBothMost && (size_t)B * ((l->M + span - 1) / span) <= 256;
     p.Rp = (l->rank + 7) / 8 * 8;
