@@ -317,8 +317,9 @@ int    ibh_kv4_evict(const ibh_kv4_cache* src, const ibh_kv4_cache* dst, const f
  * halves away from zero, exactly: codes do not depend on r.  (The codes of
  * ibh_quantize_act_g128 of y are the same but for quotients within its own
  * rounding of a border.)  r max|p| < 1e-10 gives codes 0 and s 1e-10, as there.
- * The sum and r are held in 64 bits, y and s rounded once.  A row that holds a NaN or an infinity is NaN in
- * y and s, 128 columns of p that do in s; codes are 0 there.
+ * The sum and r are held in 64 bits, y and s rounded once.  A row that holds a
+ * NaN or an infinity is NaN in y and s, 128 columns of p that do in s; codes are
+ * 0 there.
  * y or h may be x or delta themselves (rows of N floats); otherwise outputs
  * overlap nothing. */
 int ibh_add_rmsnorm(float* y, int8_t* q, float* s, float* h, const float* x, const float* delta,
@@ -327,15 +328,18 @@ int ibh_add_rmsnorm(float* y, int8_t* q, float* s, float* h, const float* x, con
 /* Low-rank adapters of many requests beside a shared projection:
  *   out[b] = base[b] + scales[i] * B_i (A_i x[b]),  i = ids[b]
  * with fp32 sums of the adapters' 16-bit numbers and x as it is (no rounding in
- * between but fp32's).  (From 65 rows on, parts of x and of A x below 2^-126 count as 0.)  base NULL stands for zeros; base may be out.  A row of a
- * negative id has no adapter: out = base.  Up to 4096 adapters.  Rows may come in any order; those of
+ * between but fp32's).  From 65 rows on, parts of x and of A x below 2^-126 count
+ * as 0, and what would be infinite may be NaN.
+ * base NULL stands for zeros; base may be out.  A row of a negative id has no
+ * adapter: out = base.  Up to 4096 adapters.  Rows may come in any order; those of
  * one adapter are served together.  ids, scales and ranks are read on the
  * device, so a captured graph follows them.  An id of n or more, or a rank
  * outside 0 .. rank, raises IBH_DEVERR_LORA (ibh_device_errors) and makes that
  * row NaN.
  * out overlaps nothing else.  `ws` >= ibh_lora_workspace_bytes (0 for few rows
- * and small adapters) on 16 bytes; NULL = the library's workspace of 4 MiB: a call that needs more is refused
- * (IBH_ERROR_MEMORY).  Calls that share one must not overlap in time. */
+ * and small adapters) on 16 bytes; NULL = the library's workspace of 4 MiB: a
+ * call that needs more is refused (IBH_ERROR_MEMORY).  Calls that share one must
+ * not overlap in time. */
 #define IBH_F16  0
 #define IBH_BF16 1
 #define IBH_LORA_MAX_RANK 256
