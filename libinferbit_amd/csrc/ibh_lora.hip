@@ -23,7 +23,6 @@ constexpr int kBoth = 512;          // threads that do both products of few rows
 constexpr int kBothOut = 4;         // the outputs of a lane group there,
 constexpr size_t kBothMost = 65536; // and the numbers of an adapter's a up to which they do
 constexpr int kSpan = 256;          // outputs that a block of the second product takes
-constexpr int kMaxSplit = 16;       // blocks that share a tile's columns
 
 typedef float f4_t __attribute__((ext_vector_type(4), aligned(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -710,9 +709,14 @@ LoraPlan plan_of(const ibh_lora_adapters* l, int B) {
     if (!p.few) {
         p.max_tiles = B / kTile + min(l->n + 2, B);
         p.plan_bytes = sizeof(Tile) * (size_t)p.max_tiles;
-        // the splits of a tile's columns: 512 columns a block, what its wavefronts
-        // have under way at once
-        p.S = min(kMaxSplit, (l->N + 511) / 512);
+        // The blocks that share a tile's columns, eights because the second product
+        // adds t up eight at a time.  More of them shorten the first product's chain
+        // and lengthen the second, the more rows the more (both kernels, eight
+        // adapters): 16 and 8 for 300 x 8192 of rank 32 take 14.3 and 16.6 us, for 1000
+        // x 8192 of rank 64 29.4 and 26.4, for 300 x 2048 10.9 and 10.6; 8 and 1 for 500
+        // x 1024 9.9 and 13.8, for 4099 x 1024 of rank 64 39.2 and 31.8; 4 as 512
+        // columns a block for 4099 x 2048 28.6 where 8 take 26.2.
+        p.S = l->N <= B / 4 ? 1 : B <= 512 && l->N > 4096 ? 16 : 8;
     }
     p.bytes = p.both ? 0 : p.plan_bytes + (size_t)p.S * B * p.Rp * 4;
     return p;
