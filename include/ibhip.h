@@ -321,7 +321,7 @@ int    ibh_kv4_evict(const ibh_kv4_cache* src, const ibh_kv4_cache* dst, const f
  * NaN or an infinity is NaN in y and s, 128 columns of p that do in s; codes are
  * 0 there.
  * y or h may be x or delta themselves (rows of N floats); otherwise outputs
- * overlap nothing. */
+ * overlap nothing.  N up to 2^30, B below 2^22. */
 int ibh_add_rmsnorm(float* y, int8_t* q, float* s, float* h, const float* x, const float* delta,
                     const float* weight, float eps, int N, int B, int x_stride, int delta_stride, void* stream);
 
@@ -331,11 +331,12 @@ int ibh_add_rmsnorm(float* y, int8_t* q, float* s, float* h, const float* x, con
  * between but fp32's).  From 65 rows on, parts of x and of A x below 2^-126 count
  * as 0, and what would be infinite may be NaN.
  * base NULL stands for zeros; base may be out.  A row of a negative id has no
- * adapter: out = base.  Up to 4096 adapters.  Rows may come in any order; those of
- * one adapter are served together.  ids, scales and ranks are read on the
- * device, so a captured graph follows them.  An id of n or more, or a rank
- * outside 0 .. rank, raises IBH_DEVERR_LORA (ibh_device_errors) and makes that
- * row NaN.
+ * adapter: out = base.  Rows may come in any order; those of one adapter are
+ * served together.  ids, scales and ranks are read on the device, so a captured
+ * graph follows them.  An id of n or more, or a rank outside 0 .. rank, raises
+ * IBH_DEVERR_LORA (ibh_device_errors) and makes that row NaN.
+ * Up to 4096 adapters, N and M up to 2^20; from 65 rows on B / 32 + min(n + 2, B)
+ * up to 65535, and times M / 256 below 2^24 (the blocks of a launch).
  * out overlaps nothing else.  `ws` >= ibh_lora_workspace_bytes (0 for few rows
  * and small adapters) on 16 bytes; NULL = the library's workspace of 4 MiB: a
  * call that needs more is refused (IBH_ERROR_MEMORY).  Calls that share one must
@@ -364,7 +365,7 @@ int    ibh_lora(const ibh_lora_adapters* l, float* out, const float* base, const
  * probability 0 and is never among the k; where fewer are left the rest is -1
  * and -infinity.  A row without any finite logit but -infinity: log-probabilities
  * -infinity, entropy 0.  A row that holds a NaN or +infinity: NaN, ids -1.
- * Outputs overlap nothing.  `ws` >= ibh_logprobs_workspace_bytes (0 for many
+ * Outputs overlap nothing.  V up to 2^30, B below 2^24.  `ws` >= ibh_logprobs_workspace_bytes (0 for many
  * calls) on 16 bytes; NULL = the library's workspace of 4 MiB: a call that needs
  * more is refused (IBH_ERROR_MEMORY).  Calls that share one must not overlap in
  * time. */

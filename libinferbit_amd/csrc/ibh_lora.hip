@@ -126,7 +126,7 @@ __device__ __forceinline__ u4_t load_rank(const Lora& l, const uint16_t* p, int 
 }
 
 // ── up to kFew rows ──────────────────────────────────────────────────────────
-// Block x belongs to row x.  The rows of its adapter are served four at a time
+// Each block belongs to a row.  The rows of its adapter are served four at a time
 // by the blocks of its first, fifth, ... row: what they share is read from
 // memory once and from L2 by the others.  A chain of waits bounds these: ids, an
 // adapter's rank, its numbers and x, sums over the block (32 rows of 4096, each
@@ -141,8 +141,8 @@ struct Few {
         return (r0 & -(i == 0)) | (r1 & -(i == 1)) | (r2 & -(i == 2)) | (r3 & -(i == 3));
     }
 };
-__device__ __forceinline__ Few few_of(const Lora& l) {
-    const int lane = threadIdx.x & 63, me = blockIdx.x;
+__device__ __forceinline__ Few few_of(const Lora& l, int me) {
+    const int lane = threadIdx.x & 63;
     const int mine = lane < l.B ? max(l.ids[lane], -1) : -2;
     Few f;
     f.id = __builtin_amdgcn_readlane(mine, me);
@@ -242,7 +242,7 @@ __device__ __forceinline__ void shrink_rows(const Lora& l, const Few& f, int r0,
 template <int KIND, bool WHOLE>
 __global__ __launch_bounds__(256) void lora_shrink_few(Lora l) {
     __shared__ float part[16][4];
-    const Few f = few_of(l);
+    const Few f = few_of(l, blockIdx.x);
     const int r0 = blockIdx.y * 4;
     if (!f.rows || f.rank <= 0 || r0 >= (f.rank + 7) / 8 * 8) return;
     auto store = [&](int i, int r, float v) { l.t[(size_t)f.row(i) * l.Rp + r] = v; };
@@ -251,8 +251,8 @@ __global__ __launch_bounds__(256) void lora_shrink_few(Lora l) {
     else shrink_rows<KIND, WHOLE, 256, 4, 4>(l, f, r0, part, store);
 }
 
-// Outputs of a block: a row of b in `1 << lg` lanes, eight numbers each; OUT
-// outputs a lane group.
+// Outputs of block `block` of a row: a row of b in `1 << lg` lanes, eight numbers
+// each; OUT outputs a lane group.
 template <int KIND, bool WHOLE, int T, int OUT, int NR>
 struct Expand {
     u4_t w[OUT];
@@ -260,9 +260,9 @@ struct Expand {
     int sub, per, m0, lg;
 
     // what does not need t
-    __device__ __forceinline__ Expand(const Lora& l, const Few& f, int lg_) : lg(lg_) {
+    __device__ __forceinline__ Expand(const Lora& l, const Few& f, int lg_, int block) : lg(lg_) {
         sub = threadIdx.x & ((1 << lg) - 1), per = T >> lg;
-        m0 = blockIdx.y * per * OUT + (threadIdx.x >> lg);
+        m0 = block * per * OUT + (threadIdx.x >> lg);
         const uint16_t* b = l.b + (size_t)f.id * l.M * l.R;
 #pragma unroll
         for (int o = 0; o < OUT; o++) {
@@ -309,10 +309,10 @@ struct Expand {
 };
 
 // Rows without an adapter: base; with one that is not in the table: NaN.
-__device__ __forceinline__ void few_without(const Lora& l, const Few& f, int span) {
-    if (f.rank < 0 && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(&ibh_lora_err, IBH_DEVERR_LORA);
+__device__ __forceinline__ void few_without(const Lora& l, const Few& f, int span, int block) {
+    if (f.rank < 0 && threadIdx.x == 0 && block == 0) atomicOr(&ibh_lora_err, IBH_DEVERR_LORA);
     if (f.rank == 0 && l.out == l.base) return;
-    const int m0 = blockIdx.y * span;
+    const int m0 = block * span;
     for (int i = 0; i < f.rows; i++)
         for (int m = m0 + threadIdx.x; m < min(m0 + span, l.M); m += blockDim.x)
             l.out[f.row(i) * l.os + m] = f.rank < 0 ? __builtin_nanf("") : l.base ? l.base[f.row(i) * l.bs + m] : 0.f;
@@ -320,25 +320,32 @@ __device__ __forceinline__ void few_without(const Lora& l, const Few& f, int spa
 
 template <int KIND, bool WHOLE, int NR>
 __device__ __forceinline__ void expand_rows(const Lora& l, const Few& f, int lg) {
-    Expand<KIND, WHOLE, 256, kOut, NR>(l, f, lg).finish(l, f, [&](int i, int r) {
+    Expand<KIND, WHOLE, 256, kOut, NR>(l, f, lg, blockIdx.x).finish(l, f, [&](int i, int r) {
         return *(const f4_t*)(l.t + (size_t)f.row(i) * l.Rp + r);
     });
 }
+// Outputs in the first dimension, rows in the second, which has room for 65535
+// blocks: 2^20 outputs in sixteens are one more (64 x 4096, rank 32: 5.6 us, rows
+// first 5.8; eight adapters instead of 64: 4.8 and 7.3; 64 x 8192, rank 256: 58
+// and 61; 16 x 4096, rank 128: 6.0 and 5.6).
 template <int KIND, bool WHOLE>
 __global__ __launch_bounds__(256) void lora_expand_few(Lora l, int lg) {
-    const Few f = few_of(l);
+    const Few f = few_of(l, blockIdx.y);
     if (!f.rows) return;
-    if (f.rank <= 0) few_without(l, f, (256 >> lg) * kOut);
+    if (f.rank <= 0) few_without(l, f, (256 >> lg) * kOut, blockIdx.x);
     else if (f.rows == 1) expand_rows<KIND, WHOLE, 1>(l, f, lg);
     else if (f.rows == 2) expand_rows<KIND, WHOLE, 2>(l, f, lg);
     else expand_rows<KIND, WHOLE, 4>(l, f, lg);
 }
 
 // Both products in one launch where an adapter's a is small: every block that
-// takes outputs of some rows works their t out by itself.
+// takes outputs of some rows works their t out by itself.  Rows in the first
+// dimension: with 8, 16, 24, ... of them a row's blocks come to one XCD, whose L2
+// reads a once for all of them (32 x 4096, rank 16: 7.2 us, 8.7 with the outputs
+// first); the second has 256 blocks at most.
 template <int KIND, bool WHOLE, int NR>
 __device__ __forceinline__ void both_rows(const Lora& l, const Few& f, int lg, float (*part)[kBoth / 64], float* t) {
-    const Expand<KIND, WHOLE, kBoth, kBothOut, NR> e(l, f, lg);
+    const Expand<KIND, WHOLE, kBoth, kBothOut, NR> e(l, f, lg, blockIdx.y);
     for (int r0 = 0; r0 < (f.rank + 7) / 8 * 8; r0 += 8) {
         if (r0) __syncthreads();
         shrink_rows<KIND, WHOLE, kBoth, 8, NR>(l, f, r0, part, [&](int i, int r, float v) { t[i * l.Rp + r] = v; });
@@ -350,9 +357,9 @@ template <int KIND, bool WHOLE>
 __global__ __launch_bounds__(kBoth) void lora_both_few(Lora l, int lg) {
     __shared__ float part[32][kBoth / 64];
     __shared__ __align__(16) float t[4 * IBH_LORA_MAX_RANK];
-    const Few f = few_of(l);
+    const Few f = few_of(l, blockIdx.x);
     if (!f.rows) return;
-    if (f.rank <= 0) few_without(l, f, (kBoth >> lg) * kBothOut);
+    if (f.rank <= 0) few_without(l, f, (kBoth >> lg) * kBothOut, blockIdx.y);
     else if (f.rows == 1) both_rows<KIND, WHOLE, 1>(l, f, lg, part, t);
     else if (f.rows == 2) both_rows<KIND, WHOLE, 2>(l, f, lg, part, t);
     else both_rows<KIND, WHOLE, 4>(l, f, lg, part, t);
@@ -733,7 +740,7 @@ void launch_shrink(const Lora& l, const LoraPlan& p, hipStream_t st) {
 template <int KIND, bool WHOLE>
 void launch_expand(const Lora& l, const LoraPlan& p, int lg, hipStream_t st) {
     const int span = (256 >> lg) * kOut;
-    if (p.few) lora_expand_few<KIND, WHOLE><<<dim3(l.B, (l.M + span - 1) / span), 256, 0, st>>>(l, lg);
+    if (p.few) lora_expand_few<KIND, WHOLE><<<dim3((l.M + span - 1) / span, l.B), 256, 0, st>>>(l, lg);
     else
         lora_expand_tile<KIND, WHOLE><<<dim3((l.M + kSpan - 1) / kSpan, l.max_tiles), 256,
                                         max(3 * kTile * ((l.R + 31) / 32 * 32 + 8) * 2, kTile * (kSpan + 4) * 4), st>>>(l);
