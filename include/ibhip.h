@@ -328,8 +328,9 @@ int ibh_add_rmsnorm(float* y, int8_t* q, float* s, float* h, const float* x, con
 /* Low-rank adapters of many requests beside a shared projection:
  *   out[b] = base[b] + scales[i] * B_i (A_i x[b]),  i = ids[b]
  * with fp32 sums of the adapters' 16-bit numbers and x as it is (no rounding in
- * between but fp32's).  From 65 rows on, parts of x and of A x below 2^-126 count
- * as 0, and what would be infinite may be NaN.
+ * between but fp32's).  From 65 rows on, what of x and of A x lies below 2^-133 is
+ * cut off (from 2^-110 on a number keeps all its bits), and what would be infinite
+ * may be NaN.
  * base NULL stands for zeros; base may be out.  A row of a negative id has no
  * adapter: out = base.  Rows may come in any order; those of one adapter are
  * served together.  ids, scales and ranks are read on the device, so a captured

@@ -452,7 +452,10 @@ __global__ __launch_bounds__(1024) void lora_plan(Lora l) {
 }
 
 // fp32 numbers as bf16 numbers, upper halves cut off one after the other: 8
-// bits each, all 24 in three, nothing lost.
+// bits each, all 24 in three.  Nothing is lost of numbers of 2^-110 and more; of
+// smaller ones what lies below 2^-133, the last place of a bf16 number (the matrix
+// cores take subnormal ones as they are).  An infinity leaves NaN below it: a sum
+// that holds one becomes NaN, as it does beside the next one of the other sign.
 __device__ __forceinline__ uint32_t upper(float a, float b) {
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
 }
