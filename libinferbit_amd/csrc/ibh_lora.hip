@@ -794,8 +794,8 @@ extern "C" size_t ibh_lora_workspace_bytes(const ibh_lora_adapters* l, int B) {
 
 extern "C" int ibh_lora(const ibh_lora_adapters* l, float* out, const float* base, const float* x, const int32_t* ids,
                         int B, int out_stride, int base_stride, int x_stride, void* ws, size_t ws_bytes, void* stream) {
-    if (!adapters_ok(l, "ibh_lora")) return IBH_ERROR_PARAM;
     if (B == 0) return IBH_OK;
+    if (!adapters_ok(l, "ibh_lora")) return IBH_ERROR_PARAM;
     if (!out || !x || !ids || B < 0 || (B > 1 && (out_stride < l->M || (base && base_stride < l->M) || x_stride < l->N))) {
         ibh_set_error("ibh_lora: invalid arguments (B=%d out_stride=%d base_stride=%d x_stride=%d)", B, out_stride,
                       base_stride, x_stride);
