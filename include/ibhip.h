@@ -338,7 +338,8 @@ int ibh_add_rmsnorm(float* y, int8_t* q, float* s, float* h, const float* x, con
  * IBH_DEVERR_LORA (ibh_device_errors) and makes that row NaN.
  * Up to 4096 adapters, N and M up to 2^20; from 65 rows on B / 32 + min(n + 2, B)
  * up to 65535, and times M / 256 below 2^24 (the blocks of a launch).
- * out overlaps nothing else.  `ws` >= ibh_lora_workspace_bytes (0 for few rows
+ * out overlaps nothing else (its rows may lie between x's or base's, all equally
+ * far apart).  `ws` >= ibh_lora_workspace_bytes (0 for few rows
  * and small adapters) on 16 bytes; NULL = the library's workspace of 4 MiB: a
  * call that needs more is refused (IBH_ERROR_MEMORY).  Calls that share one must
  * not overlap in time. */

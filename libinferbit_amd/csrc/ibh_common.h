@@ -35,6 +35,18 @@ inline bool ibh_overlap(const void* a, size_t na, const void* b, size_t nb) {
     return a && b && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
 }
 
+// The same of two sets of rows: na and nb bytes, sa and sb bytes apart.  Rows that
+// lie equally far apart may take turns, as columns of one wide array do: none of b
+// then begins within one of a or reaches its next.
+inline bool ibh_rows_overlap(size_t rows, const void* a, size_t na, size_t sa, const void* b, size_t nb, size_t sb) {
+    const size_t la = rows ? (rows - 1) * sa + na : 0, lb = rows ? (rows - 1) * sb + nb : 0;
+    if (!ibh_overlap(a, la, b, lb)) return false;
+    if (rows < 2 || sa != sb) return true;
+    const uintptr_t u = (uintptr_t)a, v = (uintptr_t)b;
+    const size_t behind = u <= v ? (v - u) % sa : (sa - (u - v) % sa) % sa;   // where a row of b begins in a's
+    return behind < na || behind + nb > sa;
+}
+
 #define IBH_HIP(call, what)                                                     \
     do {                                                                        \
         hipError_t e_ = (call);                                                 \

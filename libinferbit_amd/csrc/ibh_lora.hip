@@ -803,7 +803,9 @@ extern "C" int ibh_lora(const ibh_lora_adapters* l, float* out, const float* bas
     }
     const size_t rows = B, ob = ((rows - 1) * out_stride + l->M) * 4, bb = ((rows - 1) * base_stride + l->M) * 4;
     const size_t xb = ((rows - 1) * x_stride + l->N) * 4, n = l->n;
-    if (ibh_overlap(out, ob, x, xb) || (!(out == base && (B == 1 || out_stride == base_stride)) && ibh_overlap(out, ob, base, bb)) ||
+    const size_t om = (size_t)l->M * 4, os = (size_t)out_stride * 4;
+    if (ibh_rows_overlap(rows, out, om, os, x, (size_t)l->N * 4, (size_t)x_stride * 4) ||
+        (!(out == base && (B == 1 || out_stride == base_stride)) && ibh_rows_overlap(rows, out, om, os, base, om, (size_t)base_stride * 4)) ||
         ibh_overlap(out, ob, ids, rows * 4) || ibh_overlap(out, ob, l->a, n * l->rank * l->N * 2) ||
         ibh_overlap(out, ob, l->b, n * l->rank * l->M * 2) || ibh_overlap(out, ob, l->scales, n * 4) ||
         ibh_overlap(out, ob, l->ranks, n * 4)) {

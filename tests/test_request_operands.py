@@ -18,3 +18,27 @@ def test_no_rows_need_no_adapters():
     assert lora(0) == 0
     assert lora(0, n=0, a=None, b=None, out=None, x=None, ids=None) == 0
     assert lora(1, n=0) == -5
+
+
+def test_rows_that_take_turns():
+    """Columns of one wide array: rows of out between those of x and base, but not on them."""
+    S, at = 16384, lambda f: (3 << 40) + 4 * f
+    for x, base in ((4096, 8192), (8192, 4096), (-4096, -8192), (12288, -4096), (4096 + 3 * S, None), (4096 - 2 * S, 8192 - S)):
+        assert lora(5, x=at(x), base=None if base is None else at(base), os=S, xs=S, bs=S) == -3, (x, base)
+    for x in (0, 1, -1, 4095, -4095, 12289, -12289, S - 4095, 2 * S - 4095, -S + 4095, -2 * S + 1):
+        assert lora(5, x=at(x), os=S, xs=S) == -5, x
+        assert lora(5, base=at(x), os=S, bs=S) == (-3 if x == 0 else -5), x
+    # single rows, and rows that lie unequally far apart, by all that lies between their first and last number
+    assert lora(1, x=at(4096), os=S, xs=S) == lora(1, x=at(-4096)) == -3
+    assert lora(1, x=at(4095), os=S, xs=S) == -5
+    assert lora(2, x=at(4096), os=S, xs=S + 4096) == -5
+    assert lora(2, x=at(S + 4096), os=S, xs=S + 4096) == -3
+
+
+def test_overlap_of_rows_by_trying_all():
+    """Whether a call is refused, against the rows' numbers themselves."""
+    for s in (8, 11):
+        mine = {i * s + j for i in range(66) for j in range(5)}
+        for off in range(-3 * s, 3 * s + 1):
+            others = {off + i * s + j for i in range(66) for j in range(3)}
+            assert lora(66, N=3, M=5, x=(3 << 40) + 4 * off, os=s, xs=s) == (-5 if mine & others else -3), (s, off)
