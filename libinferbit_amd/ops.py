@@ -3,8 +3,10 @@
 Names and argument meaning follow the reference (src/threading.c,
 src/kernels/scalar.c, src/inferbit_internal.h:199-277): ``out`` first, then
 weights, scales, activations, then sizes.  Operands are torch tensors
-resident on the GPU; work is enqueued on torch's current stream so
-torch.cuda events time it.  Errors raise IbhError (the library's negative
+resident on the current GPU; work is enqueued on torch's current stream so
+torch.cuda events time it.  Calls that name another GPU for themselves (the
+4-bit cache's, and those around a batch's projections) run on their operands'
+and its current stream.  Errors raise IbhError (the library's negative
 INFERBIT_ERROR_* code plus its message).
 """
 from __future__ import annotations
@@ -21,11 +23,76 @@ SCALE_F16, SCALE_F32 = 0, 1
 
 
 def _ptr(t: torch.Tensor):
+    """The address of t, a contiguous tensor of the current GPU: a launch there reaches no other GPU's memory."""
     if not t.is_cuda:
         raise ValueError("libinferbit_amd ops take GPU tensors")
+    if t.get_device() != torch._C._cuda_getDevice():
+        raise ValueError(f"operand on {t.device}, the current GPU is cuda:{torch._C._cuda_getDevice()}")
     if not t.is_contiguous():
         raise ValueError("operand must be contiguous")
     return t.data_ptr()
+
+
+def _gpu(t) -> int:
+    """The GPU that t is on."""
+    index = t.get_device()
+    if index < 0:
+        raise ValueError("libinferbit_amd ops take GPU tensors")
+    return index
+
+
+def _on(t, index: int, dtype, shape):
+    """The address of t, a contiguous tensor of GPU `index` with the given type and shape."""
+    if t.get_device() == index and t.dtype is dtype and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
+    if t.get_device() != index:
+        raise ValueError(f"operand on {t.device}, another is on cuda:{index}")
+    if t.dtype is not dtype:
+        raise TypeError(f"operand must be {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"operand must be {list(shape)}, got {list(t.shape)}")
+    raise ValueError("operand must be contiguous")
+
+
+def _spaced(t, index: int, shape):
+    """(address, floats between rows) of t, fp32 rows [B, n] of contiguous elements on GPU `index`."""
+    if t.get_device() == index and t.dtype is torch.float32 and t.shape == shape and t.is_contiguous():
+        return t.data_ptr(), shape[1]
+    if t.get_device() != index:
+        raise ValueError(f"operand on {t.device}, another is on cuda:{index}")
+    if t.dtype is not torch.float32:
+        raise TypeError(f"operand must be torch.float32, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"operand must be {list(shape)}, got {list(t.shape)}")
+    s0, s1 = t.stride()
+    if shape[0] <= 1:
+        s0 = shape[1]
+    if (s1 != 1 and shape[1] > 1) or s0 < shape[1] or s0 > 0x7fffffff:
+        raise ValueError("rows must not overlap and their elements must be contiguous")
+    return t.data_ptr(), s0
+
+
+def _call_on(index: int, name: str, *args) -> None:
+    """A call on GPU `index`, on its current stream."""
+    # the stream's handle without the Python object around it: that takes 1.8 us of a call's 8
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = getattr(lib(), name)(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = getattr(lib(), name)(*args, stream)
+    if rc:
+        check(rc, name)
+
+
+def _scratch(ws, need: int, index: int):
+    """(address, bytes, the tensor to keep) of the given workspace, or of `need` bytes on GPU `index`."""
+    if ws is not None:
+        return _on(ws, index, torch.uint8, ws.shape), ws.numel(), ws
+    if not need:
+        return None, 0, None
+    ws = torch.empty(need, dtype=torch.uint8, device=index)
+    return ws.data_ptr(), need, ws
 
 
 def _stream():
@@ -126,7 +193,8 @@ class Kv4Cache:
         size = lib().ibh_kv4_page_bytes(n_kv, head_dim)
         if not size or pool.numel() % size:
             raise ValueError(f"the pool is not whole pages of {n_kv} heads of {head_dim}")
-        self.desc = Kv4Desc(_ptr(pool), self._on(table, torch.int32, table.numel()),
+        _gpu(pool)
+        self.desc = Kv4Desc(self._on(pool, torch.uint8, pool.numel()), self._on(table, torch.int32, table.numel()),
                             self._on(lens, torch.int32, self.n_seq), pool.numel() // size, self.n_seq, self.max_pages,
                             n_kv, head_dim)
         self.ref = ctypes.byref(self.desc)
@@ -160,22 +228,8 @@ class Kv4Cache:
             raise ValueError("rows must be evenly spaced with contiguous elements")
         return t.data_ptr(), n, s1
 
-    def _workspace(self, need: int):
-        """(address, bytes, the tensor to keep) of `need` bytes of scratch memory of the current stream."""
-        if not need:
-            return None, 0, None
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        return ws.data_ptr(), need, ws
-
     def _call(self, name: str, *args) -> None:
-        index = self.index
-        # the current stream's handle without the Python object around it: that takes 1.8 us of a call's 8
-        stream = torch._C._cuda_getCurrentRawStream(index)
-        if torch.cuda.current_device() == index:
-            check(getattr(lib(), name)(*args, stream), name)
-        else:
-            with torch.cuda.device(index):
-                check(getattr(lib(), name)(*args, stream), name)
+        _call_on(self.index, name, *args)
 
 
 def kv4_append(cache: Kv4Cache, k, v) -> None:
@@ -207,10 +261,8 @@ def kv4_attn(out, q, cache: Kv4Cache, n_heads: int, weights_in=None, weights_out
     if weights_in is not None:
         size = cache.n_seq * cache.n_kv * cache.max_pages * KV4_PAGE
         wi, wo = (cache._on(w, torch.float32, size) for w in (weights_in, weights_out))
-    if ws is None:
-        pw, nw, ws = cache._workspace(lib().ibh_kv4_attn_workspace_bytes(cache.ref, n_heads, n_q, wi is not None))
-    else:
-        pw, nw = cache._on(ws, torch.uint8, ws.numel()), ws.numel()
+    need = 0 if ws is not None else lib().ibh_kv4_attn_workspace_bytes(cache.ref, n_heads, n_q, wi is not None)
+    pw, nw, ws = _scratch(ws, need, cache.index)
     cache._call("ibh_kv4_attn", cache.ref, po, pq, n_heads, n_q, sq, wi, wo, pw, nw)
 
 
@@ -221,75 +273,11 @@ def kv4_evict(src: Kv4Cache, dst: Kv4Cache, weights_src, weights_dst, budget: in
     if dst.index != src.index:
         raise ValueError(f"the caches are on {src.device} and {dst.device}")
     n = src.n_seq * src.n_kv
-    if ws is None:
-        pw, nw, ws = src._workspace(lib().ibh_kv4_evict_workspace_bytes(src.ref))
-    else:
-        pw, nw = src._on(ws, torch.uint8, ws.numel()), ws.numel()
+    pw, nw, ws = _scratch(ws, 0 if ws is not None else lib().ibh_kv4_evict_workspace_bytes(src.ref), src.index)
     src._call("ibh_kv4_evict", src.ref, dst.ref,
               src._on(weights_src, torch.float32, n * src.max_pages * KV4_PAGE),
               src._on(weights_dst, torch.float32, n * dst.max_pages * KV4_PAGE), budget, sink, recent,
               src._on(kept, torch.int32, n * budget), pw, nw)
-
-
-def _gpu(t) -> int:
-    """The GPU that t is on."""
-    index = t.get_device()
-    if index < 0:
-        raise ValueError("libinferbit_amd ops take GPU tensors")
-    return index
-
-
-def _on(t, index: int, dtype, shape):
-    """The address of t, a contiguous tensor of GPU `index` with the given type and shape."""
-    if t.get_device() == index and t.dtype is dtype and t.shape == shape and t.is_contiguous():
-        return t.data_ptr()
-    if t.get_device() != index:
-        raise ValueError(f"operand on {t.device}, another is on cuda:{index}")
-    if t.dtype is not dtype:
-        raise TypeError(f"operand must be {dtype}, got {t.dtype}")
-    if t.shape != shape:
-        raise ValueError(f"operand must be {list(shape)}, got {list(t.shape)}")
-    raise ValueError("operand must be contiguous")
-
-
-def _spaced(t, index: int, shape):
-    """(address, floats between rows) of t, fp32 rows [B, n] of contiguous elements on GPU `index`."""
-    if t.get_device() == index and t.dtype is torch.float32 and t.shape == shape and t.is_contiguous():
-        return t.data_ptr(), shape[1]
-    if t.get_device() != index:
-        raise ValueError(f"operand on {t.device}, another is on cuda:{index}")
-    if t.dtype is not torch.float32:
-        raise TypeError(f"operand must be torch.float32, got {t.dtype}")
-    if t.shape != shape:
-        raise ValueError(f"operand must be {list(shape)}, got {list(t.shape)}")
-    s0, s1 = t.stride()
-    if shape[0] <= 1:
-        s0 = shape[1]
-    if (s1 != 1 and shape[1] > 1) or s0 < shape[1] or s0 > 0x7fffffff:
-        raise ValueError("rows must not overlap and their elements must be contiguous")
-    return t.data_ptr(), s0
-
-
-def _call_on(index: int, name: str, *args) -> None:
-    """A call on GPU `index`, on its current stream."""
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch._C._cuda_getDevice() == index:
-        rc = getattr(lib(), name)(*args, stream)
-    else:
-        with torch.cuda.device(index):
-            rc = getattr(lib(), name)(*args, stream)
-    if rc:
-        check(rc, name)
-
-
-def _scratch(ws, need: int, index: int):
-    """(address, bytes, the tensor to keep) of the given workspace, or of `need` bytes on GPU `index`."""
-    if ws is not None:
-        return _on(ws, index, torch.uint8, ws.shape), ws.numel(), ws
-    if not need:
-        return None, 0, None
-    ws = torch.empty(need, dtype=torch.uint8, device=index)
-    return ws.data_ptr(), need, ws
 
 
 def add_rmsnorm(y, x, weight, eps: float, delta=None, h=None, q=None, s=None) -> None:
@@ -467,13 +455,18 @@ class Int4gDeviceTensor:
         self.s = s
         self.M, self.N = s.M, s.N
 
+    def _here(self) -> None:
+        _ptr(self.keep[0])                               # on the current GPU still
+
     def matmul(self, x, out, act_sparse_rel: float = 0.0) -> None:
         """ib_pq_session_matmul on this tensor (src/pq_decode.c:4442-4452)."""
+        self._here()
         check(lib().ibh_int4g_matmul(ctypes.byref(self.s), _ptr(x), _ptr(out), act_sparse_rel, None, 0, _stream()),
               "ibh_int4g_matmul")
 
     def matmul_batched(self, x, out, act_sparse_rel: float = 0.0) -> None:
         """ib_pq_session_matmul_batched (src/pq_decode.c:4501-4539): x [B, N], out [B, M]."""
+        self._here()
         B = x.shape[0]
         check(lib().ibh_int4g_matmul_batched(ctypes.byref(self.s), B, _ptr(x), _ptr(out), act_sparse_rel, None, 0,
                                              _stream()), "ibh_int4g_matmul_batched")

@@ -89,10 +89,8 @@ class PqSession:
 
     def matmul(self, name: str, x, out) -> None:
         """ib_pq_session_matmul on device tensors x [N] -> out [M]."""
-        import torch
-        check(lib().ibh_v5_session_matmul(self._h, name.encode(), ctypes.c_void_p(x.data_ptr()),
-                                          ctypes.c_void_p(out.data_ptr()),
-                                          ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)),
+        from . import ops
+        check(lib().ibh_v5_session_matmul(self._h, name.encode(), ops._ptr(x), ops._ptr(out), ops._stream()),
               "ibh_v5_session_matmul")
 
     def kv_cache(self, max_seq: int) -> KvCache:
