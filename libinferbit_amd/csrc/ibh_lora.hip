@@ -21,7 +21,8 @@ constexpr int kStep = 64;           // columns of x that a wavefront takes at a 
 constexpr int kOut = 2;             // outputs of a lane group in the second product of few rows
 constexpr int kBoth = 512;          // threads that do both products of few rows,
 constexpr int kBothOut = 4;         // the outputs of a lane group there,
-constexpr size_t kBothMost = 65536; // and the numbers of an adapter's a up to which they do
+constexpr int kBothRank = 32;       // and the rank
+constexpr size_t kBothMost = 65536; // and numbers of an adapter's a up to which they do
 constexpr int kSpan = 256;          // outputs that a block of the second product takes
 
 typedef float f4_t __attribute__((ext_vector_type(4), aligned(4)));
@@ -356,7 +357,7 @@ __device__ __forceinline__ void both_rows(const Lora& l, const Few& f, int lg, f
 template <int KIND, bool WHOLE>
 __global__ __launch_bounds__(kBoth) void lora_both_few(Lora l, int lg) {
     __shared__ float part[32][kBoth / 64];
-    __shared__ __align__(16) float t[4 * IBH_LORA_MAX_RANK];
+    __shared__ __align__(16) float t[4 * kBothRank];
     const Few f = few_of(l, blockIdx.x);
     if (!f.rows) return;
     if (f.rank <= 0) few_without(l, f, (kBoth >> lg) * kBothOut, blockIdx.y);
@@ -706,12 +707,17 @@ LoraPlan plan_of(const ibh_lora_adapters* l, int B) {
     p.lg = 0;
     while (8 << p.lg < l->rank) p.lg++;
     // One launch where a is small and a block a CU holds all outputs: it reads a
-    // once for each block of outputs, but spares a launch and a workspace (kernels
-    // alone, one and two launches: 1 x 2048, rank 8: 4.3 and 5.8 us; 32 x 4096 of
-    // rank 16: 7.1 and 7.5, 10 and 14 with the call; M 14336 there: 13.1 and 9.3;
-    // 64 x 4096 of rank 32: 14.1 and 10.9).
+    // once for each block of outputs, eight ranks after eight, but spares a launch
+    // and a workspace, 4 us of a call.  Kernels alone, one and two launches, in us:
+    //   outputs     1 x 2048, rank 8: 4.2 and 5.7; 32 x 4096, rank 16: 7.4 and 7.7, its
+    //               14336 outputs: 12.8 and 9.8
+    //   numbers     32 rows, rank 16 by 3584, 5120, 6144, 8192: 6.9 and 7.3, 7.9 and 8.0,
+    //               8.4 and 8.3, 8.9 and 9.1; one row of 8192: 7.5 and 7.1; 32 rows, rank
+    //               32 by 4096: 11.4 and 9.4; of rank 8 one launch stays the faster one
+    //   rank        32 rows by 65536 numbers, rank 16, 32, 64, 128, 256: 7.4 and 7.7, 8.4
+    //               and 7.1, 11.9 and 7.2, 20 and 8.2, 67 and 11
     const int span = (kBoth >> p.lg) * kBothOut;
-    p.both = p.few && (size_t)l->rank * l->N <= kBothMost && (size_t)B * ((l->M + span - 1) / span) <= 256;
+    p.both = p.few && l->rank <= kBothRank && (size_t)l->rank * l->N <= kBothMost && (size_t)B * ((l->M + span - 1) / span) <= 256;
     p.Rp = (l->rank + 7) / 8 * 8;
     p.S = 1;
     p.max_tiles = 0;

@@ -42,3 +42,11 @@ def test_overlap_of_rows_by_trying_all():
         for off in range(-3 * s, 3 * s + 1):
             others = {off + i * s + j for i in range(66) for j in range(3)}
             assert lora(66, N=3, M=5, x=(3 << 40) + 4 * off, os=s, xs=s) == (-5 if mine & others else -3), (s, off)
+
+
+def test_large_ranks_take_two_launches():
+    """Both products of few rows in one launch (which needs no workspace) work ranks out eight after eight: up to 32."""
+    need = lambda rank, N: _lib.lib().ibh_lora_workspace_bytes(C.byref(_lib.LoraDesc(1 << 40, 2 << 40, None, None, 4, rank, N, 1024, 0)), 32)
+    assert need(8, 8192) == need(16, 4096) == need(32, 2048) == need(32, 64) == 0
+    assert need(33, 64) == 32 * 40 * 4 and need(64, 1024) == 32 * 64 * 4 and need(256, 256) == 32 * 256 * 4
+    assert need(32, 2049) == 32 * 32 * 4
