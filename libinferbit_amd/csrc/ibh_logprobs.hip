@@ -5,13 +5,15 @@
 // and e = sum e^(z - m) (z - m) of its logits, every wavefront the k best it has
 // seen.  log S = m + log s; entropy = log s - e / s.
 //
-// Memory bounds long calls: 2047 rows of 32003, 262 MB, take 50 us without
-// alternatives (5.2 TB/s, as a copy does), 57 with the 8 best and 63 with 20:
+// Memory bounds long calls: 2047 rows of 32003, 262 MB, take 49 us without
+// alternatives (5.3 TB/s, as a copy does), 59 with the 8 best and 67 with 20:
 // the candidates' instructions (a wavefront's bar is the k-th best of its first
-// 1024 logits, so each later piece has about k).  Short calls are chains: of the
-// 11.5 us of 32 x 128000 with the 20 best, 3.2 pass until the first logits are
-// there, 1.3 over the candidates, 0.6 over the sums, 2.5 over the wavefronts'
-// lists, and 4.5 us go to the launch that joins the shares.
+// 1024 logits, so each later piece has about k).  Short calls are chains: of 32 x
+// 128000 with the 20 best, 11.3 us in the first launch and 4.9 in the one that joins
+// the shares, half of the first one's blocks are done after 7.4 us (their last logits
+// there 3.3, candidates held 4.6, the block's wavefronts there 5.6, their sums joined
+// 5.8, their lists sorted 7.1), the last after 9.9.  (Kernels, traced one by one; a
+// row of calls with the 8 best takes 57 us each.)
 #include "ibh_common.h"
 
 namespace {
@@ -332,14 +334,14 @@ __global__ __launch_bounds__(64) void logprobs_join(LogArgs a) {
 
 // How a call is cut.  Rows that fill the card by themselves, and rows of one
 // round of four wavefronts' pieces, take a block of four (300 x 128000, 20 best:
-// 48 us, 45 and a launch where they are shared; 600 x 64000, 8 best: 39 and 44;
-// 60 and 52 in blocks of sixteen).  Fewer rows of up to two rounds of sixteen
-// take a block of those: one launch instead of two (1 x 32000, 5 best: 10.3 us,
-// 10.7 in two kernels and a launch; 255 rows, 20 best: 16 and 20; but 1 x 64000
-// 14 and 11, 1 x 4000 7.3 and 5.8 in one block of four).  Otherwise a row is
-// shared by blocks, whole rounds each, and the shares are joined (32 x 128000, 20
-// best, 256, 512, 1024 and 2048 blocks in all, without the join: 14.4, 11.5, 11.8
-// and 10.5 us; 8 x 260000: 9.6, 7.7, 7.6 and 7.7).
+// 49 us, shared 38 + 5.3 in two launches, 60 in a block of sixteen, of which a CU
+// holds one; 600 x 64000, 8 best: 40, 39 + 5.0 and 52).  Fewer rows of up to two
+// rounds of sixteen take a block of those: one launch instead of two (1 x 32000, 5
+// best: 10.3 us, shared 6.2 + 3.9; 255 rows, 20 best: 16 and 17 + 4.6; but 1 x 64000
+// 14.6 and 6.2 + 3.9, 1 x 4000 7.6 and 6.2 in one block of four).  Otherwise a row
+// is shared by blocks, whole rounds each, and the shares are joined (32 x 128000, 20
+// best, 256, 512 and 1024 blocks in all: 13.7 + 4.7, 11.4 + 4.8 and 10.4 + 5.1; 8 x
+// 260000, 256 and 512: 9.9 + 5.5 and 8.0 + 7.4).
 struct LogPlan {
     int W, S, seg;
     size_t part, bytes;

@@ -131,7 +131,7 @@ __device__ __forceinline__ u4_t load_rank(const Lora& l, const uint16_t* p, int 
 // by the blocks of its first, fifth, ... row: what they share is read from
 // memory once and from L2 by the others.  A chain of waits bounds these: ids, an
 // adapter's rank, its numbers and x, sums over the block (32 rows of 4096, each
-// with an adapter of rank 16: 8.4 MB in 4.2 and 3.3 us, 7.1 in one launch).
+// with an adapter of rank 16: 8.4 MB in 4.1 and 3.2 us, 7.3 in one launch).
 struct Few {
     int id, rank, rows;             // rows 0: this block has nothing to do
     // Four numbers, all of them read to pick one: one of an array, or one of four
@@ -164,7 +164,7 @@ __device__ __forceinline__ Few few_of(const Lora& l, int me) {
 }
 
 // The wavefront's sums of K numbers (2 .. 32): each step gives half of them away
-// to the lane across and takes the other half's, 31 exchanges for 32 numbers where
+// to the lane across and takes the other half's, 32 exchanges for 32 numbers where
 // one sum after the other would take 32 times six.  Returns whose sum a[0] is
 // then, -1 in the lanes that hold copies.
 template <int K>
@@ -369,7 +369,7 @@ __global__ __launch_bounds__(kBoth) void lora_both_few(Lora l, int lg) {
 // ── more rows: tiles of one adapter's rows on the matrix cores ───────────────
 // One block sorts the rows by adapter (counting; the order within one adapter
 // is left to chance and changes no result: a row's sums do not depend on its
-// place) and cuts each adapter's rows into tiles.  3.6 us for 120 rows, 5.8 for
+// place) and cuts each adapter's rows into tiles.  3.8 us for 120 rows, 6.1 for
 // 4099: 1.5 until ids are there, the rest code that is fetched once and LDS
 // atomics one behind the other.
 __global__ __launch_bounds__(1024) void lora_plan(Lora l) {
@@ -485,7 +485,7 @@ __device__ __forceinline__ void pieces(u4_t v, v8bf* p) {
 // wavefront takes 64 columns of all rows at a time, the next 64 under way: every
 // number of x is loaded, cut into pieces and multiplied by one lane, straight in
 // the matrix instructions' own order (16 rows, 32 columns in eights).  4099 x
-// 4096: 16.5 us with rank 16 in bf16 (4.1 TB/s), 22 with rank 32 in fp16, whose
+// 4096: 17 us with rank 16 in bf16 (4.1 TB/s), 22 with rank 32 in fp16, whose
 // pieces take half of the vector instructions; 26 with the pieces in LDS.
 template <int KIND, bool WHOLE, int RT>
 __global__ __launch_bounds__(256, RT <= 2 ? 3 : 2) void lora_shrink_tile(Lora l) {
@@ -708,13 +708,13 @@ LoraPlan plan_of(const ibh_lora_adapters* l, int B) {
     while (8 << p.lg < l->rank) p.lg++;
     // One launch where a is small and a block a CU holds all outputs: it reads a
     // once for each block of outputs, eight ranks after eight, but spares a launch
-    // and a workspace, 4 us of a call.  Kernels alone, one and two launches, in us:
-    //   outputs     1 x 2048, rank 8: 4.2 and 5.7; 32 x 4096, rank 16: 7.4 and 7.7, its
-    //               14336 outputs: 12.8 and 9.8
-    //   numbers     32 rows, rank 16 by 3584, 5120, 6144, 8192: 6.9 and 7.3, 7.9 and 8.0,
-    //               8.4 and 8.3, 8.9 and 9.1; one row of 8192: 7.5 and 7.1; 32 rows, rank
-    //               32 by 4096: 11.4 and 9.4; of rank 8 one launch stays the faster one
-    //   rank        32 rows by 65536 numbers, rank 16, 32, 64, 128, 256: 7.4 and 7.7, 8.4
+    // and a workspace, 4 us of an eager call.  Kernels alone, one and two launches, in us:
+    //   outputs     1 x 2048, rank 8: 4.4 and 5.5; 32 x 4096, rank 16: 7.3 in both, with
+    //               14336 outputs 12.8 and 9.6
+    //   numbers     32 rows, rank 16 by 3584, 5120, 6144, 8192: 7.0 and 7.1, 7.9 and 7.8,
+    //               8.2 and 8.1, 8.9 in both; one row of 8192: 7.4 and 7.1; 32 rows, rank
+    //               32 by 4096: 11.0 and 8.9, rank 8 by 8192: 5.9 and 7.5
+    //   rank        32 rows by 65536 numbers, rank 16, 32, 64, 128, 256: 7.3 in both, 8.4
     //               and 7.1, 11.9 and 7.2, 20 and 8.2, 67 and 11
     const int span = (kBoth >> p.lg) * kBothOut;
     p.both = p.few && l->rank <= kBothRank && (size_t)l->rank * l->N <= kBothMost && (size_t)B * ((l->M + span - 1) / span) <= 256;
@@ -727,11 +727,12 @@ LoraPlan plan_of(const ibh_lora_adapters* l, int B) {
         p.plan_bytes = sizeof(Tile) * (size_t)p.max_tiles;
         // The blocks that share a tile's columns, eights because the second product
         // adds t up eight at a time.  More of them shorten the first product's chain
-        // and lengthen the second, the more rows the more (both kernels, eight
-        // adapters): 16 and 8 for 300 x 8192 of rank 32 take 14.3 and 16.6 us, for 1000
-        // x 8192 of rank 64 29.4 and 26.4, for 300 x 2048 10.9 and 10.6; 8 and 1 for 500
-        // x 1024 9.9 and 13.8, for 4099 x 1024 of rank 64 39.2 and 31.8; 4 as 512
-        // columns a block for 4099 x 2048 28.6 where 8 take 26.2.
+        // and lengthen the second, the more rows the more (both kernels, eight bf16
+        // adapters, 4096 outputs, us): 16 and 8 for 300 x 8192 of rank 32 take 14.0 and
+        // 16.9, for 1000 x 8192 of rank 64 28.4 and 26.1, for 300 x 2048 of rank 32 11.4
+        // in both; 8 and 1 for 500 x 1024 of rank 32 11.7 and 16.4, for 4099 x 1024 of
+        // rank 64 55.3 and 49.7; 8, 4 and 1 for 4099 x 2048 of rank 16 41.1, 42.2 and 43.5;
+        // 8 and 10 for 4099 x 5120 of rank 64 74.8 and 80.9.
         p.S = l->N <= B / 4 ? 1 : B <= 512 && l->N > 4096 ? 16 : 8;
     }
     p.bytes = p.both ? 0 : p.plan_bytes + (size_t)p.S * B * p.Rp * 4;

@@ -2,9 +2,11 @@
 // for a batch of rows in one pass.
 //
 // Memory bounds it: x and delta come once, h and y or the codes go once.  4099
-// rows of 4096 with h and y, 269 MB, take 43 us (6.3 TB/s; a plain copy of a
-// gigabyte runs at 5.2), with codes 41 us; 512 rows with codes 8.5 us; one row 3
-// us, of which a launch is 2.  The sums in 64 bits cost nothing beside that.
+// rows of 4096 with h and y, 269 MB, take 43 us (6.2 TB/s; a plain copy of a
+// gigabyte runs at 5.2), with codes 37, with y and codes 49 us; 512 rows with codes
+// 8.0 us; one row 3 us, of which a launch is 2 (kernels, traced one by one; a row
+// of calls with h and y takes 47 us each).  The sums in 64 bits cost nothing beside
+// that.
 #include "ibh_common.h"
 
 namespace {
@@ -243,12 +245,14 @@ extern "C" int ibh_add_rmsnorm(float* y, int8_t* q, float* s, float* h, const fl
     }
     const NormArgs a{y, s, h, q, x, delta, weight, eps, N, G, (size_t)x_stride, (size_t)delta_stride};
     hipStream_t st = ibh_resolve_stream(stream);
-    // Threads by quads of columns: the fewest that hold the row for short rows
-    // (6000 x 200 in 64 threads 6.2 us, in 256 9.7; 4000 x 1000 in 128 11.0, in 256
-    // 13.2); then, for few rows, wide blocks, whose loads are all under way sooner
-    // (1 x 4096 in 512 threads 3.0 us, in 256 3.9; 64 rows 3.9 and 4.8; 512 rows
-    // 8.3 and 8.6), for many small ones, of which a CU holds more (4099 x 4096 in
-    // 512 50.5 us, in 256 47.1; 4099 x 2048 in 512 27.0, in 64 22.5).
+    // Threads by quads of columns, all in us of the kernel: the fewest that hold the
+    // row for short rows (6000 x 200 in 64 threads 5.9, in 256 9.5; 4000 x 1000 in
+    // 128 11.1, in 256 13.1); then, for few rows, wide blocks, whose loads are all
+    // under way sooner (1 x 4096 in 512 threads 2.8, in 256 3.8; 64 rows 3.9 and 4.8;
+    // 512 rows 8.0 and 8.4), for many small ones, of which a CU holds more (1024 rows
+    // 10.9 in both, 1500 15.5 and 14.7, 4099 44.6 and 43.2; 4099 x 2048 in 512 22.9, in
+    // 64 21.3; 8192 columns in 1024 and 512: 64 rows 4.4 and 4.5, 1024 24.1 and 22.2,
+    // 2000 46.7 and 42.8).
     const bool few = B <= 1024;
     if (N <= 256) launch<64, 1>(a, B, st);
     else if (N <= 1024) launch<128, 2>(a, B, st);
